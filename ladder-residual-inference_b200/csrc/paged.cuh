@@ -1,0 +1,66 @@
+// Paged key-value cache: layout, element types and what the kernels of its operators share.
+//
+// k_pages, v_pages [n_pages, n_kv, page, head_dim]; a page holds `page` positions of every KV head.  Position j of sequence b lies in page
+// table[b][j / page] at row j % page.  Elements are the activations' type, or e4m3 with an fp32 scale for each (page, head, row):
+// value = code * scale.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace lri {
+
+struct e4m3 {
+  uint8_t bits;
+};
+
+// two packed codes, the lower byte first, as halves: exact, every e4m3 number is one of fp16's
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+// eight elements of a cache row as they are stored, as floats
+__device__ __forceinline__ void load_cached8(const e4m3* p, float (&f)[8]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? v.x : v.y;
+    Num<__half>::unpack2(e4m3x2_to_half2(static_cast<uint16_t>(w >> (16 * (i & 1)))), f[2 * i], f[2 * i + 1]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_cached8(const T* p, float (&f)[8]) {
+  load8<T>(p, f);
+}
+
+// Pages of the sequences of a call.
+struct PageTable {
+  const int32_t* ids;  // [n_seq, max_pages], row pitch ld
+  int64_t ld;
+  int n_seq, max_pages, page;
+  int64_t n_pages;
+  __host__ __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(max_pages) * page; }
+  // page that holds position pos (0 <= pos < capacity()) of sequence b, -1: none
+  __device__ __forceinline__ int64_t find(int64_t b, int64_t pos) const {
+    const int64_t id = ids[b * ld + pos / page];
+    return id >= 0 && id < n_pages ? id : -1;
+  }
+};
+
+// Attention of one new token of each sequence (paged_attention.cu).
+struct PagedAttnParams {
+  const void* q;  // [n_seq, n_head, dim]
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  PageTable table;
+  const void* input_pos;  // [n_seq]
+  int pos_is_i64;
+  void* out;  // [n_seq, n_head, dim]
+  int n_head, n_kv, dim;
+  int64_t window;  // 0: none
+  float scale_log2;
+};
+
+}  // namespace lri

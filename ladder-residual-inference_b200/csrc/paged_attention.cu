@@ -1,0 +1,134 @@
+// Attention of one new token of each sequence over a paged key-value cache: y = softmax(q k^T scale) v over the visible positions.
+#include "paged.cuh"
+
+namespace lri {
+
+int check_paged(const char* who, int dtype, int cache_dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, const PageTable& t, int n_kv, int dim);
+
+namespace {
+
+constexpr int kWarps = 4;
+
+// One CTA per (query head, sequence); LANES threads hold a position, eight elements each.  Every group of lanes keeps its own running maximum,
+// sum and values in 32 bits; the groups of a warp are joined by shuffles, the warps through shared memory.
+template <typename T, typename C, int LANES>
+__global__ void __launch_bounds__(kWarps * 32) paged_attn_plain_kernel(const PagedAttnParams p) {
+  constexpr int kGroups = 32 / LANES;
+  __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[kWarps][LANES * 8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int head = blockIdx.x, h = head / (p.n_head / p.n_kv);
+  const int64_t b = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / LANES, e = lane % LANES * 8;
+  int64_t ctx = load_pos(p.input_pos, p.pos_is_i64, b) + 1;
+  ctx = ctx > p.table.capacity() ? p.table.capacity() : ctx;
+  const int64_t lo = p.window > 0 && ctx > p.window ? ctx - p.window : 0;
+  const int64_t at = (b * p.n_head + head) * p.dim + e;
+  float q[8] = {}, o[8] = {}, m = -INFINITY, l = 0.f;
+  if (e < p.dim) load8<T>(static_cast<const T*>(p.q) + at, q);
+  for (int64_t j0 = lo + warp * kGroups; j0 < ctx; j0 += kWarps * kGroups) {  // the warp's bounds are the same in every lane
+    const int64_t j = j0 + group;
+    const int64_t page = j < ctx ? p.table.find(b, j) : -1;
+    const int64_t row = (page * p.n_kv + h) * p.table.page + j % p.table.page;
+    float k[8] = {}, s = 0.f;
+    if (page >= 0 && e < p.dim) load_cached8(static_cast<const C*>(p.k) + row * p.dim + e, k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(q[i], k[i], s);
+#pragma unroll
+    for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    if (page < 0) continue;
+    if (p.k_scale) s *= p.k_scale[row];
+    s *= p.scale_log2;
+    const float m_new = fmaxf(m, s), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = exp2f(m - m_use), w = exp2f(s - m_use);
+    float v[8] = {};
+    if (e < p.dim) load_cached8(static_cast<const C*>(p.v) + row * p.dim + e, v);
+    const float wv = p.v_scale ? w * p.v_scale[row] : w;
+    l = l * corr + w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = o[i] * corr + wv * v[i];
+    m = m_new;
+  }
+  // join the groups of a warp
+#pragma unroll
+  for (int w = LANES; w < 32; w <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, w), l2 = __shfl_xor_sync(0xffffffffu, l, w);
+    const float m_new = fmaxf(m, m2), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float f = exp2f(m - m_use), f2 = exp2f(m2 - m_use);
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = o[i] * f + __shfl_xor_sync(0xffffffffu, o[i], w) * f2;
+    m = m_new;
+  }
+  if (lane < LANES) {
+    if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sm_o[warp][e + i] = o[i];
+  }
+  __syncthreads();
+  if (warp == 0 && lane < LANES && e < p.dim) {
+    float mm = -INFINITY, ll = 0.f, y[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w]);
+    mm = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(sm_m[w] - mm);
+      ll += sm_l[w] * f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += sm_o[w][e + i] * f;
+    }
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;  // nothing visible: zeros; a NaN stays one
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= inv;
+    store8<T>(static_cast<T*>(p.out) + at, y);
+  }
+}
+
+template <typename T, typename C>
+int launch_plain(const PagedAttnParams& p, cudaStream_t st) {
+  auto go = [&](auto kern) {
+    for (int at = 0; at < p.table.n_seq; at += 65535) {
+      PagedAttnParams part = p;
+      part.table.n_seq = p.table.n_seq - at < 65535 ? p.table.n_seq - at : 65535;
+      part.table.ids += at * p.table.ld;
+      part.q = static_cast<const T*>(p.q) + static_cast<int64_t>(at) * p.n_head * p.dim;
+      part.out = static_cast<T*>(p.out) + static_cast<int64_t>(at) * p.n_head * p.dim;
+      part.input_pos = static_cast<const char*>(p.input_pos) + static_cast<int64_t>(at) * (p.pos_is_i64 ? 8 : 4);
+      LRI_CUDA(launch_pdl(kern, dim3(p.n_head, part.table.n_seq), dim3(kWarps * 32), 0, st, part));
+      LRI_LAUNCH_CHECK("paged_attn_plain_kernel");
+    }
+    return static_cast<int>(LRI_OK);
+  };
+  if (p.dim <= 64) return go(paged_attn_plain_kernel<T, C, 8>);
+  if (p.dim <= 128) return go(paged_attn_plain_kernel<T, C, 16>);
+  return go(paged_attn_plain_kernel<T, C, 32>);
+}
+
+}  // namespace
+}  // namespace lri
+
+using namespace lri;
+
+extern "C" size_t lri_paged_attn_decode_workspace_bytes(int n_head, int n_kv, int head_dim) { return 0; }
+
+extern "C" int lri_paged_attn_decode(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale,
+                                     int64_t n_pages, int page_size, const int32_t* pages, int64_t pages_ld, int n_seq, int max_pages, const void* input_pos,
+                                     int pos_is_i64, int64_t window, float scale, void* out, int n_head, int n_kv, int head_dim, void* workspace,
+                                     size_t workspace_bytes, lri_stream_t stream) {
+  PagedAttnParams p{};
+  p.table = PageTable{pages, pages_ld, n_seq, max_pages, page_size, n_pages};
+  int rc = check_paged("paged_attn_decode", dtype, cache_dtype, k_pages, v_pages, k_scale, v_scale, p.table, n_kv, head_dim);
+  if (rc != LRI_OK) return rc;
+  LRI_REQUIRE(n_head >= 1 && n_head <= 65535 && n_head % n_kv == 0, LRI_ERR_ARG, "paged_attn_decode: n_head=%d n_kv=%d", n_head, n_kv);
+  LRI_REQUIRE(window >= 0, LRI_ERR_ARG, "paged_attn_decode: window=%lld", (long long)window);
+  if (n_seq == 0) return LRI_OK;
+  LRI_REQUIRE(q && input_pos && out, LRI_ERR_ARG, "paged_attn_decode: NULL pointer");
+  LRI_REQUIRE(aligned16(q) && aligned16(out), LRI_ERR_ALIGN, "paged_attn_decode: pointers must be 16-byte aligned");
+  p.q = q, p.k = k_pages, p.v = v_pages, p.k_scale = cache_dtype == LRI_E4M3 ? k_scale : nullptr, p.v_scale = cache_dtype == LRI_E4M3 ? v_scale : nullptr;
+  p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64, p.out = out, p.n_head = n_head, p.n_kv = n_kv, p.dim = head_dim, p.window = window;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cache_dtype == LRI_E4M3) return dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, e4m3>(p, st) : launch_plain<__half, e4m3>(p, st);
+  return dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_plain<__half, __half>(p, st);
+}

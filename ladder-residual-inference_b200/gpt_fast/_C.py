@@ -68,6 +68,16 @@ _SIGNATURES = {
                                        c_int, c_int, c_int64, c_int, c_void_p]),
     "lri_attn_prefill": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                                  c_int, c_int, c_int64, c_void_p]),
+    "lri_rope_paged_store": (c_int, [c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_int,  # .. halves
+                                     c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int,  # .. max_pages
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
+                                     c_int64, c_int, c_int, c_int, c_void_p]),
+    "lri_paged_attn_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lri_paged_attn_decode": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
+                                      c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_float,  # .. scale
+                                      c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "lri_paged_load": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
+                               c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "lri_comm_create": (c_int, [c_int, c_int, c_int64, ctypes.POINTER(c_void_p), ctypes.c_char_p]),
     "lri_comm_connect": (c_int, [c_void_p, ctypes.c_char_p]),
     "lri_allreduce": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
@@ -164,7 +174,7 @@ for _name, (_res, _args) in _SIGNATURES.items():
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
-BF16, FP16, FP32 = 0, 1, 2
+BF16, FP16, FP32, E4M3 = 0, 1, 2, 3
 GATE_SIGMOID, GATE_SILU = 0, 1
 GEMM_AUTO, GEMM_TCGEN05, GEMM_SIMT = 0, 1, 2
 
@@ -180,6 +190,11 @@ def dtype_code(dtype: torch.dtype) -> int:
 def dtype_code_any(dtype: torch.dtype) -> int:
     """dtype_code for the entry points that also run in fp32."""
     return FP32 if dtype == torch.float32 else dtype_code(dtype)
+
+
+def cache_code(dtype: torch.dtype) -> int:
+    """dtype_code for the pages of a key-value cache, which may hold 8 bits."""
+    return E4M3 if dtype == torch.float8_e4m3fn else dtype_code(dtype)
 
 
 def check(status: int) -> None:
@@ -200,6 +215,15 @@ def ptr(t):
 def stream_handle() -> int:
     # the stream object of torch.cuda.current_stream() costs a microsecond a launch
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def require_here(*tensors) -> None:
+    """require_cuda, and on the current device: the launch goes to its current stream."""
+    require_cuda(*tensors)
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise RuntimeError(f"tensors must live on the current device (cuda:{here}), not on cuda:{t.get_device()}")
 
 
 def require_cuda(*tensors) -> None:

@@ -9,6 +9,7 @@ from .gpt_ladder_TP import GPTLadder
 from .gpt_migosun_TP import GPTMigosun
 from .gpt_parallel_TP import GPTParallel
 from .gpt_patevik_TP import GPTPatevik
+from .paged import PagedKVCache
 from .tp import maybe_init_dist
 
-__all__ = ["GPTDense", "GPTDesync", "GPTLadder", "GPTMigosun", "GPTParallel", "GPTPatevik", "maybe_init_dist"]
+__all__ = ["GPTDense", "GPTDesync", "GPTLadder", "GPTMigosun", "GPTParallel", "GPTPatevik", "PagedKVCache", "maybe_init_dist"]
