@@ -229,16 +229,17 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  * [n_pages, n_kv, page_size] in fp32 (value = code * scale; not read or written otherwise, NULL then).  Position j of sequence b is row
  * j % page_size of page pages[b * pages_ld + j / page_size]; sequences may share pages.  Numbers outside 0 .. n_pages - 1 name no
  * page.  `dtype` bfloat16 or float16; head_dim a multiple of 8 up to 256; page_size a multiple of 8 up to 4096;
- * n_pages * n_kv and max_pages * page_size below 2^31.  Pages, scales, qkv, tables, q and results are 16-byte aligned.
+ * n_pages * n_kv below 2^31, max_pages * page_size up to 2^30.  Pages, scales, qkv, tables, q and results are 16-byte aligned.
  *
  * lri_rope_paged_store: rows [n_head query | n_kv key | n_kv value heads] of qkv (pitch qkv_ld, a multiple of 8), one for each new token, to
  * rotated queries q_out [tokens, n_head, head_dim] and to rotated keys and values in the pages.  Token i has position input_pos[i] in
  * sequence sequence[i], or in sequence i where `sequence` is NULL.  The first rot_dim elements of a head rotate, in adjacent pairs or (halves
  * != 0) pairs (e, e + rot_dim / 2); rope_table [table_rows, rot_dim / 2, 2] = (cos, sin) in `dtype` or (table_is_f32 != 0) fp32;
  * rot_dim 0: no rotation, no table.  fp32 from the rounded projection, rounded once.  e4m3: a row's scale is its largest magnitude / 448,
- * its codes the nearest to value * (448 / largest magnitude); a row with an infinity or NaN gets a NaN scale.  A token whose position is
+ * its codes the nearest to value * 448 / largest magnitude; a row with an infinity or NaN gets a NaN scale.  A token whose position is
  * negative or behind the table's or the pages' end, or whose sequence or page does not exist, is skipped: nothing is written for it.
- * A (page, row) may be named once in a call.
+ * A (page, row) may be named once in a call.  The calls are described by structs of the host: a step makes many of them, and a binding's
+ * cost grows with the number of arguments.
  *
  * lri_paged_attn_decode: one new token of each sequence (its row is in the cache already); query head h reads KV head
  * h / (n_head / n_kv); q, out [n_seq, n_head, head_dim].  Visible are positions 0 .. input_pos[b], with window > 0 the last `window` of
@@ -249,20 +250,40 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  * lri_paged_load: positions 0 .. last_pos[b] of each sequence into dense caches k_out, v_out [n_seq, n_kv, rows, head_dim] in `dtype`
  * (e4m3: code * scale, rounded once), with zeros in rows without a page and behind them up to a multiple of 64 positions, as far as a tile of
  * lri_attn_prefill reads; later rows are left as they were. */
-int lri_rope_paged_store(int dtype, int cache_dtype, const void* qkv, int64_t qkv_ld, const void* rope_table, int table_is_f32,
-                         int64_t table_rows, int rot_dim, int halves, const void* input_pos, int pos_is_i64, const int32_t* sequence,
-                         const int32_t* pages, int64_t pages_ld, int n_seq, int max_pages, void* q_out, void* k_pages, void* v_pages,
-                         float* k_scale, float* v_scale, int64_t n_pages, int page_size, int64_t tokens, int n_head, int n_kv,
-                         int head_dim, lri_stream_t stream);
+typedef struct {
+  const void *qkv, *rope_table, *input_pos;
+  const int32_t *sequence, *pages;
+  void *q_out, *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  lri_stream_t stream;
+  int64_t qkv_ld, table_rows, pages_ld, n_pages, tokens;
+  int dtype, cache_dtype, table_is_f32, rot_dim, halves, pos_is_i64, n_seq, max_pages, page_size, n_head, n_kv, head_dim;
+} lri_paged_store_call;
+int lri_rope_paged_store(const lri_paged_store_call* call);
+typedef struct {
+  const void *q, *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  const int32_t* pages;
+  const void* input_pos;
+  void *out, *workspace;
+  lri_stream_t stream;
+  int64_t n_pages, pages_ld, window, workspace_bytes;
+  int dtype, cache_dtype, page_size, n_seq, max_pages, pos_is_i64, n_head, n_kv, head_dim;
+  float scale;
+} lri_paged_attn_call;
 size_t lri_paged_attn_decode_workspace_bytes(int n_head, int n_kv, int head_dim);
-int lri_paged_attn_decode(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
-                          const float* v_scale, int64_t n_pages, int page_size, const int32_t* pages, int64_t pages_ld, int n_seq,
-                          int max_pages, const void* input_pos, int pos_is_i64, int64_t window, float scale, void* out, int n_head,
-                          int n_kv, int head_dim, void* workspace, size_t workspace_bytes, lri_stream_t stream);
-int lri_paged_load(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale,
-                   int64_t n_pages, int page_size, const int32_t* pages, int64_t pages_ld, int n_seq, int max_pages,
-                   const void* last_pos, int pos_is_i64, void* k_out, void* v_out, int64_t rows, int n_kv, int head_dim,
-                   lri_stream_t stream);
+int lri_paged_attn_decode(const lri_paged_attn_call* call);
+typedef struct {
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  const int32_t* pages;
+  const void* last_pos;
+  void *k_out, *v_out;
+  lri_stream_t stream;
+  int64_t n_pages, pages_ld, rows;
+  int dtype, cache_dtype, page_size, n_seq, max_pages, pos_is_i64, n_kv, head_dim;
+} lri_paged_load_call;
+int lri_paged_load(const lri_paged_load_call* call);
 
 /* ---- F8: all-reduce over peer memory (one process per GPU) -----------------------------------
  * A communicator owns, on every rank, one inbox buffer that all peers can write.  One-shot

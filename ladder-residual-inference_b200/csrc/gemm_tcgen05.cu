@@ -272,6 +272,22 @@ int make_tmap_f32(CUtensorMap* map, const float* ptr, int64_t rows, int64_t row_
   return LRI_OK;
 }
 
+int make_tmap_pages(CUtensorMap* map, int dtype, const void* ptr, int64_t slabs, int page, int dim, int box_cols, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(LRI_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
+  const int bytes = dtype == LRI_E4M3 ? 1 : 2;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(slabs)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * bytes, static_cast<cuuint64_t>(dim) * bytes * page};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = dtype == LRI_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : dtype == LRI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_cols * bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LRI_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return LRI_OK;
+}
+
 int sm_count() { return device_sm_count(); }
 
 namespace {

@@ -57,10 +57,19 @@ struct PagedAttnParams {
   PageTable table;
   const void* input_pos;  // [n_seq]
   int pos_is_i64;
-  void* out;  // [n_seq, n_head, dim]
+  void* out;  // as q
   int n_head, n_kv, dim;
   int64_t window;  // 0: none
   float scale_log2;
 };
+
+// What the operators ask of the cache and of the pages' table (paged_cache.cu).
+int check_paged(const char* who, int dtype, int cache_dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, const PageTable& t, int n_kv, int dim);
+
+// On the tensor cores (paged_attention_stream.cu).
+bool paged_attn_stream_supports(int cache_dtype, int dim);
+size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim);
+int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t workspace_bytes, cudaStream_t st);
+int paged_attn_status_read_and_clear(int* status_out);
 
 }  // namespace lri

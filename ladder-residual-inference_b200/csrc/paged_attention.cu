@@ -1,9 +1,9 @@
 // Attention of one new token of each sequence over a paged key-value cache: y = softmax(q k^T scale) v over the visible positions.
+// Here the entry point and a plain kernel for heads that the tensor-core kernel (paged_attention_stream.cu) does not take: wider than 128 elements,
+// or of e4m3 rows that are not whole 16-byte pieces.
 #include "paged.cuh"
 
 namespace lri {
-
-int check_paged(const char* who, int dtype, int cache_dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, const PageTable& t, int n_kv, int dim);
 
 namespace {
 
@@ -110,25 +110,31 @@ int launch_plain(const PagedAttnParams& p, cudaStream_t st) {
 
 using namespace lri;
 
-extern "C" size_t lri_paged_attn_decode_workspace_bytes(int n_head, int n_kv, int head_dim) { return 0; }
+extern "C" size_t lri_paged_attn_decode_workspace_bytes(int n_head, int n_kv, int head_dim) {
+  if (n_head <= 0 || n_kv <= 0 || n_head % n_kv != 0 || !paged_attn_stream_supports(LRI_BF16, head_dim)) return 0;
+  return paged_attn_stream_workspace_bytes(n_head, n_kv, head_dim);
+}
 
-extern "C" int lri_paged_attn_decode(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale,
-                                     int64_t n_pages, int page_size, const int32_t* pages, int64_t pages_ld, int n_seq, int max_pages, const void* input_pos,
-                                     int pos_is_i64, int64_t window, float scale, void* out, int n_head, int n_kv, int head_dim, void* workspace,
-                                     size_t workspace_bytes, lri_stream_t stream) {
+extern "C" int lri_paged_attn_decode(const lri_paged_attn_call* call) {
+  LRI_REQUIRE(call, LRI_ERR_ARG, "paged_attn_decode: NULL call");
+  const lri_paged_attn_call& c = *call;
   PagedAttnParams p{};
-  p.table = PageTable{pages, pages_ld, n_seq, max_pages, page_size, n_pages};
-  int rc = check_paged("paged_attn_decode", dtype, cache_dtype, k_pages, v_pages, k_scale, v_scale, p.table, n_kv, head_dim);
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  int rc = check_paged("paged_attn_decode", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
-  LRI_REQUIRE(n_head >= 1 && n_head <= 65535 && n_head % n_kv == 0, LRI_ERR_ARG, "paged_attn_decode: n_head=%d n_kv=%d", n_head, n_kv);
-  LRI_REQUIRE(window >= 0, LRI_ERR_ARG, "paged_attn_decode: window=%lld", (long long)window);
-  if (n_seq == 0) return LRI_OK;
-  LRI_REQUIRE(q && input_pos && out, LRI_ERR_ARG, "paged_attn_decode: NULL pointer");
-  LRI_REQUIRE(aligned16(q) && aligned16(out), LRI_ERR_ALIGN, "paged_attn_decode: pointers must be 16-byte aligned");
-  p.q = q, p.k = k_pages, p.v = v_pages, p.k_scale = cache_dtype == LRI_E4M3 ? k_scale : nullptr, p.v_scale = cache_dtype == LRI_E4M3 ? v_scale : nullptr;
-  p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64, p.out = out, p.n_head = n_head, p.n_kv = n_kv, p.dim = head_dim, p.window = window;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache_dtype == LRI_E4M3) return dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, e4m3>(p, st) : launch_plain<__half, e4m3>(p, st);
-  return dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_plain<__half, __half>(p, st);
+  LRI_REQUIRE(c.n_head >= 1 && c.n_head <= 65535 && c.n_head % c.n_kv == 0, LRI_ERR_ARG, "paged_attn_decode: n_head=%d n_kv=%d", c.n_head, c.n_kv);
+  LRI_REQUIRE(c.window >= 0, LRI_ERR_ARG, "paged_attn_decode: window=%lld", (long long)c.window);
+  if (c.n_seq == 0) return LRI_OK;
+  LRI_REQUIRE(c.q && c.input_pos && c.out && c.pages, LRI_ERR_ARG, "paged_attn_decode: NULL pointer");
+  LRI_REQUIRE(aligned16(c.q) && aligned16(c.out), LRI_ERR_ALIGN, "paged_attn_decode: pointers must be 16-byte aligned");
+  const bool eight = c.cache_dtype == LRI_E4M3;
+  p.q = c.q, p.k = c.k_pages, p.v = c.v_pages, p.k_scale = eight ? c.k_scale : nullptr, p.v_scale = eight ? c.v_scale : nullptr;
+  p.input_pos = c.input_pos, p.pos_is_i64 = c.pos_is_i64, p.out = c.out, p.n_head = c.n_head, p.n_kv = c.n_kv, p.dim = c.head_dim, p.window = c.window;
+  p.scale_log2 = c.scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  // option attn_mma: 0 keeps attention off the tensor cores, as in lri_attn_decode
+  if (option(OPT_ATTN_MMA) != 0 && paged_attn_stream_supports(c.cache_dtype, c.head_dim))
+    return paged_attn_stream_launch(c.dtype, c.cache_dtype, p, c.workspace, static_cast<size_t>(c.workspace_bytes), st);
+  if (eight) return c.dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, e4m3>(p, st) : launch_plain<__half, e4m3>(p, st);
+  return c.dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_plain<__half, __half>(p, st);
 }

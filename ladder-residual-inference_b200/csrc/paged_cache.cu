@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(kThreads) rope_paged_store_kernel(const StoreP
   if constexpr (!E4M3) {
     if (live) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + row * p.dim + e, x);
   } else {
-    // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded once, from the rotated value in
-    // 32 bits.  A row with an infinity or a NaN has no scale: it reads back as NaN.
+    // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
+    // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
+    // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
     float top = 0.f;
     bool finite = true;
 #pragma unroll
@@ -107,12 +108,17 @@ __global__ void __launch_bounds__(kThreads) rope_paged_store_kernel(const StoreP
     if (!live || head < p.n_head) return;
     const bool whole = top < INFINITY;
     top = fmaxf(top, kSmallest);
-    const float inv = kLargest / top;
+    // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
+    const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
+    auto scaled = [&](float v) {
+      const float n = v * up, y = n * inv;
+      return fminf(fmaxf(fmaf(fmaf(-y, den, n), inv, y), -kLargest), kLargest);
+    };
     uint32_t w[2] = {0u, 0u};
     if (whole)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 y = make_float2(fminf(fmaxf(x[2 * i] * inv, -kLargest), kLargest), fminf(fmaxf(x[2 * i + 1] * inv, -kLargest), kLargest));
+        const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
         w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
       }
     *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + row * p.dim + e) = make_uint2(w[0], w[1]);
@@ -197,8 +203,8 @@ int check_paged(const char* who, int dtype, int cache_dtype, const void* k, cons
   LRI_REQUIRE(t.page >= 8 && t.page <= 4096 && t.page % 8 == 0, LRI_ERR_UNSUPPORTED, "%s: page_size=%d (multiples of 8 up to 4096)", who, t.page);
   LRI_REQUIRE(t.n_seq >= 0 && t.max_pages >= 1 && t.ld >= t.max_pages, LRI_ERR_ARG, "%s: table of %d x %d pages, row pitch %lld", who, t.n_seq, t.max_pages, (long long)t.ld);
   LRI_REQUIRE(t.n_pages >= 1 && t.n_pages * n_kv < (1ll << 31), LRI_ERR_UNSUPPORTED, "%s: %lld pages of %d heads (below 2^31 together)", who, (long long)t.n_pages, n_kv);
-  LRI_REQUIRE(t.capacity() < (1ll << 31), LRI_ERR_UNSUPPORTED, "%s: tables of %d pages of %d positions (below 2^31 together)", who, t.max_pages, t.page);
-  LRI_REQUIRE(k && v && t.ids, LRI_ERR_ARG, "%s: NULL pointer", who);
+  LRI_REQUIRE(t.capacity() <= (1ll << 30), LRI_ERR_UNSUPPORTED, "%s: tables of %d pages of %d positions (up to 2^30 together)", who, t.max_pages, t.page);
+  LRI_REQUIRE(k && v, LRI_ERR_ARG, "%s: NULL pointer", who);
   LRI_REQUIRE(aligned16(k) && aligned16(v), LRI_ERR_ALIGN, "%s: pages must be 16-byte aligned", who);
   if (cache_dtype == LRI_E4M3) {
     LRI_REQUIRE(k_scale && v_scale, LRI_ERR_ARG, "%s: e4m3 pages need scales", who);
@@ -211,50 +217,51 @@ int check_paged(const char* who, int dtype, int cache_dtype, const void* k, cons
 
 using namespace lri;
 
-extern "C" int lri_rope_paged_store(int dtype, int cache_dtype, const void* qkv, int64_t qkv_ld, const void* rope_table, int table_is_f32, int64_t table_rows,
-                                    int rot_dim, int halves, const void* input_pos, int pos_is_i64, const int32_t* sequence, const int32_t* pages,
-                                    int64_t pages_ld, int n_seq, int max_pages, void* q_out, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
-                                    int64_t n_pages, int page_size, int64_t tokens, int n_head, int n_kv, int head_dim, lri_stream_t stream) {
+extern "C" int lri_rope_paged_store(const lri_paged_store_call* call) {
+  LRI_REQUIRE(call, LRI_ERR_ARG, "rope_paged_store: NULL call");
+  const lri_paged_store_call& c = *call;
   StoreParams p{};
-  p.table = PageTable{pages, pages_ld, n_seq, max_pages, page_size, n_pages};
-  int rc = check_paged("rope_paged_store", dtype, cache_dtype, k_pages, v_pages, k_scale, v_scale, p.table, n_kv, head_dim);
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  int rc = check_paged("rope_paged_store", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
-  LRI_REQUIRE(tokens >= 0 && n_head >= 1 && n_head <= 65535, LRI_ERR_ARG, "rope_paged_store: tokens=%lld n_head=%d", (long long)tokens, n_head);
-  LRI_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, LRI_ERR_ARG, "rope_paged_store: rot_dim=%d of head_dim=%d", rot_dim, head_dim);
-  LRI_REQUIRE(rot_dim == 0 || (rope_table && table_rows >= 1), LRI_ERR_ARG, "rope_paged_store: a rotation needs its table");
-  LRI_REQUIRE(sequence || tokens <= n_seq, LRI_ERR_ARG, "rope_paged_store: %lld tokens without sequence numbers for %d sequences", (long long)tokens, n_seq);
-  LRI_REQUIRE(qkv_ld >= static_cast<int64_t>(n_head + 2 * n_kv) * head_dim && qkv_ld % 8 == 0, LRI_ERR_ARG, "rope_paged_store: row pitch %lld", (long long)qkv_ld);
-  if (tokens == 0) return LRI_OK;
-  LRI_REQUIRE(qkv && input_pos && q_out, LRI_ERR_ARG, "rope_paged_store: NULL pointer");
-  LRI_REQUIRE(aligned16(qkv) && aligned16(rope_table) && aligned16(q_out), LRI_ERR_ALIGN, "rope_paged_store: pointers must be 16-byte aligned");
-  p.qkv = qkv, p.ld = qkv_ld, p.rope = rope_table, p.table_rows = table_rows, p.rot = rot_dim, p.halves = halves, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64;
-  p.sequence = sequence, p.q_out = q_out, p.k = k_pages, p.v = v_pages, p.k_scale = k_scale, p.v_scale = v_scale;
-  p.tokens = tokens, p.n_head = n_head, p.n_kv = n_kv, p.dim = head_dim;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool eight = cache_dtype == LRI_E4M3;
-  return dtype == LRI_BF16 ? dispatch_store<__nv_bfloat16>(p, table_is_f32 != 0, eight, st) : dispatch_store<__half>(p, table_is_f32 != 0, eight, st);
+  LRI_REQUIRE(c.tokens >= 0 && c.n_head >= 1 && c.n_head <= 65535, LRI_ERR_ARG, "rope_paged_store: tokens=%lld n_head=%d", (long long)c.tokens, c.n_head);
+  LRI_REQUIRE(c.rot_dim >= 0 && c.rot_dim <= c.head_dim && c.rot_dim % 2 == 0, LRI_ERR_ARG, "rope_paged_store: rot_dim=%d of head_dim=%d", c.rot_dim, c.head_dim);
+  LRI_REQUIRE(c.rot_dim == 0 || (c.rope_table && c.table_rows >= 1), LRI_ERR_ARG, "rope_paged_store: a rotation needs its table");
+  LRI_REQUIRE(c.sequence || c.tokens <= c.n_seq, LRI_ERR_ARG, "rope_paged_store: %lld tokens without sequence numbers for %d sequences", (long long)c.tokens, c.n_seq);
+  LRI_REQUIRE(c.qkv_ld >= static_cast<int64_t>(c.n_head + 2 * c.n_kv) * c.head_dim && c.qkv_ld % 8 == 0, LRI_ERR_ARG, "rope_paged_store: row pitch %lld", (long long)c.qkv_ld);
+  if (c.tokens == 0) return LRI_OK;
+  LRI_REQUIRE(c.qkv && c.input_pos && c.q_out && (c.pages || c.n_seq == 0), LRI_ERR_ARG, "rope_paged_store: NULL pointer");
+  LRI_REQUIRE(aligned16(c.qkv) && aligned16(c.rope_table) && aligned16(c.q_out), LRI_ERR_ALIGN, "rope_paged_store: pointers must be 16-byte aligned");
+  p.qkv = c.qkv, p.ld = c.qkv_ld, p.rope = c.rope_table, p.table_rows = c.table_rows, p.rot = c.rot_dim, p.halves = c.halves;
+  p.input_pos = c.input_pos, p.pos_is_i64 = c.pos_is_i64, p.sequence = c.sequence, p.q_out = c.q_out;
+  p.k = c.k_pages, p.v = c.v_pages, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
+  p.tokens = c.tokens, p.n_head = c.n_head, p.n_kv = c.n_kv, p.dim = c.head_dim;
+  cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  const bool eight = c.cache_dtype == LRI_E4M3, f32 = c.table_is_f32 != 0;
+  return c.dtype == LRI_BF16 ? dispatch_store<__nv_bfloat16>(p, f32, eight, st) : dispatch_store<__half>(p, f32, eight, st);
 }
 
-extern "C" int lri_paged_load(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int64_t n_pages,
-                              int page_size, const int32_t* pages, int64_t pages_ld, int n_seq, int max_pages, const void* last_pos, int pos_is_i64, void* k_out,
-                              void* v_out, int64_t rows, int n_kv, int head_dim, lri_stream_t stream) {
+extern "C" int lri_paged_load(const lri_paged_load_call* call) {
+  LRI_REQUIRE(call, LRI_ERR_ARG, "paged_load: NULL call");
+  const lri_paged_load_call& c = *call;
   LoadParams p{};
-  p.table = PageTable{pages, pages_ld, n_seq, max_pages, page_size, n_pages};
-  int rc = check_paged("paged_load", dtype, cache_dtype, k_pages, v_pages, k_scale, v_scale, p.table, n_kv, head_dim);
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  int rc = check_paged("paged_load", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
-  LRI_REQUIRE(rows >= 0 && rows < (1ll << 31) && n_seq <= 65535, LRI_ERR_ARG, "paged_load: rows=%lld n_seq=%d", (long long)rows, n_seq);
-  if (rows == 0 || n_seq == 0) return LRI_OK;
-  LRI_REQUIRE(last_pos && k_out && v_out, LRI_ERR_ARG, "paged_load: NULL pointer");
-  LRI_REQUIRE(aligned16(k_out) && aligned16(v_out), LRI_ERR_ALIGN, "paged_load: pointers must be 16-byte aligned");
-  p.k = k_pages, p.v = v_pages, p.k_scale = cache_dtype == LRI_E4M3 ? k_scale : nullptr, p.v_scale = cache_dtype == LRI_E4M3 ? v_scale : nullptr;
-  p.last_pos = last_pos, p.pos_is_i64 = pos_is_i64, p.k_out = k_out, p.v_out = v_out, p.rows = rows, p.n_kv = n_kv, p.dim = head_dim;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>((rows + kFillRows - 1) / kFillRows), static_cast<unsigned>(n_kv), static_cast<unsigned>(n_seq));
+  LRI_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) && c.n_seq <= 65535, LRI_ERR_ARG, "paged_load: rows=%lld n_seq=%d", (long long)c.rows, c.n_seq);
+  if (c.rows == 0 || c.n_seq == 0) return LRI_OK;
+  LRI_REQUIRE(c.pages && c.last_pos && c.k_out && c.v_out, LRI_ERR_ARG, "paged_load: NULL pointer");
+  LRI_REQUIRE(aligned16(c.k_out) && aligned16(c.v_out), LRI_ERR_ALIGN, "paged_load: pointers must be 16-byte aligned");
+  const bool eight = c.cache_dtype == LRI_E4M3;
+  p.k = c.k_pages, p.v = c.v_pages, p.k_scale = eight ? c.k_scale : nullptr, p.v_scale = eight ? c.v_scale : nullptr;
+  p.last_pos = c.last_pos, p.pos_is_i64 = c.pos_is_i64, p.k_out = c.k_out, p.v_out = c.v_out, p.rows = c.rows, p.n_kv = c.n_kv, p.dim = c.head_dim;
+  cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  const dim3 grid(static_cast<unsigned>((c.rows + kFillRows - 1) / kFillRows), static_cast<unsigned>(c.n_kv), static_cast<unsigned>(c.n_seq));
   auto go = [&](auto kern) {
     LRI_CUDA(launch_pdl(kern, grid, dim3(kThreads), 0, st, p));
     LRI_LAUNCH_CHECK("paged_load_kernel");
     return static_cast<int>(LRI_OK);
   };
-  if (cache_dtype == LRI_E4M3) return dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, e4m3>) : go(paged_load_kernel<__half, e4m3>);
-  return dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, __nv_bfloat16>) : go(paged_load_kernel<__half, __half>);
+  if (eight) return c.dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, e4m3>) : go(paged_load_kernel<__half, e4m3>);
+  return c.dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, __nv_bfloat16>) : go(paged_load_kernel<__half, __half>);
 }

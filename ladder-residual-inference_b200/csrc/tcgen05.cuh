@@ -189,6 +189,9 @@ int make_tmap_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, 
 // box_rows rows, not swizzled; elements past `width` read as zero
 int make_tmap_f32(CUtensorMap* map, const float* ptr, int64_t rows, int64_t row_pitch, int64_t heads, int64_t head_pitch, int64_t width,
                   int box_width, int box_rows);
+// 3-D view [slabs, page, dim] of the pages of a key-value cache (a slab is one head's part of a page), box = box_cols elements x box_rows
+// rows of one slab, swizzled over the 128 or 64 bytes of a row of the box; elements past `dim` read as zero
+int make_tmap_pages(CUtensorMap* map, int dtype, const void* ptr, int64_t slabs, int page, int dim, int box_cols, int box_rows);
 int sm_count();
 
 }  // namespace lri

@@ -6,6 +6,7 @@ fallback: if the shared library is missing the import fails with the command tha
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -30,6 +31,11 @@ class LlamaPass(ctypes.Structure):
                 + [(k, c_size_t) for k in ("ws_qkv_bytes", "ws_wo_bytes", "ws_ug_bytes", "ws_w2_bytes", "scratch_bytes")]
                 + [(k, c_void_p) for k in ("stream", "side", "events")])
 
+
+# Calls that are described by a struct, packed (a step makes many of them, and ctypes takes 0.1 us an argument); NULL pointers are 0.
+STORE_CALL = struct.Struct("@11Q5q12i")  # lri_paged_store_call
+ATTN_CALL = struct.Struct("@10Q4q9if")   # lri_paged_attn_call
+LOAD_CALL = struct.Struct("@9Q3q8i")     # lri_paged_load_call
 
 ONE_SM = 0x100  # LRI_ONE_SM
 DENSE, LADDER, LADDER_TWO_STREAMS, PARALLEL, DESYNC, PARALLEL_TWO_STREAMS = range(6)
@@ -68,16 +74,10 @@ _SIGNATURES = {
                                        c_int, c_int, c_int64, c_int, c_void_p]),
     "lri_attn_prefill": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                                  c_int, c_int, c_int64, c_void_p]),
-    "lri_rope_paged_store": (c_int, [c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_int,  # .. halves
-                                     c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int,  # .. max_pages
-                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
-                                     c_int64, c_int, c_int, c_int, c_void_p]),
+    "lri_rope_paged_store": (c_int, [c_void_p]),
     "lri_paged_attn_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
-    "lri_paged_attn_decode": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
-                                      c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_float,  # .. scale
-                                      c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
-    "lri_paged_load": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,  # .. page_size
-                               c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "lri_paged_attn_decode": (c_int, [c_void_p]),
+    "lri_paged_load": (c_int, [c_void_p]),
     "lri_comm_create": (c_int, [c_int, c_int, c_int64, ctypes.POINTER(c_void_p), ctypes.c_char_p]),
     "lri_comm_connect": (c_int, [c_void_p, ctypes.c_char_p]),
     "lri_allreduce": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
@@ -212,18 +212,28 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def address(t) -> int:
+    """ptr for a packed struct."""
+    return 0 if t is None else t.data_ptr()
+
+
 def stream_handle() -> int:
     # the stream object of torch.cuda.current_stream() costs a microsecond a launch
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def require_here(*tensors) -> None:
-    """require_cuda, and on the current device: the launch goes to its current stream."""
-    require_cuda(*tensors)
-    here = torch._C._cuda_getDevice()
+    """require_cuda, and all of them on the current device: the launch goes to its current stream."""
+    at = -1
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise RuntimeError(f"tensors must live on the current device (cuda:{here}), not on cuda:{t.get_device()}")
+        if t is None:
+            continue
+        device = t.get_device()
+        if device != at or device < 0:
+            require_cuda(t)
+            if at >= 0 or device != torch._C._cuda_getDevice():
+                raise RuntimeError(f"tensors must live on the current device (cuda:{torch._C._cuda_getDevice()}), not on cuda:{device}")
+            at = device
 
 
 def require_cuda(*tensors) -> None:

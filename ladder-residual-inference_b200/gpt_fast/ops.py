@@ -129,13 +129,16 @@ class CudaOps:
         """table None: no rotation; its second extent is half of the elements that rotate."""
         _C.require_here(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale)
         n_pages, n_kv, page, dim = k_pages.shape
-        rows, rot = (table.shape[0], 2 * table.shape[1]) if table is not None else (0, 0)
-        _C.check(_C.lib.lri_rope_paged_store(
-            _C.dtype_code(qkv.dtype), _C.cache_code(k_pages.dtype), qkv.data_ptr(), qkv.stride(0), _C.ptr(table),
-            int(table is not None and table.dtype == torch.float32), rows, rot, int(halves), input_pos.data_ptr(),
-            int(input_pos.dtype == torch.int64), _C.ptr(sequence), pages.data_ptr(), pages.stride(0), pages.shape[0], pages.shape[1],
-            q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _C.ptr(k_scale), _C.ptr(v_scale), n_pages, page, qkv.shape[0], n_head,
-            n_kv, dim, _C.stream_handle()))
+        n_seq, most = pages.shape
+        rows = rot = f32 = 0
+        if table is not None:
+            rows, half, _ = table.shape
+            rot, f32 = 2 * half, table.dtype == torch.float32
+        _C.check(_C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
+            qkv.data_ptr(), _C.address(table), input_pos.data_ptr(), _C.address(sequence), pages.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), _C.stream_handle(), qkv.stride(0), rows, pages.stride(0), n_pages,
+            qkv.shape[0], _C.dtype_code(qkv.dtype), _C.cache_code(k_pages.dtype), f32, rot, halves, input_pos.dtype == torch.int64, n_seq,
+            most, page, n_head, n_kv, dim)))
 
     @staticmethod
     def paged_attn_workspace_bytes(n_head, n_kv, head_dim):
@@ -145,20 +148,21 @@ class CudaOps:
     def paged_attention(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, window, scale, out, n_head, workspace):
         _C.require_here(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, out, workspace)
         n_pages, n_kv, page, dim = k_pages.shape
-        ws_ptr, ws_bytes = (workspace.data_ptr(), workspace.numel()) if workspace is not None else (None, 0)
-        _C.check(_C.lib.lri_paged_attn_decode(
-            _C.dtype_code(q.dtype), _C.cache_code(k_pages.dtype), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _C.ptr(k_scale),
-            _C.ptr(v_scale), n_pages, page, pages.data_ptr(), pages.stride(0), pages.shape[0], pages.shape[1], input_pos.data_ptr(),
-            int(input_pos.dtype == torch.int64), window, scale, out.data_ptr(), n_head, n_kv, dim, ws_ptr, ws_bytes, _C.stream_handle()))
+        n_seq, most = pages.shape
+        _C.check(_C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), pages.data_ptr(), input_pos.data_ptr(),
+            out.data_ptr(), workspace.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), window, workspace.numel(), _C.dtype_code(q.dtype),
+            _C.cache_code(k_pages.dtype), page, n_seq, most, input_pos.dtype == torch.int64, n_head, n_kv, dim, scale)))
 
     @staticmethod
     def paged_load(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out):
         _C.require_here(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out)
         n_pages, n_kv, page, dim = k_pages.shape
-        _C.check(_C.lib.lri_paged_load(
-            _C.dtype_code(k_out.dtype), _C.cache_code(k_pages.dtype), k_pages.data_ptr(), v_pages.data_ptr(), _C.ptr(k_scale),
-            _C.ptr(v_scale), n_pages, page, pages.data_ptr(), pages.stride(0), pages.shape[0], pages.shape[1], last_pos.data_ptr(),
-            int(last_pos.dtype == torch.int64), k_out.data_ptr(), v_out.data_ptr(), k_out.shape[2], n_kv, dim, _C.stream_handle()))
+        n_seq, most = pages.shape
+        _C.check(_C.lib.lri_paged_load(_C.LOAD_CALL.pack(
+            k_pages.data_ptr(), v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), pages.data_ptr(), last_pos.data_ptr(),
+            k_out.data_ptr(), v_out.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), k_out.shape[2], _C.dtype_code(k_out.dtype),
+            _C.cache_code(k_pages.dtype), page, n_seq, most, last_pos.dtype == torch.int64, n_kv, dim)))
 
     # ---- all layers of a pass ------------------------------------------------------------------------
     @staticmethod

@@ -59,7 +59,8 @@ def test_store_refuses(kw):
     dict(q=torch.zeros(3, 4, 32, dtype=torch.bfloat16)), dict(q=torch.zeros(3, 3, 64, dtype=torch.bfloat16)), dict(q=torch.zeros(3, 4, 64)),
     dict(q=torch.zeros(4, 3, 64, dtype=torch.bfloat16).transpose(0, 1)), dict(q=torch.zeros(3, 0, 64, dtype=torch.bfloat16)), dict(window=-1),
     dict(pages=torch.zeros(4, 2, dtype=torch.int32)), dict(input_pos=torch.zeros(4, dtype=torch.int32)), dict(input_pos=torch.zeros(3, dtype=torch.int16)),
-    dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(3, 64, 4, dtype=torch.bfloat16).transpose(1, 2))])
+    dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(3, 64, 4, dtype=torch.bfloat16).transpose(1, 2)),
+    dict(workspace=torch.zeros(16)), dict(window=1 << 62)])
 def test_attend_refuses(kw):
     a = dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), input_pos=torch.zeros(3, dtype=torch.int32), pages=torch.zeros(3, 2, dtype=torch.int32),
              workspace=torch.zeros(16, dtype=torch.uint8))
@@ -107,55 +108,66 @@ ARG, ALIGN, UNSUPPORTED = -1, -2, -3
 
 def _c_store(**kw):
     from gpt_fast import _C
-    a = dict(dtype=0, cache=0, qkv=BUF, ld=512, rope=BUF, f32=0, rows=50, rot=64, halves=0, pos=BUF, i64=0, seq=None, pages=BUF, pages_ld=2, n_seq=3, most=2, q=BUF, k=BUF,
-             v=BUF, ks=None, vs=None, n_pages=6, page=16, tokens=3, n_head=4, n_kv=2, dim=64, stream=None)
+    a = dict(qkv=BUF, rope=BUF, pos=BUF, seq=0, pages=BUF, q=BUF, k=BUF, v=BUF, ks=0, vs=0, stream=0, ld=512, rows=50, pages_ld=2, n_pages=6, tokens=3, dtype=0,
+             cache=0, f32=0, rot=64, halves=0, i64=0, n_seq=3, most=2, page=16, n_head=4, n_kv=2, dim=64)
     assert set(kw) <= set(a)
     a.update(kw)
-    return _C.lib.lri_rope_paged_store(*a.values())
+    return _C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(*a.values()))
 
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=2), UNSUPPORTED), (dict(cache=1), UNSUPPORTED), (dict(cache=3), ARG), (dict(cache=3, ks=BUF, vs=BUF + 4), ALIGN), (dict(dim=68), UNSUPPORTED),
     (dict(dim=264), UNSUPPORTED), (dict(page=20), UNSUPPORTED), (dict(page=4104), UNSUPPORTED), (dict(n_kv=0), ARG), (dict(n_head=0), ARG), (dict(n_pages=0), UNSUPPORTED),
     (dict(n_pages=1 << 30), UNSUPPORTED), (dict(most=0), ARG), (dict(most=1 << 28, pages_ld=1 << 28), UNSUPPORTED), (dict(pages_ld=1), ARG), (dict(rot=66), ARG),
-    (dict(rot=3), ARG), (dict(rot=-2), ARG), (dict(rope=None), ARG), (dict(rows=0), ARG), (dict(tokens=4), ARG), (dict(tokens=-1), ARG), (dict(ld=504), ARG),
-    (dict(ld=513), ARG), (dict(qkv=None), ARG), (dict(pos=None), ARG), (dict(q=None), ARG), (dict(k=None), ARG), (dict(v=None), ARG), (dict(pages=None), ARG),
-    (dict(qkv=BUF + 8), ALIGN), (dict(q=BUF + 8), ALIGN), (dict(k=BUF + 8), ALIGN), (dict(rope=BUF + 8), ALIGN), (dict(tokens=0, qkv=None), 0)])
+    (dict(rot=3), ARG), (dict(rot=-2), ARG), (dict(rope=0), ARG), (dict(rows=0), ARG), (dict(tokens=4), ARG), (dict(tokens=-1), ARG), (dict(ld=504), ARG),
+    (dict(ld=513), ARG), (dict(qkv=0), ARG), (dict(pos=0), ARG), (dict(q=0), ARG), (dict(k=0), ARG), (dict(v=0), ARG), (dict(pages=0), ARG),
+    (dict(qkv=BUF + 8), ALIGN), (dict(q=BUF + 8), ALIGN), (dict(k=BUF + 8), ALIGN), (dict(rope=BUF + 8), ALIGN), (dict(tokens=0, qkv=0), 0)])
 def test_c_store_refuses(kw, status):
     assert _c_store(**kw) == status
 
 
 def _c_attend(**kw):
     from gpt_fast import _C
-    a = dict(dtype=0, cache=0, q=BUF, k=BUF, v=BUF, ks=None, vs=None, n_pages=6, page=16, pages=BUF, pages_ld=2, n_seq=3, most=2, pos=BUF, i64=0, window=0, scale=1.0, out=BUF,
-             n_head=4, n_kv=2, dim=64, ws=BUF, ws_bytes=1 << 30, stream=None)
+    a = dict(q=BUF, k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, out=BUF, ws=BUF, stream=0, n_pages=6, pages_ld=2, window=0, ws_bytes=1 << 30, dtype=0, cache=0, page=16,
+             n_seq=3, most=2, i64=0, n_head=4, n_kv=2, dim=64, scale=1.0)
     assert set(kw) <= set(a)
     a.update(kw)
-    return _C.lib.lri_paged_attn_decode(*a.values())
+    return _C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(*a.values()))
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(n_head=3), ARG), (dict(n_head=0), ARG), (dict(window=-1), ARG), (dict(n_seq=-1), ARG), (dict(q=None), ARG), (dict(out=None), ARG), (dict(pos=None), ARG),
+    (dict(n_head=3), ARG), (dict(n_head=0), ARG), (dict(window=-1), ARG), (dict(n_seq=-1), ARG), (dict(q=0), ARG), (dict(out=0), ARG), (dict(pos=0), ARG),
     (dict(q=BUF + 8), ALIGN), (dict(out=BUF + 2), ALIGN), (dict(dtype=3), UNSUPPORTED), (dict(cache=2), UNSUPPORTED), (dict(cache=3, ks=BUF), ARG),
-    (dict(n_seq=0, q=None, out=None), 0)])
+    (dict(n_seq=0, q=0, out=0), 0)])
 def test_c_attend_refuses(kw, status):
     assert _c_attend(**kw) == status
 
 
 def _c_load(**kw):
     from gpt_fast import _C
-    a = dict(dtype=0, cache=0, k=BUF, v=BUF, ks=None, vs=None, n_pages=6, page=16, pages=BUF, pages_ld=2, n_seq=3, most=2, pos=BUF, i64=0, k_out=BUF, v_out=BUF, rows=32, n_kv=2,
-             dim=64, stream=None)
+    a = dict(k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, k_out=BUF, v_out=BUF, stream=0, n_pages=6, pages_ld=2, rows=32, dtype=0, cache=0, page=16, n_seq=3, most=2, i64=0,
+             n_kv=2, dim=64)
     assert set(kw) <= set(a)
     a.update(kw)
-    return _C.lib.lri_paged_load(*a.values())
+    return _C.lib.lri_paged_load(_C.LOAD_CALL.pack(*a.values()))
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(rows=-1), ARG), (dict(rows=1 << 31), ARG), (dict(n_seq=65536), ARG), (dict(pos=None), ARG), (dict(k_out=None), ARG), (dict(v_out=BUF + 8), ALIGN),
-    (dict(n_kv=65536), ARG), (dict(rows=0, k_out=None), 0), (dict(n_seq=0, pos=None), 0)])
+    (dict(rows=-1), ARG), (dict(rows=1 << 31), ARG), (dict(n_seq=65536), ARG), (dict(pos=0), ARG), (dict(k_out=0), ARG), (dict(v_out=BUF + 8), ALIGN),
+    (dict(n_kv=65536), ARG), (dict(rows=0, k_out=0), 0), (dict(n_seq=0, pos=0), 0)])
 def test_c_load_refuses(kw, status):
     assert _c_load(**kw) == status
+
+
+def test_no_call():
+    from gpt_fast import _C
+    for f in (_C.lib.lri_rope_paged_store, _C.lib.lri_paged_attn_decode, _C.lib.lri_paged_load):
+        assert f(None) == ARG
+
+
+def test_nothing_to_do():
+    """No sequences and no tokens: no launch, whatever the pointers."""
+    assert _c_attend(n_seq=0, pages=0, pos=0) == _c_load(n_seq=0, pages=0, k_out=0) == _c_store(tokens=0, n_seq=0, pages=0) == 0
 
 
 def test_device_messages_name_the_call():
