@@ -1,15 +1,19 @@
-// Paged decode attention as a stream of cache rows, with the query heads of a KV head as the rows of tensor-core tiles.
+// Paged decode attention as a stream of cache rows on the tensor cores.
 //
 // The work is cut into units of 32 or 64 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head; every CTA adds up
 // the sequences' units and takes an equal contiguous run of all of them, so that sequences of any lengths keep all SMs busy from the
-// first microsecond to the last.  One warp fetches (TMA, boxes that lie within a page, a 64 KB ring of K and V tiles), four warps
-// compute: S = Q K^T and O += P V as m16n8k16 products, online softmax per warp in 32 bits.  A pair that lies in one CTA's run is finished
-// there; the parts of one that several CTAs share go through the workspace and the last of these CTAs joins them in their order, whoever it is,
-// so that results are the same bits every time.
+// first microsecond to the last.  One warp fetches (TMA, boxes that lie within a page, a ring of K and V tiles), four warps compute, two to a
+// unit.  A pair that lies in one CTA's run is finished there; the parts of one that several CTAs share go through the workspace and the last of
+// these CTAs to arrive joins them in their order, so that results are the same bits every time.
+//
+// Products are m16n8k16 with positions, then elements of a value, as the 16 rows and the query heads that share a KV head as the 8 columns (two
+// blocks of columns for 9 to 16 heads): S^T = K Q^T, O^T += V^T P^T; P^T goes from the first product's layout to the second's by a matrix transpose
+// in registers.  Softmax in 32 bits, a running reference per head and warp that only moves when a score exceeds it by 2^4: mostly a tile needs
+// no exchange between lanes at all.
 //
 // e4m3 pages: codes become halves (exactly) on their way into the products.  Queries enter as halves too, each head's row multiplied by the power
 // of two that brings its largest element to 2^14 .. 2^15, which keeps bfloat16's digits.  The keys' scales multiply the scores; the values'
-// scales multiply the probabilities, against the largest scale so far, so that probabilities in halves neither overflow nor vanish.
+// scales multiply the probabilities, against a running reference, so that probabilities in halves neither overflow nor vanish.
 //
 // Rows that are not visible (behind the position, before the window, without a page) may hold anything: their scores are masked and
 // their values replaced by zeros.
@@ -27,12 +31,12 @@ __device__ int g_paged_attn_status = 0;
 
 constexpr int kWarps = 4;                    // that compute
 constexpr int kThreads = (kWarps + 1) * 32;  // and one that fetches
-constexpr int kTile = 16;                    // positions of a warp's products
-constexpr int kRingBytes = 64 * 1024;
+constexpr int kPairWarps = 2;                // warps that share a unit, a team
+constexpr int kTeams = kWarps / kPairWarps;
 constexpr int kMaxGroup = 16;    // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;   // of a launch
 constexpr int kMinRun = 2;       // units: a CTA without as many is not worth its part in the join
-constexpr int kPerSm = 2;
+constexpr int kMaxPerSm = 3;
 constexpr size_t kCounterBytes = 4096;
 
 struct StreamParams {
@@ -44,17 +48,22 @@ struct StreamParams {
   float* part_o;                      // [CTAs][2][tile_heads][HD]
 };
 
-template <typename C, int HD>
+// NT: blocks of eight query heads
+template <typename C, int HD, int NT>
 struct Shape {
   static constexpr int kRow = HD * static_cast<int>(sizeof(C));
   static constexpr int kChunkRow = kRow < 128 ? kRow : 128;  // bytes of a row that a box holds: the swizzle's span
   static constexpr int kChunks = kRow / kChunkRow;
   static constexpr int kUnit = kRow > 128 ? 32 : 64;
-  static constexpr int kTeams = kWarps * kTile / kUnit;  // warps that share a unit form a team
+  static constexpr int kTile = kUnit / kPairWarps;  // positions of a warp's products
   static constexpr uint32_t kChunkBytes = kUnit * kChunkRow;
   static constexpr uint32_t kHalf = kChunks * kChunkBytes;
+  static constexpr int kPerSm = NT == 1 ? 3 : 2;
+  static constexpr int kRingBytes = NT == 1 ? 48 * 1024 : 64 * 1024;
   static constexpr uint32_t kStages = kRingBytes / kHalf;  // a tile of K or of V each
-  static_assert(kStages % (2 * kTeams) == 0, "a team's tiles lie in its own stages");
+  // Each team has stages of its own, or else a warp that is ahead by a round would take the other team's phase of a barrier for its own.
+  static constexpr uint32_t kTeamStages = kStages / kTeams;
+  static_assert(kStages % kTeams == 0 && kTeamStages >= 2, "a unit takes two stages");
   // 16-byte piece c of row r within a tile: its place in the swizzled box
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     if (kChunkRow == 128) return (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -98,26 +107,37 @@ __device__ __forceinline__ int sequence_of(const int* before, int n, int u) {
   return lo;
 }
 
-template <typename T, typename C, int HD>
-__global__ void __launch_bounds__(kThreads, kPerSm)
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 matrix of 16-bit elements
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// the lower and the upper two of four codes as halves
+__device__ __forceinline__ void codes_to_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
+}
+
+template <typename T, typename C, int HD, int NT>
+__global__ void __launch_bounds__(kThreads, (Shape<C, HD, NT>::kPerSm))
 paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const StreamParams p) {
-  using S = Shape<C, HD>;
+  using S = Shape<C, HD, NT>;
   constexpr bool kEight = sizeof(C) == 1;
   constexpr bool kTwoTerm = std::is_same<C, __nv_bfloat16>::value;
   using M = typename std::conditional<kEight, __half, T>::type;  // type of the products
-  // Probabilities in halves are taken 2^14 times as large (and the sums with them), so that those down to 2^-28 of the largest keep their digits.
-  constexpr float kLift = std::is_same<M, __half>::value ? 14.f : 0.f;
-  constexpr int KB = HD / 16, OB = HD / 8, UNIT = S::kUnit;
+  // The reference of a head's scores moves when one exceeds it by kSlack (powers of two), that of the values' scales when one is four times as
+  // large.  Probabilities in halves are taken 2^kLift times as large, and the sums with them: up to 2^15, and with all digits down to 2^-23.
+  constexpr float kSlack = 4.f, kLift = std::is_same<M, __half>::value ? 9.f : 0.f;
+  constexpr int KB = HD / 16, UNIT = S::kUnit, TILE = S::kTile, RB = TILE / 16;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* tail = smem_raw + (ring - smem_u32(smem_raw)) + kRingBytes;
+  uint8_t* tail = smem_raw + (ring - smem_u32(smem_raw)) + S::kRingBytes;
   float* sm_scale = reinterpret_cast<float*>(tail);                                                    // [stages][UNIT], e4m3
   float* sm_o = sm_scale + (kEight ? S::kStages * UNIT : 0);                                           // [warps][tile_heads][HD]
   int* before = reinterpret_cast<int*>(sm_o + kWarps * p.tile_heads * HD);                             // [n_seq + 1] units before a sequence
   int* contexts = before + p.a.table.n_seq + 1;                                                        // [n_seq]
   __shared__ uint64_t bars[2 * S::kStages];
-  __shared__ uint32_t stage_boxes[S::kStages / 2];  // bit i: box i of the unit has a page
+  __shared__ uint32_t stage_boxes[S::kStages];  // bit i: box i of the unit whose keys are in this stage has a page
   __shared__ float sm_m[kWarps][kMaxGroup], sm_l[kWarps][kMaxGroup];
   __shared__ int abort_flag;
   __shared__ unsigned int ticket;
@@ -132,7 +152,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     abort_flag = 0;
     for (uint32_t s = 0; s < S::kStages; ++s) {
       mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, kWarps / S::kTeams);
+      mbar_init(empty0 + 8 * s, kPairWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -194,7 +214,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int64_t page = table.find(b, pos);
       if (page >= 0) slab = static_cast<int>(page * p.a.n_kv + pair / p.head_tiles), row = pos % table.page;
     };
-    uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait on parity 1
+    uint32_t s[kTeams], parity[kTeams];  // of each team's next stage; a fresh barrier passes a wait on parity 1
+#pragma unroll
+    for (int t = 0; t < kTeams; ++t) s[t] = 0, parity[t] = 1;
     int slab, row, next_slab, next_row;
     look_up(u0 + lane / boxes, slab, row);
     bool ok = true;
@@ -202,40 +224,43 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       look_up(base + ahead + lane / boxes, next_slab, next_row);
       const uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
       const int n = u1 - base < ahead ? u1 - base : ahead;
-      for (int i = 0; i < n && ok; ++i) {
-        const uint32_t mine = (have >> (i * boxes)) & ((1u << boxes) - 1u);
-        const uint32_t count = __popc(mine);
+      for (int i0 = 0; i0 < n && ok; i0 += kTeams)  // (`ahead` is a multiple of the teams)
 #pragma unroll
-        for (int half = 0; half < 2 && ok; ++half) {
-          const uint32_t st = s + half, full = full0 + 8 * st;
-          ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * st, parity, &abort_flag, 41, &g_paged_attn_status));
-          if (!ok) break;
-          if (lane == 0) {
-            if (half == 0) stage_boxes[s >> 1] = mine;
-            mbar_expect_tx(full, count * p.box * (S::kRow + (kEight ? 4 : 0)));
-          }
-          __syncwarp();
-          if (lane / boxes == i && slab >= 0) {
-            const int at = (lane % boxes) * p.box;
+        for (int t = 0; t < kTeams; ++t) {
+          const int i = i0 + t;
+          if (i >= n || !ok) break;
+          const uint32_t mine = (have >> (i * boxes)) & ((1u << boxes) - 1u);
+          const uint32_t count = __popc(mine);
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-              tma_load_3d(ring + st * S::kHalf + c * S::kChunkBytes + at * S::kChunkRow, half ? &tmap_v : &tmap_k, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
-            if (kEight) bulk_load(smem_u32(sm_scale + st * UNIT + at), (half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(slab) * table.page + row, p.box * 4, full);
+          for (int half = 0; half < 2 && ok; ++half) {
+            const uint32_t st = t * S::kTeamStages + s[t], full = full0 + 8 * st;
+            ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * st, parity[t], &abort_flag, 41, &g_paged_attn_status));
+            if (!ok) break;
+            if (lane == 0) {
+              if (half == 0) stage_boxes[st] = mine;
+              mbar_expect_tx(full, count * p.box * (S::kRow + (kEight ? 4 : 0)));
+            }
+            __syncwarp();
+            if (lane / boxes == i && slab >= 0) {
+              const int at = (lane % boxes) * p.box;
+#pragma unroll
+              for (int c = 0; c < S::kChunks; ++c)
+                tma_load_3d(ring + st * S::kHalf + c * S::kChunkBytes + at * S::kChunkRow, half ? &tmap_v : &tmap_k, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
+              if (kEight) bulk_load(smem_u32(sm_scale + st * UNIT + at), (half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(slab) * table.page + row, p.box * 4, full);
+            }
+            __syncwarp();
+            if (++s[t] == S::kTeamStages) s[t] = 0, parity[t] ^= 1u;
           }
-          __syncwarp();
         }
-        s += 2;
-        if (s == S::kStages) s = 0, parity ^= 1u;
-      }
       slab = next_slab, row = next_row;
     }
   } else if (u0 < u1) {
-    const int r0 = lane >> 2, r1 = r0 + 8;       // the rows (heads) whose scores this thread holds
-    const int sub = warp % (UNIT / kTile);       // which 16 positions of a unit
-    const int team = warp / (UNIT / kTile);
-    uint32_t s = 2 * team, parity = 0;           // the stage of K; V is in the next one
+    const int quad = lane >> 2, col = (lane & 3) * 2;  // a thread holds scores of positions quad, quad + 8, .. and heads col, col + 1
+    const int sub = warp % kPairWarps, team = warp / kPairWarps;
+    uint32_t s = team * S::kTeamStages, parity = 0;  // the stage whose turn it is: of keys, then of values
+    const uint32_t s_end = s + S::kTeamStages;
     bool ok = true;
-    int next = u0 + team;                        // this team's next unit
+    int next = u0 + team;  // this team's next unit
     int b = sequence_of(before, n_seq, u0);
     for (int u = u0; u < u1;) {
       while (before[b + 1] <= u) ++b;
@@ -247,252 +272,281 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int head0 = h * p.group + ht * p.tile_heads;
       const int g = p.group - ht * p.tile_heads < p.tile_heads ? p.group - ht * p.tile_heads : p.tile_heads;
 
-      // ---- Q: head i of the pass is row i; rows from g up are zero -------------------------------------------------------------------
-      uint32_t qa[KB][4];
-      float score_scale[2] = {p.a.scale_log2, p.a.scale_log2};
-      {
-        const T* qg = static_cast<const T*>(p.a.q) + (static_cast<int64_t>(b) * p.a.n_head + head0) * p.a.dim;
+      // ---- Q^T: head i of the pass is column i; columns from g up are zero -----------------------------------------------------------
+      uint32_t qb[NT][KB][2];
+      float score_scale[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int i = n * 8 + quad;
+        const T* qg = static_cast<const T*>(p.a.q) + (static_cast<int64_t>(b) * p.a.n_head + head0 + i) * p.a.dim;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 2; ++e) {
             // e4m3: a thread's four bytes of a row of keys are elements 4 t .. 4 t + 3 of the block
-            const int r = (e & 1) ? r1 : r0, col = kb * 16 + (kEight ? (lane & 3) * 4 + (e >> 1) * 2 : (lane & 3) * 2 + (e >> 1) * 8);
-            qa[kb][e] = r < g && col < p.a.dim ? *reinterpret_cast<const uint32_t*>(qg + static_cast<int64_t>(r) * p.a.dim + col) : 0u;
+            const int at = kb * 16 + (kEight ? col * 2 + e * 2 : col + e * 8);
+            qb[n][kb][e] = i < g && at < p.a.dim ? *reinterpret_cast<const uint32_t*>(qg + at) : 0u;
           }
-        if (kEight && !std::is_same<T, __half>::value) {
-          float top[2] = {0.f, 0.f};
+        score_scale[n][0] = score_scale[n][1] = p.a.scale_log2;
+        if constexpr (kEight && !std::is_same<T, __half>::value) {
+          float top = 0.f;
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               float x, y;
-              Num<T>::unpack2(qa[kb][e], x, y);
-              top[e & 1] = fmaxf(top[e & 1], fmaxf(fabsf(x), fabsf(y)));
+              Num<T>::unpack2(qb[n][kb][e], x, y);
+              top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
             }
-          float up[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            int k = 14 + 127 - static_cast<int>(__float_as_uint(top[r]) >> 23);  // 2^k brings it to 2^14 .. 2^15
-            k = k > 110 ? 110 : k;                                               // rows of nothing but tiny numbers: their scores are zero anyway
-            up[r] = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-            score_scale[r] *= __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          int k = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);  // 2^k brings it to 2^14 .. 2^15
+          k = k > 110 ? 110 : k;                                            // rows of nothing but tiny numbers: their scores are zero anyway
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               float x, y;
-              Num<T>::unpack2(qa[kb][e], x, y);
-              qa[kb][e] = pack2<__half>(x * up[e & 1], y * up[e & 1]);
+              Num<T>::unpack2(qb[n][kb][e], x, y);
+              qb[n][kb][e] = pack2<__half>(x * up, y * up);
             }
+          score_scale[n][0] *= __shfl_sync(0xffffffffu, down, col * 4);
+          score_scale[n][1] *= __shfl_sync(0xffffffffu, down, col * 4 + 4);
         }
       }
-      float o[OB][4];
+      float o[NT][KB][4];  // elements quad and quad + 8 (e4m3: 2 quad and 2 quad + 1) of a block of 16, heads col and col + 1
+      float m_run[NT][2], l_run[NT][2];
 #pragma unroll
-      for (int i = 0; i < OB; ++i)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-      float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of the largest scale of values so far
+        for (int i = 0; i < KB; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+        m_run[n][0] = m_run[n][1] = -INFINITY, l_run[n][0] = l_run[n][1] = 0.f;
+      }
+      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of v_top
 
-      auto arrived = [&](uint32_t stage) {
-        return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * stage, parity, &abort_flag, 42, &g_paged_attn_status)) != 0;
+      auto arrived = [&]() {
+        return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 42, &g_paged_attn_status)) != 0;
       };
-      auto give_back = [&](uint32_t stage) {
+      auto give_back = [&]() {
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty0 + 8 * stage);
+        if (lane == 0) mbar_arrive(empty0 + 8 * s);
+        if (++s == s_end) s -= S::kTeamStages, parity ^= 1u;
       };
-      for (; next < end && ok; next += S::kTeams) {
-        ok = arrived(s);
+      for (; next < end && ok; next += kTeams) {
+        ok = arrived();
         if (!ok) break;
-        // ---- which of the 16 positions are visible ----------------------------------------------------------------------------------
-        const int p0 = (sp.first + next - first) * UNIT + sub * kTile;
-        const uint32_t has = stage_boxes[s >> 1];
-        uint32_t vis = ((has >> ((sub * kTile) / p.box)) & 1u ? 0x00ffu : 0u) | ((has >> ((sub * kTile + 8) / p.box)) & 1u ? 0xff00u : 0u);
-        if (p0 + kTile > sp.ctx) vis &= p0 < sp.ctx ? (1u << (sp.ctx - p0)) - 1u : 0u;
-        if (p0 < sp.lo) vis &= sp.lo - p0 < kTile ? ~((1u << (sp.lo - p0)) - 1u) : 0u;
-        // ---- scores 16 heads x 16 positions, four accumulation chains ---------------------------------------------------------------
-        float sc[2][2][4];
+        // ---- which of the positions are visible --------------------------------------------------------------------------------------
+        const int p0 = (sp.first + next - first) * UNIT + sub * TILE;
+        const uint32_t has = stage_boxes[s];
+        uint32_t vis = 0u;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i >> 3][(i >> 2) & 1][i & 3] = 0.f;
-        {
-          const int row = sub * kTile + (lane & 7) + (lane >> 4) * 8;
+        for (int i = 0; i < TILE / 8; ++i) vis |= (has >> ((sub * TILE + i * 8) / p.box)) & 1u ? 0xffu << (i * 8) : 0u;
+        if (p0 + TILE > sp.ctx) vis &= p0 < sp.ctx ? (1u << (sp.ctx - p0)) - 1u : 0u;
+        if (p0 < sp.lo) vis &= sp.lo - p0 < TILE ? ~((1u << (sp.lo - p0)) - 1u) : 0u;
+        constexpr uint32_t kAll = TILE == 32 ? 0xffffffffu : (1u << (TILE & 31)) - 1u;
+        // ---- scores: TILE positions x 8 NT heads ----------------------------------------------------------------------------------------
+        float sc[RB][NT][4];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const int row = sub * TILE + rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
           const uint32_t at = ring + s * S::kHalf;
+          float part[2][NT][4];  // two chains
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[0][n][e] = part[1][n][e] = 0.f;
           if constexpr (kEight) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb += 2) {
-              uint32_t bf[4];
-              load_matrix(at + S::at(row, kb + ((lane >> 3) & 1)), bf);
+              uint32_t bf[4], a[2][4];
+              load_matrix(at + S::at(row, kb + (lane >> 4)), bf);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {  // block kb + (i & 1), positions (i >> 1) * 8 ..
-                const uint32_t b0 = e4m3x2_to_half2(static_cast<uint16_t>(bf[i])), b1 = e4m3x2_to_half2(static_cast<uint16_t>(bf[i] >> 16));
-                const uint32_t(&a)[4] = qa[kb + (i & 1)];
-                mma16816<__half>(sc[i & 1][i >> 1], a[0], a[1], a[2], a[3], b0, b1);
-              }
+              for (int i = 0; i < 4; ++i) codes_to_halves(bf[i], a[i >> 1][i & 1], a[i >> 1][2 + (i & 1)]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<M>(part[i][n], a[i][0], a[i][1], a[i][2], a[i][3], qb[n][kb + i][0], qb[n][kb + i][1]);
             }
           } else {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-              uint32_t bf[4];
-              load_matrix(at + S::at(row, kb * 2 + ((lane >> 3) & 1)), bf);
-              mma16816<M>(sc[kb & 1][0], qa[kb][0], qa[kb][1], qa[kb][2], qa[kb][3], bf[0], bf[1]);
-              mma16816<M>(sc[kb & 1][1], qa[kb][0], qa[kb][1], qa[kb][2], qa[kb][3], bf[2], bf[3]);
+              uint32_t a[4];
+              load_matrix(at + S::at(row, kb * 2 + (lane >> 4)), a);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma16816<M>(part[kb & 1][n], a[0], a[1], a[2], a[3], qb[n][kb][0], qb[n][kb][1]);
             }
           }
-        }
-        float ks[4];  // scales of positions (i >> 1) * 8 + 2 t + (i & 1)
-        if constexpr (kEight) {
-          const float* sk = sm_scale + s * UNIT + sub * kTile + (lane & 3) * 2;
-          const float2 x = *reinterpret_cast<const float2*>(sk), y = *reinterpret_cast<const float2*>(sk + 8);
-          ks[0] = x.x, ks[1] = x.y, ks[2] = y.x, ks[3] = y.y;
-        }
-        give_back(s);
-        // ---- scale, mask -------------------------------------------------------------------------------------------------------------
-        float x[2][4], mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = kEight ? score_scale[e >> 1] * ks[nb * 2 + (e & 1)] : p.a.scale_log2;
-            x[nb][e] = (vis >> (nb * 8 + (lane & 3) * 2 + (e & 1))) & 1u ? (sc[0][nb][e] + sc[1][nb][e]) * f : -INFINITY;
-            mx[e >> 1] = fmaxf(mx[e >> 1], x[nb][e]);
+            for (int e = 0; e < 4; ++e) sc[rb][n][e] = part[0][n][e] + part[1][n][e];
+          if constexpr (kEight) {
+            const float* sk = sm_scale + s * UNIT + sub * TILE + rb * 16 + quad;
+            const float ks[2] = {sk[0], sk[8]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[rb][n][e] *= ks[e >> 1] * score_scale[n][e & 1];
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[rb][n][e] *= p.a.scale_log2;
           }
         }
-        // ---- online softmax ------------------------------------------------------------------------------------------------------------
-        float corr[2];
+        give_back();
+        if (vis != kAll) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-          const float m_new = fmaxf(m_run[r], mx[r]);
-          const float m_use = m_new == -INFINITY ? 0.f : m_new;
-          corr[r] = exp2f(m_run[r] - m_use);
-          m_run[r] = m_new;
-          mx[r] = m_use - kLift;
+          for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!((vis >> (rb * 16 + (e >> 1) * 8 + quad)) & 1u))
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[rb][n][e] = -INFINITY;
         }
-        ok = arrived(s + 1);
+        // ---- references: of a head's scores, of the values' scales ------------------------------------------------------------------------
+        float mx[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            mx[n][c] = -INFINITY;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) mx[n][c] = fmaxf(mx[n][c], fmaxf(sc[rb][n][c], sc[rb][n][2 + c]));
+            moved = moved || mx[n][c] > m_run[n][c] + kSlack;
+          }
+        ok = arrived();
         if (!ok) break;
-        float vs[4], turn = 1.f;
+        float vs[RB][2], top = 0.f;
         if constexpr (kEight) {
-          const float* sv = sm_scale + (s + 1) * UNIT + sub * kTile + (lane & 3) * 2;
-          const float2 a = *reinterpret_cast<const float2*>(sv), c = *reinterpret_cast<const float2*>(sv + 8);
-          vs[0] = a.x, vs[1] = a.y, vs[2] = c.x, vs[3] = c.y;
-          float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            vs[i] = (vis >> ((i >> 1) * 8 + (lane & 3) * 2 + (i & 1))) & 1u ? vs[i] : 0.f;
-            top = fmaxf(top, fabsf(vs[i]));
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          if (top > v_top) {
-            turn = v_top / top;
-            v_top = top, v_inv = 1.f / top;
-          }
+          for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] *= v_inv;
-        }
-        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f || turn != 1.f)) {  // a maximum moved: seldom after the first tiles
-#pragma unroll
-          for (int r = 0; r < 2; ++r) l_run[r] *= corr[r];
-#pragma unroll
-          for (int i = 0; i < OB; ++i) {
-            o[i][0] *= corr[0] * turn;
-            o[i][1] *= corr[0] * turn;
-            o[i][2] *= corr[1] * turn;
-            o[i][3] *= corr[1] * turn;
-          }
-        }
-        uint32_t pa[4], pl[4];
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          float pv[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pv[e] = exp2f(x[nb][e] - mx[e >> 1]);
-            l_run[e >> 1] += pv[e];
-            if (kEight) pv[e] *= vs[nb * 2 + (e & 1)];
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            pa[nb * 2 + r] = pack2<M>(pv[2 * r], pv[2 * r + 1]);
-            if (kTwoTerm) {
-              float h0, h1;
-              Num<M>::unpack2(pa[nb * 2 + r], h0, h1);
-              pl[nb * 2 + r] = pack2<M>(pv[2 * r] - h0, pv[2 * r + 1] - h1);
+            for (int i = 0; i < 2; ++i) {
+              vs[rb][i] = sm_scale[s * UNIT + sub * TILE + rb * 16 + i * 8 + quad];
+              if (vis != kAll && !((vis >> (rb * 16 + i * 8 + quad)) & 1u)) vs[rb][i] = 0.f;
+              top = fmaxf(top, fabsf(vs[rb][i]));
             }
-          }
+          moved = moved || top > 4.f * v_top;
         }
-        // ---- O += P V (16 positions = one k block) ------------------------------------------------------------------------------------
-        const uint32_t sv = ring + (s + 1) * S::kHalf;
-        if (vis != 0xffffu) {
+        if (__any_sync(0xffffffffu, moved)) {
+          float turn = 1.f;
+          if constexpr (kEight) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            if (top > v_top) turn = v_top / top, v_top = top, v_inv = 1.f / top;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], w));
+              const float m_new = fmaxf(m_run[n][c], mx[n][c]);
+              const float corr = exp2f(m_run[n][c] - (m_new == -INFINITY ? 0.f : m_new));
+              m_run[n][c] = m_new;
+              l_run[n][c] *= corr;
+#pragma unroll
+              for (int i = 0; i < KB; ++i) o[n][i][c] *= corr * turn, o[n][i][2 + c] *= corr * turn;
+            }
+        }
+        // ---- probabilities, transposed ----------------------------------------------------------------------------------------------------
+        uint32_t pb[RB][NT][2], pl[RB][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float m0 = m_run[n][0] == -INFINITY ? 0.f : m_run[n][0] - kLift, m1 = m_run[n][1] == -INFINITY ? 0.f : m_run[n][1] - kLift;
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float x = exp2_approx(sc[rb][n][2 * i] - m0), y = exp2_approx(sc[rb][n][2 * i + 1] - m1);
+              l_run[n][0] += x, l_run[n][1] += y;
+              if (kEight) {
+                const float f = vs[rb][i] * v_inv;
+                x *= f, y *= f;
+              }
+              const uint32_t hi = pack2<M>(x, y);
+              pb[rb][n][i] = transposed(hi);
+              if (kTwoTerm) {
+                float h0, h1;
+                Num<M>::unpack2(hi, h0, h1);
+                pl[rb][n][i] = transposed(pack2<M>(x - h0, y - h1));
+              }
+            }
+        }
+        const uint32_t sv = ring + s * S::kHalf;
+        if (vis != kAll) {
           // values that are not visible may be anything, and 0 x NaN is not 0
-          for (int i = lane; i < kTile * (S::kRow / 16); i += 32) {
+          for (int i = lane; i < TILE * (S::kRow / 16); i += 32) {
             const int r = i / (S::kRow / 16), c = i % (S::kRow / 16);
-            if (!((vis >> r) & 1u)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(sub * kTile + r, c)), "r"(0u) : "memory");
+            if (!((vis >> r) & 1u)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(sub * TILE + r, c)), "r"(0u) : "memory");
           }
           __syncwarp();
         }
-        {
-          const int row = sub * kTile + (lane & 7) + ((lane >> 3) & 1) * 8;
+        // ---- O^T += V^T P^T, 16 positions at a time ----------------------------------------------------------------------------------------
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
           if constexpr (kEight) {
+            const int row = sub * TILE + rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-            for (int ch = 0; ch < KB; ch += 2) {  // 16 elements of a value: columns of an even and an odd block
-              uint32_t bf[4];
-              load_matrix_trans(sv + S::at(row, ch + (lane >> 4)), bf);
+            for (int kb = 0; kb < KB; kb += 2) {  // rows of a product: the block's even elements, then its odd ones
+              uint32_t bf[4], a[2][4];
+              load_matrix_trans(sv + S::at(row, kb + (lane >> 4)), bf);
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t w0 = __byte_perm(bf[2 * i], 0u, 0x3120), w1 = __byte_perm(bf[2 * i + 1], 0u, 0x3120);
-                mma16816<__half>(o[2 * (ch + i)], pa[0], pa[1], pa[2], pa[3], e4m3x2_to_half2(static_cast<uint16_t>(w0)), e4m3x2_to_half2(static_cast<uint16_t>(w1)));
-                mma16816<__half>(o[2 * (ch + i) + 1], pa[0], pa[1], pa[2], pa[3], e4m3x2_to_half2(static_cast<uint16_t>(w0 >> 16)), e4m3x2_to_half2(static_cast<uint16_t>(w1 >> 16)));
-              }
+              for (int i = 0; i < 4; ++i) codes_to_halves(__byte_perm(bf[i], 0u, 0x3120), a[i >> 1][(i & 1) * 2], a[i >> 1][(i & 1) * 2 + 1]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<M>(o[n][kb + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[rb][n][0], pb[rb][n][1]);
             }
           } else {
+            const int row = sub * TILE + rb * 16 + (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
-            for (int ob2 = 0; ob2 < OB / 2; ++ob2) {
-              uint32_t bf[4];
-              load_matrix_trans(sv + S::at(row, ob2 * 2 + (lane >> 4)), bf);
-              mma16816<M>(o[2 * ob2], pa[0], pa[1], pa[2], pa[3], bf[0], bf[1]);
-              mma16816<M>(o[2 * ob2 + 1], pa[0], pa[1], pa[2], pa[3], bf[2], bf[3]);
-              if (kTwoTerm) {
-                mma16816<M>(o[2 * ob2], pl[0], pl[1], pl[2], pl[3], bf[0], bf[1]);
-                mma16816<M>(o[2 * ob2 + 1], pl[0], pl[1], pl[2], pl[3], bf[2], bf[3]);
+            for (int kb = 0; kb < KB; ++kb) {
+              uint32_t a[4];
+              load_matrix_trans(sv + S::at(row, kb * 2 + ((lane >> 3) & 1)), a);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma16816<M>(o[n][kb], a[0], a[1], a[2], a[3], pb[rb][n][0], pb[rb][n][1]);
+                if (kTwoTerm) mma16816<M>(o[n][kb], a[0], a[1], a[2], a[3], pl[rb][n][0], pl[rb][n][1]);
               }
             }
           }
         }
-        if (vis != 0xffffu) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros, before the next copy
-        give_back(s + 1);
-        s += 2 * S::kTeams;
-        if (s >= S::kStages) s -= S::kStages, parity ^= 1u;
+        if (vis != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros, before the next copy
+        give_back();
       }
 
       // ---- join the warps --------------------------------------------------------------------------------------------------------------
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], w);
       warps_sync();  // the arrays' previous contents have been read
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = r ? r1 : r0;
-        if (i < g) {
-          if ((lane & 3) == 0) sm_m[warp][i] = m_run[r] - kLift, sm_l[warp][i] = l_run[r];
-          float* d = sm_o + (warp * p.tile_heads + i) * HD;
-          if constexpr (kEight) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int ch = 0; ch < KB; ++ch)
-              *reinterpret_cast<float4*>(d + ch * 16 + (lane & 3) * 4) = make_float4(o[2 * ch][2 * r] * v_top, o[2 * ch + 1][2 * r] * v_top, o[2 * ch][2 * r + 1] * v_top, o[2 * ch + 1][2 * r + 1] * v_top);
-          } else {
+        for (int c = 0; c < 2; ++c) {
+          const int i = n * 8 + col + c;
+          if (i < g) {
+            if (quad == 0) sm_m[warp][i] = m_run[n][c] - kLift, sm_l[warp][i] = l_run[n][c];
+            float* d = sm_o + (warp * p.tile_heads + i) * HD;
 #pragma unroll
-            for (int k = 0; k < OB; ++k) *reinterpret_cast<float2*>(d + k * 8 + (lane & 3) * 2) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
+            for (int k = 0; k < KB; ++k) {
+              if constexpr (kEight) {
+                *reinterpret_cast<float2*>(d + k * 16 + quad * 2) = make_float2(o[n][k][c] * v_top, o[n][k][2 + c] * v_top);
+              } else {
+                d[k * 16 + quad] = o[n][k][c], d[k * 16 + quad + 8] = o[n][k][2 + c];
+              }
+            }
           }
         }
-      }
       warps_sync();
       // result of elements e, e + 1 of head i of the pass
       auto store = [&](int i, int e, float l, float2 v) {
@@ -539,21 +593,27 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         }
         warps_sync();
         if (ticket == static_cast<unsigned int>(c_last - c_first)) {
-          for (int idx = threadIdx.x; idx < g * (HD / 2); idx += kWarps * 32) {
-            const int i = idx / (HD / 2), e = idx % (HD / 2) * 2;
-            float mm = -INFINITY, ll = 0.f;
-            float2 sum = make_float2(0.f, 0.f);
-            for (int64_t c = c_first; c <= c_last; ++c) {
-              const int64_t at = part_of(c) + i;
+          const int parts = static_cast<int>(c_last - c_first) + 1;
+          const int64_t p_first = part_of(c_first), p_rest = 2 * c_first * p.tile_heads;  // part k > 0 is the first of CTA c_first + k
+          for (int idx = threadIdx.x; idx < g * (HD / 4); idx += kWarps * 32) {
+            const int i = idx / (HD / 4), e = idx % (HD / 4) * 4;
+            // all maxima first: then no load waits for another
+            float mm = -INFINITY;
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) mm = fmaxf(mm, __ldcg(p.part_ml + ((k ? p_rest + 2 * k * p.tile_heads : p_first) + i) * 2));
+            const float m_use = mm == -INFINITY ? 0.f : mm;
+            float ll = 0.f, v[4] = {};
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) {
+              const int64_t at = (k ? p_rest + 2 * k * p.tile_heads : p_first) + i;
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD + e));
-              const float m_new = fmaxf(mm, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
-              const float w_old = exp2f(mm - m_use), w = exp2f(ml.x - m_use);
-              ll = ll * w_old + ml.y * w;
-              sum.x = sum.x * w_old + v.x * w, sum.y = sum.y * w_old + v.y * w;
-              mm = m_new;
+              const float4 w = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + e));
+              const float f = exp2f(ml.x - m_use);
+              ll += ml.y * f;
+              v[0] += w.x * f, v[1] += w.y * f, v[2] += w.z * f, v[3] += w.w * f;
             }
-            store(i, e, ll, sum);
+            store(i, e, ll, make_float2(v[0], v[1]));
+            store(i, e + 2, ll, make_float2(v[2], v[3]));
           }
           if (threadIdx.x == 0) p.counters[c_first] = 0u;  // ready for the next call
         }
@@ -573,9 +633,9 @@ int tile_heads_of(int group) {
   return (group + tiles - 1) / tiles;
 }
 
-template <typename T, typename C, int HD>
+template <typename T, typename C, int HD, int NT>
 int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
-  using S = Shape<C, HD>;
+  using S = Shape<C, HD, NT>;
   const PageTable& t = p.a.table;
   p.box = S::kUnit;
   while (t.page % p.box != 0) p.box /= 2;
@@ -591,10 +651,10 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   int64_t per = (1ll << 30) / most;
   LRI_REQUIRE(per >= 1, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %lld positions of %d heads", (long long)t.capacity(), p.a.n_kv);
   per = per < kMaxSeqs ? per : kMaxSeqs;
-  auto kern = paged_attn_stream_kernel<T, C, HD>;
-  const int fixed = 1024 + kRingBytes + (sizeof(C) == 1 ? S::kStages * S::kUnit * 4 : 0);
+  auto kern = paged_attn_stream_kernel<T, C, HD, NT>;
+  const int fixed = 1024 + S::kRingBytes + (sizeof(C) == 1 ? S::kStages * S::kUnit * 4 : 0);
   static std::atomic<unsigned long long> attr_set{0};
-  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kWarps * kMaxGroup * HD * 4 + (2 * kMaxSeqs + 1) * 4));
+  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kWarps * 8 * NT * HD * 4 + (2 * kMaxSeqs + 1) * 4));
   const PagedAttnParams all = p.a;
   for (int64_t at = 0; at < all.table.n_seq; at += per) {
     const int n = static_cast<int>(all.table.n_seq - at < per ? all.table.n_seq - at : per);
@@ -603,7 +663,7 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
     p.a.q = static_cast<const T*>(all.q) + at * all.n_head * all.dim;
     p.a.out = static_cast<T*>(all.out) + at * all.n_head * all.dim;
     p.a.input_pos = static_cast<const char*>(all.input_pos) + at * (all.pos_is_i64 ? 8 : 4);
-    const int64_t room = static_cast<int64_t>(kPerSm) * device_sm_count(), useful = (most * n + kMinRun - 1) / kMinRun;
+    const int64_t room = static_cast<int64_t>(S::kPerSm) * device_sm_count(), useful = (most * n + kMinRun - 1) / kMinRun;
     const int smem = fixed + kWarps * p.tile_heads * HD * 4 + (2 * n + 1) * 4;
     LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(kThreads), smem, st, tk, tv, p));
     LRI_LAUNCH_CHECK("paged_attn_stream_kernel");
@@ -611,10 +671,15 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   return LRI_OK;
 }
 
+template <typename T, typename C, int HD>
+int by_heads(int cache_dtype, StreamParams& p, cudaStream_t st) {
+  return p.tile_heads <= 8 ? launch<T, C, HD, 1>(cache_dtype, p, st) : launch<T, C, HD, 2>(cache_dtype, p, st);
+}
+
 template <typename T>
 int dispatch(int cache_dtype, StreamParams& p, cudaStream_t st) {
-  if (cache_dtype == LRI_E4M3) return p.a.dim <= 64 ? launch<T, e4m3, 64>(cache_dtype, p, st) : launch<T, e4m3, 128>(cache_dtype, p, st);
-  return p.a.dim <= 64 ? launch<T, T, 64>(cache_dtype, p, st) : launch<T, T, 128>(cache_dtype, p, st);
+  if (cache_dtype == LRI_E4M3) return p.a.dim <= 64 ? by_heads<T, e4m3, 64>(cache_dtype, p, st) : by_heads<T, e4m3, 128>(cache_dtype, p, st);
+  return p.a.dim <= 64 ? by_heads<T, T, 64>(cache_dtype, p, st) : by_heads<T, T, 128>(cache_dtype, p, st);
 }
 
 }  // namespace
@@ -624,13 +689,13 @@ bool paged_attn_stream_supports(int cache_dtype, int dim) { return dim <= 128 &&
 
 size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim) {
   const int hd = dim <= 64 ? 64 : 128;
-  return kCounterBytes + static_cast<size_t>(kPerSm) * device_sm_count() * 2 * tile_heads_of(n_head / n_kv) * (hd + 2) * 4;
+  return kCounterBytes + static_cast<size_t>(kMaxPerSm) * device_sm_count() * 2 * tile_heads_of(n_head / n_kv) * (hd + 2) * 4;
 }
 
 int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   LRI_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim), LRI_ERR_WORKSPACE,
               "paged_attn_decode: workspace of %zu bytes (16-byte aligned) required", paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim));
-  LRI_REQUIRE(static_cast<size_t>(kPerSm) * device_sm_count() * 4 <= kCounterBytes, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %d multiprocessors", device_sm_count());
+  LRI_REQUIRE(static_cast<size_t>(kMaxPerSm) * device_sm_count() * 4 <= kCounterBytes, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %d multiprocessors", device_sm_count());
   StreamParams p{};
   p.a = a;
   p.group = a.n_head / a.n_kv;
@@ -638,7 +703,7 @@ int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& 
   p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
   p.counters = static_cast<unsigned int*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-  p.part_ml = p.part_o + static_cast<size_t>(kPerSm) * device_sm_count() * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
+  p.part_ml = p.part_o + static_cast<size_t>(kMaxPerSm) * device_sm_count() * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
   return dtype == LRI_BF16 ? dispatch<__nv_bfloat16>(cache_dtype, p, st) : dispatch<__half>(cache_dtype, p, st);
 }
 

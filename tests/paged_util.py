@@ -49,7 +49,7 @@ def make_cache(lengths, page, n_kv, dim, dtype, eight, seed=0, device="cuda"):
     return cache, table
 
 
-def dense(cache, table, b, lo, hi):
+def dense(cache, table, b, lo, hi, with_scales=False):
     """Keys and values of positions lo .. hi - 1 of sequence b in 64 bits, [heads, positions, dim]; only positions that have a page."""
     page, n_pages = cache.k_pages.shape[2], cache.k_pages.shape[0]
     at = torch.arange(lo, hi, device=table.device)
@@ -59,23 +59,26 @@ def dense(cache, table, b, lo, hi):
     got = []
     for pages, scales in ((cache.k_pages, cache.k_scale), (cache.v_pages, cache.v_scale)):
         x = pages.view(torch.uint8 if scales is not None else pages.dtype)[ids, :, at % page].view(pages.dtype).double()
-        if scales is not None:
-            x = x * scales[ids, :, at % page].double()[..., None]
-        got.append(x.transpose(0, 1))
-    return got
+        s = torch.ones_like(x[..., 0]) if scales is None else scales[ids, :, at % page].double()
+        got.append((x * s[..., None]).transpose(0, 1))
+    return got + [x.transpose(0, 1), s.transpose(0, 1)] if with_scales else got
 
 
 def attend_64(cache, table, q, lengths, window=0, scale=None):
     """The result in 64 bits and how far a right one may be off: probabilities rounded once to the type (half a step of what they weigh), sums
     in 32 bits of the scores (dim + 2 roundings of the sum of magnitudes), 2^-18 for the exponentials and the sums over positions, and the
-    result's own rounding."""
+    result's own rounding.
+
+    Probabilities that are halves (fp16 and e4m3 pages) end at steps of 2^-24: taken 2^9 times as large, p (with e4m3 p scale / largest scale) is off by
+    up to 2^-25 2^-9 = 2^-34 however small it is.  The largest p is at least 1 in these units, so the sum that divides is too, and the result is off by up
+    to 2^-34 times the sum of |value| (e4m3: |code| times the largest scale) over the positions: it shows where all that has weight is zero."""
     n_kv, dim = cache.k_pages.shape[1], cache.k_pages.shape[3]
     scale = dim ** -0.5 if scale is None else scale
     y, tol = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
     half = half_step(q.dtype)
     for b, n in enumerate(lengths):
         n = max(0, min(n, table.shape[1] * cache.k_pages.shape[2]))
-        k, v = dense(cache, table, b, max(0, n - window) if window else 0, n)
+        k, v, codes, scales = dense(cache, table, b, max(0, n - window) if window else 0, n, True)
         if k.shape[1] == 0:
             continue
         qb = q[b].double().view(n_kv, -1, dim)
@@ -83,6 +86,9 @@ def attend_64(cache, table, q, lengths, window=0, scale=None):
         loose = (qb.abs() @ k.abs().transpose(1, 2) * abs(scale)).amax() * (dim + 2) * 2.0 ** -24
         y[b] = (w @ v).reshape(q[b].shape)
         tol[b] = (w @ v.abs()).reshape(q[b].shape) * (half + 2 * loose + 2.0 ** -18) + half * y[b].abs() + TINY[q.dtype]
+        if cache.v_scale is not None or q.dtype == torch.float16:
+            ends = 2.0 ** -34 * codes.abs().sum(1) * scales.amax(-1, keepdim=True)
+            tol[b] += ends[:, None].expand(-1, qb.shape[1], -1).reshape(q[b].shape)
     return y, tol
 
 
