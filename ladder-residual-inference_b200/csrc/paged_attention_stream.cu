@@ -1,10 +1,12 @@
-// Paged decode attention as a stream of cache rows on the tensor cores.
+// Paged decode attention as streams of cache rows on the tensor cores.
 //
-// The work is cut into units of 32 or 64 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head; every CTA adds up
-// the sequences' units and takes an equal contiguous run of all of them, so that sequences of any lengths keep all SMs busy from the
-// first microsecond to the last.  One warp fetches (TMA, boxes that lie within a page, a ring of K and V tiles), four warps compute, two to a
-// unit.  A pair that lies in one CTA's run is finished there; the parts of one that several CTAs share go through the workspace and the last of
-// these CTAs to arrive joins them in their order, so that results are the same bits every time.
+// The work is cut into units of 16 or 32 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head; every CTA (one an
+// SM) adds up the sequences' units and takes an equal contiguous run of all of them, and so does each of its warps, so that sequences of any
+// lengths keep all SMs busy from the first microsecond to the last.  A warp is on its own: it fetches the units of its run by TMA (boxes that
+// lie within a page) into a ring of its own, a tile of keys or of values each as soon as the one before in its place has been read, and multiplies
+// them; a pair that lies in its run is finished and stored without a word to the others.  Where a run begins or ends inside a pair the
+// warps' parts are joined through shared memory when all have come to their ends, and those of several CTAs through the workspace by the last
+// of these CTAs to arrive, in their order, so that results are the same bits every time.
 //
 // Products are m16n8k16 with positions, then elements of a value, as the 16 rows and the query heads that share a KV head as the 8 columns (two
 // blocks of columns for 9 to 16 heads): S^T = K Q^T, O^T += V^T P^T; P^T goes from the first product's layout to the second's by a matrix transpose
@@ -29,20 +31,19 @@ using namespace tc;
 
 __device__ int g_paged_attn_status = 0;
 
-constexpr int kWarps = 4;                    // that compute
-constexpr int kThreads = (kWarps + 1) * 32;  // and one that fetches
-constexpr int kPairWarps = 2;                // warps that share a unit, a team
-constexpr int kTeams = kWarps / kPairWarps;
-constexpr int kMaxGroup = 16;    // query heads that share a pass over the cache
-constexpr int kMaxSeqs = 1024;   // of a launch
-constexpr int kMinRun = 2;       // units: a CTA without as many is not worth its part in the join
-constexpr int kMaxPerSm = 3;
-constexpr size_t kCounterBytes = 4096;
+constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
+constexpr int kMaxSeqs = 1024;  // of a launch
+constexpr int kMinRun = 4;      // units: a CTA without as many is not worth its part in the join
+constexpr int kMaxStages = 8;
+constexpr int kSmemBytes = 227 * 1024, kStaticBytes = 2048;  // of an SM, of those what the kernel declares
+constexpr int kMaxCtas = 256;
+constexpr size_t kCounterBytes = kMaxCtas * 4;
 
 struct StreamParams {
   PagedAttnParams a;
   int group, tile_heads, head_tiles;  // query heads of a KV head, of a pass, passes
   int box;                            // positions of a TMA box
+  int stages;                         // of a warp's ring: a tile of keys or of values each
   unsigned int* counters;             // [CTAs]
   float* part_ml;                     // [CTAs][2][tile_heads][2]
   float* part_o;                      // [CTAs][2][tile_heads][HD]
@@ -51,19 +52,14 @@ struct StreamParams {
 // NT: blocks of eight query heads
 template <typename C, int HD, int NT>
 struct Shape {
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kRow = HD * static_cast<int>(sizeof(C));
   static constexpr int kChunkRow = kRow < 128 ? kRow : 128;  // bytes of a row that a box holds: the swizzle's span
   static constexpr int kChunks = kRow / kChunkRow;
-  static constexpr int kUnit = kRow > 128 ? 32 : 64;
-  static constexpr int kTile = kUnit / kPairWarps;  // positions of a warp's products
+  static constexpr int kUnit = kRow > 128 ? 16 : 32;
   static constexpr uint32_t kChunkBytes = kUnit * kChunkRow;
-  static constexpr uint32_t kHalf = kChunks * kChunkBytes;
-  static constexpr int kPerSm = NT == 1 ? 3 : 2;
-  static constexpr int kRingBytes = NT == 1 ? 48 * 1024 : 64 * 1024;
-  static constexpr uint32_t kStages = kRingBytes / kHalf;  // a tile of K or of V each
-  // Each team has stages of its own, or else a warp that is ahead by a round would take the other team's phase of a barrier for its own.
-  static constexpr uint32_t kTeamStages = kStages / kTeams;
-  static_assert(kStages % kTeams == 0 && kTeamStages >= 2, "a unit takes two stages");
+  static constexpr uint32_t kHalf = kChunks * kChunkBytes;  // a tile of keys or of values
   // 16-byte piece c of row r within a tile: its place in the swizzled box
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     if (kChunkRow == 128) return (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -71,7 +67,6 @@ struct Shape {
   }
 };
 
-__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 __device__ __forceinline__ void load_matrix(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -117,8 +112,16 @@ __device__ __forceinline__ void codes_to_halves(uint32_t v, uint32_t& lo, uint32
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
 
+// codes as halves times 2^-8, in the order (0, 2), (1, 3), by integer operations: the four bits of the exponent and the three of the mantissa move
+// into a half's fields as they are, subnormal numbers too.  Conversions run at a sixteenth of the issue rate: keys take them, values this,
+// 95 -> 70 us for 100 sequences of 300 to 6000 positions.  (The two codes of NaN count as +-480; lri_rope_paged_store writes none.)
+__device__ __forceinline__ void codes_to_halves_256th(uint32_t v, uint32_t& even, uint32_t& odd) {
+  even = ((v << 7) & 0x3f803f80u) | ((v << 8) & 0x80008000u);
+  odd = ((v >> 1) & 0x3f803f80u) | (v & 0x80008000u);
+}
+
 template <typename T, typename C, int HD, int NT>
-__global__ void __launch_bounds__(kThreads, (Shape<C, HD, NT>::kPerSm))
+__global__ void __launch_bounds__((Shape<C, HD, NT>::kThreads), 1)
 paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const StreamParams p) {
   using S = Shape<C, HD, NT>;
   constexpr bool kEight = sizeof(C) == 1;
@@ -127,37 +130,45 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   // The reference of a head's scores moves when one exceeds it by kSlack (powers of two), that of the values' scales when one is four times as
   // large.  Probabilities in halves are taken 2^kLift times as large, and the sums with them: up to 2^15, and with all digits down to 2^-23.
   constexpr float kSlack = 4.f, kLift = std::is_same<M, __half>::value ? 9.f : 0.f;
-  constexpr int KB = HD / 16, UNIT = S::kUnit, TILE = S::kTile, RB = TILE / 16;
+  constexpr int W = S::kWarps, KB = HD / 16, UNIT = S::kUnit, RB = UNIT / 16;
+  constexpr uint32_t kAll = UNIT == 32 ? 0xffffffffu : 0xffffu;
 
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* tail = smem_raw + (ring - smem_u32(smem_raw)) + S::kRingBytes;
-  float* sm_scale = reinterpret_cast<float*>(tail);                                                    // [stages][UNIT], e4m3
-  float* sm_o = sm_scale + (kEight ? S::kStages * UNIT : 0);                                           // [warps][tile_heads][HD]
-  int* before = reinterpret_cast<int*>(sm_o + kWarps * p.tile_heads * HD);                             // [n_seq + 1] units before a sequence
-  int* contexts = before + p.a.table.n_seq + 1;                                                        // [n_seq]
-  __shared__ uint64_t bars[2 * S::kStages];
-  __shared__ uint32_t stage_boxes[S::kStages];  // bit i: box i of the unit whose keys are in this stage has a page
-  __shared__ float sm_m[kWarps][kMaxGroup], sm_l[kWarps][kMaxGroup];
+  const int heads = p.tile_heads;
+  const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u, ring_bytes = p.stages * S::kHalf;
+  uint8_t* rings = smem_raw + (ring0 - smem_u32(smem_raw));                          // [W][stages][kHalf]
+  float* scales = reinterpret_cast<float*>(rings + W * ring_bytes);                  // [W][stages][UNIT], e4m3
+  float* firsts = scales + (kEight ? W * p.stages * UNIT : 0);                       // [W][heads][HD]: parts of pairs that runs begin in
+  float* part_ml = firsts + W * heads * HD;                                          // [2 W][heads][2]
+  int* before = reinterpret_cast<int*>(part_ml + 2 * W * heads * 2);                 // [n_seq + 1]: units before a sequence
+  int* contexts = before + p.a.table.n_seq + 1;                                      // [n_seq]
+  __shared__ uint64_t bars[W][kMaxStages];
+  __shared__ uint32_t stage_boxes[W][kMaxStages];  // bit i: box i of the unit whose keys are in this stage has a page
+  // The warps' parts of pairs, in order: part 2 w of the pair that warp w's run begins in, 2 w + 1 of the one it ends in.
+  struct Part {
+    int first, end;            // units of the pair, first -1: no part
+    int from, to;              // units of the part
+    int row, g;                // the pair's row of results, heads
+  };
+  __shared__ Part parts[2 * W];
+  __shared__ int group_at[2 * W + 1], groups;  // parts of the same pair follow one another
+  __shared__ unsigned int tickets[2];
   __shared__ int abort_flag;
-  __shared__ unsigned int ticket;
 
   const PageTable& table = p.a.table;
   const int n_seq = table.n_seq;
   const int pairs = p.a.n_kv * p.head_tiles;  // of a sequence
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
-  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[S::kStages]);
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (uint32_t s = 0; s < S::kStages; ++s) {
-      mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, kPairWarps);
-    }
+  const uint32_t full0 = smem_u32(&bars[warp][0]);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(full0 + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    parts[2 * warp].first = parts[2 * warp + 1].first = -1;
   }
-  if (warp == kWarps && elect_one()) {
+  if (warp == W - 1 && elect_one()) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_v) : "memory");
   }
@@ -165,7 +176,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   pdl_wait();  // q, positions, the table and the newest cache rows come from preceding kernels
 
   // ---- units of all sequences, and before each ------------------------------------------------------------------------------------
-  for (int b = threadIdx.x; b < n_seq; b += kThreads) {
+  for (int b = threadIdx.x; b < n_seq; b += S::kThreads) {
     int64_t ctx = load_pos(p.a.input_pos, p.a.pos_is_i64, b);
     ctx = ctx < 0 ? 0 : (ctx >= table.capacity() ? table.capacity() : ctx + 1);
     contexts[b] = static_cast<int>(ctx);
@@ -191,16 +202,23 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   const int64_t units = before[n_seq];
   const int64_t ctas = units < static_cast<int64_t>(gridDim.x) * kMinRun ? (units + kMinRun - 1) / kMinRun : gridDim.x;  // that have a run
   const int64_t me = blockIdx.x;
-  const int u0 = static_cast<int>(me < ctas ? units * me / ctas : units), u1 = static_cast<int>(me < ctas ? units * (me + 1) / ctas : units);
+  const int cta0 = static_cast<int>(me < ctas ? units * me / ctas : units), cta1 = static_cast<int>(me < ctas ? units * (me + 1) / ctas : units);
+  const int u0 = cta0 + (cta1 - cta0) * warp / W, u1 = cta0 + (cta1 - cta0) * (warp + 1) / W;  // this warp's run
 
   // sequences without a visible position
   for (int b = blockIdx.x; b < n_seq; b += gridDim.x)
     if (before[b] == before[b + 1]) {
       T* dst = static_cast<T*>(p.a.out) + static_cast<int64_t>(b) * p.a.n_head * p.a.dim;
-      for (int i = threadIdx.x; i < p.a.n_head * (p.a.dim >> 3); i += kThreads) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < p.a.n_head * (p.a.dim >> 3); i += S::kThreads) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
     }
 
-  if (warp == kWarps) {
+  // results of a pair are stored as they come: elements e .. of head i
+  auto row_of = [&](int row, int i) { return static_cast<T*>(p.a.out) + (static_cast<int64_t>(row) + i) * p.a.dim; };
+
+  if (u0 < u1) {
+    const uint32_t ring = ring0 + warp * ring_bytes;
+    float* my_scales = scales + warp * p.stages * UNIT;
+
     // ---- fetch: a lane looks up the page of one box, 32 boxes at a time and 32 ahead ------------------------------------------------
     const int boxes = UNIT / p.box, ahead = 32 / boxes;  // of a unit; units that 32 lanes look up
     auto look_up = [&](int u, int& slab, int& row) {     // box (lane % boxes) of unit u: slab -1 where there is nothing to fetch
@@ -214,53 +232,43 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int64_t page = table.find(b, pos);
       if (page >= 0) slab = static_cast<int>(page * p.a.n_kv + pair / p.head_tiles), row = pos % table.page;
     };
-    uint32_t s[kTeams], parity[kTeams];  // of each team's next stage; a fresh barrier passes a wait on parity 1
-#pragma unroll
-    for (int t = 0; t < kTeams; ++t) s[t] = 0, parity[t] = 1;
+    int f_unit = u0, f_base = u0, f_stage = 0, f_half = 0;  // what is fetched next; the first unit that the lanes have looked up
     int slab, row, next_slab, next_row;
     look_up(u0 + lane / boxes, slab, row);
-    bool ok = true;
-    for (int base = u0; base < u1 && ok; base += ahead) {
-      look_up(base + ahead + lane / boxes, next_slab, next_row);
-      const uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
-      const int n = u1 - base < ahead ? u1 - base : ahead;
-      for (int i0 = 0; i0 < n && ok; i0 += kTeams)  // (`ahead` is a multiple of the teams)
+    look_up(u0 + ahead + lane / boxes, next_slab, next_row);
+    uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
+    auto fetch = [&]() {  // behind a __syncwarp(): the stage has been read
+      if (f_unit >= u1) return;
+      const int i = f_unit - f_base;
+      const uint32_t mine = (have >> (i * boxes)) & ((1u << boxes) - 1u), full = full0 + 8 * f_stage;
+      if (lane == 0) {
+        if (f_half == 0) stage_boxes[warp][f_stage] = mine;
+        mbar_expect_tx(full, __popc(mine) * p.box * (S::kRow + (kEight ? 4 : 0)));
+      }
+      __syncwarp();
+      if (lane / boxes == i && slab >= 0) {
+        const int at = (lane % boxes) * p.box;
+        const CUtensorMap* map = f_half ? &tmap_v : &tmap_k;
 #pragma unroll
-        for (int t = 0; t < kTeams; ++t) {
-          const int i = i0 + t;
-          if (i >= n || !ok) break;
-          const uint32_t mine = (have >> (i * boxes)) & ((1u << boxes) - 1u);
-          const uint32_t count = __popc(mine);
-#pragma unroll
-          for (int half = 0; half < 2 && ok; ++half) {
-            const uint32_t st = t * S::kTeamStages + s[t], full = full0 + 8 * st;
-            ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * st, parity[t], &abort_flag, 41, &g_paged_attn_status));
-            if (!ok) break;
-            if (lane == 0) {
-              if (half == 0) stage_boxes[st] = mine;
-              mbar_expect_tx(full, count * p.box * (S::kRow + (kEight ? 4 : 0)));
-            }
-            __syncwarp();
-            if (lane / boxes == i && slab >= 0) {
-              const int at = (lane % boxes) * p.box;
-#pragma unroll
-              for (int c = 0; c < S::kChunks; ++c)
-                tma_load_3d(ring + st * S::kHalf + c * S::kChunkBytes + at * S::kChunkRow, half ? &tmap_v : &tmap_k, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
-              if (kEight) bulk_load(smem_u32(sm_scale + st * UNIT + at), (half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(slab) * table.page + row, p.box * 4, full);
-            }
-            __syncwarp();
-            if (++s[t] == S::kTeamStages) s[t] = 0, parity[t] ^= 1u;
-          }
-        }
-      slab = next_slab, row = next_row;
-    }
-  } else if (u0 < u1) {
+        for (int c = 0; c < S::kChunks; ++c)
+          tma_load_3d(ring + f_stage * S::kHalf + c * S::kChunkBytes + at * S::kChunkRow, map, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
+        if (kEight) bulk_load(smem_u32(my_scales + f_stage * UNIT + at), (f_half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(slab) * table.page + row, p.box * 4, full);
+      }
+      if (++f_stage == p.stages) f_stage = 0;
+      f_half ^= 1;
+      if (f_half == 0 && ++f_unit - f_base == ahead) {
+        f_base = f_unit;
+        slab = next_slab, row = next_row;
+        have = __ballot_sync(0xffffffffu, slab >= 0);
+        look_up(f_base + ahead + lane / boxes, next_slab, next_row);
+      }
+    };
+    for (int i = 0; i < p.stages; ++i) fetch();
+
     const int quad = lane >> 2, col = (lane & 3) * 2;  // a thread holds scores of positions quad, quad + 8, .. and heads col, col + 1
-    const int sub = warp % kPairWarps, team = warp / kPairWarps;
-    uint32_t s = team * S::kTeamStages, parity = 0;  // the stage whose turn it is: of keys, then of values
-    const uint32_t s_end = s + S::kTeamStages;
+    int s = 0;  // the stage whose turn it is: of keys, then of values
+    uint32_t parity = 0;
     bool ok = true;
-    int next = u0 + team;  // this team's next unit
     int b = sequence_of(before, n_seq, u0);
     for (int u = u0; u < u1;) {
       while (before[b + 1] <= u) ++b;
@@ -269,8 +277,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int first = before[b] + pair * sp.tiles;
       const int end = first + sp.tiles < u1 ? first + sp.tiles : u1;
       const int h = pair / p.head_tiles, ht = pair - h * p.head_tiles;
-      const int head0 = h * p.group + ht * p.tile_heads;
-      const int g = p.group - ht * p.tile_heads < p.tile_heads ? p.group - ht * p.tile_heads : p.tile_heads;
+      const int head0 = h * p.group + ht * heads;
+      const int g = p.group - ht * heads < heads ? p.group - ht * heads : heads;
+      const int out_row = b * p.a.n_head + head0;
 
       // ---- Q^T: head i of the pass is column i; columns from g up are zero -----------------------------------------------------------
       uint32_t qb[NT][KB][2];
@@ -278,7 +287,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int i = n * 8 + quad;
-        const T* qg = static_cast<const T*>(p.a.q) + (static_cast<int64_t>(b) * p.a.n_head + head0 + i) * p.a.dim;
+        const T* qg = static_cast<const T*>(p.a.q) + (static_cast<int64_t>(out_row) + i) * p.a.dim;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -325,33 +334,32 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
         m_run[n][0] = m_run[n][1] = -INFINITY, l_run[n][0] = l_run[n][1] = 0.f;
       }
-      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of v_top
+      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of v_top / 256
 
-      auto arrived = [&]() {
-        return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 42, &g_paged_attn_status)) != 0;
-      };
+      auto arrived = [&]() { return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 42, &g_paged_attn_status)) != 0; };
       auto give_back = [&]() {
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty0 + 8 * s);
-        if (++s == s_end) s -= S::kTeamStages, parity ^= 1u;
+        fetch();
+        if (++s == p.stages) s = 0, parity ^= 1u;
       };
-      for (; next < end && ok; next += kTeams) {
+      for (int unit = u; unit < end && ok; ++unit) {
         ok = arrived();
         if (!ok) break;
         // ---- which of the positions are visible --------------------------------------------------------------------------------------
-        const int p0 = (sp.first + next - first) * UNIT + sub * TILE;
-        const uint32_t has = stage_boxes[s];
-        uint32_t vis = 0u;
-#pragma unroll
-        for (int i = 0; i < TILE / 8; ++i) vis |= (has >> ((sub * TILE + i * 8) / p.box)) & 1u ? 0xffu << (i * 8) : 0u;
-        if (p0 + TILE > sp.ctx) vis &= p0 < sp.ctx ? (1u << (sp.ctx - p0)) - 1u : 0u;
-        if (p0 < sp.lo) vis &= sp.lo - p0 < TILE ? ~((1u << (sp.lo - p0)) - 1u) : 0u;
-        constexpr uint32_t kAll = TILE == 32 ? 0xffffffffu : (1u << (TILE & 31)) - 1u;
-        // ---- scores: TILE positions x 8 NT heads ----------------------------------------------------------------------------------------
+        const int p0 = (sp.first + unit - first) * UNIT;
+        const uint32_t has = stage_boxes[warp][s];
+        uint32_t vis = kAll;
+        if (has != (1u << boxes) - 1u) {
+          vis = 0u;
+          for (int i = 0; i < boxes; ++i) vis |= (has >> i) & 1u ? (0xffffffffu >> (32 - p.box)) << (i * p.box) : 0u;
+        }
+        if (p0 + UNIT > sp.ctx) vis &= p0 < sp.ctx ? (1u << (sp.ctx - p0)) - 1u : 0u;
+        if (p0 < sp.lo) vis &= sp.lo - p0 < UNIT ? ~((1u << (sp.lo - p0)) - 1u) : 0u;
+        // ---- scores: UNIT positions x 8 NT heads ----------------------------------------------------------------------------------------
         float sc[RB][NT][4];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-          const int row = sub * TILE + rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+          const int r = rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
           const uint32_t at = ring + s * S::kHalf;
           float part[2][NT][4];  // two chains
 #pragma unroll
@@ -362,7 +370,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
             for (int kb = 0; kb < KB; kb += 2) {
               uint32_t bf[4], a[2][4];
-              load_matrix(at + S::at(row, kb + (lane >> 4)), bf);
+              load_matrix(at + S::at(r, kb + (lane >> 4)), bf);
 #pragma unroll
               for (int i = 0; i < 4; ++i) codes_to_halves(bf[i], a[i >> 1][i & 1], a[i >> 1][2 + (i & 1)]);
 #pragma unroll
@@ -374,7 +382,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
               uint32_t a[4];
-              load_matrix(at + S::at(row, kb * 2 + (lane >> 4)), a);
+              load_matrix(at + S::at(r, kb * 2 + (lane >> 4)), a);
 #pragma unroll
               for (int n = 0; n < NT; ++n) mma16816<M>(part[kb & 1][n], a[0], a[1], a[2], a[3], qb[n][kb][0], qb[n][kb][1]);
             }
@@ -384,7 +392,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[rb][n][e] = part[0][n][e] + part[1][n][e];
           if constexpr (kEight) {
-            const float* sk = sm_scale + s * UNIT + sub * TILE + rb * 16 + quad;
+            const float* sk = my_scales + s * UNIT + rb * 16 + quad;
             const float ks[2] = {sk[0], sk[8]};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -427,7 +435,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              vs[rb][i] = sm_scale[s * UNIT + sub * TILE + rb * 16 + i * 8 + quad];
+              vs[rb][i] = my_scales[s * UNIT + rb * 16 + i * 8 + quad];
               if (vis != kAll && !((vis >> (rb * 16 + i * 8 + quad)) & 1u)) vs[rb][i] = 0.f;
               top = fmaxf(top, fabsf(vs[rb][i]));
             }
@@ -481,9 +489,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         const uint32_t sv = ring + s * S::kHalf;
         if (vis != kAll) {
           // values that are not visible may be anything, and 0 x NaN is not 0
-          for (int i = lane; i < TILE * (S::kRow / 16); i += 32) {
+          for (int i = lane; i < UNIT * (S::kRow / 16); i += 32) {
             const int r = i / (S::kRow / 16), c = i % (S::kRow / 16);
-            if (!((vis >> r) & 1u)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(sub * TILE + r, c)), "r"(0u) : "memory");
+            if (!((vis >> r) & 1u)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(r, c)), "r"(0u) : "memory");
           }
           __syncwarp();
         }
@@ -491,24 +499,24 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           if constexpr (kEight) {
-            const int row = sub * TILE + rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+            const int r = rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
             for (int kb = 0; kb < KB; kb += 2) {  // rows of a product: the block's even elements, then its odd ones
               uint32_t bf[4], a[2][4];
-              load_matrix_trans(sv + S::at(row, kb + (lane >> 4)), bf);
+              load_matrix_trans(sv + S::at(r, kb + (lane >> 4)), bf);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) codes_to_halves(__byte_perm(bf[i], 0u, 0x3120), a[i >> 1][(i & 1) * 2], a[i >> 1][(i & 1) * 2 + 1]);
+              for (int i = 0; i < 4; ++i) codes_to_halves_256th(bf[i], a[i >> 1][(i & 1) * 2], a[i >> 1][(i & 1) * 2 + 1]);
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma16816<M>(o[n][kb + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[rb][n][0], pb[rb][n][1]);
             }
           } else {
-            const int row = sub * TILE + rb * 16 + (lane & 7) + (lane >> 4) * 8;
+            const int r = rb * 16 + (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
               uint32_t a[4];
-              load_matrix_trans(sv + S::at(row, kb * 2 + ((lane >> 3) & 1)), a);
+              load_matrix_trans(sv + S::at(r, kb * 2 + ((lane >> 3) & 1)), a);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<M>(o[n][kb], a[0], a[1], a[2], a[3], pb[rb][n][0], pb[rb][n][1]);
@@ -521,112 +529,172 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         give_back();
       }
 
-      // ---- join the warps --------------------------------------------------------------------------------------------------------------
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], w);
-      warps_sync();  // the arrays' previous contents have been read
+      // ---- the end of a pair, or of the run -------------------------------------------------------------------------------------------------
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int i = n * 8 + col + c;
-          if (i < g) {
-            if (quad == 0) sm_m[warp][i] = m_run[n][c] - kLift, sm_l[warp][i] = l_run[n][c];
-            float* d = sm_o + (warp * p.tile_heads + i) * HD;
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-              if constexpr (kEight) {
-                *reinterpret_cast<float2*>(d + k * 16 + quad * 2) = make_float2(o[n][k][c] * v_top, o[n][k][2 + c] * v_top);
-              } else {
-                d[k * 16 + quad] = o[n][k][c], d[k * 16 + quad + 8] = o[n][k][2 + c];
+          for (int w = 4; w < 32; w <<= 1) l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], w);
+        }
+      const float unit_o = kEight ? v_top * 256.f : 1.f;
+      if (u == first && end == first + sp.tiles) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          // nothing visible: zeros; a NaN stays one
+          const float f0 = l_run[n][0] == 0.f ? 0.f : unit_o / l_run[n][0], f1 = l_run[n][1] == 0.f ? 0.f : unit_o / l_run[n][1];
+          const int i = n * 8 + quad;
+          T* dst = row_of(out_row, i);
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            // transposed, a thread has elements of one head: (col, col + 1) and (col + 8, ..), e4m3 (2 col, 2 col + 2) and (2 col + 1, ..)
+            const uint32_t x = transposed(pack2<T>(o[n][k][0] * f0, o[n][k][1] * f1)), y = transposed(pack2<T>(o[n][k][2] * f0, o[n][k][3] * f1));
+            if constexpr (kEight) {
+              const int e = k * 16 + 2 * col;
+              if (i < g && e < p.a.dim) *reinterpret_cast<uint2*>(dst + e) = make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+            } else {
+              const int e = k * 16 + col;
+              if (i < g && e < p.a.dim) *reinterpret_cast<uint32_t*>(dst + e) = x;
+              if (i < g && e + 8 < p.a.dim) *reinterpret_cast<uint32_t*>(dst + e + 8) = y;
+            }
+          }
+        }
+      } else {
+        // a part: the first of the run beside the rings, the last in the warp's ring, which has been read
+        const int which = 2 * warp + (u == u0 ? 0 : 1);
+        float* d0 = u == u0 ? firsts + warp * heads * HD : reinterpret_cast<float*>(rings + warp * ring_bytes);
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int i = n * 8 + col + c;
+            if (i < g) {
+              if (quad == 0) *reinterpret_cast<float2*>(part_ml + (which * heads + i) * 2) = make_float2(m_run[n][c] - kLift, l_run[n][c]);
+              float* d = d0 + i * HD;
+#pragma unroll
+              for (int k = 0; k < KB; ++k) {
+                if constexpr (kEight) {
+                  *reinterpret_cast<float2*>(d + k * 16 + quad * 2) = make_float2(o[n][k][c] * unit_o, o[n][k][2 + c] * unit_o);
+                } else {
+                  d[k * 16 + quad] = o[n][k][c], d[k * 16 + quad + 8] = o[n][k][2 + c];
+                }
               }
             }
           }
-        }
-      warps_sync();
-      // result of elements e, e + 1 of head i of the pass
-      auto store = [&](int i, int e, float l, float2 v) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing visible: zeros; a NaN stays one
-        if (e < p.a.dim)
-          *reinterpret_cast<uint32_t*>(static_cast<T*>(p.a.out) + (static_cast<int64_t>(b) * p.a.n_head + head0 + i) * p.a.dim + e) = pack2<T>(v.x * inv, v.y * inv);
-      };
-      // the CTAs that share this pair: CTA c has units units * c / ctas ..
-      const bool whole = u == first && end == first + sp.tiles;
-      const int64_t c_first = whole ? me : (static_cast<int64_t>(first + 1) * ctas - 1) / units;
-      const int64_t c_last = whole ? me : (static_cast<int64_t>(first + sp.tiles) * ctas - 1) / units;
-      // a CTA leaves at most two parts: of the pair its run begins in, and of the one it ends in
-      auto part_of = [&](int64_t c) { return (c * 2 + (c == c_first && units * c / ctas != first ? 1 : 0)) * p.tile_heads; };
-      const int64_t mine = part_of(me);
-      for (int idx = threadIdx.x; idx < g * (HD / 2); idx += kWarps * 32) {
-        const int i = idx / (HD / 2), e = idx % (HD / 2) * 2;
-        float mm = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w][i]);
-        const float m_use = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f;
-        float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float wt = exp2f(sm_m[w][i] - m_use);  // 0 for warps that saw no position
-          const float2 ow = *reinterpret_cast<const float2*>(sm_o + (w * p.tile_heads + i) * HD + e);
-          ll += sm_l[w][i] * wt;
-          v.x += ow.x * wt, v.y += ow.y * wt;
-        }
-        if (whole) {
-          store(i, e, ll, v);
-        } else {
-          *reinterpret_cast<float2*>(p.part_o + (mine + i) * HD + e) = v;
-          if (e == 0) *reinterpret_cast<float2*>(p.part_ml + (mine + i) * 2) = make_float2(mm, ll);
-        }
-      }
-      if (!whole) {
-        // ---- the last CTA of this pair joins the parts ---------------------------------------------------------------------------------
-        warps_sync();
-        if (threadIdx.x == 0) {
-          unsigned int there;  // the barrier orders the other threads' stores before this release, and their loads behind it
-          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(there) : "l"(p.counters + c_first) : "memory");
-          ticket = there;
-        }
-        warps_sync();
-        if (ticket == static_cast<unsigned int>(c_last - c_first)) {
-          const int parts = static_cast<int>(c_last - c_first) + 1;
-          const int64_t p_first = part_of(c_first), p_rest = 2 * c_first * p.tile_heads;  // part k > 0 is the first of CTA c_first + k
-          for (int idx = threadIdx.x; idx < g * (HD / 4); idx += kWarps * 32) {
-            const int i = idx / (HD / 4), e = idx % (HD / 4) * 4;
-            // all maxima first: then no load waits for another
-            float mm = -INFINITY;
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) mm = fmaxf(mm, __ldcg(p.part_ml + ((k ? p_rest + 2 * k * p.tile_heads : p_first) + i) * 2));
-            const float m_use = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f, v[4] = {};
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) {
-              const int64_t at = (k ? p_rest + 2 * k * p.tile_heads : p_first) + i;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-              const float4 w = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + e));
-              const float f = exp2f(ml.x - m_use);
-              ll += ml.y * f;
-              v[0] += w.x * f, v[1] += w.y * f, v[2] += w.z * f, v[3] += w.w * f;
-            }
-            store(i, e, ll, make_float2(v[0], v[1]));
-            store(i, e + 2, ll, make_float2(v[2], v[3]));
-          }
-          if (threadIdx.x == 0) p.counters[c_first] = 0u;  // ready for the next call
-        }
+        if (lane == 0) parts[which] = Part{first, first + sp.tiles, u, end, out_row, g};
       }
       u = end;
     }
   }
   __syncthreads();
-  if (abort_flag && threadIdx.x == 0) {
-    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
+
+  // ---- the CTA's parts of a pair become one: a result, or a part in the workspace -------------------------------------------------------------
+  if (warp == 0) {
+    const int mine = lane < 2 * W ? parts[lane].first : -1;
+    const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0);
+    const uint32_t lower = there & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, mine, lower ? 31 - __clz(lower) : 0);
+    const bool starts = mine >= 0 && (!lower || prev != mine);
+    const uint32_t start = __ballot_sync(0xffffffffu, starts);
+    if (starts) group_at[__popc(start & ((1u << lane) - 1u))] = lane;
+    if (lane == 0) groups = __popc(start), group_at[__popc(start)] = 2 * W;
   }
   __syncthreads();
+  // element e .. e + 3 of a head's result from its sum
+  auto store4 = [&](int row, int i, int e, float l, const float (&v)[4]) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (e < p.a.dim) *reinterpret_cast<uint2*>(row_of(row, i) + e) = make_uint2(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv));
+  };
+  for (int idx = threadIdx.x; idx < groups * heads * (HD / 4); idx += S::kThreads) {
+    const int k = idx / (heads * (HD / 4)), rest = idx - k * (heads * (HD / 4)), i = rest / (HD / 4), e = rest % (HD / 4) * 4;
+    const int a0 = group_at[k], a1 = group_at[k + 1];
+    const Part& head = parts[a0];
+    if (i >= head.g) continue;
+    float mm = -INFINITY;
+    int last = a0;
+    for (int a = a0; a < a1; ++a)
+      if (parts[a].first >= 0) mm = fmaxf(mm, part_ml[(a * heads + i) * 2]), last = a;
+    const float m_use = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f, v[4] = {};
+    for (int a = a0; a < a1; ++a)
+      if (parts[a].first >= 0) {
+        const float f = exp2f(part_ml[(a * heads + i) * 2] - m_use);
+        const float4 x = *reinterpret_cast<const float4*>((a & 1 ? reinterpret_cast<const float*>(rings + (a >> 1) * ring_bytes) : firsts + (a >> 1) * heads * HD) + i * HD + e);
+        ll += part_ml[(a * heads + i) * 2 + 1] * f;
+        v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
+      }
+    if (head.from == head.first && parts[last].to == head.end) {
+      store4(head.row, i, e, ll, v);
+    } else {
+      // a CTA leaves at most two parts: of the pair its run begins in, and of the one it ends in
+      const int64_t at = (me * 2 + (head.from == cta0 ? 0 : 1)) * heads + i;
+      *reinterpret_cast<float4*>(p.part_o + at * HD + e) = make_float4(v[0], v[1], v[2], v[3]);
+      if (e == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, ll);
+    }
+  }
+  // The CTAs that share a pair: CTA c has units units * c / ctas ..; the last of them to arrive joins their parts.
+  int shared_from[2], shared_to[2];  // of the first and of the last pair of this CTA, from -1: not shared
+  Part pair_of[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    shared_from[k] = shared_to[k] = -1;
+    if (groups == 0 || (k == 1 && groups == 1)) continue;
+    pair_of[k] = parts[group_at[k == 0 ? 0 : groups - 1]];
+    if (pair_of[k].first < cta0 || pair_of[k].end > cta1) {
+      shared_from[k] = static_cast<int>((static_cast<int64_t>(pair_of[k].first + 1) * ctas - 1) / units);
+      shared_to[k] = static_cast<int>((static_cast<int64_t>(pair_of[k].end) * ctas - 1) / units);
+    }
+  }
+  if (shared_from[0] >= 0 || shared_from[1] >= 0) {
+    __syncthreads();
+    if (threadIdx.x < 2 && (threadIdx.x ? shared_from[1] : shared_from[0]) >= 0) {
+      unsigned int there;  // the barrier orders the other threads' stores before this release, and their loads behind it
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(there) : "l"(p.counters + (threadIdx.x ? shared_from[1] : shared_from[0])) : "memory");
+      tickets[threadIdx.x] = there;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int n = shared_to[k] - shared_from[k] + 1;
+      if (shared_from[k] < 0 || tickets[k] != static_cast<unsigned int>(n - 1)) continue;
+      const int g = pair_of[k].g;
+      // part 0 is the last of its CTA unless that begins with the pair; part i > 0 the first of its CTA
+      const int64_t at0 = static_cast<int64_t>(shared_from[k]) * 2 * heads;
+      const int64_t at_first = at0 + (units * shared_from[k] / ctas != pair_of[k].first ? heads : 0);
+      float2* ml = reinterpret_cast<float2*>(rings);  // [n][g]
+      __syncthreads();
+      for (int i = threadIdx.x; i < n * g; i += S::kThreads) {
+        const int c = i / g;
+        ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((c ? at0 + static_cast<int64_t>(c) * 2 * heads : at_first) + i % g) * 2));
+      }
+      __syncthreads();
+      for (int idx = threadIdx.x; idx < g * (HD / 4); idx += S::kThreads) {
+        const int i = idx / (HD / 4), e = idx % (HD / 4) * 4;
+        float mm = -INFINITY;
+        for (int c = 0; c < n; ++c) mm = fmaxf(mm, ml[c * g + i].x);
+        const float m_use = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, v[4] = {};
+#pragma unroll 10
+        for (int c = 0; c < n; ++c) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c ? at0 + static_cast<int64_t>(c) * 2 * heads : at_first) + i) * HD + e));
+          const float f = exp2f(ml[c * g + i].x - m_use);
+          ll += ml[c * g + i].y * f;
+          v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
+        }
+        store4(pair_of[k].row, i, e, ll, v);
+      }
+      if (threadIdx.x == 0) p.counters[shared_from[k]] = 0u;  // ready for the next call
+    }
+  }
+  if (abort_flag) {
+    if (threadIdx.x == 0)
+      for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
+    __syncthreads();
+  }
 }
+
+int max_ctas() { return device_sm_count() < kMaxCtas ? device_sm_count() : kMaxCtas; }
 
 int tile_heads_of(int group) {
   const int tiles = (group + kMaxGroup - 1) / kMaxGroup;
@@ -652,9 +720,8 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   LRI_REQUIRE(per >= 1, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %lld positions of %d heads", (long long)t.capacity(), p.a.n_kv);
   per = per < kMaxSeqs ? per : kMaxSeqs;
   auto kern = paged_attn_stream_kernel<T, C, HD, NT>;
-  const int fixed = 1024 + S::kRingBytes + (sizeof(C) == 1 ? S::kStages * S::kUnit * 4 : 0);
   static std::atomic<unsigned long long> attr_set{0};
-  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kWarps * 8 * NT * HD * 4 + (2 * kMaxSeqs + 1) * 4));
+  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes - kStaticBytes));
   const PagedAttnParams all = p.a;
   for (int64_t at = 0; at < all.table.n_seq; at += per) {
     const int n = static_cast<int>(all.table.n_seq - at < per ? all.table.n_seq - at : per);
@@ -663,9 +730,14 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
     p.a.q = static_cast<const T*>(all.q) + at * all.n_head * all.dim;
     p.a.out = static_cast<T*>(all.out) + at * all.n_head * all.dim;
     p.a.input_pos = static_cast<const char*>(all.input_pos) + at * (all.pos_is_i64 ? 8 : 4);
-    const int64_t room = static_cast<int64_t>(S::kPerSm) * device_sm_count(), useful = (most * n + kMinRun - 1) / kMinRun;
-    const int smem = fixed + kWarps * p.tile_heads * HD * 4 + (2 * n + 1) * 4;
-    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(kThreads), smem, st, tk, tv, p));
+    // all that the parts and the sequences leave of shared memory goes to the rings
+    const int fixed = 1024 + S::kWarps * p.tile_heads * (HD * 4 + 2 * 8) + (2 * n + 1) * 4;
+    const int stage = S::kWarps * static_cast<int>(S::kHalf + (sizeof(C) == 1 ? S::kUnit * 4 : 0));
+    const int fits = (kSmemBytes - kStaticBytes - fixed) / stage;
+    p.stages = fits < kMaxStages ? fits : kMaxStages;
+    LRI_REQUIRE(p.stages >= 2, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %d heads of %d with %d sequences", p.tile_heads, HD, n);
+    const int64_t room = max_ctas(), useful = (most * n + kMinRun - 1) / kMinRun;
+    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(S::kThreads), fixed + p.stages * stage, st, tk, tv, p));
     LRI_LAUNCH_CHECK("paged_attn_stream_kernel");
   }
   return LRI_OK;
@@ -689,13 +761,12 @@ bool paged_attn_stream_supports(int cache_dtype, int dim) { return dim <= 128 &&
 
 size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim) {
   const int hd = dim <= 64 ? 64 : 128;
-  return kCounterBytes + static_cast<size_t>(kMaxPerSm) * device_sm_count() * 2 * tile_heads_of(n_head / n_kv) * (hd + 2) * 4;
+  return kCounterBytes + static_cast<size_t>(max_ctas()) * 2 * tile_heads_of(n_head / n_kv) * (hd + 2) * 4;
 }
 
 int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   LRI_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim), LRI_ERR_WORKSPACE,
               "paged_attn_decode: workspace of %zu bytes (16-byte aligned) required", paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim));
-  LRI_REQUIRE(static_cast<size_t>(kMaxPerSm) * device_sm_count() * 4 <= kCounterBytes, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %d multiprocessors", device_sm_count());
   StreamParams p{};
   p.a = a;
   p.group = a.n_head / a.n_kv;
@@ -703,7 +774,7 @@ int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& 
   p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
   p.counters = static_cast<unsigned int*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-  p.part_ml = p.part_o + static_cast<size_t>(kMaxPerSm) * device_sm_count() * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
+  p.part_ml = p.part_o + static_cast<size_t>(max_ctas()) * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
   return dtype == LRI_BF16 ? dispatch<__nv_bfloat16>(cache_dtype, p, st) : dispatch<__half>(cache_dtype, p, st);
 }
 
