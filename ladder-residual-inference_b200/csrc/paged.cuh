@@ -43,8 +43,8 @@ struct PageTable {
   int64_t n_pages;
   __host__ __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(max_pages) * page; }
   // page that holds position pos (0 <= pos < capacity()) of sequence b, -1: none
-  __device__ __forceinline__ int64_t find(int64_t b, int64_t pos) const {
-    const int64_t id = ids[b * ld + pos / page];
+  __device__ __forceinline__ int find(int64_t b, int pos) const {
+    const int id = ids[b * ld + pos / page];
     return id >= 0 && id < n_pages ? id : -1;
   }
 };

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_plain_kernel(const Pag
   if (e < p.dim) load8<T>(static_cast<const T*>(p.q) + at, q);
   for (int64_t j0 = lo + warp * kGroups; j0 < ctx; j0 += kWarps * kGroups) {  // the warp's bounds are the same in every lane
     const int64_t j = j0 + group;
-    const int64_t page = j < ctx ? p.table.find(b, j) : -1;
+    const int64_t page = j < ctx ? p.table.find(b, static_cast<int>(j)) : -1;
     const int64_t row = (page * p.n_kv + h) * p.table.page + j % p.table.page;
     float k[8] = {}, s = 0.f;
     if (page >= 0 && e < p.dim) load_cached8(static_cast<const C*>(p.k) + row * p.dim + e, k);

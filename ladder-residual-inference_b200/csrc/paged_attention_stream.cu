@@ -1,8 +1,9 @@
 // Paged decode attention as streams of cache rows on the tensor cores.
 //
-// The work is cut into units of 16 or 32 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head; every CTA (one an
-// SM) adds up the sequences' units and takes an equal contiguous run of all of them, and so does each of its warps, so that sequences of any
-// lengths keep all SMs busy from the first microsecond to the last.  A warp is on its own: it fetches the units of its run by TMA (boxes that
+// The work is cut into units of 16 or 32 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head.  They lie on a
+// line, kStep apart, with kGap more behind each pair for what its beginning and end cost (1.0 to 1.2 us where a unit takes 2.6).  Every CTA (one an SM)
+// adds up the sequences and takes an equal stretch of the line, and so does each of its warps, so that sequences of any lengths keep
+// all SMs busy from the first microsecond to the last.  A warp is on its own: it fetches the units of its run by TMA (boxes that
 // lie within a page) into a ring of its own, a tile of keys or of values each as soon as the one before in its place has been read, and multiplies
 // them; a pair that lies in its run is finished and stored without a word to the others.  Where a run begins or ends inside a pair the
 // warps' parts are joined through shared memory when all have come to their ends, and those of several CTAs through the workspace by the last
@@ -33,9 +34,10 @@ __device__ int g_paged_attn_status = 0;
 
 constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;  // of a launch
-constexpr int kMinRun = 4;      // units: a CTA without as many is not worth its part in the join
+constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of the line
+constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
 constexpr int kMaxStages = 8;
-constexpr int kSmemBytes = 227 * 1024, kStaticBytes = 2048;  // of an SM, of those what the kernel declares
+constexpr int kSmemBytes = 227 * 1024, kStaticBytes = 3072;  // of an SM, of those what the kernel declares
 constexpr int kMaxCtas = 256;
 constexpr size_t kCounterBytes = kMaxCtas * 4;
 
@@ -91,16 +93,17 @@ __device__ __forceinline__ Span span_of(int ctx, int64_t window) {
   return s;
 }
 
-// the sequence whose units hold unit u: the last b with before[b] <= u among those with units
-__device__ __forceinline__ int sequence_of(const int* before, int n, int u) {
+// the last b with begins[b] <= at, which begins a sequence that has units where `at` is below begins[n]
+__device__ __forceinline__ int sequence_of(const int* begins, int n, int at) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (before[mid] <= u) lo = mid;
+    if (begins[mid] <= at) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
+__device__ __forceinline__ int length_of(int tiles) { return tiles > 0 ? tiles * kStep + kGap : 0; }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 matrix of 16-bit elements
   uint32_t r;
@@ -140,8 +143,11 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   float* scales = reinterpret_cast<float*>(rings + W * ring_bytes);                  // [W][stages][UNIT], e4m3
   float* firsts = scales + (kEight ? W * p.stages * UNIT : 0);                       // [W][heads][HD]: parts of pairs that runs begin in
   float* part_ml = firsts + W * heads * HD;                                          // [2 W][heads][2]
-  int* before = reinterpret_cast<int*>(part_ml + 2 * W * heads * 2);                 // [n_seq + 1]: units before a sequence
-  int* contexts = before + p.a.table.n_seq + 1;                                      // [n_seq]
+  float* part_w = part_ml + 2 * W * heads * 2;                                       // [2 W][heads]
+  float* part_m = part_w + 2 * W * heads;                                            // [2 W][heads]
+  int* before = reinterpret_cast<int*>(part_m + 2 * W * heads);                      // [n_seq + 1]: units before a sequence
+  int* line = before + p.a.table.n_seq + 1;                                          // [n_seq + 1]: where it begins on the line
+  int* contexts = line + p.a.table.n_seq + 1;                                        // [n_seq]
   __shared__ uint64_t bars[W][kMaxStages];
   __shared__ uint32_t stage_boxes[W][kMaxStages];  // bit i: box i of the unit whose keys are in this stage has a page
   // The warps' parts of pairs, in order: part 2 w of the pair that warp w's run begins in, 2 w + 1 of the one it ends in.
@@ -149,10 +155,12 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     int first, end;            // units of the pair, first -1: no part
     int from, to;              // units of the part
     int row, g;                // the pair's row of results, heads
+    int line;                  // where it begins on the line
   };
   __shared__ Part parts[2 * W];
-  __shared__ int group_at[2 * W + 1], groups;  // parts of the same pair follow one another
+  __shared__ int order[2 * W], group_at[2 * W + 1], groups;  // the parts that there are, and where in `order` those of a pair begin
   __shared__ unsigned int tickets[2];
+  __shared__ int2 warp_sums[W];
   __shared__ int abort_flag;
 
   const PageTable& table = p.a.table;
@@ -175,35 +183,55 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   pdl_launch_dependents();
   pdl_wait();  // q, positions, the table and the newest cache rows come from preceding kernels
 
-  // ---- units of all sequences, and before each ------------------------------------------------------------------------------------
-  for (int b = threadIdx.x; b < n_seq; b += S::kThreads) {
-    int64_t ctx = load_pos(p.a.input_pos, p.a.pos_is_i64, b);
-    ctx = ctx < 0 ? 0 : (ctx >= table.capacity() ? table.capacity() : ctx + 1);
-    contexts[b] = static_cast<int>(ctx);
-    before[b] = span_of<UNIT>(static_cast<int>(ctx), p.a.window).tiles * pairs;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int b0 = 0; b0 < n_seq; b0 += 32) {
-      const int n = b0 + lane < n_seq ? before[b0 + lane] : 0;
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      if (b0 + lane < n_seq) before[b0 + lane] = carry + sum - n;
-      carry += __shfl_sync(0xffffffffu, sum, 31);
+  // ---- units before each sequence, and where it begins on the line --------------------------------------------------------------------
+  int units = 0, length = 0;
+  for (int b0 = 0; b0 < n_seq; b0 += S::kThreads) {
+    const int b = b0 + threadIdx.x;
+    int2 n = make_int2(0, 0);
+    if (b < n_seq) {
+      int64_t ctx = load_pos(p.a.input_pos, p.a.pos_is_i64, b);
+      ctx = ctx < 0 ? 0 : (ctx >= table.capacity() ? table.capacity() : ctx + 1);
+      contexts[b] = static_cast<int>(ctx);
+      const int tiles = span_of<UNIT>(static_cast<int>(ctx), p.a.window).tiles;
+      n = make_int2(tiles * pairs, length_of(tiles) * pairs);
     }
-    if (lane == 0) before[n_seq] = carry;
+    int2 sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+      if (lane >= o) sum.x += x, sum.y += y;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    int2 lower = make_int2(units, length);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int2 v = warp_sums[w];
+      if (w < warp) lower.x += v.x, lower.y += v.y;
+      units += v.x, length += v.y;
+    }
+    if (b < n_seq) before[b] = lower.x + sum.x - n.x, line[b] = lower.y + sum.y - n.y;
+    if (threadIdx.x == 0) before[n_seq] = units, line[n_seq] = length;
+    __syncthreads();
   }
-  __syncthreads();
-  const int64_t units = before[n_seq];
-  const int64_t ctas = units < static_cast<int64_t>(gridDim.x) * kMinRun ? (units + kMinRun - 1) / kMinRun : gridDim.x;  // that have a run
-  const int64_t me = blockIdx.x;
-  const int cta0 = static_cast<int>(me < ctas ? units * me / ctas : units), cta1 = static_cast<int>(me < ctas ? units * (me + 1) / ctas : units);
-  const int u0 = cta0 + (cta1 - cta0) * warp / W, u1 = cta0 + (cta1 - cta0) * (warp + 1) / W;  // this warp's run
+  // CTA c of those that have work takes length c / ctas .. of the line
+  const int ctas = length < static_cast<int64_t>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
+  const int me = blockIdx.x;
+  auto line_of = [&](int c) { return static_cast<int>(static_cast<int64_t>(length) * c / ctas); };
+  auto cta_at = [&](int at) { return static_cast<int>((static_cast<int64_t>(at + 1) * ctas - 1) / length); };
+  int u0 = 0, u1 = 0, cta0 = 0, cta1 = 0;  // units of this warp, of this CTA
+  if (me < ctas) {
+    // lanes 0 .. 3: the first unit at or behind a place
+    const int from = line_of(me), n = line_of(me + 1) - from, at = from + (lane & 3 ? (lane & 3) == 1 ? n : n * (warp + (lane & 3) - 2) / W : 0);
+    int u = units;
+    if (at < length) {
+      const int b = sequence_of(line, n_seq, at), tiles = (before[b + 1] - before[b]) / pairs, rest = at - line[b], pair = rest / length_of(tiles);
+      const int unit = (rest - pair * length_of(tiles) + kStep - 1) / kStep;
+      u = before[b] + pair * tiles + (unit < tiles ? unit : tiles);
+    }
+    cta0 = __shfl_sync(0xffffffffu, u, 0), cta1 = __shfl_sync(0xffffffffu, u, 1);
+    u0 = __shfl_sync(0xffffffffu, u, 2), u1 = __shfl_sync(0xffffffffu, u, 3);
+  }
 
   // sequences without a visible position
   for (int b = blockIdx.x; b < n_seq; b += gridDim.x)
@@ -229,13 +257,12 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int rest = u - before[b], pair = rest / s.tiles;
       const int pos = (s.first + rest - pair * s.tiles) * UNIT + (lane % boxes) * p.box;
       if (pos >= s.ctx || pos + p.box <= s.lo) return;
-      const int64_t page = table.find(b, pos);
-      if (page >= 0) slab = static_cast<int>(page * p.a.n_kv + pair / p.head_tiles), row = pos % table.page;
+      const int page = table.find(b, pos);
+      if (page >= 0) slab = page * p.a.n_kv + pair / p.head_tiles, row = pos % table.page;
     };
     int f_unit = u0, f_base = u0, f_stage = 0, f_half = 0;  // what is fetched next; the first unit that the lanes have looked up
-    int slab, row, next_slab, next_row;
+    int slab, row, next_slab = -1, next_row = 0;
     look_up(u0 + lane / boxes, slab, row);
-    look_up(u0 + ahead + lane / boxes, next_slab, next_row);
     uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
     auto fetch = [&]() {  // behind a __syncwarp(): the stage has been read
       if (f_unit >= u1) return;
@@ -263,7 +290,8 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         look_up(f_base + ahead + lane / boxes, next_slab, next_row);
       }
     };
-    for (int i = 0; i < p.stages; ++i) fetch();
+    for (int i = 0; i < p.stages; ++i) fetch();  // (up to four units; a look-up is of eight or more)
+    look_up(f_base + ahead + lane / boxes, next_slab, next_row);
 
     const int quad = lane >> 2, col = (lane & 3) * 2;  // a thread holds scores of positions quad, quad + 8, .. and heads col, col + 1
     int s = 0;  // the stage whose turn it is: of keys, then of values
@@ -582,7 +610,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
               }
             }
           }
-        if (lane == 0) parts[which] = Part{first, first + sp.tiles, u, end, out_row, g};
+        if (lane == 0) parts[which] = Part{first, first + sp.tiles, u, end, out_row, g, line[b] + pair * length_of(sp.tiles)};
       }
       u = end;
     }
@@ -590,15 +618,29 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   __syncthreads();
 
   // ---- the CTA's parts of a pair become one: a result, or a part in the workspace -------------------------------------------------------------
-  if (warp == 0) {
+  // what a part of a head weighs: 2 to the power of its reference minus the largest of the pair's in this CTA
+  for (int idx = threadIdx.x; idx < 2 * W * heads; idx += S::kThreads) {
+    const int a = idx / heads, i = idx - a * heads, pair = parts[a].first;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 2 * W; ++c) {
+      const float m = part_ml[(c * heads + i) * 2];
+      if (parts[c].first == pair) mm = fmaxf(mm, m);
+    }
+    mm = mm == -INFINITY ? 0.f : mm;
+    part_w[idx] = exp2f(part_ml[idx * 2] - mm);
+    part_m[idx] = mm;
+  }
+  // parts of the same pair follow one another
+  if (warp == W - 1) {
     const int mine = lane < 2 * W ? parts[lane].first : -1;
-    const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0);
-    const uint32_t lower = there & ((1u << lane) - 1u);
+    const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0), lower = there & ((1u << lane) - 1u);
     const int prev = __shfl_sync(0xffffffffu, mine, lower ? 31 - __clz(lower) : 0);
     const bool starts = mine >= 0 && (!lower || prev != mine);
     const uint32_t start = __ballot_sync(0xffffffffu, starts);
-    if (starts) group_at[__popc(start & ((1u << lane) - 1u))] = lane;
-    if (lane == 0) groups = __popc(start), group_at[__popc(start)] = 2 * W;
+    if (mine >= 0) order[__popc(lower)] = lane;
+    if (starts) group_at[__popc(start & ((1u << lane) - 1u))] = __popc(lower);
+    if (lane == 0) groups = __popc(start), group_at[__popc(start)] = __popc(there);
   }
   __syncthreads();
   // element e .. e + 3 of a head's result from its sum
@@ -608,42 +650,38 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   };
   for (int idx = threadIdx.x; idx < groups * heads * (HD / 4); idx += S::kThreads) {
     const int k = idx / (heads * (HD / 4)), rest = idx - k * (heads * (HD / 4)), i = rest / (HD / 4), e = rest % (HD / 4) * 4;
-    const int a0 = group_at[k], a1 = group_at[k + 1];
-    const Part& head = parts[a0];
+    const int n0 = group_at[k], n1 = group_at[k + 1];
+    const Part& head = parts[order[n0]];
     if (i >= head.g) continue;
-    float mm = -INFINITY;
-    int last = a0;
-    for (int a = a0; a < a1; ++a)
-      if (parts[a].first >= 0) mm = fmaxf(mm, part_ml[(a * heads + i) * 2]), last = a;
-    const float m_use = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f, v[4] = {};
-    for (int a = a0; a < a1; ++a)
-      if (parts[a].first >= 0) {
-        const float f = exp2f(part_ml[(a * heads + i) * 2] - m_use);
-        const float4 x = *reinterpret_cast<const float4*>((a & 1 ? reinterpret_cast<const float*>(rings + (a >> 1) * ring_bytes) : firsts + (a >> 1) * heads * HD) + i * HD + e);
-        ll += part_ml[(a * heads + i) * 2 + 1] * f;
-        v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
-      }
-    if (head.from == head.first && parts[last].to == head.end) {
+#pragma unroll 4
+    for (int n = n0; n < n1; ++n) {
+      const int a = order[n];
+      const float f = part_w[a * heads + i];
+      const float4 x = *reinterpret_cast<const float4*>((a & 1 ? reinterpret_cast<const float*>(rings + (a >> 1) * ring_bytes) : firsts + (a >> 1) * heads * HD) + i * HD + e);
+      ll += part_ml[(a * heads + i) * 2 + 1] * f;
+      v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
+    }
+    if (head.from == head.first && parts[order[n1 - 1]].to == head.end) {
       store4(head.row, i, e, ll, v);
     } else {
       // a CTA leaves at most two parts: of the pair its run begins in, and of the one it ends in
-      const int64_t at = (me * 2 + (head.from == cta0 ? 0 : 1)) * heads + i;
+      const int64_t at = (static_cast<int64_t>(me) * 2 + (head.from == cta0 ? 0 : 1)) * heads + i;
       *reinterpret_cast<float4*>(p.part_o + at * HD + e) = make_float4(v[0], v[1], v[2], v[3]);
-      if (e == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, ll);
+      if (e == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(ll == 0.f ? -INFINITY : part_m[order[n0] * heads + i], ll);
     }
   }
-  // The CTAs that share a pair: CTA c has units units * c / ctas ..; the last of them to arrive joins their parts.
+  // The CTAs that share a pair, from that of its first unit to that of its last: the last of them to arrive joins their parts.
   int shared_from[2], shared_to[2];  // of the first and of the last pair of this CTA, from -1: not shared
   Part pair_of[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     shared_from[k] = shared_to[k] = -1;
     if (groups == 0 || (k == 1 && groups == 1)) continue;
-    pair_of[k] = parts[group_at[k == 0 ? 0 : groups - 1]];
+    pair_of[k] = parts[order[group_at[k == 0 ? 0 : groups - 1]]];
     if (pair_of[k].first < cta0 || pair_of[k].end > cta1) {
-      shared_from[k] = static_cast<int>((static_cast<int64_t>(pair_of[k].first + 1) * ctas - 1) / units);
-      shared_to[k] = static_cast<int>((static_cast<int64_t>(pair_of[k].end) * ctas - 1) / units);
+      shared_from[k] = cta_at(pair_of[k].line);
+      shared_to[k] = cta_at(pair_of[k].line + (pair_of[k].end - pair_of[k].first - 1) * kStep);
     }
   }
   if (shared_from[0] >= 0 || shared_from[1] >= 0) {
@@ -659,9 +697,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int n = shared_to[k] - shared_from[k] + 1;
       if (shared_from[k] < 0 || tickets[k] != static_cast<unsigned int>(n - 1)) continue;
       const int g = pair_of[k].g;
-      // part 0 is the last of its CTA unless that begins with the pair; part i > 0 the first of its CTA
+      // part 0 is the last of its CTA unless the unit in front of it lies before that CTA's stretch; part i > 0 the first of its CTA
       const int64_t at0 = static_cast<int64_t>(shared_from[k]) * 2 * heads;
-      const int64_t at_first = at0 + (units * shared_from[k] / ctas != pair_of[k].first ? heads : 0);
+      const int64_t at_first = at0 + (pair_of[k].line > 0 && pair_of[k].line - kGap - kStep >= line_of(shared_from[k]) ? heads : 0);
       float2* ml = reinterpret_cast<float2*>(rings);  // [n][g]
       __syncthreads();
       for (int i = threadIdx.x; i < n * g; i += S::kThreads) {
@@ -713,9 +751,9 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   if (rc != LRI_OK) return rc;
   rc = make_tmap_pages(&tv, cache_dtype, p.a.v, slabs, t.page, p.a.dim, S::kChunkRow / static_cast<int>(sizeof(C)), p.box);
   if (rc != LRI_OK) return rc;
-  // units of a sequence at most, and sequences whose units stay below 2^30
+  // what a sequence takes of the line at most, and sequences that stay below 2^30 together
   const int64_t longest = p.a.window > 0 && p.a.window < t.capacity() ? p.a.window + S::kUnit : t.capacity();
-  const int64_t most = ((longest + S::kUnit - 1) / S::kUnit + 1) * p.a.n_kv * p.head_tiles;
+  const int64_t most = (((longest + S::kUnit - 1) / S::kUnit + 1) * kStep + kGap) * p.a.n_kv * p.head_tiles;
   int64_t per = (1ll << 30) / most;
   LRI_REQUIRE(per >= 1, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %lld positions of %d heads", (long long)t.capacity(), p.a.n_kv);
   per = per < kMaxSeqs ? per : kMaxSeqs;
@@ -731,7 +769,7 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
     p.a.out = static_cast<T*>(all.out) + at * all.n_head * all.dim;
     p.a.input_pos = static_cast<const char*>(all.input_pos) + at * (all.pos_is_i64 ? 8 : 4);
     // all that the parts and the sequences leave of shared memory goes to the rings
-    const int fixed = 1024 + S::kWarps * p.tile_heads * (HD * 4 + 2 * 8) + (2 * n + 1) * 4;
+    const int fixed = 1024 + S::kWarps * p.tile_heads * (HD * 4 + 2 * 16) + (3 * n + 2) * 4;
     const int stage = S::kWarps * static_cast<int>(S::kHalf + (sizeof(C) == 1 ? S::kUnit * 4 : 0));
     const int fits = (kSmemBytes - kStaticBytes - fixed) / stage;
     p.stages = fits < kMaxStages ? fits : kMaxStages;

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) rope_paged_store_kernel(const StoreP
     pos = load_pos(p.input_pos, p.pos_is_i64, token);
     const int64_t b = p.sequence ? p.sequence[token] : token;
     live = pos >= 0 && pos < p.table.capacity() && (p.rot == 0 || pos < p.table_rows) && b >= 0 && b < p.table.n_seq;
-    if (live) page = p.table.find(b, pos);
+    if (live) page = p.table.find(b, static_cast<int>(pos));
     live = page >= 0 && e < p.dim;
   }
   float x[8] = {};
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) paged_load_kernel(const LoadParams p
     const int64_t pos = first + i / vecs;
     const int e = i % vecs * 8;
     float k[8] = {}, v[8] = {};
-    const int64_t page = pos < n ? p.table.find(b, pos) : -1;
+    const int64_t page = pos < n ? p.table.find(b, static_cast<int>(pos)) : -1;
     if (page >= 0) {
       const int64_t row = (page * p.n_kv + h) * p.table.page + pos % p.table.page;
       load_cached8(static_cast<const C*>(p.k) + row * p.dim + e, k);
