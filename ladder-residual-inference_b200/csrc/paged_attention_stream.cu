@@ -36,8 +36,7 @@ constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;  // of a launch
 constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of the line
 constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
-constexpr int kMaxStages = 8;
-constexpr int kSmemBytes = 227 * 1024, kStaticBytes = 3072;  // of an SM, of those what the kernel declares
+constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
 constexpr int kMaxCtas = 256;
 constexpr size_t kCounterBytes = kMaxCtas * 4;
 
@@ -45,7 +44,6 @@ struct StreamParams {
   PagedAttnParams a;
   int group, tile_heads, head_tiles;  // query heads of a KV head, of a pass, passes
   int box;                            // positions of a TMA box
-  int stages;                         // of a warp's ring: a tile of keys or of values each
   unsigned int* counters;             // [CTAs]
   float* part_ml;                     // [CTAs][2][tile_heads][2]
   float* part_o;                      // [CTAs][2][tile_heads][HD]
@@ -115,14 +113,6 @@ __device__ __forceinline__ void codes_to_halves(uint32_t v, uint32_t& lo, uint32
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
 
-// codes as halves times 2^-8, in the order (0, 2), (1, 3), by integer operations: the four bits of the exponent and the three of the mantissa move
-// into a half's fields as they are, subnormal numbers too.  Conversions run at a sixteenth of the issue rate: keys take them, values this,
-// 95 -> 70 us for 100 sequences of 300 to 6000 positions.  (The two codes of NaN count as +-480; lri_rope_paged_store writes none.)
-__device__ __forceinline__ void codes_to_halves_256th(uint32_t v, uint32_t& even, uint32_t& odd) {
-  even = ((v << 7) & 0x3f803f80u) | ((v << 8) & 0x80008000u);
-  odd = ((v >> 1) & 0x3f803f80u) | (v & 0x80008000u);
-}
-
 template <typename T, typename C, int HD, int NT>
 __global__ void __launch_bounds__((Shape<C, HD, NT>::kThreads), 1)
 paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const StreamParams p) {
@@ -138,18 +128,17 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 
   extern __shared__ uint8_t smem_raw[];
   const int heads = p.tile_heads;
-  const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u, ring_bytes = p.stages * S::kHalf;
-  uint8_t* rings = smem_raw + (ring0 - smem_u32(smem_raw));                          // [W][stages][kHalf]
-  float* scales = reinterpret_cast<float*>(rings + W * ring_bytes);                  // [W][stages][UNIT], e4m3
-  float* firsts = scales + (kEight ? W * p.stages * UNIT : 0);                       // [W][heads][HD]: parts of pairs that runs begin in
+  const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u, ring_bytes = kStages * S::kHalf;
+  uint8_t* rings = smem_raw + (ring0 - smem_u32(smem_raw));                          // [W][kStages][kHalf]
+  float* scales = reinterpret_cast<float*>(rings + W * ring_bytes);                  // [W][kStages][UNIT], e4m3
+  float* firsts = scales + (kEight ? W * kStages * UNIT : 0);                       // [W][heads][HD]: parts of pairs that runs begin in
   float* part_ml = firsts + W * heads * HD;                                          // [2 W][heads][2]
   float* part_w = part_ml + 2 * W * heads * 2;                                       // [2 W][heads]
   float* part_m = part_w + 2 * W * heads;                                            // [2 W][heads]
   int* before = reinterpret_cast<int*>(part_m + 2 * W * heads);                      // [n_seq + 1]: units before a sequence
   int* line = before + p.a.table.n_seq + 1;                                          // [n_seq + 1]: where it begins on the line
   int* contexts = line + p.a.table.n_seq + 1;                                        // [n_seq]
-  __shared__ uint64_t bars[W][kMaxStages];
-  __shared__ uint32_t stage_boxes[W][kMaxStages];  // bit i: box i of the unit whose keys are in this stage has a page
+  __shared__ uint64_t bars[W][kStages];
   // The warps' parts of pairs, in order: part 2 w of the pair that warp w's run begins in, 2 w + 1 of the one it ends in.
   struct Part {
     int first, end;            // units of the pair, first -1: no part
@@ -171,7 +160,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   const uint32_t full0 = smem_u32(&bars[warp][0]);
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane == 0) {
-    for (int i = 0; i < p.stages; ++i) mbar_init(full0 + 8 * i, 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(full0 + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     parts[2 * warp].first = parts[2 * warp + 1].first = -1;
@@ -245,7 +234,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 
   if (u0 < u1) {
     const uint32_t ring = ring0 + warp * ring_bytes;
-    float* my_scales = scales + warp * p.stages * UNIT;
+    const float* my_scales = scales + warp * kStages * UNIT;
 
     // ---- fetch: a lane looks up the page of one box, 32 boxes at a time and 32 ahead ------------------------------------------------
     const int boxes = UNIT / p.box, ahead = 32 / boxes;  // of a unit; units that 32 lanes look up
@@ -260,42 +249,31 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int page = table.find(b, pos);
       if (page >= 0) slab = page * p.a.n_kv + pair / p.head_tiles, row = pos % table.page;
     };
-    int f_unit = u0, f_base = u0, f_stage = 0, f_half = 0;  // what is fetched next; the first unit that the lanes have looked up
+    int base = u0;  // the first unit that the lanes have looked up
     int slab, row, next_slab = -1, next_row = 0;
     look_up(u0 + lane / boxes, slab, row);
     uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
-    auto fetch = [&]() {  // behind a __syncwarp(): the stage has been read
-      if (f_unit >= u1) return;
-      const int i = f_unit - f_base;
-      const uint32_t mine = (have >> (i * boxes)) & ((1u << boxes) - 1u), full = full0 + 8 * f_stage;
-      if (lane == 0) {
-        if (f_half == 0) stage_boxes[warp][f_stage] = mine;
-        mbar_expect_tx(full, __popc(mine) * p.box * (S::kRow + (kEight ? 4 : 0)));
-      }
-      __syncwarp();
-      if (lane / boxes == i && slab >= 0) {
-        const int at = (lane % boxes) * p.box;
-        const CUtensorMap* map = f_half ? &tmap_v : &tmap_k;
+    // the tile of keys (0) or of values (1) of unit u; the one before in its place has been read by all lanes
+    auto fetch = [&](int half, int u) {
+      const uint32_t full = full0 + 8 * half, dst = ring + half * S::kHalf;
+      const uint32_t mine = (have >> ((u - base) * boxes)) & ((1u << boxes) - 1u);
+      if (elect_one()) mbar_expect_tx(full, __popc(mine) * p.box * (S::kRow + (kEight ? 4 : 0)));
+      for (int i = 0; i < boxes; ++i) {
+        const int from = (u - base) * boxes + i, z = __shfl_sync(0xffffffffu, slab, from), y = __shfl_sync(0xffffffffu, row, from);
+        if (z >= 0 && elect_one()) {
 #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c)
-          tma_load_3d(ring + f_stage * S::kHalf + c * S::kChunkBytes + at * S::kChunkRow, map, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
-        if (kEight) bulk_load(smem_u32(my_scales + f_stage * UNIT + at), (f_half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(slab) * table.page + row, p.box * 4, full);
-      }
-      if (++f_stage == p.stages) f_stage = 0;
-      f_half ^= 1;
-      if (f_half == 0 && ++f_unit - f_base == ahead) {
-        f_base = f_unit;
-        slab = next_slab, row = next_row;
-        have = __ballot_sync(0xffffffffu, slab >= 0);
-        look_up(f_base + ahead + lane / boxes, next_slab, next_row);
+          for (int c = 0; c < S::kChunks; ++c)
+            tma_load_3d(dst + c * S::kChunkBytes + i * p.box * S::kChunkRow, half ? &tmap_v : &tmap_k, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), y, z);
+          if (kEight) bulk_load(smem_u32(my_scales + half * UNIT + i * p.box), (half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(z) * table.page + y, p.box * 4, full);
+        }
       }
     };
-    for (int i = 0; i < p.stages; ++i) fetch();  // (up to four units; a look-up is of eight or more)
-    look_up(f_base + ahead + lane / boxes, next_slab, next_row);
+    fetch(0, u0);
+    fetch(1, u0);
+    look_up(base + ahead + lane / boxes, next_slab, next_row);
 
     const int quad = lane >> 2, col = (lane & 3) * 2;  // a thread holds scores of positions quad, quad + 8, .. and heads col, col + 1
-    int s = 0;  // the stage whose turn it is: of keys, then of values
-    uint32_t parity = 0;
+    uint32_t parity = 0, has = have & ((1u << boxes) - 1u);  // of the unit whose turn it is: bit i: box i has a page
     bool ok = true;
     int b = sequence_of(before, n_seq, u0);
     for (int u = u0; u < u1;) {
@@ -362,33 +340,34 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
         m_run[n][0] = m_run[n][1] = -INFINITY, l_run[n][0] = l_run[n][1] = 0.f;
       }
-      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of v_top / 256
+      float v_top = 0x1p-120f, v_inv = 0x1p120f;  // e4m3: O is in units of v_top
 
-      auto arrived = [&]() { return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 42, &g_paged_attn_status)) != 0; };
-      auto give_back = [&]() {
-        __syncwarp();
-        fetch();
-        if (++s == p.stages) s = 0, parity ^= 1u;
-      };
+      auto arrived = [&](int half) { return __all_sync(0xffffffffu, mbar_wait(full0 + 8 * half, parity, &abort_flag, 42, &g_paged_attn_status)) != 0; };
       for (int unit = u; unit < end && ok; ++unit) {
-        ok = arrived();
-        if (!ok) break;
         // ---- which of the positions are visible --------------------------------------------------------------------------------------
         const int p0 = (sp.first + unit - first) * UNIT;
-        const uint32_t has = stage_boxes[warp][s];
         uint32_t vis = kAll;
-        if (has != (1u << boxes) - 1u) {
+        if (has != (1u << boxes) - 1u || p0 + UNIT > sp.ctx || p0 < sp.lo) {
           vis = 0u;
           for (int i = 0; i < boxes; ++i) vis |= (has >> i) & 1u ? (0xffffffffu >> (32 - p.box)) << (i * p.box) : 0u;
+          if (p0 + UNIT > sp.ctx) vis &= (1u << (sp.ctx - p0)) - 1u;
+          if (p0 < sp.lo) vis &= ~((1u << (sp.lo - p0)) - 1u);
         }
-        if (p0 + UNIT > sp.ctx) vis &= p0 < sp.ctx ? (1u << (sp.ctx - p0)) - 1u : 0u;
-        if (p0 < sp.lo) vis &= sp.lo - p0 < UNIT ? ~((1u << (sp.lo - p0)) - 1u) : 0u;
+        const int next = unit + 1;
+        if (next - base == ahead) {
+          base = next, slab = next_slab, row = next_row;
+          have = __ballot_sync(0xffffffffu, slab >= 0);
+          look_up(base + ahead + lane / boxes, next_slab, next_row);
+        }
+        has = (have >> ((next - base) * boxes)) & ((1u << boxes) - 1u);
+        ok = arrived(0);
+        if (!ok) break;
         // ---- scores: UNIT positions x 8 NT heads ----------------------------------------------------------------------------------------
         float sc[RB][NT][4];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           const int r = rb * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-          const uint32_t at = ring + s * S::kHalf;
+          const uint32_t at = ring;
           float part[2][NT][4];  // two chains
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -420,7 +399,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[rb][n][e] = part[0][n][e] + part[1][n][e];
           if constexpr (kEight) {
-            const float* sk = my_scales + s * UNIT + rb * 16 + quad;
+            const float* sk = my_scales + rb * 16 + quad;
             const float ks[2] = {sk[0], sk[8]};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -433,7 +412,8 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
               for (int e = 0; e < 4; ++e) sc[rb][n][e] *= p.a.scale_log2;
           }
         }
-        give_back();
+        __syncwarp();
+        if (next < u1) fetch(0, next);
         if (vis != kAll) {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
@@ -455,7 +435,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
             for (int rb = 0; rb < RB; ++rb) mx[n][c] = fmaxf(mx[n][c], fmaxf(sc[rb][n][c], sc[rb][n][2 + c]));
             moved = moved || mx[n][c] > m_run[n][c] + kSlack;
           }
-        ok = arrived();
+        ok = arrived(1);
         if (!ok) break;
         float vs[RB][2], top = 0.f;
         if constexpr (kEight) {
@@ -463,7 +443,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              vs[rb][i] = my_scales[s * UNIT + rb * 16 + i * 8 + quad];
+              vs[rb][i] = my_scales[UNIT + rb * 16 + i * 8 + quad];
               if (vis != kAll && !((vis >> (rb * 16 + i * 8 + quad)) & 1u)) vs[rb][i] = 0.f;
               top = fmaxf(top, fabsf(vs[rb][i]));
             }
@@ -514,7 +494,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
               }
             }
         }
-        const uint32_t sv = ring + s * S::kHalf;
+        const uint32_t sv = ring + S::kHalf;
         if (vis != kAll) {
           // values that are not visible may be anything, and 0 x NaN is not 0
           for (int i = lane; i < UNIT * (S::kRow / 16); i += 32) {
@@ -533,7 +513,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
               uint32_t bf[4], a[2][4];
               load_matrix_trans(sv + S::at(r, kb + (lane >> 4)), bf);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) codes_to_halves_256th(bf[i], a[i >> 1][(i & 1) * 2], a[i >> 1][(i & 1) * 2 + 1]);
+              for (int i = 0; i < 4; ++i) codes_to_halves(__byte_perm(bf[i], 0u, 0x3120), a[i >> 1][(i & 1) * 2], a[i >> 1][(i & 1) * 2 + 1]);
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -554,7 +534,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           }
         }
         if (vis != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros, before the next copy
-        give_back();
+        __syncwarp();
+        if (next < u1) fetch(1, next);
+        parity ^= 1u;
       }
 
       // ---- the end of a pair, or of the run -------------------------------------------------------------------------------------------------
@@ -565,7 +547,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], w);
         }
-      const float unit_o = kEight ? v_top * 256.f : 1.f;
+      const float unit_o = kEight ? v_top : 1.f;
       if (u == first && end == first + sp.tiles) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -758,8 +740,12 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   LRI_REQUIRE(per >= 1, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %lld positions of %d heads", (long long)t.capacity(), p.a.n_kv);
   per = per < kMaxSeqs ? per : kMaxSeqs;
   auto kern = paged_attn_stream_kernel<T, C, HD, NT>;
+  // with the most heads and sequences
+  constexpr int kRings = kStages * static_cast<int>(S::kHalf + (sizeof(C) == 1 ? S::kUnit * 4 : 0));
+  constexpr int kSmem = 1024 + S::kWarps * (8 * NT * (HD * 4 + 2 * 16) + kRings) + (3 * kMaxSeqs + 2) * 4;
+  static_assert(kSmem + 4096 <= 227 * 1024, "rings, parts and sequences fit an SM, beside what the kernel declares");
   static std::atomic<unsigned long long> attr_set{0};
-  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes - kStaticBytes));
+  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const PagedAttnParams all = p.a;
   for (int64_t at = 0; at < all.table.n_seq; at += per) {
     const int n = static_cast<int>(all.table.n_seq - at < per ? all.table.n_seq - at : per);
@@ -768,14 +754,9 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
     p.a.q = static_cast<const T*>(all.q) + at * all.n_head * all.dim;
     p.a.out = static_cast<T*>(all.out) + at * all.n_head * all.dim;
     p.a.input_pos = static_cast<const char*>(all.input_pos) + at * (all.pos_is_i64 ? 8 : 4);
-    // all that the parts and the sequences leave of shared memory goes to the rings
-    const int fixed = 1024 + S::kWarps * p.tile_heads * (HD * 4 + 2 * 16) + (3 * n + 2) * 4;
-    const int stage = S::kWarps * static_cast<int>(S::kHalf + (sizeof(C) == 1 ? S::kUnit * 4 : 0));
-    const int fits = (kSmemBytes - kStaticBytes - fixed) / stage;
-    p.stages = fits < kMaxStages ? fits : kMaxStages;
-    LRI_REQUIRE(p.stages >= 2, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %d heads of %d with %d sequences", p.tile_heads, HD, n);
+    const int smem = 1024 + S::kWarps * (p.tile_heads * (HD * 4 + 2 * 16) + kRings) + (3 * n + 2) * 4;
     const int64_t room = max_ctas(), useful = (most * n + kMinRun - 1) / kMinRun;
-    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(S::kThreads), fixed + p.stages * stage, st, tk, tv, p));
+    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(S::kThreads), smem, st, tk, tv, p));
     LRI_LAUNCH_CHECK("paged_attn_stream_kernel");
   }
   return LRI_OK;
