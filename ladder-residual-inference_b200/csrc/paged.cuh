@@ -35,18 +35,33 @@ __device__ __forceinline__ void load_cached8(const T* p, float (&f)[8]) {
   load8<T>(p, f);
 }
 
+// n / d for 0 <= n < 2^31 by a product: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d), n m / 2^(31 + s) exceeds n / d by less than
+// n / 2^31 / d, which does not reach the next whole number.
+struct FastDiv {
+  uint32_t mul, shift;
+  static FastDiv of(int d) {
+    FastDiv f{0u, 31u};
+    while ((1ll << (f.shift - 31)) < d) ++f.shift;
+    f.mul = static_cast<uint32_t>(((1ull << f.shift) + d - 1) / d);
+    return f;
+  }
+  __host__ __device__ __forceinline__ int operator()(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift); }
+};
+
 // Pages of the sequences of a call.
 struct PageTable {
   const int32_t* ids;  // [n_seq, max_pages], row pitch ld
   int64_t ld;
   int n_seq, max_pages, page;
   int64_t n_pages;
+  FastDiv by_page;
   __host__ __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(max_pages) * page; }
   // page that holds position pos (0 <= pos < capacity()) of sequence b, -1: none
   __device__ __forceinline__ int find(int64_t b, int pos) const {
-    const int id = ids[b * ld + pos / page];
+    const int id = ids[b * ld + by_page(pos)];
     return id >= 0 && id < n_pages ? id : -1;
   }
+  __device__ __forceinline__ int row_of(int pos) const { return pos - by_page(pos) * page; }  // within its page
 };
 
 // Attention of one new token of each sequence (paged_attention.cu).

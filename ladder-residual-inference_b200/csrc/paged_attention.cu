@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_plain_kernel(const Pag
   for (int64_t j0 = lo + warp * kGroups; j0 < ctx; j0 += kWarps * kGroups) {  // the warp's bounds are the same in every lane
     const int64_t j = j0 + group;
     const int64_t page = j < ctx ? p.table.find(b, static_cast<int>(j)) : -1;
-    const int64_t row = (page * p.n_kv + h) * p.table.page + j % p.table.page;
+    const int64_t row = (page * p.n_kv + h) * p.table.page + p.table.row_of(static_cast<int>(j));
     float k[8] = {}, s = 0.f;
     if (page >= 0 && e < p.dim) load_cached8(static_cast<const C*>(p.k) + row * p.dim + e, k);
 #pragma unroll
@@ -119,9 +119,10 @@ extern "C" int lri_paged_attn_decode(const lri_paged_attn_call* call) {
   LRI_REQUIRE(call, LRI_ERR_ARG, "paged_attn_decode: NULL call");
   const lri_paged_attn_call& c = *call;
   PagedAttnParams p{};
-  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages, {}};
   int rc = check_paged("paged_attn_decode", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
+  p.table.by_page = FastDiv::of(c.page_size);
   LRI_REQUIRE(c.n_head >= 1 && c.n_head <= 65535 && c.n_head % c.n_kv == 0, LRI_ERR_ARG, "paged_attn_decode: n_head=%d n_kv=%d", c.n_head, c.n_kv);
   LRI_REQUIRE(c.window >= 0, LRI_ERR_ARG, "paged_attn_decode: window=%lld", (long long)c.window);
   if (c.n_seq == 0) return LRI_OK;

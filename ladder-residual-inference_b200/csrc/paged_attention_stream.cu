@@ -247,7 +247,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int pos = (s.first + rest - pair * s.tiles) * UNIT + (lane % boxes) * p.box;
       if (pos >= s.ctx || pos + p.box <= s.lo) return;
       const int page = table.find(b, pos);
-      if (page >= 0) slab = page * p.a.n_kv + pair / p.head_tiles, row = pos % table.page;
+      if (page >= 0) slab = page * p.a.n_kv + pair / p.head_tiles, row = table.row_of(pos);
     };
     int base = u0;  // the first unit that the lanes have looked up
     int slab, row, next_slab = -1, next_row = 0;

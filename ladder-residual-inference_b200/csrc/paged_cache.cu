@@ -7,6 +7,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLargest = 448.f;            // of e4m3
 constexpr float kSmallest = 0x1p-100f;       // rows of smaller values are stored against it, so that no scale is zero or subnormal
+constexpr int kManyTokens = 1024;            // from here on a thread takes several tokens
 constexpr int kFillRows = 64;                // lri_paged_load: zeros up to a multiple of this
 
 struct StoreParams {
@@ -28,101 +29,132 @@ struct StoreParams {
 
 // Rotation of elements e .. e + 7 of a head: pair i turns by the angle whose cosine and sine the table row holds at 2 i.  Products are
 // rounded before they are added (no contraction), so that a result does not depend on the layout or on the kernel.
-template <typename T, typename TT>
-__device__ __forceinline__ void rotate8(const StoreParams& p, const T* head, int e, const TT* row, float (&x)[8]) {
-  if (!p.halves) {
-    if ((p.rot & 7) == 0) {  // table rows are aligned, and vectors lie within or behind what rotates
+// Halves: `other` holds the elements that these are paired with.  VECTORS: eight elements have their table entries and partners in whole vectors.
+template <typename TT, bool VECTORS>
+__device__ __forceinline__ void rotate8(int rot, int halves, int e, const TT* row, const float (&other)[8], float (&x)[8]) {
+  if constexpr (VECTORS) {
+    if (!halves) {
       float cs[8];
       load8<TT>(row + e, cs);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) rope_pair(x[i], x[i + 1], cs[i], cs[i + 1], x[i], x[i + 1]);
     } else {
-      for (int i = 0; i < 8; i += 2)
-        if (e + i < p.rot) rope_pair(x[i], x[i + 1], Num<TT>::to_f(row[e + i]), Num<TT>::to_f(row[e + i + 1]), x[i], x[i + 1]);
-    }
-    return;
-  }
-  const int half = p.rot >> 1;
+      const bool low = e < rot >> 1;
+      const TT* at = row + 2 * (low ? e : e - (rot >> 1));
+      float cs[2][8];
+      load8<TT>(at, cs[0]);
+      load8<TT>(at + 8, cs[1]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int at = e + i;
-    if (at >= p.rot) continue;
-    const bool low = at < half;
-    const int pair = low ? at : at - half;
-    const float other = Num<T>::to_f(head[low ? at + half : pair]);
-    const float c = Num<TT>::to_f(row[2 * pair]), s = Num<TT>::to_f(row[2 * pair + 1]);
-    float a, b;
-    rope_pair(low ? x[i] : other, low ? other : x[i], c, s, a, b);
-    x[i] = low ? a : b;
+      for (int i = 0; i < 8; ++i) {
+        float a, b;
+        rope_pair(low ? x[i] : other[i], low ? other[i] : x[i], cs[i >> 2][2 * (i & 3)], cs[i >> 2][2 * (i & 3) + 1], a, b);
+        x[i] = low ? a : b;
+      }
+    }
+  } else if (!halves) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      if (e + i < rot) rope_pair(x[i], x[i + 1], Num<TT>::to_f(row[e + i]), Num<TT>::to_f(row[e + i + 1]), x[i], x[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (e + i >= rot) continue;
+      const bool low = e + i < rot >> 1;
+      const int pair = low ? e + i : e + i - (rot >> 1);
+      float a, b;
+      rope_pair(low ? x[i] : other[i], low ? other[i] : x[i], Num<TT>::to_f(row[2 * pair]), Num<TT>::to_f(row[2 * pair + 1]), a, b);
+      x[i] = low ? a : b;
+    }
   }
 }
 
-// LANES threads hold a head, eight elements each.
-template <typename T, typename TT, bool E4M3, int LANES>
+// LANES threads hold a head, eight elements each, of R tokens: blockIdx.y says which heads, blockIdx.x which tokens.  Bound by HBM for prompts:
+// what a thread reads does not wait for what says where it goes, and R tokens are on their way at once (8192 tokens of 32 + 2 x 8 heads of 128:
+// MEASURE_STORE).  For single tokens it is a chain of two loads and a store.
+template <typename T, typename TT, bool E4M3, bool VECTORS, int LANES, int R>
 __global__ void __launch_bounds__(kThreads) rope_paged_store_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t heads = static_cast<uint32_t>(p.n_head + 2 * p.n_kv);
-  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
-  const int64_t token = static_cast<int64_t>(item / heads);
-  const int head = static_cast<int>(item - static_cast<uint64_t>(token) * heads);
-  const int e = static_cast<int>(threadIdx.x % LANES) * 8;
-  bool live = token < p.tokens;
-  int64_t pos = 0, page = -1;
-  if (live) {
-    pos = load_pos(p.input_pos, p.pos_is_i64, token);
-    const int64_t b = p.sequence ? p.sequence[token] : token;
-    live = pos >= 0 && pos < p.table.capacity() && (p.rot == 0 || pos < p.table_rows) && b >= 0 && b < p.table.n_seq;
-    if (live) page = p.table.find(b, static_cast<int>(pos));
-    live = page >= 0 && e < p.dim;
-  }
-  float x[8] = {};
-  if (live) {
+  const int at = blockIdx.y * blockDim.x + threadIdx.x, head = at / LANES, e = at % LANES * 8;
+  const bool mine = head < p.n_head + 2 * p.n_kv && e < p.dim;
+  const bool turns = mine && head < p.n_head + p.n_kv && e < p.rot, is_v = head >= p.n_head + p.n_kv;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * R;
+  const int half = p.rot >> 1;
+
+  uint4 raw[R], pair[R];
+  int64_t pos[R], seq[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t token = token0 + r;
+    raw[r] = pair[r] = make_uint4(0, 0, 0, 0);
+    pos[r] = -1, seq[r] = token;
+    if (token >= p.tokens) continue;
+    pos[r] = load_pos(p.input_pos, p.pos_is_i64, token);
+    if (p.sequence) seq[r] = p.sequence[token];
+    if (!mine) continue;
     const T* src = static_cast<const T*>(p.qkv) + token * p.ld + static_cast<int64_t>(head) * p.dim;
-    load8<T>(src + e, x);
-    if (head < p.n_head + p.n_kv && e < p.rot) rotate8<T, TT>(p, src, e, static_cast<const TT*>(p.rope) + pos * p.rot, x);
+    raw[r] = *reinterpret_cast<const uint4*>(src + e);
+    if (VECTORS && turns && p.halves) pair[r] = *reinterpret_cast<const uint4*>(src + (e < half ? e + half : e - half));
   }
-  if (head < p.n_head) {
-    if (live) store8<T>(static_cast<T*>(p.q_out) + (token * p.n_head + head) * p.dim + e, x);
-    if (!E4M3) return;
+  int page[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool there = pos[r] >= 0 && pos[r] < p.table.capacity() && (p.rot == 0 || pos[r] < p.table_rows) && seq[r] >= 0 && seq[r] < p.table.n_seq;
+    page[r] = there ? p.table.find(seq[r], static_cast<int>(pos[r])) : -1;
   }
-  const bool is_v = head >= p.n_head + p.n_kv;
-  const int h = head - p.n_head - (is_v ? p.n_kv : 0);
-  const int64_t row = (page * p.n_kv + h) * p.table.page + pos % p.table.page;
-  if constexpr (!E4M3) {
-    if (live) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + row * p.dim + e, x);
-  } else {
-    // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
-    // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
-    // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
-    float top = 0.f;
-    bool finite = true;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      top = fmaxf(top, fabsf(x[i]));
-      finite = finite && fabsf(x[i]) < INFINITY;
-    }
-    if (!finite) top = INFINITY;
+  for (int r = 0; r < R; ++r) {
+    const int64_t token = token0 + r;
+    const bool live = mine && page[r] >= 0;
+    float x[8], other[8];
+    unpack8<T>(raw[r], x);
+    unpack8<T>(pair[r], other);
+    if (live && turns) {
+      if (!VECTORS && p.halves) {
+        const T* src = static_cast<const T*>(p.qkv) + token * p.ld + static_cast<int64_t>(head) * p.dim;
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!live || head < p.n_head) return;
-    const bool whole = top < INFINITY;
-    top = fmaxf(top, kSmallest);
-    // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
-    const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
-    auto scaled = [&](float v) {
-      const float n = v * up, y = n * inv;
-      return fminf(fmaxf(fmaf(fmaf(-y, den, n), inv, y), -kLargest), kLargest);
-    };
-    uint32_t w[2] = {0u, 0u};
-    if (whole)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
-        w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
+        for (int i = 0; i < 8; ++i) other[i] = e + i < p.rot ? Num<T>::to_f(src[e + i < half ? e + i + half : e + i - half]) : 0.f;
       }
-    *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + row * p.dim + e) = make_uint2(w[0], w[1]);
-    if (e == 0) (is_v ? p.v_scale : p.k_scale)[row] = whole ? top / kLargest : NAN;
+      rotate8<TT, VECTORS>(p.rot, p.halves, e, static_cast<const TT*>(p.rope) + pos[r] * p.rot, other, x);
+    }
+    if (live && head < p.n_head) store8<T>(static_cast<T*>(p.q_out) + (token * p.n_head + head) * p.dim + e, x);
+    const int h = head - p.n_head - (is_v ? p.n_kv : 0);
+    const int64_t row = live ? (static_cast<int64_t>(page[r]) * p.n_kv + h) * p.table.page + p.table.row_of(static_cast<int>(pos[r])) : 0;
+    if constexpr (!E4M3) {
+      if (live && head >= p.n_head) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + row * p.dim + e, x);
+    } else {
+      // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
+      // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
+      // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
+      float top = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        top = fmaxf(top, fabsf(x[i]));
+        finite = finite && fabsf(x[i]) < INFINITY;
+      }
+      if (!finite) top = INFINITY;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!live || head < p.n_head) continue;
+      const bool whole = top < INFINITY;
+      top = fmaxf(top, kSmallest);
+      // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
+      const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
+      auto scaled = [&](float v) {
+        const float n = v * up, y = n * inv;
+        return fminf(fmaxf(fmaf(fmaf(-y, den, n), inv, y), -kLargest), kLargest);
+      };
+      uint32_t w[2] = {0u, 0u};
+      if (whole)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
+          w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
+        }
+      *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + row * p.dim + e) = make_uint2(w[0], w[1]);
+      if (e == 0) (is_v ? p.v_scale : p.k_scale)[row] = whole ? top / kLargest : NAN;
+    }
   }
 }
 
@@ -137,59 +169,107 @@ struct LoadParams {
   int n_kv, dim;
 };
 
-// A CTA reads 64 positions of a (sequence, head).
-template <typename T, typename C>
+// eight elements of a cache row as they are stored
+template <typename C>
+struct Raw8 {
+  using type = uint4;
+};
+template <>
+struct Raw8<e4m3> {
+  using type = uint2;
+};
+
+// A CTA reads 64 positions of a (sequence, head); LANES threads hold a row, eight elements each.  Bound by HBM: all pages are looked up before
+// the first row is asked for, and all rows before the first is stored (MEASURE_LOAD).
+template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(kThreads) paged_load_kernel(const LoadParams p) {
+  using V = typename Raw8<C>::type;
+  constexpr int kRows = kThreads / LANES, R = kFillRows / kRows;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t b = blockIdx.z, h = blockIdx.y, first = static_cast<int64_t>(blockIdx.x) * kFillRows;
-  int64_t n = load_pos(p.last_pos, p.pos_is_i64, b) + 1;
+  const int64_t b = blockIdx.z;
+  const int h = blockIdx.y, first = blockIdx.x * kFillRows;
+  int64_t last = load_pos(p.last_pos, p.pos_is_i64, b);
   const int64_t most = p.rows < p.table.capacity() ? p.rows : p.table.capacity();
-  n = n < 0 ? 0 : (n > most ? most : n);
-  if (first >= n) return;
-  const int vecs = p.dim >> 3;
-  const int64_t end = first + kFillRows < p.rows ? first + kFillRows : p.rows;
-  for (int i = threadIdx.x; i < (end - first) * vecs; i += kThreads) {
-    const int64_t pos = first + i / vecs;
-    const int e = i % vecs * 8;
-    float k[8] = {}, v[8] = {};
-    const int64_t page = pos < n ? p.table.find(b, static_cast<int>(pos)) : -1;
-    if (page >= 0) {
-      const int64_t row = (page * p.n_kv + h) * p.table.page + pos % p.table.page;
-      load_cached8(static_cast<const C*>(p.k) + row * p.dim + e, k);
-      load_cached8(static_cast<const C*>(p.v) + row * p.dim + e, v);
-      if (p.k_scale) {
-        const float ks = p.k_scale[row], vs = p.v_scale[row];
+  const int n = static_cast<int>(last < 0 ? 0 : (last >= most ? most : last + 1));
+  const int e = threadIdx.x % LANES * 8;
+  if (first >= n || e >= p.dim) return;
+  int page[R];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) k[c] *= ks, v[c] *= vs;
-      }
-    }
+  for (int r = 0; r < R; ++r) {
+    const int pos = first + r * kRows + threadIdx.x / LANES;
+    page[r] = pos < n ? p.table.find(b, pos) : -1;
+  }
+  V k[R], v[R];
+  float ks[R], vs[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    k[r] = v[r] = V{}, ks[r] = vs[r] = 0.f;
+    if (page[r] < 0) continue;
+    const int pos = first + r * kRows + threadIdx.x / LANES;
+    const int64_t row = (static_cast<int64_t>(page[r]) * p.n_kv + h) * p.table.page + p.table.row_of(pos);
+    k[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.k) + row * p.dim + e);
+    v[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.v) + row * p.dim + e);
+    if constexpr (sizeof(C) == 1) ks[r] = p.k_scale[row], vs[r] = p.v_scale[row];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t pos = first + r * kRows + threadIdx.x / LANES;
+    if (pos >= p.rows) continue;
     const int64_t to = ((b * p.n_kv + h) * p.rows + pos) * p.dim + e;
-    store8<T>(static_cast<T*>(p.k_out) + to, k);
-    store8<T>(static_cast<T*>(p.v_out) + to, v);
+    if constexpr (sizeof(C) == 1) {
+      auto scaled = [&](const V& codes, float scale, void* out) {
+        float x[8];
+        load_cached8(reinterpret_cast<const e4m3*>(&codes), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= scale;
+        store8<T>(static_cast<T*>(out) + to, x);
+      };
+      scaled(k[r], ks[r], p.k_out);
+      scaled(v[r], vs[r], p.v_out);
+    } else {
+      *reinterpret_cast<V*>(static_cast<T*>(p.k_out) + to) = k[r];
+      *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + to) = v[r];
+    }
   }
 }
 
-template <typename T, typename TT, bool E4M3>
+template <typename T, typename TT, bool E4M3, bool VECTORS>
 int launch_store(const StoreParams& p, cudaStream_t st) {
   const int vecs = p.dim / 8;
-  const int64_t items = p.tokens * (p.n_head + 2 * p.n_kv);
-  auto go = [&](auto kern, int lanes) {
-    const int64_t per = kThreads / lanes, grid = (items + per - 1) / per;
-    LRI_REQUIRE(grid < (1ll << 31), LRI_ERR_UNSUPPORTED, "rope_paged_store: %lld tokens", (long long)p.tokens);
-    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, p));
+  auto go = [&](auto kern, int lanes, int tokens) {
+    const int threads = (p.n_head + 2 * p.n_kv) * lanes, blocks = (threads + kThreads - 1) / kThreads;
+    const int block = ((threads + blocks - 1) / blocks + 31) / 32 * 32;
+    const int64_t grid = (p.tokens + tokens - 1) / tokens;
+    LRI_REQUIRE(grid < (1ll << 31) && blocks <= 65535, LRI_ERR_UNSUPPORTED, "rope_paged_store: %lld tokens of %d heads", (long long)p.tokens, p.n_head + 2 * p.n_kv);
+    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(blocks)), dim3(block), 0, st, p));
     LRI_LAUNCH_CHECK("rope_paged_store_kernel");
     return static_cast<int>(LRI_OK);
   };
-  if (vecs <= 8) return go(rope_paged_store_kernel<T, TT, E4M3, 8>, 8);
-  if (vecs <= 16) return go(rope_paged_store_kernel<T, TT, E4M3, 16>, 16);
-  return go(rope_paged_store_kernel<T, TT, E4M3, 32>, 32);
+  const bool many = p.tokens >= kManyTokens;
+  if (vecs <= 8) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 4>, 8, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 1>, 8, 1);
+  if (vecs <= 16) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 4>, 16, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 1>, 16, 1);
+  return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 4>, 32, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 1>, 32, 1);
 }
 
-template <typename T>
-int dispatch_store(const StoreParams& p, bool table_f32, bool eight, cudaStream_t st) {
-  if (table_f32) return eight ? launch_store<T, float, true>(p, st) : launch_store<T, float, false>(p, st);
-  return eight ? launch_store<T, T, true>(p, st) : launch_store<T, T, false>(p, st);
+template <typename T, typename TT>
+int dispatch_store(const StoreParams& p, bool eight, cudaStream_t st) {
+  // table rows of whole vectors, and halves of whole vectors
+  const bool vectors = p.rot % (p.halves ? 16 : 8) == 0;
+  if (eight) return vectors ? launch_store<T, TT, true, true>(p, st) : launch_store<T, TT, true, false>(p, st);
+  return vectors ? launch_store<T, TT, false, true>(p, st) : launch_store<T, TT, false, false>(p, st);
+}
+
+template <typename T, typename C>
+int launch_load(const LoadParams& p, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((p.rows + kFillRows - 1) / kFillRows), static_cast<unsigned>(p.n_kv), static_cast<unsigned>(p.table.n_seq));
+  auto go = [&](auto kern) {
+    LRI_CUDA(launch_pdl(kern, grid, dim3(kThreads), 0, st, p));
+    LRI_LAUNCH_CHECK("paged_load_kernel");
+    return static_cast<int>(LRI_OK);
+  };
+  const int vecs = p.dim / 8;
+  return vecs <= 8 ? go(paged_load_kernel<T, C, 8>) : vecs <= 16 ? go(paged_load_kernel<T, C, 16>) : go(paged_load_kernel<T, C, 32>);
 }
 
 }  // namespace
@@ -221,9 +301,10 @@ extern "C" int lri_rope_paged_store(const lri_paged_store_call* call) {
   LRI_REQUIRE(call, LRI_ERR_ARG, "rope_paged_store: NULL call");
   const lri_paged_store_call& c = *call;
   StoreParams p{};
-  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages, {}};
   int rc = check_paged("rope_paged_store", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
+  p.table.by_page = FastDiv::of(c.page_size);
   LRI_REQUIRE(c.tokens >= 0 && c.n_head >= 1 && c.n_head <= 65535, LRI_ERR_ARG, "rope_paged_store: tokens=%lld n_head=%d", (long long)c.tokens, c.n_head);
   LRI_REQUIRE(c.rot_dim >= 0 && c.rot_dim <= c.head_dim && c.rot_dim % 2 == 0, LRI_ERR_ARG, "rope_paged_store: rot_dim=%d of head_dim=%d", c.rot_dim, c.head_dim);
   LRI_REQUIRE(c.rot_dim == 0 || (c.rope_table && c.table_rows >= 1), LRI_ERR_ARG, "rope_paged_store: a rotation needs its table");
@@ -238,16 +319,18 @@ extern "C" int lri_rope_paged_store(const lri_paged_store_call* call) {
   p.tokens = c.tokens, p.n_head = c.n_head, p.n_kv = c.n_kv, p.dim = c.head_dim;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   const bool eight = c.cache_dtype == LRI_E4M3, f32 = c.table_is_f32 != 0;
-  return c.dtype == LRI_BF16 ? dispatch_store<__nv_bfloat16>(p, f32, eight, st) : dispatch_store<__half>(p, f32, eight, st);
+  if (c.dtype == LRI_BF16) return f32 ? dispatch_store<__nv_bfloat16, float>(p, eight, st) : dispatch_store<__nv_bfloat16, __nv_bfloat16>(p, eight, st);
+  return f32 ? dispatch_store<__half, float>(p, eight, st) : dispatch_store<__half, __half>(p, eight, st);
 }
 
 extern "C" int lri_paged_load(const lri_paged_load_call* call) {
   LRI_REQUIRE(call, LRI_ERR_ARG, "paged_load: NULL call");
   const lri_paged_load_call& c = *call;
   LoadParams p{};
-  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages};
+  p.table = PageTable{c.pages, c.pages_ld, c.n_seq, c.max_pages, c.page_size, c.n_pages, {}};
   int rc = check_paged("paged_load", c.dtype, c.cache_dtype, c.k_pages, c.v_pages, c.k_scale, c.v_scale, p.table, c.n_kv, c.head_dim);
   if (rc != LRI_OK) return rc;
+  p.table.by_page = FastDiv::of(c.page_size);
   LRI_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) && c.n_seq <= 65535, LRI_ERR_ARG, "paged_load: rows=%lld n_seq=%d", (long long)c.rows, c.n_seq);
   if (c.rows == 0 || c.n_seq == 0) return LRI_OK;
   LRI_REQUIRE(c.pages && c.last_pos && c.k_out && c.v_out, LRI_ERR_ARG, "paged_load: NULL pointer");
@@ -256,12 +339,6 @@ extern "C" int lri_paged_load(const lri_paged_load_call* call) {
   p.k = c.k_pages, p.v = c.v_pages, p.k_scale = eight ? c.k_scale : nullptr, p.v_scale = eight ? c.v_scale : nullptr;
   p.last_pos = c.last_pos, p.pos_is_i64 = c.pos_is_i64, p.k_out = c.k_out, p.v_out = c.v_out, p.rows = c.rows, p.n_kv = c.n_kv, p.dim = c.head_dim;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
-  const dim3 grid(static_cast<unsigned>((c.rows + kFillRows - 1) / kFillRows), static_cast<unsigned>(c.n_kv), static_cast<unsigned>(c.n_seq));
-  auto go = [&](auto kern) {
-    LRI_CUDA(launch_pdl(kern, grid, dim3(kThreads), 0, st, p));
-    LRI_LAUNCH_CHECK("paged_load_kernel");
-    return static_cast<int>(LRI_OK);
-  };
-  if (eight) return c.dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, e4m3>) : go(paged_load_kernel<__half, e4m3>);
-  return c.dtype == LRI_BF16 ? go(paged_load_kernel<__nv_bfloat16, __nv_bfloat16>) : go(paged_load_kernel<__half, __half>);
+  if (eight) return c.dtype == LRI_BF16 ? launch_load<__nv_bfloat16, e4m3>(p, st) : launch_load<__half, e4m3>(p, st);
+  return c.dtype == LRI_BF16 ? launch_load<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_load<__half, __half>(p, st);
 }
