@@ -15,21 +15,20 @@ struct e4m3 {
   uint8_t bits;
 };
 
-// two packed codes, the lower byte first, as halves: exact, every e4m3 number is one of fp16's
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+// the lower and the upper two of four codes as halves: exact, every e4m3 number is one of fp16's
+__device__ __forceinline__ void codes_to_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
+}
+__device__ __forceinline__ void codes_to_floats(const uint2& v, float (&f)[8]) {
+  uint32_t h[4];
+  codes_to_halves(v.x, h[0], h[1]);
+  codes_to_halves(v.y, h[2], h[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) Num<__half>::unpack2(h[i], f[2 * i], f[2 * i + 1]);
 }
 
 // eight elements of a cache row as they are stored, as floats
-__device__ __forceinline__ void load_cached8(const e4m3* p, float (&f)[8]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? v.x : v.y;
-    Num<__half>::unpack2(e4m3x2_to_half2(static_cast<uint16_t>(w >> (16 * (i & 1)))), f[2 * i], f[2 * i + 1]);
-  }
-}
+__device__ __forceinline__ void load_cached8(const e4m3* p, float (&f)[8]) { codes_to_floats(*reinterpret_cast<const uint2*>(p), f); }
 template <typename T>
 __device__ __forceinline__ void load_cached8(const T* p, float (&f)[8]) {
   load8<T>(p, f);

@@ -108,11 +108,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 mat
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// the lower and the upper two of four codes as halves
-__device__ __forceinline__ void codes_to_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
-}
-
 template <typename T, typename C, int HD, int NT>
 __global__ void __launch_bounds__((Shape<C, HD, NT>::kThreads), 1)
 paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const StreamParams p) {

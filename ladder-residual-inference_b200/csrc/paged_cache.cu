@@ -7,7 +7,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLargest = 448.f;            // of e4m3
 constexpr float kSmallest = 0x1p-100f;       // rows of smaller values are stored against it, so that no scale is zero or subnormal
-constexpr int kManyTokens = 1024;            // from here on a thread takes several tokens
+constexpr int kManyTokens = 1024;            // from here on a thread takes several tokens,
+constexpr int kRound = 4, kPerSm = 3;        // whole rounds of them, in as many CTAs an SM
+constexpr int kStoreSmem = 40 * 1024;        // of a CTA
 constexpr int kFillRows = 64;                // lri_paged_load: zeros up to a multiple of this
 
 struct StoreParams {
@@ -25,6 +27,7 @@ struct StoreParams {
   float *k_scale, *v_scale;
   int64_t tokens;
   int n_head, n_kv, dim;
+  int per;  // tokens of a CTA
 };
 
 // Rotation of elements e .. e + 7 of a head: pair i turns by the angle whose cosine and sine the table row holds at 2 i.  Products are
@@ -68,93 +71,130 @@ __device__ __forceinline__ void rotate8(int rot, int halves, int e, const TT* ro
   }
 }
 
-// LANES threads hold a head, eight elements each, of R tokens: blockIdx.y says which heads, blockIdx.x which tokens.  Bound by HBM for prompts:
-// what a thread reads does not wait for what says where it goes, and R tokens are on their way at once (8192 tokens of 32 + 2 x 8 heads of 128:
-// MEASURE_STORE).  For single tokens it is a chain of two loads and a store.
+// LANES threads hold a head, eight elements each; blockIdx.y says which heads, blockIdx.x which `per` tokens.  The CTA first finds out where its
+// tokens go and brings their rows of the table into shared memory, while the first rows of the projection are on their way; then R tokens at a
+// time, the next R asked for before.  Bound by HBM for prompts (8192 tokens of 32 + 2 x 8 heads of 128: MEASURE_STORE), where bytes in flight and
+// what is repeated for every vector count: with each token's place looked up by every thread, 186 instructions for a vector and 67 us.  For
+// single tokens it is a chain of three loads and a store.
 template <typename T, typename TT, bool E4M3, bool VECTORS, int LANES, int R>
-__global__ void __launch_bounds__(kThreads) rope_paged_store_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(const StoreParams p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  TT* table = reinterpret_cast<TT*>(smem_raw);                                                                     // [per][rot], VECTORS
+  int64_t* rows = reinterpret_cast<int64_t*>(smem_raw + (VECTORS ? p.per * p.rot * static_cast<int>(sizeof(TT)) : 0));  // [per]: of the token's first KV head, -1: skipped
+  int* positions = reinterpret_cast<int*>(rows + p.per);                                                           // [per]
   pdl_launch_dependents();
   pdl_wait();
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.per;
+  const int n = p.tokens - token0 < p.per ? static_cast<int>(p.tokens - token0) : p.per;
   const int at = blockIdx.y * blockDim.x + threadIdx.x, head = at / LANES, e = at % LANES * 8;
   const bool mine = head < p.n_head + 2 * p.n_kv && e < p.dim;
-  const bool turns = mine && head < p.n_head + p.n_kv && e < p.rot, is_v = head >= p.n_head + p.n_kv;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * R;
+  const bool turns = mine && head < p.n_head + p.n_kv && e < p.rot, is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
   const int half = p.rot >> 1;
+  const int h = head - p.n_head - (is_v ? p.n_kv : 0);
+  const T* src = static_cast<const T*>(p.qkv) + token0 * p.ld + static_cast<int64_t>(head) * p.dim + e;
+  T* q_dst = static_cast<T*>(p.q_out) + (token0 * p.n_head + head) * p.dim + e;
 
-  uint4 raw[R], pair[R];
-  int64_t pos[R], seq[R];
+  auto ask = [&](int t0, uint4 (&raw)[R]) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t token = token0 + r;
-    raw[r] = pair[r] = make_uint4(0, 0, 0, 0);
-    pos[r] = -1, seq[r] = token;
-    if (token >= p.tokens) continue;
-    pos[r] = load_pos(p.input_pos, p.pos_is_i64, token);
-    if (p.sequence) seq[r] = p.sequence[token];
-    if (!mine) continue;
-    const T* src = static_cast<const T*>(p.qkv) + token * p.ld + static_cast<int64_t>(head) * p.dim;
-    raw[r] = *reinterpret_cast<const uint4*>(src + e);
-    if (VECTORS && turns && p.halves) pair[r] = *reinterpret_cast<const uint4*>(src + (e < half ? e + half : e - half));
-  }
-  int page[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const bool there = pos[r] >= 0 && pos[r] < p.table.capacity() && (p.rot == 0 || pos[r] < p.table_rows) && seq[r] >= 0 && seq[r] < p.table.n_seq;
-    page[r] = there ? p.table.find(seq[r], static_cast<int>(pos[r])) : -1;
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t token = token0 + r;
-    const bool live = mine && page[r] >= 0;
-    float x[8], other[8];
-    unpack8<T>(raw[r], x);
-    unpack8<T>(pair[r], other);
-    if (live && turns) {
-      if (!VECTORS && p.halves) {
-        const T* src = static_cast<const T*>(p.qkv) + token * p.ld + static_cast<int64_t>(head) * p.dim;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) other[i] = e + i < p.rot ? Num<T>::to_f(src[e + i < half ? e + i + half : e + i - half]) : 0.f;
-      }
-      rotate8<TT, VECTORS>(p.rot, p.halves, e, static_cast<const TT*>(p.rope) + pos[r] * p.rot, other, x);
+    for (int r = 0; r < R; ++r) {
+      raw[r] = make_uint4(0, 0, 0, 0);
+      if (t0 + r < n && mine) raw[r] = *reinterpret_cast<const uint4*>(src + (t0 + r) * p.ld);
     }
-    if (live && head < p.n_head) store8<T>(static_cast<T*>(p.q_out) + (token * p.n_head + head) * p.dim + e, x);
-    const int h = head - p.n_head - (is_v ? p.n_kv : 0);
-    const int64_t row = live ? (static_cast<int64_t>(page[r]) * p.n_kv + h) * p.table.page + p.table.row_of(static_cast<int>(pos[r])) : 0;
-    if constexpr (!E4M3) {
-      if (live && head >= p.n_head) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + row * p.dim + e, x);
-    } else {
-      // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
-      // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
-      // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
-      float top = 0.f;
-      bool finite = true;
+  };
+  uint4 now[R], then[R];
+  ask(0, now);
+  ask(R, then);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t token = token0 + i, pos = load_pos(p.input_pos, p.pos_is_i64, token), seq = p.sequence ? p.sequence[token] : token;
+    int64_t row = -1;
+    if (pos >= 0 && pos < p.table.capacity() && (p.rot == 0 || pos < p.table_rows) && seq >= 0 && seq < p.table.n_seq) {
+      const int page = p.table.find(seq, static_cast<int>(pos));
+      if (page >= 0) row = static_cast<int64_t>(page) * p.n_kv * p.table.page + p.table.row_of(static_cast<int>(pos));
+    }
+    rows[i] = row;
+    positions[i] = row >= 0 ? static_cast<int>(pos) : -1;
+  }
+  __syncthreads();
+  if (VECTORS && p.rot > 0) {
+    constexpr int kVec = 16 / sizeof(TT);
+    const int vecs = p.rot / kVec;
+    for (int i = threadIdx.x; i < n * vecs; i += blockDim.x) {
+      const int t = i / vecs, c = i - t * vecs, pos = positions[t];
+      if (pos >= 0) reinterpret_cast<uint4*>(table)[i] = *reinterpret_cast<const uint4*>(static_cast<const TT*>(p.rope) + static_cast<int64_t>(pos) * p.rot + c * kVec);
+    }
+    __syncthreads();
+  }
+
+  auto process = [&](int t0, const uint4 (&raw)[R]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        top = fmaxf(top, fabsf(x[i]));
-        finite = finite && fabsf(x[i]) < INFINITY;
-      }
-      if (!finite) top = INFINITY;
+    for (int r = 0; r < R; ++r) {
+      if (t0 + r >= n) break;
+      int64_t row = rows[t0 + r];
+      if (row < 0) continue;  // the same in all threads
+      float x[8];
+      unpack8<T>(raw[r], x);
+      float other[8] = {};
+      if (p.halves) {
+        if (VECTORS) {  // in the lane that holds the other half's vector
+          const int lane = threadIdx.x & 31, from = turns ? lane + (e < half ? half >> 3 : -(half >> 3)) : lane;
+          uint4 o;
+          o.x = __shfl_sync(0xffffffffu, raw[r].x, from), o.y = __shfl_sync(0xffffffffu, raw[r].y, from);
+          o.z = __shfl_sync(0xffffffffu, raw[r].z, from), o.w = __shfl_sync(0xffffffffu, raw[r].w, from);
+          unpack8<T>(o, other);
+        } else if (turns) {
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!live || head < p.n_head) continue;
-      const bool whole = top < INFINITY;
-      top = fmaxf(top, kSmallest);
-      // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
-      const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
-      auto scaled = [&](float v) {
-        const float n = v * up, y = n * inv;
-        return fminf(fmaxf(fmaf(fmaf(-y, den, n), inv, y), -kLargest), kLargest);
-      };
-      uint32_t w[2] = {0u, 0u};
-      if (whole)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
-          w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
+          for (int i = 0; i < 8; ++i)
+            if (e + i < p.rot) other[i] = Num<T>::to_f(src[(t0 + r) * p.ld + i + (e + i < half ? half : -half)]);
         }
-      *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + row * p.dim + e) = make_uint2(w[0], w[1]);
-      if (e == 0) (is_v ? p.v_scale : p.k_scale)[row] = whole ? top / kLargest : NAN;
+      }
+      if (turns) {
+        const TT* angles = VECTORS ? table + (t0 + r) * p.rot : static_cast<const TT*>(p.rope) + static_cast<int64_t>(positions[t0 + r]) * p.rot;
+        rotate8<TT, VECTORS>(p.rot, p.halves, e, angles, other, x);
+      }
+      if (mine && is_q) store8<T>(q_dst + static_cast<int64_t>(t0 + r) * p.n_head * p.dim, x);
+      const int64_t to = (row + static_cast<int64_t>(h) * p.table.page) * p.dim + e;
+      if constexpr (!E4M3) {
+        if (mine && !is_q) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + to, x);
+      } else {
+        // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
+        // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
+        // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
+        float top = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          top = fmaxf(top, fabsf(x[i]));
+          finite = finite && fabsf(x[i]) < INFINITY;
+        }
+        if (!finite) top = INFINITY;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (!mine || is_q) continue;
+        const bool whole = top < INFINITY;
+        top = fmaxf(top, kSmallest);
+        // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
+        const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
+        auto scaled = [&](float v) {
+          const float num = v * up, y = num * inv;
+          return fminf(fmaxf(fmaf(fmaf(-y, den, num), inv, y), -kLargest), kLargest);
+        };
+        uint32_t w[2] = {0u, 0u};
+        if (whole)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
+            w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
+          }
+        *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + to) = make_uint2(w[0], w[1]);
+        if (e == 0) (is_v ? p.v_scale : p.k_scale)[row + static_cast<int64_t>(h) * p.table.page] = whole ? top / kLargest : NAN;
+      }
     }
+  };
+  for (int t0 = 0; t0 < n; t0 += 2 * R) {
+    process(t0, now);
+    ask(t0 + 2 * R, now);
+    process(t0 + R, then);
+    ask(t0 + 3 * R, then);
   }
 }
 
@@ -179,12 +219,14 @@ struct Raw8<e4m3> {
   using type = uint2;
 };
 
-// A CTA reads 64 positions of a (sequence, head); LANES threads hold a row, eight elements each.  Bound by HBM: all pages are looked up before
-// the first row is asked for, and all rows before the first is stored (MEASURE_LOAD).
+// A CTA reads 64 positions of a (sequence, head); LANES threads hold a row, eight elements each.  Bound by HBM: its first threads look the pages up and
+// fetch the scales, and all rows are asked for before the first is stored (eight users of 500 to 16000 positions from e4m3: MEASURE_LOAD).
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(kThreads) paged_load_kernel(const LoadParams p) {
   using V = typename Raw8<C>::type;
   constexpr int kRows = kThreads / LANES, R = kFillRows / kRows;
+  __shared__ int64_t at[kFillRows];   // of a row in the pages, -1: none
+  __shared__ float2 scales[kFillRows];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t b = blockIdx.z;
@@ -192,64 +234,75 @@ __global__ void __launch_bounds__(kThreads) paged_load_kernel(const LoadParams p
   int64_t last = load_pos(p.last_pos, p.pos_is_i64, b);
   const int64_t most = p.rows < p.table.capacity() ? p.rows : p.table.capacity();
   const int n = static_cast<int>(last < 0 ? 0 : (last >= most ? most : last + 1));
-  const int e = threadIdx.x % LANES * 8;
-  if (first >= n || e >= p.dim) return;
-  int page[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int pos = first + r * kRows + threadIdx.x / LANES;
-    page[r] = pos < n ? p.table.find(b, pos) : -1;
+  if (first >= n) return;
+  int64_t looked_up = -1;
+  if (threadIdx.x < kFillRows) {
+    const int pos = first + threadIdx.x, page = pos < n ? p.table.find(b, pos) : -1;
+    if (page >= 0) looked_up = (static_cast<int64_t>(page) * p.n_kv + h) * p.table.page + p.table.row_of(pos);
+    at[threadIdx.x] = looked_up;
   }
+  __syncthreads();
+  const int e = threadIdx.x % LANES * 8, t = threadIdx.x / LANES;
+  const bool mine = e < p.dim;
   V k[R], v[R];
-  float ks[R], vs[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    k[r] = v[r] = V{}, ks[r] = vs[r] = 0.f;
-    if (page[r] < 0) continue;
-    const int pos = first + r * kRows + threadIdx.x / LANES;
-    const int64_t row = (static_cast<int64_t>(page[r]) * p.n_kv + h) * p.table.page + p.table.row_of(pos);
-    k[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.k) + row * p.dim + e);
-    v[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.v) + row * p.dim + e);
-    if constexpr (sizeof(C) == 1) ks[r] = p.k_scale[row], vs[r] = p.v_scale[row];
+    const int64_t row = at[r * kRows + t];
+    k[r] = v[r] = V{};
+    if (row >= 0 && mine) {
+      k[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.k) + row * p.dim + e);
+      v[r] = *reinterpret_cast<const V*>(static_cast<const C*>(p.v) + row * p.dim + e);
+    }
   }
+  if constexpr (sizeof(C) == 1) {
+    if (threadIdx.x < kFillRows) scales[threadIdx.x] = looked_up >= 0 ? make_float2(p.k_scale[looked_up], p.v_scale[looked_up]) : make_float2(0.f, 0.f);
+    __syncthreads();
+  }
+  const int64_t to = ((b * p.n_kv + h) * p.rows + first + t) * p.dim + e;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t pos = first + r * kRows + threadIdx.x / LANES;
-    if (pos >= p.rows) continue;
-    const int64_t to = ((b * p.n_kv + h) * p.rows + pos) * p.dim + e;
+    if (!mine || first + r * kRows + t >= p.rows) continue;
+    T *k_out = static_cast<T*>(p.k_out) + to + r * kRows * p.dim, *v_out = static_cast<T*>(p.v_out) + to + r * kRows * p.dim;
     if constexpr (sizeof(C) == 1) {
-      auto scaled = [&](const V& codes, float scale, void* out) {
-        float x[8];
-        load_cached8(reinterpret_cast<const e4m3*>(&codes), x);
+      const float2 scale = scales[r * kRows + t];
+      float x[8], y[8];
+      codes_to_floats(k[r], x);
+      codes_to_floats(v[r], y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= scale;
-        store8<T>(static_cast<T*>(out) + to, x);
-      };
-      scaled(k[r], ks[r], p.k_out);
-      scaled(v[r], vs[r], p.v_out);
+      for (int i = 0; i < 8; ++i) x[i] *= scale.x, y[i] *= scale.y;
+      store8<T>(k_out, x);
+      store8<T>(v_out, y);
     } else {
-      *reinterpret_cast<V*>(static_cast<T*>(p.k_out) + to) = k[r];
-      *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + to) = v[r];
+      *reinterpret_cast<V*>(k_out) = k[r];
+      *reinterpret_cast<V*>(v_out) = v[r];
     }
   }
 }
 
 template <typename T, typename TT, bool E4M3, bool VECTORS>
-int launch_store(const StoreParams& p, cudaStream_t st) {
+int launch_store(StoreParams p, cudaStream_t st) {
   const int vecs = p.dim / 8;
-  auto go = [&](auto kern, int lanes, int tokens) {
+  auto go = [&](auto kern, int lanes, bool many) {
     const int threads = (p.n_head + 2 * p.n_kv) * lanes, blocks = (threads + kThreads - 1) / kThreads;
     const int block = ((threads + blocks - 1) / blocks + 31) / 32 * 32;
-    const int64_t grid = (p.tokens + tokens - 1) / tokens;
+    const int row = (VECTORS ? p.rot * static_cast<int>(sizeof(TT)) : 0) + 12;  // of shared memory
+    p.per = 1;
+    if (many) {
+      // CTAs for kPerSm on every SM, of whole rounds of tokens, that share the shared memory
+      const int64_t even = (p.tokens * blocks + static_cast<int64_t>(kPerSm) * device_sm_count() - 1) / (static_cast<int64_t>(kPerSm) * device_sm_count());
+      const int64_t most = kStoreSmem / row / kRound * kRound;
+      p.per = static_cast<int>(even < most ? (even + kRound - 1) / kRound * kRound : most);
+    }
+    const int64_t grid = (p.tokens + p.per - 1) / p.per;
     LRI_REQUIRE(grid < (1ll << 31) && blocks <= 65535, LRI_ERR_UNSUPPORTED, "rope_paged_store: %lld tokens of %d heads", (long long)p.tokens, p.n_head + 2 * p.n_kv);
-    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(blocks)), dim3(block), 0, st, p));
+    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(blocks)), dim3(block), static_cast<size_t>(p.per) * row, st, p));
     LRI_LAUNCH_CHECK("rope_paged_store_kernel");
     return static_cast<int>(LRI_OK);
   };
   const bool many = p.tokens >= kManyTokens;
-  if (vecs <= 8) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 4>, 8, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 1>, 8, 1);
-  if (vecs <= 16) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 4>, 16, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 1>, 16, 1);
-  return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 4>, 32, 4) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 1>, 32, 1);
+  if (vecs <= 8) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 4>, 8, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 1>, 8, false);
+  if (vecs <= 16) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 4>, 16, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 1>, 16, false);
+  return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 4>, 32, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 1>, 32, false);
 }
 
 template <typename T, typename TT>

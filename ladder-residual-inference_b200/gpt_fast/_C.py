@@ -175,6 +175,7 @@ for _name, (_res, _args) in _SIGNATURES.items():
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 BF16, FP16, FP32, E4M3 = 0, 1, 2, 3
+CODES = {torch.bfloat16: BF16, torch.float16: FP16}
 GATE_SIGMOID, GATE_SILU = 0, 1
 GEMM_AUTO, GEMM_TCGEN05, GEMM_SIMT = 0, 1, 2
 
@@ -192,11 +193,6 @@ def dtype_code_any(dtype: torch.dtype) -> int:
     return FP32 if dtype == torch.float32 else dtype_code(dtype)
 
 
-def cache_code(dtype: torch.dtype) -> int:
-    """dtype_code for the pages of a key-value cache, which may hold 8 bits."""
-    return E4M3 if dtype == torch.float8_e4m3fn else dtype_code(dtype)
-
-
 def check(status: int) -> None:
     if status < 0:
         raise RuntimeError(f"lri_b200 error {status}: {lib.lri_last_error().decode()}")
@@ -212,28 +208,22 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def address(t) -> int:
-    """ptr for a packed struct."""
-    return 0 if t is None else t.data_ptr()
-
-
 def stream_handle() -> int:
     # the stream object of torch.cuda.current_stream() costs a microsecond a launch
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def require_here(*tensors) -> None:
-    """require_cuda, and all of them on the current device: the launch goes to its current stream."""
-    at = -1
-    for t in tensors:
-        if t is None:
-            continue
-        device = t.get_device()
-        if device != at or device < 0:
-            require_cuda(t)
-            if at >= 0 or device != torch._C._cuda_getDevice():
-                raise RuntimeError(f"tensors must live on the current device (cuda:{torch._C._cuda_getDevice()}), not on cuda:{device}")
-            at = device
+def require_here(first, *others) -> None:
+    """require_cuda, and all of them (None: no tensor) on the current device: the launch goes to its current stream."""
+    here = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != here:
+            break
+    else:
+        if here >= 0 and here == torch._C._cuda_getDevice():
+            return
+    require_cuda(first, *others)
+    raise RuntimeError(f"tensors must live on the current device (cuda:{torch._C._cuda_getDevice()})")
 
 
 def require_cuda(*tensors) -> None:

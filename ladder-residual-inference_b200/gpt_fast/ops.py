@@ -124,45 +124,57 @@ class CudaOps:
 
 
     # ---- paged key-value cache ---------------------------------------------------------------------
+    # (A step of a small batch is bound by the host: what the caller has looked up of the shapes is handed on, 100 to 250 ns a look.)
     @staticmethod
-    def rope_paged_store(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale, n_head, halves):
+    def rope_paged_store(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale, n_head, halves, tokens, pages_shape,
+                         cache_shape):
         """table None: no rotation; its second extent is half of the elements that rotate."""
-        _C.require_here(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale)
-        n_pages, n_kv, page, dim = k_pages.shape
-        n_seq, most = pages.shape
-        rows = rot = f32 = 0
+        _C.require_here(qkv, input_pos, pages, q_out, k_pages, v_pages, table, sequence, k_scale, v_scale)
+        n_pages, n_kv, page, dim = cache_shape
+        n_seq, most = pages_shape
+        at = rows = rot = f32 = 0
         if table is not None:
             rows, half, _ = table.shape
-            rot, f32 = 2 * half, table.dtype == torch.float32
-        _C.check(_C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
-            qkv.data_ptr(), _C.address(table), input_pos.data_ptr(), _C.address(sequence), pages.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), _C.stream_handle(), qkv.stride(0), rows, pages.stride(0), n_pages,
-            qkv.shape[0], _C.dtype_code(qkv.dtype), _C.cache_code(k_pages.dtype), f32, rot, halves, input_pos.dtype == torch.int64, n_seq,
-            most, page, n_head, n_kv, dim)))
+            at, rot, f32 = table.data_ptr(), 2 * half, table.dtype is torch.float32
+        dtype = _C.CODES[qkv.dtype]
+        ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
+        status = _C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
+            qkv.data_ptr(), at, input_pos.data_ptr(), 0 if sequence is None else sequence.data_ptr(), pages.data_ptr(), q_out.data_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, _C.stream_handle(), qkv.stride(0), rows, pages.stride(0), n_pages, tokens, dtype,
+            cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
+        if status < 0:
+            _C.check(status)
 
     @staticmethod
     def paged_attn_workspace_bytes(n_head, n_kv, head_dim):
         return _C.lib.lri_paged_attn_decode_workspace_bytes(n_head, n_kv, head_dim)
 
     @staticmethod
-    def paged_attention(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, window, scale, out, n_head, workspace):
-        _C.require_here(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, out, workspace)
-        n_pages, n_kv, page, dim = k_pages.shape
-        n_seq, most = pages.shape
-        _C.check(_C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), pages.data_ptr(), input_pos.data_ptr(),
-            out.data_ptr(), workspace.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), window, workspace.numel(), _C.dtype_code(q.dtype),
-            _C.cache_code(k_pages.dtype), page, n_seq, most, input_pos.dtype == torch.int64, n_head, n_kv, dim, scale)))
+    def paged_attention(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, window, scale, out, workspace, n_head, pages_shape, cache_shape):
+        _C.require_here(q, pages, input_pos, out, workspace, k_pages, v_pages, k_scale, v_scale)
+        n_pages, n_kv, page, dim = cache_shape
+        n_seq, most = pages_shape
+        dtype = _C.CODES[q.dtype]
+        ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
+        status = _C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), input_pos.data_ptr(), out.data_ptr(),
+            workspace.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), window, workspace.numel(), dtype, cache_dtype, page, n_seq, most,
+            input_pos.dtype is torch.int64, n_head, n_kv, dim, scale))
+        if status < 0:
+            _C.check(status)
 
     @staticmethod
-    def paged_load(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out):
-        _C.require_here(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out)
-        n_pages, n_kv, page, dim = k_pages.shape
-        n_seq, most = pages.shape
-        _C.check(_C.lib.lri_paged_load(_C.LOAD_CALL.pack(
-            k_pages.data_ptr(), v_pages.data_ptr(), _C.address(k_scale), _C.address(v_scale), pages.data_ptr(), last_pos.data_ptr(),
-            k_out.data_ptr(), v_out.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), k_out.shape[2], _C.dtype_code(k_out.dtype),
-            _C.cache_code(k_pages.dtype), page, n_seq, most, last_pos.dtype == torch.int64, n_kv, dim)))
+    def paged_load(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out, rows, pages_shape, cache_shape):
+        _C.require_here(k_pages, v_pages, pages, last_pos, k_out, v_out, k_scale, v_scale)
+        n_pages, n_kv, page, dim = cache_shape
+        n_seq, most = pages_shape
+        dtype = _C.CODES[k_out.dtype]
+        ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
+        status = _C.lib.lri_paged_load(_C.LOAD_CALL.pack(
+            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), last_pos.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+            _C.stream_handle(), n_pages, pages.stride(0), rows, dtype, cache_dtype, page, n_seq, most, last_pos.dtype is torch.int64, n_kv, dim))
+        if status < 0:
+            _C.check(status)
 
     # ---- all layers of a pass ------------------------------------------------------------------------
     @staticmethod

@@ -21,10 +21,12 @@ def _said(t):
     return f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}"
 
 
-def _check_rows(rows, input_pos, pages):
-    if not ((input_pos.dtype is torch.int32 or input_pos.dtype is torch.int64) and input_pos.shape == (rows,) and input_pos.is_contiguous()):
+def _check_rows(rows, input_pos, pages, pages_shape):
+    dtype = input_pos.dtype
+    if not ((dtype is torch.int32 or dtype is torch.int64) and input_pos.shape == (rows,) and input_pos.is_contiguous()):
         raise ValueError(f"positions: {rows} contiguous int32 or int64 numbers, not {_said(input_pos)}")
-    if not (pages.dtype is torch.int32 and pages.dim() == 2 and pages.shape[1] >= 1 and (pages.is_contiguous() or pages.stride(1) == 1 <= pages.stride(0))):
+    if not (pages.dtype is torch.int32 and len(pages_shape) == 2 and pages_shape[1] >= 1 and
+            (pages.is_contiguous() or pages.stride(1) == 1 <= pages.stride(0))):
         raise ValueError(f"pages: an int32 table [sequences, most pages] with contiguous rows, not {_said(pages)}")
 
 
@@ -65,15 +67,16 @@ class PagedKVCache(nn.Module):
         without their meaning."""
         b = self._buffers
         k, v, ks, vs = b["k_pages"], b["v_pages"], b["k_scale"], b["v_scale"]
-        ok = k.dtype is v.dtype and k.shape == v.shape and k.is_contiguous() and v.is_contiguous()
+        dtype, shape = k.dtype, k.shape
+        ok = dtype is v.dtype and shape == v.shape and k.is_contiguous() and v.is_contiguous()
         if ks is None:
-            ok = ok and vs is None and k.dtype is self.dtype
+            ok = ok and vs is None and dtype is self.dtype
         else:
-            ok = (ok and vs is not None and k.dtype is _E4M3 and ks.dtype is vs.dtype is torch.float32 and ks.shape == vs.shape == k.shape[:3] and
+            ok = (ok and vs is not None and dtype is _E4M3 and ks.dtype is vs.dtype is torch.float32 and ks.shape == vs.shape == shape[:3] and
                   ks.is_contiguous() and vs.is_contiguous())
         if not ok:
             raise ValueError(f"contiguous pages of {self.dtype} without scales, or of float8_e4m3fn with fp32 scales [n_pages, n_heads, page_size]")
-        return k, v, ks, vs
+        return k, v, ks, vs, shape
 
     def store(self, qkv: Tensor, table: Optional[Tensor], input_pos: Tensor, pages: Tensor, n_head: int,
               sequence: Optional[Tensor] = None, halves: bool = False, out: Optional[Tensor] = None) -> Tensor:
@@ -83,25 +86,27 @@ class PagedKVCache(nn.Module):
         fp32, None for no rotation: the first rot elements of a head turn, in adjacent pairs (utils.precompute_freqs_cis) or in halves.
         A token without a position (negative, behind the table) or without a page is left out, its query row too.  One call
         may name a (sequence, position) once."""
-        k, v, ks, vs = self._tensors()
-        _, n_kv, _, dim = k.shape
-        dtype = self.dtype
-        if not (qkv.dim() == 2 and n_head >= 1 and qkv.shape[1] == (n_head + 2 * n_kv) * dim and qkv.dtype is dtype and
+        k, v, ks, vs, cache_shape = self._tensors()
+        _, n_kv, _, dim = cache_shape
+        dtype, shape, pages_shape = self.dtype, qkv.shape, pages.shape
+        if not (len(shape) == 2 and n_head >= 1 and shape[1] == (n_head + 2 * n_kv) * dim and qkv.dtype is dtype and
                 (qkv.is_contiguous() or qkv.stride(1) == 1)):
             raise ValueError(f"qkv: rows of {n_head} + 2 * {n_kv} heads of {dim} in {dtype}, not {_said(qkv)}")
-        tokens = qkv.shape[0]
-        _check_rows(tokens, input_pos, pages)
-        if not (tokens == pages.shape[0] if sequence is None else
+        tokens = shape[0]
+        _check_rows(tokens, input_pos, pages, pages_shape)
+        if not (tokens == pages_shape[0] if sequence is None else
                 sequence.dtype is torch.int32 and sequence.shape == (tokens,) and sequence.is_contiguous()):
-            raise ValueError(f"sequence: {tokens} contiguous int32 numbers, or None for one token of each of {pages.shape[0]} sequences")
-        if table is not None and not (table.dim() == 3 and table.shape[2] == 2 and 2 <= 2 * table.shape[1] <= dim and table.is_contiguous() and
-                                      (table.dtype is dtype or table.dtype is torch.float32)):
-            raise ValueError(f"table: [positions, rot / 2, 2] in {dtype} or float32, rot up to {dim}, not {_said(table)}")
+            raise ValueError(f"sequence: {tokens} contiguous int32 numbers, or None for one token of each of {pages_shape[0]} sequences")
+        if table is not None:
+            shape = table.shape
+            if not (len(shape) == 3 and shape[2] == 2 and 2 <= 2 * shape[1] <= dim and table.is_contiguous() and
+                    (table.dtype is dtype or table.dtype is torch.float32)):
+                raise ValueError(f"table: [positions, rot / 2, 2] in {dtype} or float32, rot up to {dim}, not {_said(table)}")
         if out is None:
-            out = torch.empty(tokens, n_head, dim, dtype=dtype, device=qkv.device)
+            out = qkv.new_empty((tokens, n_head, dim))
         else:
             _check_like(out, dtype, (tokens, n_head, dim))
-        self.ops.rope_paged_store(qkv, table, input_pos, sequence, pages, out, k, v, ks, vs, n_head, halves)
+        self.ops.rope_paged_store(qkv, table, input_pos, sequence, pages, out, k, v, ks, vs, n_head, bool(halves), tokens, pages_shape, cache_shape)
         return out
 
     def attend_workspace(self, n_head: int) -> Tensor:
@@ -114,14 +119,15 @@ class PagedKVCache(nn.Module):
         """Attention of one new token of each sequence, whose row is in the cache: q [sequences, n_head, head_dim] over positions
         0 .. input_pos[b] (the last `window` of them if it is not 0); zeros where that is none.  scale: 1 / sqrt(head_dim) by default.
         workspace: from attend_workspace(n_head); allocated for the call if None."""
-        k, v, ks, vs = self._tensors()
-        _, n_kv, _, dim = k.shape
-        if not (q.dim() == 3 and q.dtype is self.dtype and q.is_contiguous() and q.shape[2] == dim and q.shape[1] >= 1 and q.shape[1] % n_kv == 0):
+        k, v, ks, vs, cache_shape = self._tensors()
+        _, n_kv, _, dim = cache_shape
+        shape, pages_shape = q.shape, pages.shape
+        if not (len(shape) == 3 and q.dtype is self.dtype and q.is_contiguous() and shape[2] == dim and shape[1] >= 1 and shape[1] % n_kv == 0):
             raise ValueError(f"q: contiguous [sequences, a multiple of {n_kv}, {dim}] in {self.dtype}, not {_said(q)}")
-        n_seq, n_head, _ = q.shape
-        _check_rows(n_seq, input_pos, pages)
-        if pages.shape[0] != n_seq:
-            raise ValueError(f"pages of {pages.shape[0]} sequences for {n_seq}")
+        n_seq, n_head, _ = shape
+        _check_rows(n_seq, input_pos, pages, pages_shape)
+        if pages_shape[0] != n_seq:
+            raise ValueError(f"pages of {pages_shape[0]} sequences for {n_seq}")
         if not 0 <= window < 1 << 62:
             raise ValueError(f"window={window}")
         if workspace is None:
@@ -131,8 +137,9 @@ class PagedKVCache(nn.Module):
         if out is None:
             out = torch.empty_like(q)
         else:
-            _check_like(out, q.dtype, q.shape)
-        self.ops.paged_attention(q, k, v, ks, vs, pages, input_pos, window, dim ** -0.5 if scale is None else scale, out, n_head, workspace)
+            _check_like(out, q.dtype, shape)
+        self.ops.paged_attention(q, k, v, ks, vs, pages, input_pos, window, dim ** -0.5 if scale is None else scale, out, workspace, n_head, pages_shape,
+                                 cache_shape)
         return out
 
     def load(self, last_pos: Tensor, pages: Tensor, rows: Optional[int] = None, out: Optional[Tuple[Tensor, Tensor]] = None):
@@ -140,18 +147,18 @@ class PagedKVCache(nn.Module):
         type, as KVCache holds them: what prompt attention works on.  `out` is written in place: rows behind the last position up to
         a multiple of 64 become zeros, later ones stay as they were.  Without it caches of `rows` positions (default: all that the
         table's pages hold) are made, zero behind the last position."""
-        k, v, ks, vs = self._tensors()
-        _, n_kv, page, dim = k.shape
-        n_seq = pages.shape[0]
-        _check_rows(n_seq, last_pos, pages)
+        k, v, ks, vs, cache_shape = self._tensors()
+        _, n_kv, page, dim = cache_shape
+        pages_shape = pages.shape
+        n_seq = pages_shape[0] if len(pages_shape) else 0
+        _check_rows(n_seq, last_pos, pages, pages_shape)
         if out is None:
-            shape = (n_seq, n_kv, pages.shape[1] * page if rows is None else rows, dim)
+            shape = (n_seq, n_kv, pages_shape[1] * page if rows is None else rows, dim)
             out = torch.zeros(shape, dtype=self.dtype, device=k.device), torch.zeros(shape, dtype=self.dtype, device=k.device)
         k_out, v_out = out
-        if k_out.dim() != 4:
-            raise ValueError(f"out: two caches [{n_seq}, {n_kv}, rows, {dim}], not {_said(k_out)}")
-        shape = (n_seq, n_kv, k_out.shape[2], dim)
+        rows = k_out.shape[2] if k_out.dim() == 4 else -1
+        shape = (n_seq, n_kv, rows, dim)
         _check_like(k_out, self.dtype, shape)
         _check_like(v_out, self.dtype, shape)
-        self.ops.paged_load(k, v, ks, vs, pages, last_pos, k_out, v_out)
+        self.ops.paged_load(k, v, ks, vs, pages, last_pos, k_out, v_out, rows, pages_shape, cache_shape)
         return out
