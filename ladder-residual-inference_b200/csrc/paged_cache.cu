@@ -7,8 +7,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLargest = 448.f;            // of e4m3
 constexpr float kSmallest = 0x1p-100f;       // rows of smaller values are stored against it, so that no scale is zero or subnormal
-constexpr int kManyTokens = 1024;            // from here on a thread takes several tokens,
-constexpr int kRound = 4, kPerSm = 3;        // whole rounds of them, in as many CTAs an SM
+constexpr int kPerSm = 3;                    // CTAs that store, on an SM
 constexpr int kStoreSmem = 40 * 1024;        // of a CTA
 constexpr int kFillRows = 64;                // lri_paged_load: zeros up to a multiple of this
 
@@ -30,44 +29,63 @@ struct StoreParams {
   int per;  // tokens of a CTA
 };
 
+// Pieces of 16 bytes from one row of the table to the next in shared memory.
+__host__ __device__ __forceinline__ int table_pitch(int rot, int size) { return (rot * size / 16 + 3) / 4 * 4; }
+
 // Rotation of elements e .. e + 7 of a head: pair i turns by the angle whose cosine and sine the table row holds at 2 i.  Products are
 // rounded before they are added (no contraction), so that a result does not depend on the layout or on the kernel.
-// Halves: `other` holds the elements that these are paired with.  VECTORS: eight elements have their table entries and partners in whole vectors.
-template <typename TT, bool VECTORS>
-__device__ __forceinline__ void rotate8(int rot, int halves, int e, const TT* row, const float (&other)[8], float (&x)[8]) {
-  if constexpr (VECTORS) {
-    if (!halves) {
-      float cs[8];
-      load8<TT>(row + e, cs);
+// Halves: `other` holds the elements that these are paired with.
+// In whole vectors, with the row of the table in shared memory: 16-byte piece q of a row lies at place_of(q), so that threads that read 16, 32 or 64
+// bytes each, one behind the other, find them in different banks (fp32 halves in plain order took a wavefront for every two threads).
+__device__ __forceinline__ int place_of(int q) { return q ^ ((q >> 3) & 3); }
+template <typename TT>
+__device__ __forceinline__ void rotate8_vectors(int rot, int halves, int e, const TT* row, const float (&other)[8], float (&x)[8]) {
+  constexpr int kPiece = 16 / sizeof(TT), N = 8 / kPiece;  // entries of a piece, pieces of eight entries
+  auto fetch = [&](int entry, float (&f)[8]) {
+    TT raw[8];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) rope_pair(x[i], x[i + 1], cs[i], cs[i + 1], x[i], x[i + 1]);
-    } else {
-      const bool low = e < rot >> 1;
-      const TT* at = row + 2 * (low ? e : e - (rot >> 1));
-      float cs[2][8];
-      load8<TT>(at, cs[0]);
-      load8<TT>(at + 8, cs[1]);
+    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(row)[place_of(entry / kPiece + i)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float a, b;
-        rope_pair(low ? x[i] : other[i], low ? other[i] : x[i], cs[i >> 2][2 * (i & 3)], cs[i >> 2][2 * (i & 3) + 1], a, b);
-        x[i] = low ? a : b;
-      }
+    for (int i = 0; i < 8; ++i) f[i] = Num<TT>::to_f(raw[i]);
+  };
+  float cs[8];
+  if (!halves) {
+    fetch(e, cs);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) rope_pair(x[i], x[i + 1], cs[i], cs[i + 1], x[i], x[i + 1]);
+    return;
+  }
+  const bool low = e < rot >> 1;
+  const int pair = low ? e : e - (rot >> 1);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    fetch(2 * pair + 8 * k, cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      const float mine = x[4 * k + i], its = other[4 * k + i];
+      rope_pair(low ? mine : its, low ? its : mine, cs[2 * i], cs[2 * i + 1], a, b);
+      x[4 * k + i] = low ? a : b;
     }
-  } else if (!halves) {
+  }
+}
+// of any sizes, from the table itself
+template <typename TT>
+__device__ __forceinline__ void rotate8_any(int rot, int halves, int e, const TT* row, const float (&other)[8], float (&x)[8]) {
+  if (!halves) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2)
       if (e + i < rot) rope_pair(x[i], x[i + 1], Num<TT>::to_f(row[e + i]), Num<TT>::to_f(row[e + i + 1]), x[i], x[i + 1]);
-  } else {
+    return;
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (e + i >= rot) continue;
-      const bool low = e + i < rot >> 1;
-      const int pair = low ? e + i : e + i - (rot >> 1);
-      float a, b;
-      rope_pair(low ? x[i] : other[i], low ? other[i] : x[i], Num<TT>::to_f(row[2 * pair]), Num<TT>::to_f(row[2 * pair + 1]), a, b);
-      x[i] = low ? a : b;
-    }
+  for (int i = 0; i < 8; ++i) {
+    if (e + i >= rot) continue;
+    const bool low = e + i < rot >> 1;
+    const int pair = low ? e + i : e + i - (rot >> 1);
+    float a, b;
+    rope_pair(low ? x[i] : other[i], low ? other[i] : x[i], Num<TT>::to_f(row[2 * pair]), Num<TT>::to_f(row[2 * pair + 1]), a, b);
+    x[i] = low ? a : b;
   }
 }
 
@@ -79,9 +97,10 @@ __device__ __forceinline__ void rotate8(int rot, int halves, int e, const TT* ro
 template <typename T, typename TT, bool E4M3, bool VECTORS, int LANES, int R>
 __global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(const StoreParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  TT* table = reinterpret_cast<TT*>(smem_raw);                                                                     // [per][rot], VECTORS
-  int64_t* rows = reinterpret_cast<int64_t*>(smem_raw + (VECTORS ? p.per * p.rot * static_cast<int>(sizeof(TT)) : 0));  // [per]: of the token's first KV head, -1: skipped
-  int* positions = reinterpret_cast<int*>(rows + p.per);                                                           // [per]
+  uint4* table = reinterpret_cast<uint4*>(smem_raw);                                    // [per][pitch] pieces, VECTORS
+  const int pitch = VECTORS ? table_pitch(p.rot, sizeof(TT)) : 0;
+  int64_t* rows = reinterpret_cast<int64_t*>(smem_raw + static_cast<size_t>(p.per) * pitch * 16);  // [per]: of the token's first KV head, -1: skipped
+  int* positions = reinterpret_cast<int*>(rows + p.per);                                // [per]
   pdl_launch_dependents();
   pdl_wait();
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.per;
@@ -116,11 +135,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(cons
   }
   __syncthreads();
   if (VECTORS && p.rot > 0) {
-    constexpr int kVec = 16 / sizeof(TT);
-    const int vecs = p.rot / kVec;
-    for (int i = threadIdx.x; i < n * vecs; i += blockDim.x) {
-      const int t = i / vecs, c = i - t * vecs, pos = positions[t];
-      if (pos >= 0) reinterpret_cast<uint4*>(table)[i] = *reinterpret_cast<const uint4*>(static_cast<const TT*>(p.rope) + static_cast<int64_t>(pos) * p.rot + c * kVec);
+    constexpr int kPiece = 16 / sizeof(TT);
+    const int pieces = p.rot / kPiece;
+    for (int i = threadIdx.x; i < n * pieces; i += blockDim.x) {
+      const int t = i / pieces, q = i - t * pieces, pos = positions[t];
+      if (pos >= 0) table[t * pitch + place_of(q)] = *reinterpret_cast<const uint4*>(static_cast<const TT*>(p.rope) + static_cast<int64_t>(pos) * p.rot + q * kPiece);
     }
     __syncthreads();
   }
@@ -148,44 +167,40 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(cons
         }
       }
       if (turns) {
-        const TT* angles = VECTORS ? table + (t0 + r) * p.rot : static_cast<const TT*>(p.rope) + static_cast<int64_t>(positions[t0 + r]) * p.rot;
-        rotate8<TT, VECTORS>(p.rot, p.halves, e, angles, other, x);
+        if (VECTORS) rotate8_vectors<TT>(p.rot, p.halves, e, reinterpret_cast<const TT*>(table + (t0 + r) * pitch), other, x);
+        else rotate8_any<TT>(p.rot, p.halves, e, static_cast<const TT*>(p.rope) + static_cast<int64_t>(positions[t0 + r]) * p.rot, other, x);
       }
-      if (mine && is_q) store8<T>(q_dst + static_cast<int64_t>(t0 + r) * p.n_head * p.dim, x);
+      if (is_q) {
+        if (mine) store8<T>(q_dst + static_cast<int64_t>(t0 + r) * p.n_head * p.dim, x);
+        continue;
+      }
       const int64_t to = (row + static_cast<int64_t>(h) * p.table.page) * p.dim + e;
       if constexpr (!E4M3) {
-        if (mine && !is_q) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + to, x);
+        if (mine) store8<T>(static_cast<T*>(is_v ? p.v : p.k) + to, x);
       } else {
         // The largest magnitude of the row goes to 448, the largest number of e4m3.  Each element is rounded from the rotated value in 32 bits,
         // divided exactly: rows of 16-bit values hit the midpoints between codes, which a product with the rounded reciprocal moves to either
-        // side.  A row with an infinity or a NaN has no scale: it reads back as NaN.
-        float top = 0.f;
-        bool finite = true;
+        // side.  A row with an infinity or a NaN, whose bits are larger than any number's, has no scale: it reads back as NaN.
+        uint32_t bits = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          top = fmaxf(top, fabsf(x[i]));
-          finite = finite && fabsf(x[i]) < INFINITY;
-        }
-        if (!finite) top = INFINITY;
+        for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(x[i]) & 0x7fffffffu);
+        const uint32_t lanes = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));  // of this head
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (!mine || is_q) continue;
-        const bool whole = top < INFINITY;
-        top = fmaxf(top, kSmallest);
+        for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(lanes, bits, o));
+        if (!mine) continue;
+        const bool whole = bits < 0x7f800000u;
+        const float top = fmaxf(__uint_as_float(bits), kSmallest);
         // x * 448 / top: a quotient of two roundings, mended by its remainder (Markstein); both sides smaller where 448 x would overflow
         const float down = top > 0x1p100f ? 0x1p-64f : 1.f, den = top * down, inv = 1.f / den, up = kLargest * down;
         auto scaled = [&](float v) {
           const float num = v * up, y = num * inv;
-          return fminf(fmaxf(fmaf(fmaf(-y, den, num), inv, y), -kLargest), kLargest);
+          return fmaf(fmaf(-y, den, num), inv, y);
         };
-        uint32_t w[2] = {0u, 0u};
-        if (whole)
+        uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 y = make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1]));
-            w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
-          }
-        *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + to) = make_uint2(w[0], w[1]);
+        for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(scaled(x[2 * i]), scaled(x[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+        const uint2 codes = whole ? make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16) : make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(static_cast<e4m3*>(is_v ? p.v : p.k) + to) = codes;
         if (e == 0) (is_v ? p.v_scale : p.k_scale)[row + static_cast<int64_t>(h) * p.table.page] = whole ? top / kLargest : NAN;
       }
     }
@@ -282,27 +297,24 @@ __global__ void __launch_bounds__(kThreads) paged_load_kernel(const LoadParams p
 template <typename T, typename TT, bool E4M3, bool VECTORS>
 int launch_store(StoreParams p, cudaStream_t st) {
   const int vecs = p.dim / 8;
-  auto go = [&](auto kern, int lanes, bool many) {
-    const int threads = (p.n_head + 2 * p.n_kv) * lanes, blocks = (threads + kThreads - 1) / kThreads;
+  const int lanes = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+  const int threads = (p.n_head + 2 * p.n_kv) * lanes, blocks = (threads + kThreads - 1) / kThreads;
+  // kPerSm CTAs on every SM share the tokens, as far as shared memory holds their table rows.  With no more than that a thread has one token.
+  const int64_t even = (p.tokens * blocks + static_cast<int64_t>(kPerSm) * device_sm_count() - 1) / (static_cast<int64_t>(kPerSm) * device_sm_count());
+  const bool many = even > 1;
+  auto go = [&](auto kern) {
     const int block = ((threads + blocks - 1) / blocks + 31) / 32 * 32;
-    const int row = (VECTORS ? p.rot * static_cast<int>(sizeof(TT)) : 0) + 12;  // of shared memory
-    p.per = 1;
-    if (many) {
-      // CTAs for kPerSm on every SM, of whole rounds of tokens, that share the shared memory
-      const int64_t even = (p.tokens * blocks + static_cast<int64_t>(kPerSm) * device_sm_count() - 1) / (static_cast<int64_t>(kPerSm) * device_sm_count());
-      const int64_t most = kStoreSmem / row / kRound * kRound;
-      p.per = static_cast<int>(even < most ? (even + kRound - 1) / kRound * kRound : most);
-    }
+    const int row = (VECTORS ? table_pitch(p.rot, sizeof(TT)) * 16 : 0) + 12;  // of shared memory
+    p.per = many ? static_cast<int>(even < kStoreSmem / row ? even : kStoreSmem / row) : 1;
     const int64_t grid = (p.tokens + p.per - 1) / p.per;
     LRI_REQUIRE(grid < (1ll << 31) && blocks <= 65535, LRI_ERR_UNSUPPORTED, "rope_paged_store: %lld tokens of %d heads", (long long)p.tokens, p.n_head + 2 * p.n_kv);
     LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(blocks)), dim3(block), static_cast<size_t>(p.per) * row, st, p));
     LRI_LAUNCH_CHECK("rope_paged_store_kernel");
     return static_cast<int>(LRI_OK);
   };
-  const bool many = p.tokens >= kManyTokens;
-  if (vecs <= 8) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 4>, 8, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 1>, 8, false);
-  if (vecs <= 16) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 4>, 16, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 1>, 16, false);
-  return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 4>, 32, true) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 1>, 32, false);
+  if (lanes == 8) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 2>) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 8, 1>);
+  if (lanes == 16) return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 2>) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 16, 1>);
+  return many ? go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 2>) : go(rope_paged_store_kernel<T, TT, E4M3, VECTORS, 32, 1>);
 }
 
 template <typename T, typename TT>
