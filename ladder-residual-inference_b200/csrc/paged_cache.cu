@@ -34,7 +34,7 @@ __host__ __device__ __forceinline__ int table_pitch(int rot, int size) { return 
 
 // Rotation of elements e .. e + 7 of a head: pair i turns by the angle whose cosine and sine the table row holds at 2 i.  Products are
 // rounded before they are added (no contraction), so that a result does not depend on the layout or on the kernel.
-// Halves: `other` holds the elements that these are paired with.
+// Halves: `other` holds the elements that these are paired with, negated (rotate8_vectors) in the lower half.
 // In whole vectors, with the row of the table in shared memory: 16-byte piece q of a row lies at place_of(q), so that threads that read 16, 32 or 64
 // bytes each, one behind the other, find them in different banks (fp32 halves in plain order took a wavefront for every two threads).
 __device__ __forceinline__ int place_of(int q) { return q ^ ((q >> 3) & 3); }
@@ -55,18 +55,13 @@ __device__ __forceinline__ void rotate8_vectors(int rot, int halves, int e, cons
     for (int i = 0; i < 8; i += 2) rope_pair(x[i], x[i + 1], cs[i], cs[i + 1], x[i], x[i + 1]);
     return;
   }
-  const bool low = e < rot >> 1;
-  const int pair = low ? e : e - (rot >> 1);
+  // x0 c - x1 s and x1 c + x0 s are one formula where the partners of the lower half come with their signs turned
+  const int pair = e < rot >> 1 ? e : e - (rot >> 1);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     fetch(2 * pair + 8 * k, cs);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a, b;
-      const float mine = x[4 * k + i], its = other[4 * k + i];
-      rope_pair(low ? mine : its, low ? its : mine, cs[2 * i], cs[2 * i + 1], a, b);
-      x[4 * k + i] = low ? a : b;
-    }
+    for (int i = 0; i < 4; ++i) x[4 * k + i] = __fadd_rn(__fmul_rn(x[4 * k + i], cs[2 * i]), __fmul_rn(other[4 * k + i], cs[2 * i + 1]));
   }
 }
 // of any sizes, from the table itself
@@ -159,6 +154,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(cons
           uint4 o;
           o.x = __shfl_sync(0xffffffffu, raw[r].x, from), o.y = __shfl_sync(0xffffffffu, raw[r].y, from);
           o.z = __shfl_sync(0xffffffffu, raw[r].z, from), o.w = __shfl_sync(0xffffffffu, raw[r].w, from);
+          const uint32_t sign = e < half ? 0x80008000u : 0u;
+          o.x ^= sign, o.y ^= sign, o.z ^= sign, o.w ^= sign;
           unpack8<T>(o, other);
         } else if (turns) {
 #pragma unroll
