@@ -38,6 +38,7 @@ constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of
 constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
 constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
 constexpr int kMaxCtas = 256;
+constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once
 constexpr size_t kCounterBytes = kMaxCtas * 4;
 
 struct StreamParams {
@@ -198,11 +199,11 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     if (threadIdx.x == 0) before[n_seq] = units, line[n_seq] = length;
     __syncthreads();
   }
-  // CTA c of those that have work takes length c / ctas .. of the line
-  const int ctas = length < static_cast<int64_t>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
-  const int me = blockIdx.x;
-  auto line_of = [&](int c) { return static_cast<int>(static_cast<int64_t>(length) * c / ctas); };
-  auto cta_at = [&](int at) { return static_cast<int>((static_cast<int64_t>(at + 1) * ctas - 1) / length); };
+  // The CTAs that have work take equal stretches of the line, the first `longer` of them one more.
+  const int ctas = length < static_cast<int>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
+  const int me = blockIdx.x, stretch = ctas > 0 ? length / ctas : 1, longer = length - stretch * ctas;
+  auto line_of = [&](int c) { return stretch * c + (c < longer ? c : longer); };
+  auto cta_at = [&](int at) { return at < (stretch + 1) * longer ? at / (stretch + 1) : (at - longer) / stretch; };
   int u0 = 0, u1 = 0, cta0 = 0, cta1 = 0;  // units of this warp, of this CTA
   if (me < ctas) {
     // lanes 0 .. 3: the first unit at or behind a place
@@ -677,25 +678,36 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       // part 0 is the last of its CTA unless the unit in front of it lies before that CTA's stretch; part i > 0 the first of its CTA
       const int64_t at0 = static_cast<int64_t>(shared_from[k]) * 2 * heads;
       const int64_t at_first = at0 + (pair_of[k].line > 0 && pair_of[k].line - kGap - kStep >= line_of(shared_from[k]) ? heads : 0);
-      float2* ml = reinterpret_cast<float2*>(rings);  // [n][g]
-      __syncthreads();
-      for (int i = threadIdx.x; i < n * g; i += S::kThreads) {
-        const int c = i / g;
-        ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((c ? at0 + static_cast<int64_t>(c) * 2 * heads : at_first) + i % g) * 2));
-      }
-      __syncthreads();
       for (int idx = threadIdx.x; idx < g * (HD / 4); idx += S::kThreads) {
         const int i = idx / (HD / 4), e = idx % (HD / 4) * 4;
-        float mm = -INFINITY;
-        for (int c = 0; c < n; ++c) mm = fmaxf(mm, ml[c * g + i].x);
-        const float m_use = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f, v[4] = {};
-#pragma unroll 10
-        for (int c = 0; c < n; ++c) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c ? at0 + static_cast<int64_t>(c) * 2 * heads : at_first) + i) * HD + e));
-          const float f = exp2f(ml[c * g + i].x - m_use);
-          ll += ml[c * g + i].y * f;
-          v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
+        float mm = -INFINITY, ll = 0.f, v[4] = {};
+        for (int c0 = 0; c0 < n; c0 += kJoin) {  // kJoin parts on their way at once
+          float2 ml[kJoin];
+          float4 x[kJoin];
+#pragma unroll
+          for (int c = 0; c < kJoin; ++c) {
+            if (c0 + c < n) {
+              const int64_t at = (c0 + c ? at0 + static_cast<int64_t>(c0 + c) * 2 * heads : at_first) + i;
+              ml[c] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+              x[c] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + e));
+            } else {
+              ml[c] = make_float2(-INFINITY, 0.f), x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+          float m_new = mm;
+#pragma unroll
+          for (int c = 0; c < kJoin; ++c) m_new = fmaxf(m_new, ml[c].x);
+          const float m_use = m_new == -INFINITY ? 0.f : m_new, old = exp2f(mm - m_use);
+          mm = m_new;
+          ll *= old;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) v[d] *= old;
+#pragma unroll
+          for (int c = 0; c < kJoin; ++c) {
+            const float f = exp2f(ml[c].x - m_use);
+            ll += ml[c].y * f;
+            v[0] += x[c].x * f, v[1] += x[c].y * f, v[2] += x[c].z * f, v[3] += x[c].w * f;
+          }
         }
         store4(pair_of[k].row, i, e, ll, v);
       }
