@@ -38,6 +38,7 @@ constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of
 constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
 constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
 constexpr int kMaxCtas = 256;
+constexpr int kHintLines = 8192;  // of 128 bytes
 constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once
 constexpr size_t kCounterBytes = kMaxCtas * 4;
 
@@ -164,6 +165,12 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   if (warp == W - 1 && elect_one()) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_v) : "memory");
+  }
+  {
+    // while the preceding kernel still runs: ask the L2 for the table, as far as that is little, and the positions (0.4 to 0.6 us)
+    const int64_t lines = ((static_cast<int64_t>(n_seq - 1) * table.ld + table.max_pages) * 4 + 127) / 128, mine = static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x;
+    if (lines <= kHintLines && mine < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(table.ids) + mine * 128));
+    if (threadIdx.x * 32 < n_seq) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.a.input_pos) + threadIdx.x * 32 * (p.a.pos_is_i64 ? 8 : 4)));
   }
   pdl_launch_dependents();
   pdl_wait();  // q, positions, the table and the newest cache rows come from preceding kernels

@@ -45,16 +45,19 @@ class Engine:
         self.ops = ops if ops is not None else CudaOps
         self.comm = comm if comm is not None else make_comm()
         self.ready = False
+        self.paged = False  # whether the layers' caches are pages (setup_paged)
+        self._pages = None  # the table of the step in hand
         self._norm_pushes = False  # set per step by _reduce_plan
 
     # ------------------------------------------------------------------------------------------
-    def setup(self, max_batch, max_seq, device, dtype):
+    def setup(self, max_batch, max_seq, device, dtype, rows=None):
+        """rows: the most token rows of a pass, max_batch * max_seq by default."""
         cfg, t = self.cfg, self.comm.world
         self.nh, self.nkv, self.hd = cfg.n_head // t, cfg.n_local_heads // t, cfg.head_dim
         self.inter = cfg.intermediate_size // t
         self.d, self.dtype = cfg.dim, dtype
         self.max_batch, self.max_seq = max_batch, max_seq
-        rows = max_batch * max_seq
+        rows = max_batch * max_seq if rows is None else rows
         self.max_rows = rows
 
         def buf(cols, n=rows):
@@ -96,6 +99,22 @@ class Engine:
                 e.record()  # an event has a handle from its first recording on
         self.ready = True
 
+    def setup_paged(self, max_sequences, max_prompt, max_length, device, dtype):
+        """Buffers of a model whose caches are pages: steps of up to max_sequences new tokens, prompts of one sequence of up to max_prompt at a time,
+        sequences of up to max_length positions."""
+        self.setup(max_sequences, max_prompt, device, dtype, rows=max(max_sequences, max_prompt))
+        n = (self.nh + 2 * self.nkv) * self.hd
+        self.qkv = torch.empty(self.max_rows, n, dtype=dtype, device=device)
+        nbytes = max(self.ops.linear_workspace_bytes(self.max_rows, n), self.ops.linear_workspace_bytes(min(self.max_rows, 64), n))
+        self.ws_qkv_rows = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        caches = [layer.attention.kv_cache for layer in self.model.layers]
+        self.ws_paged = caches[0].attend_workspace(self.nh)
+        # a prompt's attention works on a dense copy of its sequence's pages, which the layers share
+        rows = -(-max_length // 64) * 64
+        self.dense_k, self.dense_v = (torch.zeros(1, self.nkv, rows, self.hd, dtype=dtype, device=device) for _ in range(2))
+        self.one_sequence = torch.zeros(self.max_rows, dtype=torch.int32, device=device)
+        self.paged = True
+
     def _setup_head(self, max_batch, device, dtype):
         """Buffers of the output projection and of the token choice."""
         cfg, t = self.cfg, self.comm.world
@@ -127,14 +146,28 @@ class Engine:
     def _attention(self, att, w_qkv, rows, B, S, pos, out, push=0):
         """push > 0: the output projection also pushes its partial to the peers on that channel."""
         ops = self.ops
-        kc, vc = att.kv_cache.k_cache, att.kv_cache.v_cache
-        ops.qkv_rope_kvcache(self.normed, w_qkv, self.model.freqs_cis, False, pos, self.q, kc, vc, B, S, self.nh,
-                             self.nkv, self.hd, self.ws_qkv)
-        ops.attention(self.q, kc, vc, pos, self.y, B, S, self.nh, self.nkv, self.hd, self.scratch, self._splits)
+        if self.paged:
+            self._paged_attention(att.kv_cache, w_qkv, rows, S, pos)
+        else:
+            kc, vc = att.kv_cache.k_cache, att.kv_cache.v_cache
+            ops.qkv_rope_kvcache(self.normed, w_qkv, self.model.freqs_cis, False, pos, self.q, kc, vc, B, S, self.nh,
+                                 self.nkv, self.hd, self.ws_qkv)
+            ops.attention(self.q, kc, vc, pos, self.y, B, S, self.nh, self.nkv, self.hd, self.scratch, self._splits)
         if push:
             self.comm.linear_push(self.y, att.wo.weight, out, rows, push)
         else:
             ops.linear(self.y, att.wo.weight, out, rows, workspace=self.ws_wo)
+
+    def _paged_attention(self, cache, w_qkv, rows, S, pos):
+        """self.normed -> self.y: one new token of each sequence over its pages, or a prompt of one sequence over a dense copy of them."""
+        ops, qkv, q = self.ops, self.qkv[:rows], self.q[:rows].view(rows, self.nh, self.hd)
+        ops.linear(self.normed, w_qkv, qkv, rows, workspace=self.ws_qkv_rows)
+        cache.store(qkv, self.model.freqs_cis, pos, self._pages, self.nh, sequence=None if S == 1 else self.one_sequence[:rows], out=q)
+        if S == 1:
+            cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
+        else:
+            k, v = cache.load(pos[-1:], self._pages, out=(self.dense_k, self.dense_v))
+            ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)
 
     def _mlp(self, w1, w2, rows, out, addend=None, normed=None, push=0):
         self.ops.gateup_swiglu(self.normed if normed is None else normed, w1, self.h, rows, self.ws_ug)
@@ -177,12 +210,18 @@ class Engine:
         return self.comm.all_reduce_async(buf, rows)
 
     # ------------------------------------------------------------------------------------------
-    def _trunk(self, idx, input_pos):
+    def _trunk(self, idx, input_pos, pages=None):
         """Everything up to the final norm; leaves the normalised hidden states in self.normed."""
         assert self.ready, "Caches must be initialized first"
         B, S = idx.shape
-        assert input_pos.shape[0] == S, "input_pos must hold one position per token column"
-        assert B <= self.max_batch and S <= self.max_seq, "batch or sequence exceeds setup_caches() sizes"
+        assert (pages is not None) == self.paged, "a table of pages belongs to the caches of setup_paged_caches(), and these need one"
+        if self.paged:
+            assert B == 1 or S == 1, "with pages: one new token of each sequence, or a prompt of one sequence"
+            assert input_pos.shape[0] == B * S and pages.shape[0] == B, "with pages: a position for every token, a row of pages for every sequence"
+        else:
+            assert input_pos.shape[0] == S, "input_pos must hold one position per token column"
+        assert B <= self.max_batch and S <= self.max_seq, "batch or sequence exceeds the sizes that the caches were set up for"
+        self._pages = pages
         if input_pos.dtype not in (torch.int32, torch.int64):
             input_pos = input_pos.to(torch.int64)
         rows = B * S
@@ -191,7 +230,7 @@ class Engine:
 
     def _body(self, idx, rows, B, S, input_pos):
         """Embedding, layers and final norm; leaves the normalised hidden states in self.normed."""
-        self._splits = decode_splits(B, self.nh, self.nkv, self.model.max_seq_length, self.hd) if S == 1 else 1
+        self._splits = decode_splits(B, self.nh, self.nkv, self.model.max_seq_length, self.hd) if S == 1 and not self.paged else 1
         self.ops.embedding(self.model.tok_embeddings.weight, idx, self.resid)
         if not self._run_native(B, S, input_pos):
             getattr(self, "_run_" + self.family)(rows, B, S, input_pos)
@@ -279,26 +318,26 @@ class Engine:
         return True
 
     @torch.no_grad()
-    def forward(self, idx, input_pos):
-        B, S, rows = self._trunk(idx, input_pos)
+    def forward(self, idx, input_pos, pages=None):
+        B, S, rows = self._trunk(idx, input_pos, pages)
         logits = torch.empty(B, S, self.cfg.vocab_size, dtype=self.dtype, device=self.resid.device)
         self.ops.linear(self.normed, self.model.output.weight, logits, rows, workspace=self._head_workspace(rows))
         return logits
 
     @torch.no_grad()
-    def forward_last(self, idx, input_pos):
+    def forward_last(self, idx, input_pos, pages=None):
         """Prompt pass that returns the logits of the last position only, [B, 1, V].  The reference
         computes the output projection for every position (gpt_fast/gpt_ladder_TP.py:282-283) although
         its generation loop reads only the last one (benchmark.py:82-83); for a long prompt that is
         most of the LM-head work (32 x 4096 positions x 128256 logits = 33.6 GB of output)."""
-        B, S, rows = self._trunk(idx, input_pos)
+        B, S, rows = self._trunk(idx, input_pos, pages)
         last = self.normed[:rows].view(B, S, self.d)[:, -1].contiguous()
         logits = torch.empty(B, 1, self.cfg.vocab_size, dtype=self.dtype, device=self.resid.device)
         self.ops.linear(last, self.model.output.weight, logits, B, workspace=self._head_workspace(B))
         return logits
 
     @torch.no_grad()
-    def forward_greedy(self, idx, input_pos):
+    def forward_greedy(self, idx, input_pos, pages=None):
         """Decode step that returns the arg-max token of every sequence, int32 [B, 1], instead of logits.
 
         The output projection is replicated on every rank (reference gpt_fast/gpt_ladder_TP.py:218, 283),
@@ -312,7 +351,7 @@ class Engine:
         a near-tie may resolve differently.
         """
         import torch.distributed as dist
-        B, S, rows = self._trunk(idx, input_pos)
+        B, S, rows = self._trunk(idx, input_pos, pages)
         assert S == 1, "forward_greedy is a decode step (one position per sequence)"
         n = self.vocab_hi - self.vocab_lo
         t = self.comm.world
@@ -343,7 +382,7 @@ class Engine:
         return winner.to(torch.int32).view(B, 1)
 
     @torch.no_grad()
-    def forward_sample(self, idx, input_pos, temperature=1.0, top_k=None, generator=None):
+    def forward_sample(self, idx, input_pos, temperature=1.0, top_k=None, generator=None, pages=None):
         """Decode step that returns one sampled token per sequence, int32 [B, 1], from the reference's
         sampling rule (benchmark.py:56-77: logits / max(temperature, 1e-5), optional top-k cut at the
         k-th largest value, softmax, argmax(probs / q) with q ~ Exponential(1)), with the output
@@ -356,7 +395,7 @@ class Engine:
         reference's softmax output is, so the draw is the reference's up to the rounding of the
         normaliser (summation order differs)."""
         import torch.distributed as dist
-        B, S, rows = self._trunk(idx, input_pos)
+        B, S, rows = self._trunk(idx, input_pos, pages)
         assert S == 1, "forward_sample is a decode step (one position per sequence)"
         t, V = self.comm.world, self.cfg.vocab_size
         n = self.vocab_hi - self.vocab_lo

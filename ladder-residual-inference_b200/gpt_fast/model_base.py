@@ -12,6 +12,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .engine import Engine
+from .paged import PagedKVCache
 from .utils import KVCache, RMSNorm, precompute_freqs_cis
 
 
@@ -75,7 +76,7 @@ class TPModelBase(nn.Module):
         self._engine = None
 
     def setup_caches(self, max_batch_size, max_seq_length):
-        if self.max_seq_length >= max_seq_length and self.max_batch_size >= max_batch_size:
+        if self.max_seq_length >= max_seq_length and self.max_batch_size >= max_batch_size and not self._engine.paged:
             return
         max_seq_length = find_multiple(max_seq_length, 8)
         self.max_seq_length = max_seq_length
@@ -92,41 +93,65 @@ class TPModelBase(nn.Module):
         for b in self.layers:
             b.attention.kv_cache = KVCache(max_batch_size, max_seq_length, cfg.n_local_heads // dist.get_world_size(),
                                            head_dim, dtype).to(device)
-        self.freqs_cis = precompute_freqs_cis(cfg.block_size, head_dim, cfg.rope_base, dtype,
-                                              cfg.rope_scaling).to(device).contiguous()
+        self._setup_table(dtype, device)
         # kept because callers of the reference may read it; the kernels derive causality from input_pos
         self.causal_mask = torch.tril(torch.ones(max_seq_length, max_seq_length, dtype=torch.bool, device=device))
+
+    def setup_paged_caches(self, max_sequences, n_pages, page_size=32, max_length=None, max_prompt=512, cache_dtype=None):
+        """Caches in pages, for sequences of unequal lengths that come and go: the calls below then take `pages`, an int32 table [sequences,
+        most pages] on the device that names each sequence's pages in order (-1: none), and a position for every token: a step of up to
+        max_sequences new tokens (idx [B, 1], input_pos [B]; -1 for an idle row), or a prompt of one sequence, whole or in portions of up to
+        max_prompt tokens (idx [1, S], consecutive input_pos [S], pages [1, most pages]).  max_length: the most positions of a sequence, the
+        model's block_size by default.  cache_dtype: the model's type, or torch.float8_e4m3fn.  No counterpart in the reference, whose
+        sequences share their positions (gpt_fast/gpt_ladder_TP.py:252-284)."""
+        if self.engine_class is not Engine:
+            raise TypeError(f"the layers of {type(self).__name__} keep caches of their own kinds, not pages")
+        cfg = self.config
+        max_length = cfg.block_size if max_length is None else max_length
+        assert 1 <= max_prompt <= max_length <= cfg.block_size, "prompts fit a sequence, sequences the model's block_size"
+        dtype, device, head_dim = self.output.weight.dtype, self.output.weight.device, cfg.dim // cfg.n_head
+        for b in self.layers:
+            b.attention.kv_cache = PagedKVCache(n_pages, page_size, cfg.n_local_heads // dist.get_world_size(), head_dim, dtype, cache_dtype, device)
+        self.max_batch_size, self.max_seq_length = max_sequences, max_length
+        self._setup_table(dtype, device)
+        self._engine = self.engine_class(self, self.family)
+        self._engine.setup_paged(max_sequences, max_prompt, max_length, device, dtype)
+
+    def _setup_table(self, dtype, device):
+        cfg = self.config
+        self.freqs_cis = precompute_freqs_cis(cfg.block_size, cfg.dim // cfg.n_head, cfg.rope_base, dtype,
+                                              cfg.rope_scaling).to(device).contiguous()
 
     def recurrent_state(self):
         """Tensors a step reads and overwrites, so that repeating a step needs them restored (none for attention
         caches: rewriting a position with the same values changes nothing)."""
         return []
 
-    def forward(self, idx: Tensor, input_pos: Optional[Tensor] = None) -> Tensor:
+    def forward(self, idx: Tensor, input_pos: Optional[Tensor] = None, pages: Optional[Tensor] = None) -> Tensor:
         assert self._engine is not None, "Caches must be initialized first"
-        return self._engine.forward(idx, input_pos)
+        return self._engine.forward(idx, input_pos, pages)
 
-    def prefill_last(self, idx: Tensor, input_pos: Tensor) -> Tensor:
+    def prefill_last(self, idx: Tensor, input_pos: Tensor, pages: Optional[Tensor] = None) -> Tensor:
         """forward(idx, input_pos)[:, -1:] without computing the other positions' logits (no
         counterpart in the reference, whose forward always projects every position)."""
         assert self._engine is not None, "Caches must be initialized first"
-        return self._engine.forward_last(idx, input_pos)
+        return self._engine.forward_last(idx, input_pos, pages)
 
-    def decode_greedy(self, idx: Tensor, input_pos: Tensor) -> Tensor:
+    def decode_greedy(self, idx: Tensor, input_pos: Tensor, pages: Optional[Tensor] = None) -> Tensor:
         """Arg-max next token of every sequence, int32 [B, 1]; equal to
         `forward(idx, input_pos)[:, -1].argmax(-1)` but with the output projection split by
         vocabulary over the tensor-parallel ranks (no counterpart in the reference, which
         samples from the replicated logits, benchmark.py:74-92)."""
         assert self._engine is not None, "Caches must be initialized first"
-        return self._engine.forward_greedy(idx, input_pos)
+        return self._engine.forward_greedy(idx, input_pos, pages)
 
     def decode_sample(self, idx: Tensor, input_pos: Tensor, temperature: float = 1.0, top_k: Optional[int] = None,
-                      generator=None) -> Tensor:
+                      generator=None, pages: Optional[Tensor] = None) -> Tensor:
         """One sampled next token per sequence, int32 [B, 1], by the reference's rule
         (`sample(model(idx, input_pos), temperature, top_k)[0]`, benchmark.py:56-92), computed on the
         vocabulary-split output projection; see Engine.forward_sample."""
         assert self._engine is not None, "Caches must be initialized first"
-        return self._engine.forward_sample(idx, input_pos, temperature, top_k, generator)
+        return self._engine.forward_sample(idx, input_pos, temperature, top_k, generator, pages)
 
 
 class BlockBase(nn.Module):
