@@ -229,7 +229,8 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  * [n_pages, n_kv, page_size] in fp32 (value = code * scale; not read or written otherwise, NULL then).  Position j of sequence b is row
  * j % page_size of page pages[b * pages_ld + j / page_size]; sequences may share pages.  Numbers outside 0 .. n_pages - 1 name no
  * page.  `dtype` bfloat16 or float16; head_dim a multiple of 8 up to 256; page_size a multiple of 8 up to 4096;
- * n_pages * n_kv below 2^31, max_pages * page_size up to 2^30.  Pages, scales, qkv, tables, q and results are 16-byte aligned.
+ * n_pages * n_kv below 2^31, max_pages * page_size up to 2^30.  Pages, scales, qkv, tables, q and results are 16-byte aligned,
+ * and results overlap nothing else.
  *
  * lri_rope_paged_store: rows [n_head query | n_kv key | n_kv value heads] of qkv (pitch qkv_ld, a multiple of 8), one for each new token, to
  * rotated queries q_out [tokens, n_head, head_dim] and to rotated keys and values in the pages.  Token i has position input_pos[i] in

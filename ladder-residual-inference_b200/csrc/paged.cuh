@@ -77,6 +77,11 @@ struct PagedAttnParams {
   float scale_log2;
 };
 
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
 // What the operators ask of the cache and of the pages' table (paged_cache.cu).
 int check_paged(const char* who, int dtype, int cache_dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, const PageTable& t, int n_kv, int dim);
 

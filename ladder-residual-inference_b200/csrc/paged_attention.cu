@@ -128,6 +128,8 @@ extern "C" int lri_paged_attn_decode(const lri_paged_attn_call* call) {
   if (c.n_seq == 0) return LRI_OK;
   LRI_REQUIRE(c.q && c.input_pos && c.out && c.pages, LRI_ERR_ARG, "paged_attn_decode: NULL pointer");
   LRI_REQUIRE(aligned16(c.q) && aligned16(c.out), LRI_ERR_ALIGN, "paged_attn_decode: pointers must be 16-byte aligned");
+  const int64_t q_bytes = static_cast<int64_t>(c.n_seq) * c.n_head * c.head_dim * 2;
+  LRI_REQUIRE(!overlap(c.q, q_bytes, c.out, q_bytes), LRI_ERR_ARG, "paged_attn_decode: q and out overlap");  // a head's warps read q at different times
   const bool eight = c.cache_dtype == LRI_E4M3;
   p.q = c.q, p.k = c.k_pages, p.v = c.v_pages, p.k_scale = eight ? c.k_scale : nullptr, p.v_scale = eight ? c.v_scale : nullptr;
   p.input_pos = c.input_pos, p.pos_is_i64 = c.pos_is_i64, p.out = c.out, p.n_head = c.n_head, p.n_kv = c.n_kv, p.dim = c.head_dim, p.window = c.window;

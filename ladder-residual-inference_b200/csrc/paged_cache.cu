@@ -375,6 +375,9 @@ extern "C" int lri_rope_paged_store(const lri_paged_store_call* call) {
   if (c.tokens == 0) return LRI_OK;
   LRI_REQUIRE(c.qkv && c.input_pos && c.q_out && (c.pages || c.n_seq == 0), LRI_ERR_ARG, "rope_paged_store: NULL pointer");
   LRI_REQUIRE(aligned16(c.qkv) && aligned16(c.rope_table) && aligned16(c.q_out), LRI_ERR_ALIGN, "rope_paged_store: pointers must be 16-byte aligned");
+  const int64_t q_row = static_cast<int64_t>(c.n_head) * c.head_dim;
+  LRI_REQUIRE(!overlap(c.q_out, c.tokens * q_row * 2, c.qkv, ((c.tokens - 1) * c.qkv_ld + q_row + 2ll * c.n_kv * c.head_dim) * 2), LRI_ERR_ARG,
+              "rope_paged_store: q_out and qkv overlap");
   p.qkv = c.qkv, p.ld = c.qkv_ld, p.rope = c.rope_table, p.table_rows = c.table_rows, p.rot = c.rot_dim, p.halves = c.halves;
   p.input_pos = c.input_pos, p.pos_is_i64 = c.pos_is_i64, p.sequence = c.sequence, p.q_out = c.q_out;
   p.k = c.k_pages, p.v = c.v_pages, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
@@ -397,6 +400,8 @@ extern "C" int lri_paged_load(const lri_paged_load_call* call) {
   if (c.rows == 0 || c.n_seq == 0) return LRI_OK;
   LRI_REQUIRE(c.pages && c.last_pos && c.k_out && c.v_out, LRI_ERR_ARG, "paged_load: NULL pointer");
   LRI_REQUIRE(aligned16(c.k_out) && aligned16(c.v_out), LRI_ERR_ALIGN, "paged_load: pointers must be 16-byte aligned");
+  const int64_t out_bytes = static_cast<int64_t>(c.n_seq) * c.n_kv * c.rows * c.head_dim * 2;
+  LRI_REQUIRE(!overlap(c.k_out, out_bytes, c.v_out, out_bytes), LRI_ERR_ARG, "paged_load: k_out and v_out overlap");
   const bool eight = c.cache_dtype == LRI_E4M3;
   p.k = c.k_pages, p.v = c.v_pages, p.k_scale = eight ? c.k_scale : nullptr, p.v_scale = eight ? c.v_scale : nullptr;
   p.last_pos = c.last_pos, p.pos_is_i64 = c.pos_is_i64, p.k_out = c.k_out, p.v_out = c.v_out, p.rows = c.rows, p.n_kv = c.n_kv, p.dim = c.head_dim;

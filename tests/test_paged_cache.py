@@ -108,7 +108,7 @@ ARG, ALIGN, UNSUPPORTED = -1, -2, -3
 
 def _c_store(**kw):
     from gpt_fast import _C
-    a = dict(qkv=BUF, rope=BUF, pos=BUF, seq=0, pages=BUF, q=BUF, k=BUF, v=BUF, ks=0, vs=0, stream=0, ld=512, rows=50, pages_ld=2, n_pages=6, tokens=3, dtype=0,
+    a = dict(qkv=BUF, rope=BUF, pos=BUF, seq=0, pages=BUF, q=2 * BUF, k=BUF, v=BUF, ks=0, vs=0, stream=0, ld=512, rows=50, pages_ld=2, n_pages=6, tokens=3, dtype=0,
              cache=0, f32=0, rot=64, halves=0, i64=0, n_seq=3, most=2, page=16, n_head=4, n_kv=2, dim=64)
     assert set(kw) <= set(a)
     a.update(kw)
@@ -121,14 +121,15 @@ def _c_store(**kw):
     (dict(n_pages=1 << 30), UNSUPPORTED), (dict(most=0), ARG), (dict(most=1 << 28, pages_ld=1 << 28), UNSUPPORTED), (dict(pages_ld=1), ARG), (dict(rot=66), ARG),
     (dict(rot=3), ARG), (dict(rot=-2), ARG), (dict(rope=0), ARG), (dict(rows=0), ARG), (dict(tokens=4), ARG), (dict(tokens=-1), ARG), (dict(ld=504), ARG),
     (dict(ld=513), ARG), (dict(qkv=0), ARG), (dict(pos=0), ARG), (dict(q=0), ARG), (dict(k=0), ARG), (dict(v=0), ARG), (dict(pages=0), ARG),
-    (dict(qkv=BUF + 8), ALIGN), (dict(q=BUF + 8), ALIGN), (dict(k=BUF + 8), ALIGN), (dict(rope=BUF + 8), ALIGN), (dict(tokens=0, qkv=0), 0)])
+    (dict(qkv=BUF + 8), ALIGN), (dict(q=2 * BUF + 8), ALIGN), (dict(k=BUF + 8), ALIGN), (dict(rope=BUF + 8), ALIGN), (dict(tokens=0, qkv=0), 0), (dict(q=BUF), ARG),
+    (dict(q=BUF + 2 * 512 * 2 + 512 * 2 - 16), ARG), (dict(q=BUF - 3 * 256 * 2 + 16), ARG)])
 def test_c_store_refuses(kw, status):
     assert _c_store(**kw) == status
 
 
 def _c_attend(**kw):
     from gpt_fast import _C
-    a = dict(q=BUF, k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, out=BUF, ws=BUF, stream=0, n_pages=6, pages_ld=2, window=0, ws_bytes=1 << 30, dtype=0, cache=0, page=16,
+    a = dict(q=BUF, k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, out=2 * BUF, ws=BUF, stream=0, n_pages=6, pages_ld=2, window=0, ws_bytes=1 << 30, dtype=0, cache=0, page=16,
              n_seq=3, most=2, i64=0, n_head=4, n_kv=2, dim=64, scale=1.0)
     assert set(kw) <= set(a)
     a.update(kw)
@@ -137,7 +138,7 @@ def _c_attend(**kw):
 
 @pytest.mark.parametrize("kw,status", [
     (dict(n_head=3), ARG), (dict(n_head=0), ARG), (dict(window=-1), ARG), (dict(n_seq=-1), ARG), (dict(q=0), ARG), (dict(out=0), ARG), (dict(pos=0), ARG),
-    (dict(q=BUF + 8), ALIGN), (dict(out=BUF + 2), ALIGN), (dict(dtype=3), UNSUPPORTED), (dict(cache=2), UNSUPPORTED), (dict(cache=3, ks=BUF), ARG),
+    (dict(q=BUF + 8), ALIGN), (dict(out=2 * BUF + 2), ALIGN), (dict(out=BUF), ARG), (dict(out=BUF + 3 * 4 * 64 * 2 - 16), ARG), (dict(dtype=3), UNSUPPORTED), (dict(cache=2), UNSUPPORTED), (dict(cache=3, ks=BUF), ARG),
     (dict(n_seq=0, q=0, out=0), 0)])
 def test_c_attend_refuses(kw, status):
     assert _c_attend(**kw) == status
@@ -145,7 +146,7 @@ def test_c_attend_refuses(kw, status):
 
 def _c_load(**kw):
     from gpt_fast import _C
-    a = dict(k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, k_out=BUF, v_out=BUF, stream=0, n_pages=6, pages_ld=2, rows=32, dtype=0, cache=0, page=16, n_seq=3, most=2, i64=0,
+    a = dict(k=BUF, v=BUF, ks=0, vs=0, pages=BUF, pos=BUF, k_out=BUF, v_out=2 * BUF, stream=0, n_pages=6, pages_ld=2, rows=32, dtype=0, cache=0, page=16, n_seq=3, most=2, i64=0,
              n_kv=2, dim=64)
     assert set(kw) <= set(a)
     a.update(kw)
@@ -153,7 +154,7 @@ def _c_load(**kw):
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(rows=-1), ARG), (dict(rows=1 << 31), ARG), (dict(n_seq=65536), ARG), (dict(pos=0), ARG), (dict(k_out=0), ARG), (dict(v_out=BUF + 8), ALIGN),
+    (dict(rows=-1), ARG), (dict(rows=1 << 31), ARG), (dict(n_seq=65536), ARG), (dict(pos=0), ARG), (dict(k_out=0), ARG), (dict(v_out=2 * BUF + 8), ALIGN), (dict(v_out=BUF), ARG), (dict(v_out=BUF + 3 * 2 * 32 * 64 * 2 - 16), ARG),
     (dict(n_kv=65536), ARG), (dict(rows=0, k_out=0), 0), (dict(n_seq=0, pos=0), 0)])
 def test_c_load_refuses(kw, status):
     assert _c_load(**kw) == status

@@ -142,10 +142,11 @@ def _attend(cache, table, q, lengths, **kw):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("eight", [False, True])
-@pytest.mark.parametrize("n_head,n_kv,dim", [(32, 8, 128), (12, 12, 64), (8, 1, 64), (20, 1, 128), (10, 2, 80), (3, 3, 72), (34, 2, 48), (16, 1, 128), (4, 2, 192)])
+@pytest.mark.parametrize("n_head,n_kv,dim", [(32, 8, 128), (12, 12, 64), (8, 1, 64), (20, 1, 128), (10, 2, 80), (3, 3, 72), (34, 2, 48), (16, 1, 128), (4, 2, 192),
+                                             (2, 2, 8), (6, 2, 16), (3, 1, 24), (9, 1, 112)])
 @pytest.mark.parametrize("page,lengths,window", [
     (16, [1], 0), (8, [0, 1, 7, 8, 9, 31, 32, 33], 0), (24, [500, 0, 23, 24, 25, 129, 1], 0), (64, [1025, 3], 0), (128, [2000, 1, 65, 0], 100),
-    (8, [257, 64, 40], 1), (40, [300, 41, 1000], 64), (16, [5000], 0)])
+    (8, [257, 64, 40], 1), (40, [300, 41, 1000], 64), (16, [5000], 0), (4096, [4097, 4096, 1], 0)])
 def test_attend(dtype, eight, n_head, n_kv, dim, page, lengths, window):
     cache, table = make_cache(lengths, page, n_kv, dim, dtype, eight, seed=n_head + page)
     q = torch.randn(len(lengths), n_head, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).to(dtype)
@@ -285,6 +286,42 @@ def test_attend_on_another_stream():
         got = _attend(cache, table, q, lengths)
     torch.cuda.current_stream().wait_stream(stream)
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dim", [64, 192])
+def test_attend_more_sequences_than_a_launch_takes(eight, dim):
+    lengths = [(7 * i) % 40 for i in range(1100)]
+    cache, table = make_cache(lengths, 8, 1, dim, torch.bfloat16, eight)
+    q = torch.randn(1100, 2, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(torch.bfloat16)
+    want, tol = attend_64(cache, table, q, lengths)
+    assert ((_attend(cache, table, q, lengths).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dim", [128, 160])
+def test_offsets_beyond_32_bits(dim):
+    """A cache of more than 2^31 elements, the sequence's pages at its end: stored, read by attention, read back."""
+    n_kv, page, n_head, n = 8, 64, 16, 150
+    n_pages = 2 ** 31 // (n_kv * page * dim) + 64
+    from gpt_fast import PagedKVCache
+    cache = PagedKVCache(n_pages, page, n_kv, dim, torch.bfloat16, cache_dtype=E4M3, device="cuda")
+    table = torch.tensor([[n_pages - 1, n_pages - 9, n_pages - 4]], dtype=torch.int32, device="cuda")
+    qkv = torch.randn(n, (n_head + 2 * n_kv) * dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0)).to(torch.bfloat16)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    q = cache.store(qkv, None, pos, table, n_head, sequence=torch.zeros(n, dtype=torch.int32, device="cuda"))
+    k, v = dense(cache, table, 0, 0, n)
+    x = qkv.double().view(n, n_head + 2 * n_kv, dim).transpose(0, 1)
+    for got, want in ((k, x[n_head:n_head + n_kv]), (v, x[n_head + n_kv:])):
+        # half a step of e4m3: 2^-4 of the value, of the smallest numbers 2^-10 of the scale
+        assert ((got - want).abs() <= want.abs() * (2.0 ** -4 + 2.0 ** -20) + want.abs().amax(-1, keepdim=True) / 448 * 2.0 ** -10 * (1 + 2.0 ** -20)).all()
+    last = q[n - 1:].contiguous()
+    want, tol = attend_64(cache, table, last, [n])
+    assert ((cache.attend(last, pos[n - 1:], table).double() - want).abs() <= tol).all()
+    back = cache.load(pos[n - 1:], table)
+    assert ((back[0][0, :, :n].double() - k).abs() <= k.abs() * half_step(torch.bfloat16) * (1 + 2.0 ** -8)).all()
+    assert ((back[1][0, :, :n].double() - v).abs() <= v.abs() * half_step(torch.bfloat16) * (1 + 2.0 ** -8)).all()
+    # and nothing in front of them
+    assert not any(int(t.view(torch.uint8)[: n_pages - 9].amax()) for t in (cache.k_pages, cache.v_pages))
 
 
 # ---- load ------------------------------------------------------------------------------------------------------------------------
