@@ -255,23 +255,38 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     int slab, row, next_slab = -1, next_row = 0;
     look_up(u0 + lane / boxes, slab, row);
     uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
-    // the tile of keys (0) or of values (1) of unit u; the one before in its place has been read by all lanes
-    auto fetch = [&](int half, int u) {
+    // The tile of keys (0) or of values (1) of a unit; the one before in its place has been read by all lanes.  `slot` is the unit's place among those
+    // looked up, z and y its box where it has only one: then one lane does it all.
+    auto fetch = [&](int half, int slot, int z, int y) {
       const uint32_t full = full0 + 8 * half, dst = ring + half * S::kHalf;
-      const uint32_t mine = (have >> ((u - base) * boxes)) & ((1u << boxes) - 1u);
+      const CUtensorMap* map = half ? &tmap_v : &tmap_k;
+      const float* scale = half ? p.a.v_scale : p.a.k_scale;
+      constexpr int kColumns = S::kChunkRow / static_cast<int>(sizeof(C));
+      if (boxes == 1) {
+        if (elect_one()) {
+          mbar_expect_tx(full, z >= 0 ? S::kHalf + (kEight ? UNIT * 4 : 0) : 0u);
+          if (z >= 0) {
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) tma_load_3d(dst + c * S::kChunkBytes, map, full, c * kColumns, y, z);
+            if (kEight) bulk_load(smem_u32(my_scales + half * UNIT), scale + static_cast<int64_t>(z) * table.page + y, UNIT * 4, full);
+          }
+        }
+        return;
+      }
+      const uint32_t mine = (have >> (slot * boxes)) & ((1u << boxes) - 1u);
       if (elect_one()) mbar_expect_tx(full, __popc(mine) * p.box * (S::kRow + (kEight ? 4 : 0)));
       for (int i = 0; i < boxes; ++i) {
-        const int from = (u - base) * boxes + i, z = __shfl_sync(0xffffffffu, slab, from), y = __shfl_sync(0xffffffffu, row, from);
-        if (z >= 0 && elect_one()) {
+        const int bz = __shfl_sync(0xffffffffu, slab, slot * boxes + i), by = __shfl_sync(0xffffffffu, row, slot * boxes + i);
+        if (bz >= 0 && elect_one()) {
 #pragma unroll
-          for (int c = 0; c < S::kChunks; ++c)
-            tma_load_3d(dst + c * S::kChunkBytes + i * p.box * S::kChunkRow, half ? &tmap_v : &tmap_k, full, c * (S::kChunkRow / static_cast<int>(sizeof(C))), y, z);
-          if (kEight) bulk_load(smem_u32(my_scales + half * UNIT + i * p.box), (half ? p.a.v_scale : p.a.k_scale) + static_cast<int64_t>(z) * table.page + y, p.box * 4, full);
+          for (int c = 0; c < S::kChunks; ++c) tma_load_3d(dst + c * S::kChunkBytes + i * p.box * S::kChunkRow, map, full, c * kColumns, by, bz);
+          if (kEight) bulk_load(smem_u32(my_scales + half * UNIT + i * p.box), scale + static_cast<int64_t>(bz) * table.page + by, p.box * 4, full);
         }
       }
     };
-    fetch(0, u0);
-    fetch(1, u0);
+    int z = __shfl_sync(0xffffffffu, slab, 0), y = __shfl_sync(0xffffffffu, row, 0);
+    fetch(0, 0, z, y);
+    fetch(1, 0, z, y);
     look_up(base + ahead + lane / boxes, next_slab, next_row);
 
     const int quad = lane >> 2, col = (lane & 3) * 2;  // a thread holds scores of positions quad, quad + 8, .. and heads col, col + 1
@@ -361,7 +376,9 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           have = __ballot_sync(0xffffffffu, slab >= 0);
           look_up(base + ahead + lane / boxes, next_slab, next_row);
         }
-        has = (have >> ((next - base) * boxes)) & ((1u << boxes) - 1u);
+        const int slot = next - base;
+        has = (have >> (slot * boxes)) & ((1u << boxes) - 1u);
+        if (boxes == 1) z = __shfl_sync(0xffffffffu, slab, slot), y = __shfl_sync(0xffffffffu, row, slot);
         ok = arrived(0);
         if (!ok) break;
         // ---- scores: UNIT positions x 8 NT heads ----------------------------------------------------------------------------------------
@@ -415,7 +432,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           }
         }
         __syncwarp();
-        if (next < u1) fetch(0, next);
+        if (next < u1) fetch(0, slot, z, y);
         if (vis != kAll) {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
@@ -540,7 +557,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         }
         if (vis != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros, before the next copy
         __syncwarp();
-        if (next < u1) fetch(1, next);
+        if (next < u1) fetch(1, slot, z, y);
         parity ^= 1u;
       }
 
