@@ -46,9 +46,10 @@ struct StreamParams {
   PagedAttnParams a;
   int group, tile_heads, head_tiles;  // query heads of a KV head, of a pass, passes
   int box;                            // positions of a TMA box
-  unsigned int* counters;             // [CTAs]
-  float* part_ml;                     // [CTAs][2][tile_heads][2]
-  float* part_o;                      // [CTAs][2][tile_heads][HD]
+  int ctas;                           // at most
+  unsigned int* counters;             // [ctas]
+  float* part_ml;                     // [ctas][2][tile_heads][2]
+  float* part_o;                      // [ctas][2][tile_heads][HD]
 };
 
 // NT: blocks of eight query heads
@@ -788,8 +789,8 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
     p.a.out = static_cast<T*>(all.out) + at * all.n_head * all.dim;
     p.a.input_pos = static_cast<const char*>(all.input_pos) + at * (all.pos_is_i64 ? 8 : 4);
     const int smem = 1024 + S::kWarps * (p.tile_heads * (HD * 4 + 2 * 16) + kRings) + (3 * n + 2) * 4;
-    const int64_t room = max_ctas(), useful = (most * n + kMinRun - 1) / kMinRun;
-    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(room < useful ? room : useful)), dim3(S::kThreads), smem, st, tk, tv, p));
+    const int64_t useful = (most * n + kMinRun - 1) / kMinRun;
+    LRI_CUDA(launch_pdl(kern, dim3(static_cast<unsigned>(p.ctas < useful ? p.ctas : useful)), dim3(S::kThreads), smem, st, tk, tv, p));
     LRI_LAUNCH_CHECK("paged_attn_stream_kernel");
   }
   return LRI_OK;
@@ -811,22 +812,22 @@ int dispatch(int cache_dtype, StreamParams& p, cudaStream_t st) {
 // rows of whole 16-byte pieces that fit the tiles
 bool paged_attn_stream_supports(int cache_dtype, int dim) { return dim <= 128 && dim % (cache_dtype == LRI_E4M3 ? 16 : 8) == 0; }
 
-size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim) {
-  const int hd = dim <= 64 ? 64 : 128;
-  return kCounterBytes + static_cast<size_t>(max_ctas()) * 2 * tile_heads_of(n_head / n_kv) * (hd + 2) * 4;
-}
+size_t workspace_bytes(int ctas, int group, int dim) { return kCounterBytes + static_cast<size_t>(ctas) * 2 * tile_heads_of(group) * ((dim <= 64 ? 64 : 128) + 2) * 4; }
 
-int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
-  LRI_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim), LRI_ERR_WORKSPACE,
-              "paged_attn_decode: workspace of %zu bytes (16-byte aligned) required", paged_attn_stream_workspace_bytes(a.n_head, a.n_kv, a.dim));
+size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim) { return workspace_bytes(max_ctas(), n_head / n_kv, dim); }
+
+int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t bytes, cudaStream_t st) {
   StreamParams p{};
   p.a = a;
+  p.ctas = max_ctas();
   p.group = a.n_head / a.n_kv;
+  LRI_REQUIRE(workspace && aligned16(workspace) && bytes >= workspace_bytes(p.ctas, p.group, a.dim), LRI_ERR_WORKSPACE,
+              "paged_attn_decode: workspace of %zu bytes (16-byte aligned) required", workspace_bytes(p.ctas, p.group, a.dim));
   p.tile_heads = tile_heads_of(p.group);
   p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
   p.counters = static_cast<unsigned int*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-  p.part_ml = p.part_o + static_cast<size_t>(max_ctas()) * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
+  p.part_ml = p.part_o + static_cast<size_t>(p.ctas) * 2 * p.tile_heads * (a.dim <= 64 ? 64 : 128);
   return dtype == LRI_BF16 ? dispatch<__nv_bfloat16>(cache_dtype, p, st) : dispatch<__half>(cache_dtype, p, st);
 }
 

@@ -297,7 +297,7 @@ int launch_store(StoreParams p, cudaStream_t st) {
   const int lanes = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
   const int threads = (p.n_head + 2 * p.n_kv) * lanes, blocks = (threads + kThreads - 1) / kThreads;
   // kPerSm CTAs on every SM share the tokens, as far as shared memory holds their table rows.  With no more than that a thread has one token.
-  const int64_t even = (p.tokens * blocks + static_cast<int64_t>(kPerSm) * device_sm_count() - 1) / (static_cast<int64_t>(kPerSm) * device_sm_count());
+  const int64_t room = static_cast<int64_t>(kPerSm) * device_sm_count(), even = (p.tokens * blocks + room - 1) / room;
   const bool many = even > 1;
   auto go = [&](auto kern) {
     const int block = ((threads + blocks - 1) / blocks + 31) / 32 * 32;

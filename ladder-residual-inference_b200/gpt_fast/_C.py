@@ -208,22 +208,19 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
 def stream_handle() -> int:
     # the stream object of torch.cuda.current_stream() costs a microsecond a launch
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def require_here(first, *others) -> None:
-    """require_cuda, and all of them (None: no tensor) on the current device: the launch goes to its current stream."""
-    here = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != here:
-            break
-    else:
-        if here >= 0 and here == torch._C._cuda_getDevice():
-            return
-    require_cuda(first, *others)
-    raise RuntimeError(f"tensors must live on the current device (cuda:{torch._C._cuda_getDevice()})")
+def refuse_devices(*tensors) -> None:
+    """Of tensors (None: no tensor) that do not all live on the current device, to whose current stream a launch goes."""
+    require_cuda(*tensors)
+    raise RuntimeError(f"tensors must live on the current device (cuda:{current_device()})")
 
 
 def require_cuda(*tensors) -> None:

@@ -129,7 +129,11 @@ class CudaOps:
     def rope_paged_store(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale, n_head, halves, tokens, pages_shape,
                          cache_shape):
         """table None: no rotation; its second extent is half of the elements that rotate."""
-        _C.require_here(qkv, input_pos, pages, q_out, k_pages, v_pages, table, sequence, k_scale, v_scale)
+        here = qkv.get_device()
+        if not (0 <= here == torch._C._cuda_getDevice() == input_pos.get_device() == pages.get_device() == q_out.get_device() == k_pages.get_device() ==
+                v_pages.get_device() and (sequence is None or sequence.get_device() == here) and (table is None or table.get_device() == here) and
+                (k_scale is None or k_scale.get_device() == here == v_scale.get_device())):
+            _C.refuse_devices(qkv, input_pos, pages, q_out, k_pages, v_pages, table, sequence, k_scale, v_scale)
         n_pages, n_kv, page, dim = cache_shape
         n_seq, most = pages_shape
         at = rows = rot = f32 = 0
@@ -140,7 +144,7 @@ class CudaOps:
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
             qkv.data_ptr(), at, input_pos.data_ptr(), 0 if sequence is None else sequence.data_ptr(), pages.data_ptr(), q_out.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, _C.stream_handle(), qkv.stride(0), rows, pages.stride(0), n_pages, tokens, dtype,
+            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, torch._C._cuda_getCurrentRawStream(here), qkv.stride(0), rows, pages.stride(0), n_pages, tokens, dtype,
             cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
         if status < 0:
             _C.check(status)
@@ -151,28 +155,34 @@ class CudaOps:
 
     @staticmethod
     def paged_attention(q, k_pages, v_pages, k_scale, v_scale, pages, input_pos, window, scale, out, workspace, n_head, pages_shape, cache_shape):
-        _C.require_here(q, pages, input_pos, out, workspace, k_pages, v_pages, k_scale, v_scale)
+        here = q.get_device()
+        if not (0 <= here == torch._C._cuda_getDevice() == pages.get_device() == input_pos.get_device() == out.get_device() == workspace.get_device() ==
+                k_pages.get_device() == v_pages.get_device() and (k_scale is None or k_scale.get_device() == here == v_scale.get_device())):
+            _C.refuse_devices(q, pages, input_pos, out, workspace, k_pages, v_pages, k_scale, v_scale)
         n_pages, n_kv, page, dim = cache_shape
         n_seq, most = pages_shape
         dtype = _C.CODES[q.dtype]
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), input_pos.data_ptr(), out.data_ptr(),
-            workspace.data_ptr(), _C.stream_handle(), n_pages, pages.stride(0), window, workspace.numel(), dtype, cache_dtype, page, n_seq, most,
+            workspace.data_ptr(), torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0), window, workspace.numel(), dtype, cache_dtype, page, n_seq, most,
             input_pos.dtype is torch.int64, n_head, n_kv, dim, scale))
         if status < 0:
             _C.check(status)
 
     @staticmethod
     def paged_load(k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out, rows, pages_shape, cache_shape):
-        _C.require_here(k_pages, v_pages, pages, last_pos, k_out, v_out, k_scale, v_scale)
+        here = k_pages.get_device()
+        if not (0 <= here == torch._C._cuda_getDevice() == v_pages.get_device() == pages.get_device() == last_pos.get_device() == k_out.get_device() ==
+                v_out.get_device() and (k_scale is None or k_scale.get_device() == here == v_scale.get_device())):
+            _C.refuse_devices(k_pages, v_pages, pages, last_pos, k_out, v_out, k_scale, v_scale)
         n_pages, n_kv, page, dim = cache_shape
         n_seq, most = pages_shape
         dtype = _C.CODES[k_out.dtype]
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_paged_load(_C.LOAD_CALL.pack(
             k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), last_pos.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-            _C.stream_handle(), n_pages, pages.stride(0), rows, dtype, cache_dtype, page, n_seq, most, last_pos.dtype is torch.int64, n_kv, dim))
+            torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0), rows, dtype, cache_dtype, page, n_seq, most, last_pos.dtype is torch.int64, n_kv, dim))
         if status < 0:
             _C.check(status)
 
