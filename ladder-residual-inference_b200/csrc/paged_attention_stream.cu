@@ -38,7 +38,6 @@ constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of
 constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
 constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
 constexpr int kMaxCtas = 256;
-constexpr int kHintLines = 8192;  // of 128 bytes
 constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once
 constexpr size_t kCounterBytes = kMaxCtas * 4;
 
@@ -104,6 +103,21 @@ __device__ __forceinline__ int sequence_of(const int* begins, int n, int at) {
   }
   return lo;
 }
+// loads that see what has been written by now, whatever was read before
+__device__ __forceinline__ int load_fresh(const int32_t* at) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ int64_t load_pos_fresh(const void* input_pos, int pos_is_i64, int64_t i) {
+  if (!pos_is_i64) return load_fresh(static_cast<const int32_t*>(input_pos) + i);
+  int64_t v;
+  asm volatile("ld.relaxed.gpu.global.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const int64_t*>(input_pos) + i) : "memory");
+  return v;
+}
+__device__ __forceinline__ void hint_3d(const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
+}
 __device__ __forceinline__ int length_of(int tiles) { return tiles > 0 ? tiles * kStep + kGap : 0; }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 matrix of 16-bit elements
@@ -166,63 +180,113 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_v) : "memory");
   }
-  {
-    // while the preceding kernel still runs: ask the L2 for the table, as far as that is little, and the positions (0.4 to 0.6 us)
-    const int64_t lines = ((static_cast<int64_t>(n_seq - 1) * table.ld + table.max_pages) * 4 + 127) / 128, mine = static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x;
-    if (lines <= kHintLines && mine < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(table.ids) + mine * 128));
-    if (threadIdx.x * 32 < n_seq) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.a.input_pos) + threadIdx.x * 32 * (p.a.pos_is_i64 ? 8 : 4)));
-  }
   pdl_launch_dependents();
-  pdl_wait();  // q, positions, the table and the newest cache rows come from preceding kernels
 
-  // ---- units before each sequence, and where it begins on the line --------------------------------------------------------------------
-  int units = 0, length = 0;
-  for (int b0 = 0; b0 < n_seq; b0 += S::kThreads) {
-    const int b = b0 + threadIdx.x;
-    int2 n = make_int2(0, 0);
-    if (b < n_seq) {
-      int64_t ctx = load_pos(p.a.input_pos, p.a.pos_is_i64, b);
-      ctx = ctx < 0 ? 0 : (ctx >= table.capacity() ? table.capacity() : ctx + 1);
-      contexts[b] = static_cast<int>(ctx);
-      const int tiles = span_of<UNIT>(static_cast<int>(ctx), p.a.window).tiles;
-      n = make_int2(tiles * pairs, length_of(tiles) * pairs);
-    }
-    int2 sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
-      if (lane >= o) sum.x += x, sum.y += y;
-    }
-    if (lane == 31) warp_sums[warp] = sum;
-    __syncthreads();
-    int2 lower = make_int2(units, length);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int2 v = warp_sums[w];
-      if (w < warp) lower.x += v.x, lower.y += v.y;
-      units += v.x, length += v.y;
-    }
-    if (b < n_seq) before[b] = lower.x + sum.x - n.x, line[b] = lower.y + sum.y - n.y;
-    if (threadIdx.x == 0) before[n_seq] = units, line[n_seq] = length;
-    __syncthreads();
-  }
-  // The CTAs that have work take equal stretches of the line, the first `longer` of them one more.
-  const int ctas = length < static_cast<int>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
-  const int me = blockIdx.x, stretch = ctas > 0 ? length / ctas : 1, longer = length - stretch * ctas;
+  // ---- the plan, made while the preceding kernel still runs --------------------------------------------------------------------------------
+  // Positions and table may be about to change: what is read of them here is checked behind the wait and the plan made again if it does not hold.
+  // Mostly it does, and a chain of two loads and a search is out of the way (calls behind one another, 24 ragged sequences 28.2 -> 25.8 us).  These loads do not go by the L1, which would keep
+  // what they brought.
+  auto context_of = [&](int b) {
+    int64_t ctx = load_pos_fresh(p.a.input_pos, p.a.pos_is_i64, b);
+    ctx = ctx < 0 ? 0 : (ctx >= table.capacity() ? table.capacity() : ctx + 1);
+    return static_cast<int>(ctx);
+  };
+  const int me = blockIdx.x;
+  int units = 0, length = 0;       // in all; of the line
+  int ctas = 0, stretch = 1, longer = 0;  // the CTAs that have work take equal stretches of the line, the first `longer` of them one more
+  int u0 = 0, u1 = 0, cta0 = 0, cta1 = 0;  // units of this warp, of this CTA
   auto line_of = [&](int c) { return stretch * c + (c < longer ? c : longer); };
   auto cta_at = [&](int at) { return at < (stretch + 1) * longer ? at / (stretch + 1) : (at - longer) / stretch; };
-  int u0 = 0, u1 = 0, cta0 = 0, cta1 = 0;  // units of this warp, of this CTA
-  if (me < ctas) {
-    // lanes 0 .. 3: the first unit at or behind a place
-    const int from = line_of(me), n = line_of(me + 1) - from, at = from + (lane & 3 ? (lane & 3) == 1 ? n : n * (warp + (lane & 3) - 2) / W : 0);
-    int u = units;
-    if (at < length) {
-      const int b = sequence_of(line, n_seq, at), tiles = (before[b + 1] - before[b]) / pairs, rest = at - line[b], pair = rest / length_of(tiles);
-      const int unit = (rest - pair * length_of(tiles) + kStep - 1) / kStep;
-      u = before[b] + pair * tiles + (unit < tiles ? unit : tiles);
+  auto make_plan = [&]() {
+    units = length = 0;
+    for (int b0 = 0; b0 < n_seq; b0 += S::kThreads) {
+      const int b = b0 + threadIdx.x;
+      int2 n = make_int2(0, 0);
+      if (b < n_seq) {
+        contexts[b] = context_of(b);
+        const int tiles = span_of<UNIT>(contexts[b], p.a.window).tiles;
+        n = make_int2(tiles * pairs, length_of(tiles) * pairs);
+      }
+      int2 sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+        if (lane >= o) sum.x += x, sum.y += y;
+      }
+      if (lane == 31) warp_sums[warp] = sum;
+      __syncthreads();
+      int2 lower = make_int2(units, length);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int2 v = warp_sums[w];
+        if (w < warp) lower.x += v.x, lower.y += v.y;
+        units += v.x, length += v.y;
+      }
+      if (b < n_seq) before[b] = lower.x + sum.x - n.x, line[b] = lower.y + sum.y - n.y;
+      if (threadIdx.x == 0) before[n_seq] = units, line[n_seq] = length;
+      __syncthreads();
     }
-    cta0 = __shfl_sync(0xffffffffu, u, 0), cta1 = __shfl_sync(0xffffffffu, u, 1);
-    u0 = __shfl_sync(0xffffffffu, u, 2), u1 = __shfl_sync(0xffffffffu, u, 3);
+    ctas = length < static_cast<int>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
+    stretch = ctas > 0 ? length / ctas : 1, longer = length - stretch * ctas;
+    u0 = u1 = cta0 = cta1 = 0;
+    if (me < ctas) {
+      // lanes 0 .. 3: the first unit at or behind a place
+      const int from = line_of(me), n = line_of(me + 1) - from, at = from + (lane & 3 ? (lane & 3) == 1 ? n : n * (warp + (lane & 3) - 2) / W : 0);
+      int u = units;
+      if (at < length) {
+        const int b = sequence_of(line, n_seq, at), tiles = (before[b + 1] - before[b]) / pairs, rest = at - line[b], pair = rest / length_of(tiles);
+        const int unit = (rest - pair * length_of(tiles) + kStep - 1) / kStep;
+        u = before[b] + pair * tiles + (unit < tiles ? unit : tiles);
+      }
+      cta0 = __shfl_sync(0xffffffffu, u, 0), cta1 = __shfl_sync(0xffffffffu, u, 1);
+      u0 = __shfl_sync(0xffffffffu, u, 2), u1 = __shfl_sync(0xffffffffu, u, 3);
+    }
+  };
+  // A lane looks up the page of one box, 32 boxes at a time and 32 ahead.
+  const int boxes = UNIT / p.box, ahead = 32 / boxes;  // of a unit; units that 32 lanes look up
+  // box (lane % boxes) of unit u: where the table names its page, NULL where there is nothing to fetch
+  auto entry_of = [&](int u, int& head, int& row) -> const int32_t* {
+    head = row = 0;
+    if (u >= u1) return nullptr;
+    const int b = sequence_of(before, n_seq, u);
+    const Span s = span_of<UNIT>(contexts[b], p.a.window);
+    const int rest = u - before[b], pair = rest / s.tiles;
+    const int pos = (s.first + rest - pair * s.tiles) * UNIT + (lane % boxes) * p.box;
+    if (pos >= s.ctx || pos + p.box <= s.lo) return nullptr;
+    head = pair / p.head_tiles, row = table.row_of(pos);
+    return table.ids + b * table.ld + table.by_page(pos);
+  };
+  auto slab_of = [&](int page, int head) { return page >= 0 && page < table.n_pages ? page * p.a.n_kv + head : -1; };
+  auto look_up = [&](int u, int& slab, int& row) {
+    int head;
+    const int32_t* at = entry_of(u, head, row);
+    slab = at ? slab_of(load_fresh(at), head) : -1;
+  };
+
+  make_plan();
+  int slab, row, next_slab = -1, next_row = 0;
+  {
+    int head;
+    const int32_t* at = entry_of(u0 + lane / boxes, head, row);
+    const int page = at ? load_fresh(at) : -1;
+    slab = slab_of(page, head);
+    if (u0 < u1 && slab >= 0 && lane < boxes) {  // the first unit, into the L2
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c) {
+        hint_3d(&tmap_k, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
+        hint_3d(&tmap_v, c * (S::kChunkRow / static_cast<int>(sizeof(C))), row, slab);
+      }
+    }
+    pdl_wait();  // q, positions, the table and the newest cache rows come from preceding kernels
+    bool held = true;
+    for (int b = threadIdx.x; b < n_seq; b += S::kThreads) held = held && context_of(b) == contexts[b];
+    const int page_now = at ? load_fresh(at) : -1;
+    if (__syncthreads_or(!held)) {
+      make_plan();
+      look_up(u0 + lane / boxes, slab, row);
+    } else {
+      slab = slab_of(page_now, head);
+    }
   }
 
   // sequences without a visible position
@@ -239,22 +303,7 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     const uint32_t ring = ring0 + warp * ring_bytes;
     const float* my_scales = scales + warp * kStages * UNIT;
 
-    // ---- fetch: a lane looks up the page of one box, 32 boxes at a time and 32 ahead ------------------------------------------------
-    const int boxes = UNIT / p.box, ahead = 32 / boxes;  // of a unit; units that 32 lanes look up
-    auto look_up = [&](int u, int& slab, int& row) {     // box (lane % boxes) of unit u: slab -1 where there is nothing to fetch
-      slab = -1, row = 0;
-      if (u >= u1) return;
-      const int b = sequence_of(before, n_seq, u);
-      const Span s = span_of<UNIT>(contexts[b], p.a.window);
-      const int rest = u - before[b], pair = rest / s.tiles;
-      const int pos = (s.first + rest - pair * s.tiles) * UNIT + (lane % boxes) * p.box;
-      if (pos >= s.ctx || pos + p.box <= s.lo) return;
-      const int page = table.find(b, pos);
-      if (page >= 0) slab = page * p.a.n_kv + pair / p.head_tiles, row = table.row_of(pos);
-    };
     int base = u0;  // the first unit that the lanes have looked up
-    int slab, row, next_slab = -1, next_row = 0;
-    look_up(u0 + lane / boxes, slab, row);
     uint32_t have = __ballot_sync(0xffffffffu, slab >= 0);
     // The tile of keys (0) or of values (1) of a unit; the one before in its place has been read by all lanes.  `slot` is the unit's place among those
     // looked up, z and y its box where it has only one: then one lane does it all.

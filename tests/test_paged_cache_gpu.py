@@ -275,6 +275,39 @@ def test_attend_two_graphs_share_a_workspace():
             assert ((out.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dim", [128, 192])
+def test_attend_behind_a_kernel_that_writes_its_table(eight, dim):
+    """Table and positions come from the kernel directly in front, which lets this one begin before it is done: two tables in turn, copied as the
+    bits of a small cache's rows (a `load`), never waited for on the host."""
+    from gpt_fast import PagedKVCache
+    lengths = [[700, 40, 1300, 0], [32, 1200, 64, 333]]
+    cache, table = make_cache([max(a, b) for a, b in zip(*lengths)], 16, 2, dim, torch.bfloat16, eight)
+    order = [table, table[:, [1, 0] + list(range(2, table.shape[1]))].contiguous()]  # the second's first two pages change places
+    most = 128  # entries of a sequence: four rows of 32 numbers
+    notes = PagedKVCache(2, 16, 1, 64, torch.bfloat16, device="cuda")  # a page's rows hold a table as bits, its values' first row the positions
+    for i in range(2):
+        wide = torch.full((4, most), -1, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = order[i]
+        notes.k_pages[i, 0] = wide.view(torch.bfloat16).view(16, 64)
+        at = torch.full((32,), -1, dtype=torch.int32, device="cuda")
+        at[:4] = torch.tensor(lengths[i], dtype=torch.int32, device="cuda") - 1
+        notes.v_pages[i, 0, 0] = at.view(torch.bfloat16)
+    which = [torch.tensor([[i]], dtype=torch.int32, device="cuda") for i in range(2)]
+    last = torch.tensor([15], dtype=torch.int32, device="cuda")
+    out = tuple(torch.zeros(1, 1, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pages, pos = out[0].view(torch.int32).view(4, most), out[1].view(torch.int32).view(-1)[:4]
+    q = torch.randn(4, 8, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(torch.bfloat16)
+    ws = cache.attend_workspace(8)
+    want = [attend_64(cache, order[i], q, lengths[i]) for i in range(2)]
+    got = []
+    for n in range(30):
+        notes.load(last, which[n % 2], out=out)
+        got.append(cache.attend(q, pos, pages, workspace=ws))
+    for n, y in enumerate(got):
+        assert ((y.double() - want[n % 2][0]).abs() <= want[n % 2][1]).all()
+
+
 def test_attend_on_another_stream():
     lengths = [700, 20, 1300]
     cache, table = make_cache(lengths, 16, 4, 128, torch.bfloat16, True)
