@@ -36,16 +36,23 @@ class _Timed:
 
 class EngineTrace:
     OPS = ("embedding", "add_rmsnorm", "linear", "qkv_rope_kvcache", "gateup_swiglu", "attention", "lm_head_argmax")
+    PAGED = ("rope_paged_store", "paged_attention", "paged_load")  # called by the layers' caches
     COMM = ("all_reduce", "all_reduce_async", "wait", "linear_push", "add_rmsnorm_gather")
 
     def __init__(self, engine):
         self.engine, self.log = engine, []
         self._ops, self._comm = engine.ops, engine.comm
+        self._caches = [layer.attention.kv_cache for layer in engine.model.layers] if engine.paged else []
+        self._cache_ops = [cache.ops for cache in self._caches]
+        for cache in self._caches:
+            cache.ops = _Timed(cache.ops, self.PAGED, self.log)
         engine.ops = _Timed(engine.ops, self.OPS, self.log)
         engine.comm = _Timed(engine.comm, self.COMM, self.log, prefix="comm.")
 
     def stop(self):
         self.engine.ops, self.engine.comm = self._ops, self._comm
+        for cache, ops in zip(self._caches, self._cache_ops):
+            cache.ops = ops
 
     def report(self):
         """{name: (calls, device milliseconds, host milliseconds)} over everything recorded so far."""

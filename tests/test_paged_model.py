@@ -195,3 +195,22 @@ def test_captured_steps(family):
             assert (chosen == want[live, -1].argmax(-1))[decided].all()
             drawn = model.decode_sample(idx, pos, top_k=1, pages=pages)[live, 0].long()
             assert (drawn == want[live, -1].argmax(-1))[decided].all()
+
+
+@pytest.mark.gpu
+def test_trace_names_the_paged_operators():
+    """The per-operation times of a step and of a prompt hold what the layers' caches call; afterwards the caches call the library itself again."""
+    from gpt_fast.ops import CudaOps
+    from gpt_fast.trace import trace_engine
+    with torch.no_grad():
+        model, tokens = _model("ladder", "cuda"), _tokens()
+        pages, n_pages = table_for([PROMPTS[0] + STEPS], PAGE)
+        model.setup_paged_caches(1, n_pages, PAGE, max_length=128, max_prompt=96)
+        n, layers = PROMPTS[0], len(model.layers)
+        trace = trace_engine(model._engine)
+        model.prefill_last(tokens[0][None, :n].cuda(), torch.arange(n, dtype=torch.int32, device="cuda"), pages)
+        model(tokens[0][None, n:n + 1].cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), pages)
+        report = trace.report()
+        trace.stop()
+        assert report["rope_paged_store"][0] == 2 * layers and report["paged_attention"][0] == report["paged_load"][0] == layers
+        assert all(layer.attention.kv_cache.ops is CudaOps for layer in model.layers)
