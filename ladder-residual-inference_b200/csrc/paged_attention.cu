@@ -20,8 +20,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_plain_kernel(const Pag
   const int head = blockIdx.x, h = head / (p.n_head / p.n_kv);
   const int64_t b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / LANES, e = lane % LANES * 8;
-  int64_t ctx = load_pos(p.input_pos, p.pos_is_i64, b) + 1;
-  ctx = ctx > p.table.capacity() ? p.table.capacity() : ctx;
+  const int64_t pos = load_pos(p.input_pos, p.pos_is_i64, b), ctx = pos < p.table.capacity() ? pos + 1 : p.table.capacity();
   const int64_t lo = p.window > 0 && ctx > p.window ? ctx - p.window : 0;
   const int64_t at = (b * p.n_head + head) * p.dim + e;
   float q[8] = {}, o[8] = {}, m = -INFINITY, l = 0.f;

@@ -321,6 +321,56 @@ def test_attend_on_another_stream():
     assert ((got.double() - want).abs() <= tol).all()
 
 
+def test_attend_on_two_streams_at_once():
+    """Calls that may overlap on the device, each with a workspace of its own: the same bits as one behind the other."""
+    cases = []
+    for seed, lengths in ((1, [3000, 40, 900]), (2, [17, 2500])):
+        cache, table = make_cache(lengths, 16, 8, 128, torch.bfloat16, False, seed=seed)
+        q = torch.randn(len(lengths), 32, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(torch.bfloat16)
+        pos = torch.tensor([n - 1 for n in lengths], dtype=torch.int32, device="cuda")
+        cases.append((cache, q, pos, table, cache.attend_workspace(32), torch.cuda.Stream()))
+    want = [cache.attend(q, pos, table, workspace=ws) for cache, q, pos, table, ws, _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (cache, q, pos, table, ws, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                got[i].append(cache.attend(q, pos, table, workspace=ws))
+    torch.cuda.synchronize()
+    for y, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in y)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dim", [128, 192])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attend_scales_that_are_not_positive(eight, dim, scale):
+    lengths = [300, 1, 40]
+    cache, table = make_cache(lengths, 16, 2, dim, torch.bfloat16, eight)
+    q = torch.randn(3, 8, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(torch.bfloat16)
+    want, tol = attend_64(cache, table, q, lengths, scale=scale)
+    got = cache.attend(q, torch.tensor([n - 1 for n in lengths], dtype=torch.int32, device="cuda"), table, scale=scale)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dim", [128, 192])
+def test_positions_at_the_ends_of_64_bits(dim):
+    """The largest position is one behind the pages (attention and reading back: all of them; storing: left out), the smallest an idle row."""
+    cache, table = make_cache([48, 48], 16, 2, dim, torch.bfloat16, False)
+    table = table[:, :3]
+    pos = torch.tensor([2 ** 63 - 1, -2 ** 63], dtype=torch.int64, device="cuda")
+    q = torch.randn(2, 4, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).to(torch.bfloat16)
+    want, tol = attend_64(cache, table, q, [48, 0])
+    got = cache.attend(q, pos, table)
+    assert ((got.double() - want).abs() <= tol).all() and not got[1].any()
+    k, v = cache.load(pos, table)
+    for x, y in zip((k, v), dense(cache, table, 0, 0, 48)):
+        assert torch.equal(x[0].double(), y) and not x[1].any()
+    before, out = cache.k_pages.clone(), torch.full((2, 4, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    cache.store(torch.randn(2, 8 * dim, device="cuda").to(torch.bfloat16), None, pos, table, 4, out=out)
+    assert torch.equal(before.view(torch.int16), cache.k_pages.view(torch.int16)) and (out == 7).all()
+
+
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("dim", [64, 192])
 def test_attend_more_sequences_than_a_launch_takes(eight, dim):
