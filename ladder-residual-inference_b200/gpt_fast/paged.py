@@ -111,7 +111,7 @@ class PagedKVCache(nn.Module):
         return out
 
     def attend_workspace(self, n_head: int) -> Tensor:
-        """The workspace of `attend`: kept by the caller and shared by calls that do not overlap on the device."""
+        """The workspace of `attend`: shared by calls that do not overlap on the device, and kept by the caller as long as graphs captured with it."""
         k = self.k_pages
         return torch.zeros(self.ops.paged_attn_workspace_bytes(n_head, k.shape[1], k.shape[3]), dtype=torch.uint8, device=k.device)
 
