@@ -2,7 +2,7 @@
 //
 // The work is cut into units of 16 or 32 positions of one (sequence, KV head) pair, numbered sequence by sequence, head by head.  They lie on a
 // line, kStep apart, with kGap more behind each pair for what its beginning and end cost (1.0 to 1.2 us where a unit takes 2.6).  Every CTA (one an SM)
-// adds up the sequences and takes an equal stretch of the line, and so does each of its warps, so that sequences of any lengths keep
+// adds up the sequences and takes an equal stretch of the line (the last a shorter one), and so does each of its warps, so that sequences of any lengths keep
 // all SMs busy from the first microsecond to the last.  A warp is on its own: it fetches the units of its run by TMA (boxes that
 // lie within a page) into a ring of its own, a tile of keys or of values each as soon as the one before in its place has been read, and multiplies
 // them; a pair that lies in its run is finished and stored without a word to the others.  Where a run begins or ends inside a pair the
@@ -36,6 +36,11 @@ constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;  // of a launch
 constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of the line
 constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
+// CTAs are placed in the order of their numbers, and the last find their SMs taken by the preceding kernel to its end: behind a store of 16 rows the
+// last 16 of 148 have their first tiles 3 us after the others.  Of a full grid they take kLateBy of the line less, half their stretch at most (store and
+// attention in a graph, us, without and with: 8 sequences of 50 to 950 positions 14.1, 13.5; 16 of 300 14.9, 13.8; 16 of 1025 21.3, 20.6; 16 of 4000
+// 48.8, 48.7; by half of it 21.0 for the third, by half as much again 20.5 with 15.1 for the second).
+constexpr int kLateCtas = 16, kLateBy = 10 * kStep;
 constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
 constexpr int kMaxCtas = 256;
 constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once
@@ -194,9 +199,14 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   const int me = blockIdx.x;
   int units = 0, length = 0;       // in all; of the line
   int ctas = 0, stretch = 1, longer = 0;  // the CTAs that have work take equal stretches of the line, the first `longer` of them one more
+  int early = 0, late = 0;                // and those from `early` up `late` less
   int u0 = 0, u1 = 0, cta0 = 0, cta1 = 0;  // units of this warp, of this CTA
-  auto line_of = [&](int c) { return stretch * c + (c < longer ? c : longer); };
-  auto cta_at = [&](int at) { return at < (stretch + 1) * longer ? at / (stretch + 1) : (at - longer) / stretch; };
+  auto line_of = [&](int c) { return stretch * c + (c < longer ? c : longer) - (c > early ? (c - early) * late : 0); };
+  auto cta_at = [&](int at) {  // whose stretch holds this place
+    int c = 0, size = stretch, more = longer;
+    if (at >= line_of(early)) at -= line_of(early), c = early, size = stretch - late, more = longer > early ? longer - early : 0;
+    return c + (at < (size + 1) * more ? at / (size + 1) : (at - more) / size);
+  };
   auto make_plan = [&]() {
     units = length = 0;
     for (int b0 = 0; b0 < n_seq; b0 += S::kThreads) {
@@ -227,7 +237,10 @@ paged_attn_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       __syncthreads();
     }
     ctas = length < static_cast<int>(gridDim.x) * kMinRun ? (length + kMinRun - 1) / kMinRun : static_cast<int>(gridDim.x);
-    stretch = ctas > 0 ? length / ctas : 1, longer = length - stretch * ctas;
+    early = ctas, late = 0;
+    if (ctas == p.ctas && ctas > kLateCtas) early = ctas - kLateCtas, late = min(kLateBy, length / ctas / 2);
+    const int whole = length + (ctas - early) * late;
+    stretch = ctas > 0 ? whole / ctas : 1, longer = whole - stretch * ctas;
     u0 = u1 = cta0 = cta1 = 0;
     if (me < ctas) {
       // lanes 0 .. 3: the first unit at or behind a place
