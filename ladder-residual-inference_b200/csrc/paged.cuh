@@ -47,6 +47,19 @@ struct FastDiv {
   __host__ __device__ __forceinline__ int operator()(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift); }
 };
 
+// loads that see what has been written by now, whatever was read before
+__device__ __forceinline__ int load_fresh(const int32_t* at) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ int64_t load_pos_fresh(const void* input_pos, int pos_is_i64, int64_t i) {
+  if (!pos_is_i64) return load_fresh(static_cast<const int32_t*>(input_pos) + i);
+  int64_t v;
+  asm volatile("ld.relaxed.gpu.global.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const int64_t*>(input_pos) + i) : "memory");
+  return v;
+}
+
 // Pages of the sequences of a call.
 struct PageTable {
   const int32_t* ids;  // [n_seq, max_pages], row pitch ld

@@ -108,18 +108,6 @@ __device__ __forceinline__ int sequence_of(const int* begins, int n, int at) {
   }
   return lo;
 }
-// loads that see what has been written by now, whatever was read before
-__device__ __forceinline__ int load_fresh(const int32_t* at) {
-  int v;
-  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ int64_t load_pos_fresh(const void* input_pos, int pos_is_i64, int64_t i) {
-  if (!pos_is_i64) return load_fresh(static_cast<const int32_t*>(input_pos) + i);
-  int64_t v;
-  asm volatile("ld.relaxed.gpu.global.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const int64_t*>(input_pos) + i) : "memory");
-  return v;
-}
 __device__ __forceinline__ void hint_3d(const CUtensorMap* map, int x, int y, int z) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
 }

@@ -108,6 +108,49 @@ def test_store_skips_tokens_without_a_place(eight):
     _check_store(cache, out, qkv, rope, pos, pages, seq, n_head, False, live)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("tokens", [5, 700])
+def test_store_behind_a_kernel_that_writes_what_it_reads(eight, tokens):
+    """Positions, sequence numbers, pages and angles come from the kernels directly in front, which let this one begin before they are done: two sets in
+    turn, copied as the bits of a small cache's rows (a `load`), never waited for on the host."""
+    from gpt_fast import PagedKVCache
+    n_head, n_kv, dim, page, most, dtype = 4, 2, 64, 16, 16, torch.bfloat16
+    notes = PagedKVCache(2, 64, 1, 64, dtype, device="cuda")  # keys: the pages' table, then positions and sequences as bits; values: unused
+    angles = PagedKVCache(2, 256, 1, 64, dtype, device="cuda")
+    g = torch.Generator().manual_seed(0)
+    per = -(-tokens // 4)
+    sets = []
+    for i in range(2):
+        pages = torch.randperm(4 * most, generator=g).to(torch.int32).view(4, most)
+        pages[i, 3] = -1
+        at = torch.arange(4 * per)
+        seq, pos = ((at // per + i) % 4).to(torch.int32)[:tokens], (at % per + 5 + 20 * i).to(torch.int32)[:tokens]
+        pos[1 + i] = -1
+        words = torch.zeros(64 * 32, dtype=torch.int32)
+        words[:64], words[64:64 + tokens], words[1024:1024 + tokens] = pages.view(-1), pos, seq
+        notes.k_pages[i, 0] = words.view(dtype).view(64, 64).cuda()
+        angles.k_pages[i, 0] = torch.randn(256, 64, generator=g).to(dtype).cuda()
+        sets.append((pages.cuda(), pos.cuda(), seq.cuda(), angles.k_pages[i, 0].view(256, 32, 2)))
+    which = [torch.tensor([[i]], dtype=torch.int32, device="cuda") for i in range(2)]
+    last = torch.tensor([255], dtype=torch.int32, device="cuda")
+    words, spare = (torch.zeros(1, 1, 64, 64, dtype=dtype, device="cuda") for _ in range(2))
+    rope, spare2 = (torch.zeros(1, 1, 256, 64, dtype=dtype, device="cuda") for _ in range(2))
+    w = words.view(torch.int32).view(-1)
+    qkv = (torch.randn(tokens, (n_head + 2 * n_kv) * dim, generator=g) * 3).to(dtype).cuda()
+    caches = [PagedKVCache(4 * most, page, n_kv, dim, dtype, cache_dtype=E4M3 if eight else dtype, device="cuda") for _ in range(12)]
+    got = []
+    torch.cuda.synchronize()
+    for n, cache in enumerate(caches):
+        loads = [lambda i=n % 2: notes.load(last, which[i], out=(words, spare)), lambda i=n % 2: angles.load(last, which[i], out=(rope, spare2))]
+        for load in loads if n % 4 < 2 else loads[::-1]:
+            load()
+        got.append(cache.store(qkv, rope.view(256, 32, 2), w[64:64 + tokens], w[:64].view(4, most), n_head, sequence=w[1024:1024 + tokens]))
+    for n, (cache, q) in enumerate(zip(caches, got)):
+        pages, pos, seq, table = sets[n % 2]
+        live = (pos >= 0) & (pages[seq.long(), pos.clamp(min=0).long() // page] >= 0)
+        _check_store(cache, q, qkv, table, pos, pages, seq, n_head, False, live)
+
+
 def test_store_values_at_the_edges_of_e4m3():
     """Rows of zeros, of the smallest and largest numbers, with an infinity or a NaN."""
     from gpt_fast import PagedKVCache
