@@ -210,8 +210,9 @@ class Engine:
         return self.comm.all_reduce_async(buf, rows)
 
     # ------------------------------------------------------------------------------------------
-    def _trunk(self, idx, input_pos, pages=None):
+    def _trunk(self, idx, input_pos):
         """Everything up to the final norm; leaves the normalised hidden states in self.normed."""
+        pages = self._pages
         assert self.ready, "Caches must be initialized first"
         B, S = idx.shape
         assert (pages is not None) == self.paged, "a table of pages belongs to the caches of setup_paged_caches(), and these need one"
@@ -221,7 +222,6 @@ class Engine:
         else:
             assert input_pos.shape[0] == S, "input_pos must hold one position per token column"
         assert B <= self.max_batch and S <= self.max_seq, "batch or sequence exceeds the sizes that the caches were set up for"
-        self._pages = pages
         if input_pos.dtype not in (torch.int32, torch.int64):
             input_pos = input_pos.to(torch.int64)
         rows = B * S
@@ -319,7 +319,8 @@ class Engine:
 
     @torch.no_grad()
     def forward(self, idx, input_pos, pages=None):
-        B, S, rows = self._trunk(idx, input_pos, pages)
+        self._pages = pages
+        B, S, rows = self._trunk(idx, input_pos)
         logits = torch.empty(B, S, self.cfg.vocab_size, dtype=self.dtype, device=self.resid.device)
         self.ops.linear(self.normed, self.model.output.weight, logits, rows, workspace=self._head_workspace(rows))
         return logits
@@ -330,7 +331,8 @@ class Engine:
         computes the output projection for every position (gpt_fast/gpt_ladder_TP.py:282-283) although
         its generation loop reads only the last one (benchmark.py:82-83); for a long prompt that is
         most of the LM-head work (32 x 4096 positions x 128256 logits = 33.6 GB of output)."""
-        B, S, rows = self._trunk(idx, input_pos, pages)
+        self._pages = pages
+        B, S, rows = self._trunk(idx, input_pos)
         last = self.normed[:rows].view(B, S, self.d)[:, -1].contiguous()
         logits = torch.empty(B, 1, self.cfg.vocab_size, dtype=self.dtype, device=self.resid.device)
         self.ops.linear(last, self.model.output.weight, logits, B, workspace=self._head_workspace(B))
@@ -351,7 +353,8 @@ class Engine:
         a near-tie may resolve differently.
         """
         import torch.distributed as dist
-        B, S, rows = self._trunk(idx, input_pos, pages)
+        self._pages = pages
+        B, S, rows = self._trunk(idx, input_pos)
         assert S == 1, "forward_greedy is a decode step (one position per sequence)"
         n = self.vocab_hi - self.vocab_lo
         t = self.comm.world
@@ -395,7 +398,8 @@ class Engine:
         reference's softmax output is, so the draw is the reference's up to the rounding of the
         normaliser (summation order differs)."""
         import torch.distributed as dist
-        B, S, rows = self._trunk(idx, input_pos, pages)
+        self._pages = pages
+        B, S, rows = self._trunk(idx, input_pos)
         assert S == 1, "forward_sample is a decode step (one position per sequence)"
         t, V = self.comm.world, self.cfg.vocab_size
         n = self.vocab_hi - self.vocab_lo
