@@ -35,13 +35,15 @@ __device__ int g_paged_attn_status = 0;
 constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;  // of a launch
 constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of the line
-constexpr int kMinRun = 12 * kStep;  // of the line: a CTA without as much is not worth its part in the join
+// of the line: a CTA without as much is not worth its part in the join (one sequence of 1025 positions, us: 4, 8, 12, 24 units 11.8, 11.0, 11.1, 13.1)
+constexpr int kMinRun = 12 * kStep;
 // CTAs are placed in the order of their numbers, and the last find their SMs taken by the preceding kernel to its end: behind a store of 16 rows the
 // last 16 of 148 have their first tiles 3 us after the others.  Of a full grid they take kLateBy of the line less, half their stretch at most (store and
 // attention in a graph, us, without and with: 8 sequences of 50 to 950 positions 14.1, 13.5; 16 of 300 14.9, 13.8; 16 of 1025 21.3, 20.6; 16 of 4000
 // 48.8, 48.7; by half of it 21.0 for the third, by half as much again 20.5 with 15.1 for the second).
 constexpr int kLateCtas = 16, kLateBy = 10 * kStep;
-constexpr int kStages = 2;      // of a warp's ring: the keys of a unit, the values of a unit
+// of a warp's ring: the keys of a unit, the values of a unit (40 fp16 sequences, us: 2, 3, 4 units 64.1, 67.2, 67.6: SMs far from memory fall behind)
+constexpr int kStages = 2;
 constexpr int kMaxCtas = 256;
 constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once
 constexpr size_t kCounterBytes = kMaxCtas * 4;
@@ -59,11 +61,12 @@ struct StreamParams {
 // NT: blocks of eight query heads
 template <typename C, int HD, int NT>
 struct Shape {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;  // as many as the registers of an SM hold (100 e4m3 sequences, us: 8, 12, 16 83.1, 76.2, 77.2)
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRow = HD * static_cast<int>(sizeof(C));
   static constexpr int kChunkRow = kRow < 128 ? kRow : 128;  // bytes of a row that a box holds: the swizzle's span
   static constexpr int kChunks = kRow / kChunkRow;
+  // 4 KB of keys (us, this and twice as many: 40 fp16 sequences 64.2, 66.4; 100 e4m3 74.8, 78)
   static constexpr int kUnit = kRow > 128 ? 16 : 32;
   static constexpr uint32_t kChunkBytes = kUnit * kChunkRow;
   static constexpr uint32_t kHalf = kChunks * kChunkBytes;  // a tile of keys or of values

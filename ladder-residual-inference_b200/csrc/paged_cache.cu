@@ -86,7 +86,7 @@ __device__ __forceinline__ void rotate8_any(int rot, int halves, int e, const TT
 
 // LANES threads hold a head, eight elements each; blockIdx.y says which heads, blockIdx.x which `per` tokens.  The CTA first finds out where its
 // tokens go and brings their rows of the table into shared memory, while the first rows of the projection are on their way; then R tokens at a
-// time, the next R asked for before.  Bound by HBM for prompts (8192 tokens of 32 + 2 x 8 heads of 128, bf16: 39 us, 5.2 TB/s; e4m3 with halves from an
+// time, the next R asked for before.  Bound by HBM for prompts (8192 tokens of 32 + 2 x 8 heads of 128, bf16: 38 us, 5.3 TB/s; e4m3 with halves from an
 // fp32 table, where the arithmetic is half of it: 59 us), so bytes in flight and what is repeated for every vector count: with each token's place
 // looked up by every thread, 186 instructions for a vector and 67 us.  For single tokens it is a chain of loads and a store (3 us).
 template <typename T, typename TT, bool E4M3, bool VECTORS, int LANES, int R>
