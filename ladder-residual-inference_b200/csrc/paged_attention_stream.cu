@@ -42,7 +42,7 @@ constexpr int kMinRun = 12 * kStep;
 // attention in a graph, us, without and with: 8 sequences of 50 to 950 positions 14.1, 13.5; 16 of 300 14.9, 13.8; 16 of 1025 21.3, 20.6; 16 of 4000
 // 48.8, 48.7; by half of it 21.0 for the third, by half as much again 20.5 with 15.1 for the second).
 constexpr int kLateCtas = 16, kLateBy = 10 * kStep;
-// of a warp's ring: the keys of a unit, the values of a unit (40 fp16 sequences, us: 2, 3, 4 units 64.1, 67.2, 67.6: SMs far from memory fall behind)
+// of a warp's ring: the keys of a unit, the values of a unit (40 fp16 sequences, us: 2, 3, 4 places 64.1, 67.2, 67.6: SMs far from memory fall behind)
 constexpr int kStages = 2;
 constexpr int kMaxCtas = 256;
 constexpr int kJoin = 9;  // parts of other CTAs that are fetched at once

@@ -109,6 +109,18 @@ def test_store_skips_tokens_without_a_place(eight):
 
 
 @pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("rot", [0, 8])
+def test_store_many_tokens_of_few_heads(eight, rot):
+    """Blocks with more tokens than threads."""
+    dtype, n_head, n_kv, dim = torch.bfloat16, 1, 1, 8
+    cache, qkv, rope, pos, pages, seq = _store_case(dtype, eight, n_head, n_kv, dim, 64, [0, 9, 100], [30000, 1, 5003], rot, False, dtype)
+    pos[17::1000] = -1
+    live = pos >= 0
+    q = cache.store(qkv, rope, pos, pages, n_head, sequence=seq)
+    _check_store(cache, q, qkv, rope, pos, pages, seq, n_head, False, live)
+
+
+@pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("tokens", [5, 700])
 def test_store_behind_a_kernel_that_writes_what_it_reads(eight, tokens):
     """Positions, sequence numbers, pages and angles come from the kernels directly in front, which let this one begin before they are done: two sets in
