@@ -231,6 +231,10 @@ class Engine:
     def _body(self, idx, rows, B, S, input_pos):
         """Embedding, layers and final norm; leaves the normalised hidden states in self.normed."""
         self._splits = decode_splits(B, self.nh, self.nkv, self.model.max_seq_length, self.hd) if S == 1 and not self.paged else 1
+        if self.paged:
+            # The store leaves the query of a token without a place as it was: the same rows in every layer of a pass, which must not hold another
+            # pass's queries.
+            self.q[:rows].zero_()
         self.ops.embedding(self.model.tok_embeddings.weight, idx, self.resid)
         if not self._run_native(B, S, input_pos):
             getattr(self, "_run_" + self.family)(rows, B, S, input_pos)
