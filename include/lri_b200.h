@@ -250,7 +250,11 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  *
  * lri_paged_load: positions 0 .. last_pos[b] of each sequence into dense caches k_out, v_out [n_seq, n_kv, rows, head_dim] in `dtype`
  * (e4m3: code * scale, rounded once), with zeros in rows without a page and behind them up to a multiple of 64 positions, as far as a tile of
- * lri_attn_prefill reads; later rows are left as they were. */
+ * lri_attn_prefill reads; later rows are left as they were.
+ *
+ * lri_attn_prefill_pages: lri_attn_prefill of one sequence over such a copy of its pages (k_cache, v_cache [1, n_kv, smax, head_dim], read back up
+ * to the largest position), with each query's own position input_pos[s]: it sees positions 0 .. input_pos[s], as far as they have pages, as the one new
+ * token of lri_paged_attn_decode does; zeros with none visible (a negative position).  pages [max_pages]: the sequence's row of the table. */
 typedef struct {
   const void *qkv, *rope_table, *input_pos;
   const int32_t *sequence, *pages;
@@ -285,6 +289,9 @@ typedef struct {
   int dtype, cache_dtype, page_size, n_seq, max_pages, pos_is_i64, n_kv, head_dim;
 } lri_paged_load_call;
 int lri_paged_load(const lri_paged_load_call* call);
+int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos, int pos_is_i64, void* out,
+                           int S, int n_head, int n_kv, int head_dim, int64_t smax, const int32_t* pages, int max_pages, int page_size,
+                           int64_t n_pages, lri_stream_t stream);
 
 /* ---- F8: all-reduce over peer memory (one process per GPU) -----------------------------------
  * A communicator owns, on every rank, one inbox buffer that all peers can write.  One-shot

@@ -5,7 +5,7 @@
 // device memory, use fp32 softmax state, and round the output once to the storage type.
 #include <cstdlib>
 
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace lri {
 // cluster form of the decode kernel (attention_cluster.cu)
@@ -23,7 +23,7 @@ int attn_decode_stream_launch(int dtype, const void* q, const void* k_cache, con
 bool attn_prefill_tc_supports(int B, int S, int n_head, int n_kv, int head_dim, int64_t smax);
 int attn_prefill_tc_launch(int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos,
                            int pos_is_i64, void* out, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax,
-                           float scale_log2, cudaStream_t st);
+                           float scale_log2, const PageTable* table, cudaStream_t st);
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -274,6 +274,7 @@ struct PrefillParams {
   int S, n_head, n_kv;
   int64_t smax;
   float scale_log2;
+  PageTable table;  // PAGES
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -313,8 +314,8 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
 
 // Grid (ceil(S / 64), n_head, B).  Each of the 4 warps owns 16 query rows; K and V tiles of 64
 // positions are staged in shared memory with padded rows (HD + 8 elements) so that ldmatrix
-// reads are bank-conflict free.
-template <typename T, int HD>
+// reads are bank-conflict free.  PAGES as in attention_tc.cu: queries have positions of their own, keys without a page are masked.
+template <typename T, int HD, bool PAGES>
 __global__ void __launch_bounds__(kPfThreads) attn_prefill_kernel(const PrefillParams p) {
   constexpr int LDS = HD + 8;          // padded row length in elements
   constexpr int KB = HD / 16;          // k blocks of the QK^T product
@@ -336,6 +337,14 @@ __global__ void __launch_bounds__(kPfThreads) attn_prefill_kernel(const PrefillP
   const int q_end = (q0 + kPfBlockM < p.S) ? q0 + kPfBlockM : p.S;
   int64_t kv_end = pos0 + q_end;  // keys 0 .. pos0 + q_end - 1 are visible to the last row
   kv_end = kv_end > p.smax ? p.smax : kv_end;
+  __shared__ int last_of[4];  // PAGES: the last position that a warp's queries see
+  auto own_pos = [&](int s) { return s < p.S ? p.table.clamped(load_pos(p.input_pos, p.pos_is_i64, s), p.smax) : -1; };
+  if (PAGES) {
+    const int last = __reduce_max_sync(0xffffffffu, own_pos(q0 + warp * 16 + (lane & 15)));
+    if (lane == 0) last_of[warp] = last;
+    __syncthreads();
+    kv_end = 1 + max(max(last_of[0], last_of[1]), max(last_of[2], last_of[3]));
+  }
 
   const T* qg = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.S * p.n_head + head) * HD;
   const T* kg = static_cast<const T*>(p.k_cache) + (static_cast<int64_t>(b) * p.n_kv + kvh) * p.smax * HD;
@@ -367,8 +376,8 @@ __global__ void __launch_bounds__(kPfThreads) attn_prefill_kernel(const PrefillP
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   // absolute positions of the two query rows this thread holds scores for
-  const int64_t qpos0 = pos0 + q0 + warp * 16 + (lane >> 2);
-  const int64_t qpos1 = qpos0 + 8;
+  const int64_t qpos0 = PAGES ? own_pos(q0 + warp * 16 + (lane >> 2)) : pos0 + q0 + warp * 16 + (lane >> 2);
+  const int64_t qpos1 = PAGES ? own_pos(q0 + warp * 16 + (lane >> 2) + 8) : qpos0 + 8;
 
   const int n_tiles = static_cast<int>((kv_end + kPfBlockN - 1) / kPfBlockN);
   for (int t = 0; t < n_tiles; ++t) {
@@ -407,6 +416,8 @@ __global__ void __launch_bounds__(kPfThreads) attn_prefill_kernel(const PrefillP
 
     // ---- scale, causal mask, online softmax -----------------------------------------------------------
     float mx[2] = {-INFINITY, -INFINITY};
+    uint64_t paged = ~0ull;  // the keys of this tile that have a page
+    if (PAGES) paged = p.table.named64(t * kPfBlockN, lane);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int64_t key = kv0 + nb * 8 + (lane & 3) * 2;
@@ -414,7 +425,8 @@ __global__ void __launch_bounds__(kPfThreads) attn_prefill_kernel(const PrefillP
       for (int e = 0; e < 4; ++e) {
         const int64_t kj = key + (e & 1);
         const int64_t qp = (e < 2) ? qpos0 : qpos1;
-        const float v = (kj <= qp && kj < kv_end) ? sc[nb][e] * p.scale_log2 : -INFINITY;
+        const bool there = !PAGES || ((paged >> (kj - kv0)) & 1u);
+        const float v = (kj <= qp && kj < kv_end && there) ? sc[nb][e] * p.scale_log2 : -INFINITY;
         sc[nb][e] = v;
         mx[e >> 1] = fmaxf(mx[e >> 1], v);
       }
@@ -505,10 +517,10 @@ int launch_decode(const DecodeParams& p, int B, cudaStream_t st) {
   return LRI_OK;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool PAGES>
 int launch_prefill(const PrefillParams& p, int B, cudaStream_t st) {
   constexpr int smem = (kPfBlockM + 2 * kPfBlockN) * (HD + 8) * 2;
-  auto kern = attn_prefill_kernel<T, HD>;
+  auto kern = attn_prefill_kernel<T, HD, PAGES>;
   static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
   LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   dim3 grid((p.S + kPfBlockM - 1) / kPfBlockM, p.n_head, B);
@@ -655,28 +667,53 @@ extern "C" int lri_attn_decode(int dtype, const void* q, const void* k_cache, co
   return head_dim == 128 ? launch_decode<__half, 128>(p, B, st) : launch_decode<__half, 64>(p, B, st);
 }
 
+namespace lri {
+namespace {
+// What both forms of prompt attention ask, and which kernel they run; `table` not NULL: over a copy of one sequence's pages.
+int prefill(const char* who, int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos, int pos_is_i64, void* out, int B,
+            int S, int n_head, int n_kv, int head_dim, int64_t smax, const PageTable* table, cudaStream_t st) {
+  int rc = check_attn(who, dtype, B, n_head, n_kv, head_dim, smax);
+  if (rc != LRI_OK) return rc;
+  LRI_REQUIRE(q && k_cache && v_cache && input_pos && out, LRI_ERR_ARG, "%s: NULL pointer", who);
+  LRI_REQUIRE(S >= 0 && S <= (1 << 22), LRI_ERR_ARG, "%s: S=%d", who, S);
+  LRI_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), LRI_ERR_ALIGN, "%s: pointers must be 16-byte aligned", who);
+  if (B == 0 || S == 0) return LRI_OK;
+  const float scale_log2 = kLog2e / sqrtf(static_cast<float>(head_dim));
+  // option attn_prefill_tc: 1 = the tcgen05 / TMEM kernel (default), 0 = the mma.sync kernel above
+  if (option(OPT_ATTN_PREFILL_TC) != 0 && attn_prefill_tc_supports(B, S, n_head, n_kv, head_dim, smax))
+    return attn_prefill_tc_launch(dtype, q, k_cache, v_cache, input_pos, pos_is_i64, out, B, S, n_head, n_kv, head_dim, smax, scale_log2, table, st);
+  PrefillParams p{};
+  p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64, p.out = out;
+  p.S = S, p.n_head = n_head, p.n_kv = n_kv, p.smax = smax, p.scale_log2 = scale_log2;
+  if (table) p.table = *table;
+  auto go = [&](auto pages) {
+    constexpr bool kPages = decltype(pages)::value;
+    if (dtype == LRI_BF16)
+      return head_dim == 128 ? launch_prefill<__nv_bfloat16, 128, kPages>(p, B, st) : launch_prefill<__nv_bfloat16, 64, kPages>(p, B, st);
+    return head_dim == 128 ? launch_prefill<__half, 128, kPages>(p, B, st) : launch_prefill<__half, 64, kPages>(p, B, st);
+  };
+  return table ? go(std::true_type{}) : go(std::false_type{});
+}
+}  // namespace
+}  // namespace lri
+
 extern "C" int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* v_cache,
                                 const void* input_pos, int pos_is_i64, void* out, int B, int S, int n_head, int n_kv,
                                 int head_dim, int64_t smax, lri_stream_t stream) {
-  int rc = check_attn("attn_prefill", dtype, B, n_head, n_kv, head_dim, smax);
-  if (rc != LRI_OK) return rc;
-  LRI_REQUIRE(q && k_cache && v_cache && input_pos && out, LRI_ERR_ARG, "attn_prefill: NULL pointer");
-  LRI_REQUIRE(S >= 0 && S <= (1 << 22), LRI_ERR_ARG, "attn_prefill: S=%d", S);
-  LRI_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), LRI_ERR_ALIGN,
-              "attn_prefill: pointers must be 16-byte aligned");
-  if (B == 0 || S == 0) return LRI_OK;
-  // option attn_prefill_tc: 1 = the tcgen05 / TMEM kernel (default), 0 = the mma.sync kernel below
-  if (option(OPT_ATTN_PREFILL_TC) != 0 && attn_prefill_tc_supports(B, S, n_head, n_kv, head_dim, smax))
-    return attn_prefill_tc_launch(dtype, q, k_cache, v_cache, input_pos, pos_is_i64, out, B, S, n_head, n_kv, head_dim,
-                                  smax, kLog2e / sqrtf(static_cast<float>(head_dim)), static_cast<cudaStream_t>(stream));
-  PrefillParams p{};
-  p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64, p.out = out;
-  p.S = S, p.n_head = n_head, p.n_kv = n_kv, p.smax = smax;
-  p.scale_log2 = kLog2e / sqrtf(static_cast<float>(head_dim));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LRI_BF16)
-    return head_dim == 128 ? launch_prefill<__nv_bfloat16, 128>(p, B, st) : launch_prefill<__nv_bfloat16, 64>(p, B, st);
-  return head_dim == 128 ? launch_prefill<__half, 128>(p, B, st) : launch_prefill<__half, 64>(p, B, st);
+  return prefill("attn_prefill", dtype, q, k_cache, v_cache, input_pos, pos_is_i64, out, B, S, n_head, n_kv, head_dim, smax, nullptr,
+                 static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos, int pos_is_i64, void* out,
+                                      int S, int n_head, int n_kv, int head_dim, int64_t smax, const int32_t* pages, int max_pages, int page_size,
+                                      int64_t n_pages, lri_stream_t stream) {
+  PageTable t{pages, max_pages, 1, max_pages, page_size, n_pages, {}};
+  LRI_REQUIRE(pages, LRI_ERR_ARG, "attn_prefill_pages: NULL pointer");
+  LRI_REQUIRE(max_pages >= 1 && n_pages >= 1 && page_size >= 8 && page_size <= 4096 && page_size % 8 == 0 && t.capacity() <= (1ll << 30), LRI_ERR_ARG,
+              "attn_prefill_pages: %d of %lld pages of %d positions", max_pages, (long long)n_pages, page_size);
+  t.by_page = FastDiv::of(page_size);
+  return prefill("attn_prefill_pages", dtype, q, k_cache, v_cache, input_pos, pos_is_i64, out, 1, S, n_head, n_kv, head_dim, smax, &t,
+                 static_cast<cudaStream_t>(stream));
 }
 
 // =====================================================================================================

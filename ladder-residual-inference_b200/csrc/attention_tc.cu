@@ -22,6 +22,11 @@
 //
 // Rows of the KV cache past the newest position must hold finite values (they are multiplied by
 // P = 0); the cache module zero-initialises them, as the reference's does (gpt_fast/utils.py:47-48).
+//
+// PAGES: the cache is a dense copy of a sequence's pages.  Every query has a position of its own, negative for none, and keys without a page are
+// masked, so that a prompt sees what single tokens at its positions would.  A softmax warp looks the pages of a tile's keys up (two a lane) before it
+// waits for the tile's scores.
+#include "paged.cuh"
 #include "tcgen05.cuh"
 
 namespace lri {
@@ -44,9 +49,10 @@ struct FaParams {
   int S, n_head, n_kv;
   int64_t smax;
   float scale_log2;
+  PageTable table;  // PAGES
 };
 
-template <typename T, int HD>
+template <typename T, int HD, bool PAGES>
 __global__ void __launch_bounds__(kFaThreads, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const FaParams p) {
@@ -68,6 +74,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   __shared__ uint64_t bars[1 + 2 * kFaStages + 6];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
+  __shared__ int last_of[4];  // PAGES: the last position that a softmax warp's queries see
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // uniform for the compiler too
   const int lane = threadIdx.x & 31;
@@ -104,23 +111,31 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  int own_pos = -1;  // PAGES: of this thread's query
+  if (PAGES && warp >= 2) {
+    const int s = q0 + (warp & 3) * 32 + lane;
+    if (s < p.S) own_pos = p.table.clamped(load_pos(p.input_pos, p.pos_is_i64, s), p.smax);
+    const int last = __reduce_max_sync(0xffffffffu, own_pos);
+    if (lane == 0) last_of[warp & 3] = last;
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
 
-  int64_t pos0 = load_pos(p.input_pos, p.pos_is_i64, 0);
+  int64_t pos0 = PAGES ? 0 : load_pos(p.input_pos, p.pos_is_i64, 0);
   pos0 = pos0 < 0 ? 0 : pos0;
   const int q_end = (q0 + kFaM < p.S) ? q0 + kFaM : p.S;
   int64_t kv_end = pos0 + q_end;  // keys 0 .. pos0 + q_end - 1 are visible to the last row of the tile
   kv_end = kv_end > p.smax ? p.smax : kv_end;
-  const int n_tiles = static_cast<int>((kv_end + kFaN - 1) / kFaN);  // >= 1
+  if (PAGES) kv_end = 1 + max(max(last_of[0], last_of[1]), max(last_of[2], last_of[3]));
+  const int n_tiles = static_cast<int>((kv_end + kFaN - 1) / kFaN);  // >= 1 (PAGES: 0 where no query of the tile has a position)
   const int kv_row0_hi = static_cast<int>((static_cast<int64_t>(b) * p.n_kv + kvh) * p.smax);  // row of key 0 in the [rows, HD] view
 
   // warp-uniform loops, one elected lane issues: a loop run by one lane takes 74 cycles a product (see gemm_pair.cu), and a tile
   // has HD / 16 + 4 of them
   if (warp == 0) {
-    if (elect_one()) {
+    if ((!PAGES || n_tiles > 0) && elect_one()) {
       mbar_expect_tx(q_full, kQBytes);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
@@ -151,7 +166,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                                   (static_cast<uint32_t>(HD >> 3) << 17) | (static_cast<uint32_t>(kFaM >> 4) << 24);
     constexpr uint32_t v_lbo = kKvChunkBytes;  // between the 64-column chunks of head_dim
     constexpr uint32_t v_sbo = 1024u;           // between groups of 8 keys
-    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, &abort_flag, 2, &g_attn_tc_status));
+    bool ok = (!PAGES || n_tiles > 0) && __all_sync(0xffffffffu, mbar_wait(q_full, 0, &abort_flag, 2, &g_attn_tc_status));
 
     auto issue_qk = [&](int j) {
       const uint32_t s = j % kFaStages, round = j / kFaStages;
@@ -200,11 +215,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const int quarter = warp & 3;       // TMEM lanes a warp may touch: 32 * (warp id mod 4)
     const int i = quarter * 32 + lane;  // query row of this thread
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const int64_t qpos = pos0 + q0 + i;
+    const int64_t qpos = PAGES ? own_pos : pos0 + q0 + i;
     float m_ref = -INFINITY, l = 0.f;
     bool alive = true;
     for (int j = 0; j < n_tiles; ++j) {
       const uint32_t sb = static_cast<uint32_t>(j & 1);
+      uint64_t paged = ~0ull;  // the keys of this tile that have a page
+      if (PAGES) paged = p.table.named64(j * kFaN, lane);
       const bool ready = mbar_wait(s_full0 + 8 * sb, (static_cast<uint32_t>(j) >> 1) & 1u, &abort_flag, 5, &g_attn_tc_status);
       if (!__all_sync(0xffffffffu, ready)) {
         alive = false;
@@ -225,7 +242,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       const int64_t key0 = static_cast<int64_t>(j) * kFaN;
       // tiles that reach past the first row's position or past the end of the visible keys need the mask
-      if (key0 + kFaN - 1 > pos0 + q0 || key0 + kFaN > kv_end) {
+      if constexpr (PAGES) {
+        if (__any_sync(0xffffffffu, key0 + kFaN - 1 > qpos) || paged != ~0ull) {
+#pragma unroll
+          for (int e = 0; e < kFaN; ++e)
+            if (key0 + e > qpos || !((paged >> e) & 1u)) sv[e] = -INFINITY;
+        }
+      } else if (key0 + kFaN - 1 > pos0 + q0 || key0 + kFaN > kv_end) {
 #pragma unroll
         for (int e = 0; e < kFaN; ++e) {
           const int64_t kj = key0 + e;
@@ -238,7 +261,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       for (int e = 4; e < kFaN; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], sv[e]);
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;  // in log2 units
       if (j == 0) {
-        m_ref = mx;  // tile 0 holds key 0, which every query sees: finite
+        m_ref = mx;  // tile 0 holds key 0, which every query sees: finite (PAGES: -inf until a key is visible, O and l zero)
       } else {
         const bool need = mx > m_ref + kFaRescaleLog2;
         if (__any_sync(0xffffffffu, need)) {
@@ -284,6 +307,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(p_full0 + 8 * sb);
     }
+    if (PAGES && n_tiles == 0) {  // no position: zeros
+      alive = false;
+      T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.S + q0 + i) * p.n_head + head) * HD;
+      if (q0 + i < p.S)
+        for (int v = 0; v < HD / 8; ++v) reinterpret_cast<uint4*>(dst)[v] = make_uint4(0, 0, 0, 0);
+    }
     if (alive) {
       const uint32_t ob = static_cast<uint32_t>((n_tiles - 1) & 1);
       const bool done = mbar_wait(o_done0 + 8 * ob, (static_cast<uint32_t>(n_tiles - 1) >> 1) & 1u, &abort_flag, 7,
@@ -324,7 +353,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool PAGES>
 int launch_fa(int dtype, const void* q, const void* k_cache, const void* v_cache, const FaParams& p, int B,
               cudaStream_t st) {
   CUtensorMap tq, tk, tv;
@@ -337,7 +366,7 @@ int launch_fa(int dtype, const void* q, const void* k_cache, const void* v_cache
   if (rc != LRI_OK) return rc;
   constexpr int kChunks = HD / 64;
   constexpr int smem = kChunks * kFaM * 128 + kFaStages * 2 * kChunks * kFaN * 128 + 1024;
-  auto kern = attn_prefill_tc_kernel<T, HD>;
+  auto kern = attn_prefill_tc_kernel<T, HD, PAGES>;
   static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
   LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   dim3 grid((p.S + kFaM - 1) / kFaM, p.n_head, B);
@@ -356,17 +385,23 @@ bool attn_prefill_tc_supports(int B, int S, int n_head, int n_kv, int head_dim, 
   return kv_rows < (1ll << 31) && q_rows < (1ll << 31) && static_cast<int64_t>(n_head) * head_dim < (1ll << 31);
 }
 
+// `table` not NULL: PAGES, of one sequence
 int attn_prefill_tc_launch(int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos,
                            int pos_is_i64, void* out, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax,
-                           float scale_log2, cudaStream_t st) {
+                           float scale_log2, const PageTable* table, cudaStream_t st) {
   FaParams p{};
   p.out = out, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64;
   p.S = S, p.n_head = n_head, p.n_kv = n_kv, p.smax = smax, p.scale_log2 = scale_log2;
-  if (dtype == LRI_BF16)
-    return head_dim == 128 ? launch_fa<__nv_bfloat16, 128>(dtype, q, k_cache, v_cache, p, B, st)
-                           : launch_fa<__nv_bfloat16, 64>(dtype, q, k_cache, v_cache, p, B, st);
-  return head_dim == 128 ? launch_fa<__half, 128>(dtype, q, k_cache, v_cache, p, B, st)
-                         : launch_fa<__half, 64>(dtype, q, k_cache, v_cache, p, B, st);
+  if (table) p.table = *table;
+  auto go = [&](auto pages) {
+    constexpr bool kPages = decltype(pages)::value;
+    if (dtype == LRI_BF16)
+      return head_dim == 128 ? launch_fa<__nv_bfloat16, 128, kPages>(dtype, q, k_cache, v_cache, p, B, st)
+                             : launch_fa<__nv_bfloat16, 64, kPages>(dtype, q, k_cache, v_cache, p, B, st);
+    return head_dim == 128 ? launch_fa<__half, 128, kPages>(dtype, q, k_cache, v_cache, p, B, st)
+                           : launch_fa<__half, 64, kPages>(dtype, q, k_cache, v_cache, p, B, st);
+  };
+  return table ? go(std::true_type{}) : go(std::false_type{});
 }
 
 int attn_prefill_tc_status_read_and_clear(int* status_out) {

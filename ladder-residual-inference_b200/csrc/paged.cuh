@@ -74,6 +74,17 @@ struct PageTable {
     return id >= 0 && id < n_pages ? id : -1;
   }
   __device__ __forceinline__ int row_of(int pos) const { return pos - by_page(pos) * page; }  // within its page
+  // a position as attention takes it: -1 where it is negative, the last of the pages (or of `most` rows) where it lies behind them
+  __device__ __forceinline__ int clamped(int64_t pos, int64_t most) const {
+    most = most < capacity() ? most : capacity();
+    return static_cast<int>(pos < 0 ? -1 : (pos < most ? pos : most - 1));
+  }
+  // which of the positions first .. first + 63 of sequence 0 have a page: bit i is position first + i; by a whole warp
+  __device__ __forceinline__ uint64_t named64(int first, int lane) const {
+    const int a = first + lane, b = a + 32;
+    const uint32_t lo = __ballot_sync(0xffffffffu, a < capacity() && find(0, a) >= 0), hi = __ballot_sync(0xffffffffu, b < capacity() && find(0, b) >= 0);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+  }
 };
 
 // Attention of one new token of each sequence (paged_attention.cu).

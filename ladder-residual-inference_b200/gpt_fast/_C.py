@@ -78,6 +78,8 @@ _SIGNATURES = {
     "lri_paged_attn_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "lri_paged_attn_decode": (c_int, [c_void_p]),
     "lri_paged_load": (c_int, [c_void_p]),
+    "lri_attn_prefill_pages": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_void_p,
+                                       c_int, c_int, c_int64, c_void_p]),
     "lri_comm_create": (c_int, [c_int, c_int, c_int64, ctypes.POINTER(c_void_p), ctypes.c_char_p]),
     "lri_comm_connect": (c_int, [c_void_p, ctypes.c_char_p]),
     "lri_allreduce": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),

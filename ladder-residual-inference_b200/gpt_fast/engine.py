@@ -167,7 +167,11 @@ class Engine:
             cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
         else:
             k, v = cache.load(pos[-1:], self._pages, out=(self.dense_k, self.dense_v))
-            ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)
+            if hasattr(ops, "attention_pages"):
+                n_pages, _, page, _ = cache.k_pages.shape
+                ops.attention_pages(q, k, v, pos, self._pages, page, n_pages, self.y, S, self.nh, self.nkv, self.hd)
+            else:  # an ops object without it takes prompts whose positions all have pages
+                ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)
 
     def _mlp(self, w1, w2, rows, out, addend=None, normed=None, push=0):
         self.ops.gateup_swiglu(self.normed if normed is None else normed, w1, self.h, rows, self.ws_ug)

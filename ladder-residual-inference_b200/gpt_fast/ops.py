@@ -186,6 +186,14 @@ class CudaOps:
         if status < 0:
             _C.check(status)
 
+    @staticmethod
+    def attention_pages(q, k_cache, v_cache, input_pos, pages, page, n_pages, out, S, n_head, n_kv, head_dim):
+        """Prompt attention of one sequence over a dense copy of its pages (paged_load): what has no page is left out, as in paged_attention."""
+        _C.require_cuda(q, k_cache, v_cache, input_pos, pages, out)
+        _C.check(_C.lib.lri_attn_prefill_pages(_C.dtype_code(q.dtype), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), input_pos.data_ptr(),
+                                               int(input_pos.dtype == torch.int64), out.data_ptr(), S, n_head, n_kv, head_dim, k_cache.shape[2],
+                                               pages.data_ptr(), pages.shape[1], page, n_pages, _C.stream_handle()))
+
     # ---- all layers of a pass ------------------------------------------------------------------------
     @staticmethod
     def run_layers(schedule, layers, above, events, main, side, sizes, eps, workspaces, row_ws, **tensors):

@@ -35,7 +35,7 @@ class _Timed:
 
 
 class EngineTrace:
-    OPS = ("embedding", "add_rmsnorm", "linear", "qkv_rope_kvcache", "gateup_swiglu", "attention", "lm_head_argmax")
+    OPS = ("embedding", "add_rmsnorm", "linear", "qkv_rope_kvcache", "gateup_swiglu", "attention", "attention_pages", "lm_head_argmax")
     PAGED = ("rope_paged_store", "paged_attention", "paged_load")  # called by the layers' caches
     COMM = ("all_reduce", "all_reduce_async", "wait", "linear_push", "add_rmsnorm_gather")
 

@@ -18,6 +18,29 @@ class Ops(PagedOps, CpuOps):
         named = torch.where((pages >= 0) & (pages < n_pages), pages, -1)
         return PagedOps._rows(stored, scales, named, b, lo, min(hi, pages.shape[1] * page))
 
+    @classmethod
+    def paged_load(cls, k_pages, v_pages, k_scale, v_scale, pages, last_pos, k_out, v_out, rows, pages_shape, cache_shape):
+        n_pages, _, page, _ = cache_shape
+        for b, last in enumerate(last_pos.tolist()):
+            n = max(0, min(last + 1, rows, pages_shape[1] * page))
+            at = torch.arange(n)
+            ids = pages[b].long()[at // page]
+            there = (ids >= 0) & (ids < n_pages)
+            for t, s, out in ((k_pages, k_scale, k_out), (v_pages, v_scale, v_out)):
+                out[b, :, :-(-n // 64) * 64] = 0
+                out[b][:, at[there]] = cls._rows(t, s, pages, b, 0, n).transpose(0, 1).to(out.dtype)
+
+    @staticmethod
+    def attention_pages(q, k_cache, v_cache, input_pos, pages, page, n_pages, out, S, n_head, n_kv, head_dim):
+        most = min(k_cache.shape[2], pages.shape[1] * page)
+        at = torch.arange(most)
+        ids = pages[0].long()[at // page]
+        seen = (at <= input_pos.long()[:, None]) & (ids >= 0) & (ids < n_pages)
+        k, v = (t[0, :, :most].float().repeat_interleave(n_head // n_kv, 0) for t in (k_cache, v_cache))
+        scores = (q.float().view(S, n_head, head_dim).transpose(0, 1) @ k.transpose(1, 2) * head_dim ** -0.5).masked_fill(~seen, float("-inf"))
+        w = torch.softmax(scores, -1).nan_to_num(0.0)  # nothing visible: zeros
+        out[:S] = (w @ v).transpose(0, 1).reshape(S, -1).to(out.dtype)
+
 
 BOTH = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -61,3 +84,46 @@ def test_a_step_without_its_page_depends_on_nothing_before_it(family, device, mo
             # row 0: no page at its position; row 1: all there; row 2: a position behind the table
             got.append(model(idx, torch.tensor([32, 40, 6 * PAGE], dtype=torch.int32, device=device), table).float().cpu())
         assert got[0].isfinite().all() and torch.equal(got[0], got[1])
+
+
+def _same(got, want):
+    """The tolerance of the other whole-model tests."""
+    assert got.isfinite().all() and ((got - want).norm() / want.norm()).item() < 2e-2
+
+
+def _singles(model, tokens, positions, table, device):
+    return torch.cat([model(tokens[:, i:i + 1].to(device), torch.tensor([p], dtype=torch.int32, device=device), table)[0].float().cpu()
+                      for i, p in enumerate(positions)])
+
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("family", ["dense", "ladder"])
+@pytest.mark.parametrize("gone", [[0, 1], [2], [5], [0, 3, 4, 5]])
+def test_a_portion_sees_what_single_steps_see(family, device, gone, monkeypatch):
+    """Pages of earlier positions that were freed, and pages that some of the new tokens lack: a portion of a prompt and the same tokens one at a time."""
+    with torch.no_grad():
+        model = _setup(monkeypatch, family, device, 1, 12, PAGE, max_length=128, max_prompt=96)
+        table = torch.arange(8, dtype=torch.int32, device=device)[None].clone()
+        model(_tokens(70, 1).to(device), _positions(0, 70, device), table)
+        table[0, gone] = -1
+        table[0, 7] = 12  # names no page either
+        tokens = _tokens(40, 2)
+        got = model(tokens.to(device), _positions(70, 110, device), table)[0].float().cpu()
+        _same(got, _singles(model, tokens, range(70, 110), table, device))
+
+
+# The C ABI checks sizes and pointers before it touches a device: addresses that are never read stand in for device memory.
+BUF = 1 << 20
+ARG, ALIGN, UNSUPPORTED = -1, -2, -3
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(pages=0), ARG), (dict(most=0), ARG), (dict(n_pages=0), ARG), (dict(page=12), ARG), (dict(page=0), ARG), (dict(page=8192), ARG),
+    (dict(most=1 << 28), ARG), (dict(q=0), ARG), (dict(pos=0), ARG), (dict(out=BUF + 8), ALIGN), (dict(S=-1), ARG), (dict(n_head=3), ARG), (dict(dim=80), UNSUPPORTED),
+    (dict(smax=0), ARG), (dict(dtype=3), UNSUPPORTED), (dict(S=0), 0)])
+def test_c_prompt_over_pages_refuses(kw, status):
+    from gpt_fast import _C
+    a = dict(dtype=0, q=BUF, k=BUF, v=BUF, pos=BUF, i64=0, out=BUF, S=4, n_head=4, n_kv=2, dim=64, smax=64, pages=BUF, most=4, page=16, n_pages=6, stream=0)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    assert _C.lib.lri_attn_prefill_pages(*a.values()) == status
