@@ -46,7 +46,7 @@ class Engine:
         self.comm = comm if comm is not None else make_comm()
         self.ready = False
         self.paged = False  # whether the layers' caches are pages (setup_paged)
-        self._pages = None  # the table of the step in hand
+        self._pages = self._last = None  # the table of the pass in hand, and a prompt's last position
         self._norm_pushes = False  # set per step by _reduce_plan
 
     # ------------------------------------------------------------------------------------------
@@ -166,7 +166,7 @@ class Engine:
         if S == 1:
             cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
         else:
-            k, v = cache.load(pos[-1:], self._pages, out=(self.dense_k, self.dense_v))
+            k, v = cache.load(self._last, self._pages, out=(self.dense_k, self.dense_v))
             if hasattr(ops, "attention_pages"):
                 n_pages, _, page, _ = cache.k_pages.shape
                 ops.attention_pages(q, k, v, pos, self._pages, page, n_pages, self.y, S, self.nh, self.nkv, self.hd)
@@ -239,6 +239,8 @@ class Engine:
             # The store leaves the query of a token without a place as it was: the same rows in every layer of a pass, which must not hold another
             # pass's queries.
             self.q[:rows].zero_()
+            if S > 1:
+                self._last = input_pos.amax(0, keepdim=True)  # what a prompt's copy of its pages reaches to; padding may be anywhere
         self.ops.embedding(self.model.tok_embeddings.weight, idx, self.resid)
         if not self._run_native(B, S, input_pos):
             getattr(self, "_run_" + self.family)(rows, B, S, input_pos)

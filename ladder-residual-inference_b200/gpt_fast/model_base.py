@@ -101,10 +101,11 @@ class TPModelBase(nn.Module):
         """Caches in pages, for sequences of unequal lengths that come and go: the calls below then take `pages`, an int32 table [sequences,
         most pages] on the device that names each sequence's pages in order (-1: none), and a position for every token: a step of up to
         max_sequences new tokens (idx [B, 1], input_pos [B]; -1 for an idle row), or a prompt of one sequence, whole or in portions of up to
-        max_prompt tokens (idx [1, S], consecutive input_pos [S], pages [1, most pages]).  max_length: the most positions of a sequence, the
-        model's block_size by default.  cache_dtype: the model's type, or torch.float8_e4m3fn.  A new token sees the
-        positions up to its own that have a page, in a prompt as in a step.  A token whose position has no page, or lies behind the table's pages or the
-        model's block_size, is not stored; its logits mean nothing, but come from this call and the sequence's pages alone.  No counterpart in the reference, whose sequences share their positions (gpt_fast/gpt_ladder_TP.py:252-284)."""
+        max_prompt tokens (idx [1, S], input_pos [S], -1 for padding, pages [1, most pages]).  max_length: the most positions of a sequence, the
+        model's block_size by default.  cache_dtype: the model's type, or torch.float8_e4m3fn.  A new token sees the positions up to its own
+        that have a page, in a prompt as in a step.  A token whose position has no page, or lies behind the table's pages or the model's
+        block_size, is not stored; its logits mean nothing, but come from this call and the sequence's pages alone.  No counterpart in the
+        reference, whose sequences share their positions (gpt_fast/gpt_ladder_TP.py:252-284)."""
         if self.engine_class is not Engine:
             raise TypeError(f"the layers of {type(self).__name__} keep caches of their own kinds, not pages")
         cfg = self.config

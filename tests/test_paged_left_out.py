@@ -112,6 +112,32 @@ def test_a_portion_sees_what_single_steps_see(family, device, gone, monkeypatch)
         _same(got, _singles(model, tokens, range(70, 110), table, device))
 
 
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("family", ["dense", "ladder"])
+def test_a_padded_portion(family, device, monkeypatch):
+    """Tokens without a position at the end of a portion, and in it: the others' logits are those of single steps, and nothing comes from another sequence's
+    prompt, whose copy lay in the same place."""
+    with torch.no_grad():
+        model = _setup(monkeypatch, family, device, 1, 24, PAGE, max_length=128, max_prompt=96)
+        table, other = (torch.arange(8, dtype=torch.int32, device=device)[None] + i for i in (0, 12))
+        model(_tokens(30, 1).to(device), _positions(0, 30, device), table)
+        tokens, live = _tokens(40, 2), list(range(6)) + list(range(9, 33))
+        positions = torch.full((40,), -1, dtype=torch.int32, device=device)
+        positions[live] = _positions(30, 60, device)
+        got = []
+        for seed in (3, 4):
+            model(_tokens(90, seed).to(device), _positions(0, 90, device), other)
+            got.append(model(tokens.to(device), positions, table)[0].float().cpu())
+        assert torch.equal(*got)
+        _same(got[0][live], _singles(model, tokens[:, live], range(30, 60), table, device))
+        nothing = torch.full((40,), -1, dtype=torch.int32, device=device)
+        got = []
+        for seed in (3, 4):
+            model(_tokens(90, seed).to(device), _positions(0, 90, device), other)
+            got.append(model(tokens.to(device), nothing, table)[0].float().cpu())
+        assert torch.equal(*got)
+
+
 # The C ABI checks sizes and pointers before it touches a device: addresses that are never read stand in for device memory.
 BUF = 1 << 20
 ARG, ALIGN, UNSUPPORTED = -1, -2, -3
