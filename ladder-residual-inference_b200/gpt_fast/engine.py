@@ -109,11 +109,21 @@ class Engine:
         self.ws_qkv_rows = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         caches = [layer.attention.kv_cache for layer in self.model.layers]
         self.ws_paged = caches[0].attend_workspace(self.nh)
-        # a prompt's attention works on a dense copy of its sequence's pages, which the layers share
-        rows = -(-max_length // 64) * 64
-        self.dense_k, self.dense_v = (torch.zeros(1, self.nkv, rows, self.hd, dtype=dtype, device=device) for _ in range(2))
+        self._copies = [self._copy(max_length, device)]
         self.one_sequence = torch.zeros(self.max_rows, dtype=torch.int32, device=device)
         self.paged = True
+
+    def _copy(self, positions, device):
+        """Where a prompt's attention finds its sequence's pages one behind the other; the layers share it."""
+        return tuple(torch.zeros(1, self.nkv, -(-positions // 64) * 64, self.hd, dtype=self.dtype, device=device) for _ in range(2))
+
+    def _copy_for(self, pages, page):
+        """The copy for a prompt with this table: of max_length positions, or a larger one where the table names more (up to the model's block_size:
+        none behind it are stored).  Smaller ones stay, for graphs that were captured with them."""
+        positions = min(pages.shape[1] * page, self.cfg.block_size)
+        if positions > self._copies[-1][0].shape[2]:
+            self._copies.append(self._copy(positions, pages.device))
+        return self._copies[-1]
 
     def _setup_head(self, max_batch, device, dtype):
         """Buffers of the output projection and of the token choice."""
@@ -166,9 +176,9 @@ class Engine:
         if S == 1:
             cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
         else:
-            k, v = cache.load(self._last, self._pages, out=(self.dense_k, self.dense_v))
+            n_pages, _, page, _ = cache.k_pages.shape
+            k, v = cache.load(self._last, self._pages, out=self._copy_for(self._pages, page))
             if hasattr(ops, "attention_pages"):
-                n_pages, _, page, _ = cache.k_pages.shape
                 ops.attention_pages(q, k, v, pos, self._pages, page, n_pages, self.y, S, self.nh, self.nkv, self.hd)
             else:  # an ops object without it takes prompts whose positions all have pages
                 ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)

@@ -102,7 +102,7 @@ class TPModelBase(nn.Module):
         most pages] on the device that names each sequence's pages in order (-1: none), and a position for every token: a step of up to
         max_sequences new tokens (idx [B, 1], input_pos [B]; -1 for an idle row), or a prompt of one sequence, whole or in portions of up to
         max_prompt tokens (idx [1, S], input_pos [S], -1 for padding, pages [1, most pages]).  max_length: the most positions of a sequence, the
-        model's block_size by default.  cache_dtype: the model's type, or torch.float8_e4m3fn.  A new token sees the positions up to its own
+        model's block_size by default (a prompt whose row of the table names more makes a larger copy of its pages to work on).  cache_dtype: the model's type, or torch.float8_e4m3fn.  A new token sees the positions up to its own
         that have a page, in a prompt as in a step.  A token whose position has no page, or lies behind the table's pages or the model's
         block_size, is not stored; its logits mean nothing, but come from this call and the sequence's pages alone.  No counterpart in the
         reference, whose sequences share their positions (gpt_fast/gpt_ladder_TP.py:252-284)."""

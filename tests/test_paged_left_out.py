@@ -138,6 +138,19 @@ def test_a_padded_portion(family, device, monkeypatch):
         assert torch.equal(*got)
 
 
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("family", ["dense", "ladder"])
+def test_portions_behind_max_length(family, device, monkeypatch):
+    """A table with room for more positions than max_length: portions behind it see all of the sequence, as steps do."""
+    with torch.no_grad():
+        model = _setup(monkeypatch, family, device, 1, 24, PAGE, max_length=64, max_prompt=64)
+        table = torch.arange(24, dtype=torch.int32, device=device)[None]
+        for at in (0, 50, 100, 150):
+            tokens = _tokens(50, at)
+            got = model(tokens.to(device), _positions(at, at + 50, device), table)[0].float().cpu()
+        _same(got, _singles(model, tokens, range(150, 200), table, device))
+
+
 # The C ABI checks sizes and pointers before it touches a device: addresses that are never read stand in for device memory.
 BUF = 1 << 20
 ARG, ALIGN, UNSUPPORTED = -1, -2, -3
