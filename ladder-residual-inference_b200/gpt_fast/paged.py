@@ -67,17 +67,17 @@ class PagedKVCache(nn.Module):
         without their meaning."""
         b = self._buffers
         k, v, ks, vs = b["k_pages"], b["v_pages"], b["k_scale"], b["v_scale"]
-        dtype, n = k.dtype, k.numel()
-        ok = dtype is v.dtype and n == v.numel() and k.is_contiguous() and v.is_contiguous()
+        dtype, shape = k.dtype, k.shape
+        ok = dtype is v.dtype and len(shape) == 4 and shape == v.shape and k.is_contiguous() and v.is_contiguous()
         if ks is None:
             ok = ok and vs is None and dtype is self.dtype
         else:
-            rows = n // k.shape[3]
-            ok = (ok and vs is not None and dtype is _E4M3 and ks.dtype is vs.dtype is torch.float32 and ks.numel() == vs.numel() == rows and
+            ok = (ok and vs is not None and dtype is _E4M3 and ks.dtype is vs.dtype is torch.float32 and ks.shape == vs.shape == shape[:3] and
                   ks.is_contiguous() and vs.is_contiguous())
         if not ok:
-            raise ValueError(f"contiguous pages of {self.dtype} without scales, or of float8_e4m3fn with fp32 scales [n_pages, n_heads, page_size]")
-        return k, v, ks, vs, k.shape
+            raise ValueError(f"contiguous pages [n_pages, n_heads, page_size, head_dim] of {self.dtype} without scales, or of float8_e4m3fn with fp32 scales "
+                             "[n_pages, n_heads, page_size]")
+        return k, v, ks, vs, shape
 
     def store(self, qkv: Tensor, table: Optional[Tensor], input_pos: Tensor, pages: Tensor, n_head: int,
               sequence: Optional[Tensor] = None, halves: bool = False, out: Optional[Tensor] = None) -> Tensor:
