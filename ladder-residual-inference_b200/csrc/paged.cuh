@@ -111,6 +111,7 @@ int check_paged(const char* who, int dtype, int cache_dtype, const void* k, cons
 
 // On the tensor cores (paged_attention_stream.cu).
 bool paged_attn_stream_supports(int cache_dtype, int dim);
+bool paged_attn_stream_fits(int cache_dtype, const PagedAttnParams& a);
 size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim);
 int paged_attn_stream_launch(int dtype, int cache_dtype, const PagedAttnParams& a, void* workspace, size_t workspace_bytes, cudaStream_t st);
 int paged_attn_status_read_and_clear(int* status_out);

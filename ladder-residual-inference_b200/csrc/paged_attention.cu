@@ -1,6 +1,6 @@
 // Attention of one new token of each sequence over a paged key-value cache: y = softmax(q k^T scale) v over the visible positions.
-// Here the entry point and a plain kernel for heads that the tensor-core kernel (paged_attention_stream.cu) does not take: wider than 128 elements,
-// or of e4m3 rows that are not whole 16-byte pieces.
+// Here the entry point and a plain kernel for what the tensor-core kernel (paged_attention_stream.cu) does not take: heads wider than 128 elements,
+// e4m3 rows that are not whole 16-byte pieces, tables of more than some 2^32 positions times KV heads.
 #include "paged.cuh"
 
 namespace lri {
@@ -135,7 +135,7 @@ extern "C" int lri_paged_attn_decode(const lri_paged_attn_call* call) {
   p.scale_log2 = c.scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   // option attn_mma: 0 keeps attention off the tensor cores, as in lri_attn_decode
-  if (option(OPT_ATTN_MMA) != 0 && paged_attn_stream_supports(c.cache_dtype, c.head_dim))
+  if (option(OPT_ATTN_MMA) != 0 && paged_attn_stream_supports(c.cache_dtype, c.head_dim) && paged_attn_stream_fits(c.cache_dtype, p))
     return paged_attn_stream_launch(c.dtype, c.cache_dtype, p, c.workspace, static_cast<size_t>(c.workspace_bytes), st);
   if (eight) return c.dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, e4m3>(p, st) : launch_plain<__half, e4m3>(p, st);
   return c.dtype == LRI_BF16 ? launch_plain<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_plain<__half, __half>(p, st);

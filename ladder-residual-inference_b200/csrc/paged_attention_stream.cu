@@ -808,6 +808,17 @@ int tile_heads_of(int group) {
   return (group + tiles - 1) / tiles;
 }
 
+constexpr int64_t kLine = 1ll << 30;  // places are 32-bit numbers
+
+constexpr int unit_of(int bytes, int hd) { return hd * bytes > 128 ? 16 : 32; }
+
+// what a sequence of the longest that the table allows takes of the line
+int64_t most_of_the_line(int cache_dtype, const PagedAttnParams& a) {
+  const int group = a.n_head / a.n_kv, tiles = (group + kMaxGroup - 1) / kMaxGroup, unit = unit_of(cache_dtype == LRI_E4M3 ? 1 : 2, a.dim <= 64 ? 64 : 128);
+  const int64_t capacity = a.table.capacity(), longest = a.window > 0 && a.window < capacity ? a.window + unit : capacity;
+  return (((longest + unit - 1) / unit + 1) * kStep + kGap) * a.n_kv * tiles;
+}
+
 template <typename T, typename C, int HD, int NT>
 int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   using S = Shape<C, HD, NT>;
@@ -820,12 +831,9 @@ int launch(int cache_dtype, StreamParams& p, cudaStream_t st) {
   if (rc != LRI_OK) return rc;
   rc = make_tmap_pages(&tv, cache_dtype, p.a.v, slabs, t.page, p.a.dim, S::kChunkRow / static_cast<int>(sizeof(C)), p.box);
   if (rc != LRI_OK) return rc;
-  // what a sequence takes of the line at most, and sequences that stay below 2^30 together
-  const int64_t longest = p.a.window > 0 && p.a.window < t.capacity() ? p.a.window + S::kUnit : t.capacity();
-  const int64_t most = (((longest + S::kUnit - 1) / S::kUnit + 1) * kStep + kGap) * p.a.n_kv * p.head_tiles;
-  int64_t per = (1ll << 30) / most;
-  LRI_REQUIRE(per >= 1, LRI_ERR_UNSUPPORTED, "paged_attn_decode: %lld positions of %d heads", (long long)t.capacity(), p.a.n_kv);
-  per = per < kMaxSeqs ? per : kMaxSeqs;
+  static_assert(S::kUnit == unit_of(sizeof(C), HD), "units by the bytes of a row");
+  const int64_t most = most_of_the_line(cache_dtype, p.a);
+  const int64_t per = kLine / most < kMaxSeqs ? kLine / most : kMaxSeqs;  // sequences that stay on the line together
   auto kern = paged_attn_stream_kernel<T, C, HD, NT>;
   // with the most heads and sequences
   constexpr int kRings = kStages * static_cast<int>(S::kHalf + (sizeof(C) == 1 ? S::kUnit * 4 : 0));
@@ -864,6 +872,10 @@ int dispatch(int cache_dtype, StreamParams& p, cudaStream_t st) {
 
 // rows of whole 16-byte pieces that fit the tiles
 bool paged_attn_stream_supports(int cache_dtype, int dim) { return dim <= 128 && dim % (cache_dtype == LRI_E4M3 ? 16 : 8) == 0; }
+
+// Tables of so many positions that the longest sequence would not fit the line go to the plain kernel, whatever the lengths are: of more than about 2^32
+// positions times KV heads (units of 16 positions; of 32, twice as many).
+bool paged_attn_stream_fits(int cache_dtype, const PagedAttnParams& a) { return most_of_the_line(cache_dtype, a) <= kLine; }
 
 size_t workspace_bytes(int ctas, int group, int dim) { return kCounterBytes + static_cast<size_t>(ctas) * 2 * tile_heads_of(group) * ((dim <= 64 ? 64 : 128) + 2) * 4; }
 
