@@ -97,20 +97,23 @@ class TPModelBase(nn.Module):
         # kept because callers of the reference may read it; the kernels derive causality from input_pos
         self.causal_mask = torch.tril(torch.ones(max_seq_length, max_seq_length, dtype=torch.bool, device=device))
 
-    def setup_paged_caches(self, max_sequences, n_pages, page_size=32, max_length=None, max_prompt=512, cache_dtype=None):
-        """Caches in pages, for sequences of unequal lengths that come and go: the calls below then take `pages`, an int32 table [sequences,
-        most pages] on the device that names each sequence's pages in order (-1: none), and a position for every token: a step of up to
-        max_sequences new tokens (idx [B, 1], input_pos [B]; -1 for an idle row), or a prompt of one sequence, whole or in portions of up to
-        max_prompt tokens (idx [1, S], input_pos [S], -1 for padding, pages [1, most pages]).  max_length: the most positions of a sequence, the
-        model's block_size by default (a prompt whose row of the table names more makes a larger copy of its pages to work on).  cache_dtype: the model's type, or torch.float8_e4m3fn.  A new token sees the positions up to its own
-        that have a page, in a prompt as in a step.  A token whose position has no page, or lies behind the table's pages or the model's
-        block_size, is not stored; its logits mean nothing, but come from this call and the sequence's pages alone.  No counterpart in the
-        reference, whose sequences share their positions (gpt_fast/gpt_ladder_TP.py:252-284)."""
+    def setup_paged_caches(self, max_sequences, n_pages, page_size=32, max_length=None, max_prompt=None, cache_dtype=None):
+        """Caches in pages, for sequences of unequal lengths that come and go: the calls below then take `pages`, an int32 table [sequences, most
+        pages] on the device that names each sequence's pages in order (-1: none), and a position for every token: a step of up to max_sequences
+        new tokens (idx [B, 1], input_pos [B]; -1 for an idle row), or a prompt of one sequence, whole or in portions of up to max_prompt tokens
+        (512 by default, or max_length; idx [1, S], input_pos [S], -1 for padding, pages [1, most pages]). max_length: the most positions of a
+        sequence, the model's block_size by default (a prompt whose row of the table names more makes a larger copy of its pages to work on).
+        cache_dtype: the model's type, or torch.float8_e4m3fn. A new token sees the positions up to its own that have a page, in a prompt as in a
+        step. A token whose position has no page, or lies behind the table's pages or the model's block_size, is not stored; its logits mean
+        nothing, but come from this call and the sequence's pages alone. No counterpart in the reference, whose sequences share their positions
+        (gpt_fast/gpt_ladder_TP.py:252-284)."""
         if self.engine_class is not Engine:
             raise TypeError(f"the layers of {type(self).__name__} keep caches of their own kinds, not pages")
         cfg = self.config
         max_length = cfg.block_size if max_length is None else max_length
-        assert 1 <= max_prompt <= max_length <= cfg.block_size, "prompts fit a sequence, sequences the model's block_size"
+        assert 1 <= max_length <= cfg.block_size, f"max_length={max_length}: 1 to the model's block_size, {cfg.block_size}"
+        max_prompt = min(512, max_length) if max_prompt is None else max_prompt
+        assert 1 <= max_prompt <= max_length, f"max_prompt={max_prompt}: 1 to max_length, {max_length}"
         dtype, device, head_dim = self.output.weight.dtype, self.output.weight.device, cfg.dim // cfg.n_head
         for b in self.layers:
             b.attention.kv_cache = PagedKVCache(n_pages, page_size, cfg.n_local_heads // dist.get_world_size(), head_dim, dtype, cache_dtype, device)

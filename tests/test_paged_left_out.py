@@ -151,6 +151,24 @@ def test_portions_behind_max_length(family, device, monkeypatch):
         _same(got, _singles(model, tokens, range(150, 200), table, device))
 
 
+@pytest.mark.parametrize("kw,most", [(dict(), 256), (dict(max_length=100), 100), (dict(max_length=1), 1), (dict(max_prompt=40), 40), (dict(max_length=64, max_prompt=64), 64)])
+def test_the_longest_prompt(kw, most, monkeypatch):
+    """By default 512 tokens, or as many as a sequence has."""
+    with torch.no_grad():
+        model = _setup(monkeypatch, "dense", "cpu", 1, 16, PAGE, **kw)
+        table = torch.arange(16, dtype=torch.int32)[None]
+        assert model(_tokens(most, 0), _positions(0, most, "cpu"), table).shape == (1, most, SHAPE["vocab_size"])
+        with pytest.raises(AssertionError):
+            model(_tokens(most + 1, 0), _positions(0, most + 1, "cpu"), table)
+
+
+@pytest.mark.parametrize("kw,named", [(dict(max_length=257), "max_length=257"), (dict(max_length=0), "max_length=0"), (dict(max_length=64, max_prompt=65), "max_prompt=65"),
+                                      (dict(max_prompt=0), "max_prompt=0")])
+def test_set_up_names_what_it_refuses(kw, named, monkeypatch):
+    with pytest.raises(AssertionError, match=named):
+        _setup(monkeypatch, "dense", "cpu", 1, 16, PAGE, **kw)
+
+
 # The C ABI checks sizes and pointers before it touches a device: addresses that are never read stand in for device memory.
 BUF = 1 << 20
 ARG, ALIGN, UNSUPPORTED = -1, -2, -3
