@@ -124,7 +124,8 @@ class CudaOps:
 
 
     # ---- paged key-value cache ---------------------------------------------------------------------
-    # (A step of a small batch is bound by the host: what the caller has looked up of the shapes is handed on, 100 to 250 ns a look.)
+    # (A step of a small batch is bound by the host: what the caller has looked up of the shapes is handed on, 100 to 250 ns a look.
+    # The pitch of a single row says nothing: it may be any number.)
     @staticmethod
     def rope_paged_store(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale, n_head, halves, tokens, pages_shape,
                          cache_shape):
@@ -144,8 +145,8 @@ class CudaOps:
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
             qkv.data_ptr(), at, input_pos.data_ptr(), 0 if sequence is None else sequence.data_ptr(), pages.data_ptr(), q_out.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, torch._C._cuda_getCurrentRawStream(here), qkv.stride(0), rows, pages.stride(0), n_pages, tokens, dtype,
-            cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
+            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, torch._C._cuda_getCurrentRawStream(here),
+            qkv.stride(0) if tokens > 1 else (n_head + 2 * n_kv) * dim, rows, pages.stride(0) if n_seq > 1 else most, n_pages, tokens, dtype, cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
         if status < 0:
             _C.check(status)
 
@@ -165,8 +166,8 @@ class CudaOps:
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_paged_attn_decode(_C.ATTN_CALL.pack(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), input_pos.data_ptr(), out.data_ptr(),
-            workspace.data_ptr(), torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0), window, workspace.numel(), dtype, cache_dtype, page, n_seq, most,
-            input_pos.dtype is torch.int64, n_head, n_kv, dim, scale))
+            workspace.data_ptr(), torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0) if n_seq > 1 else most, window, workspace.numel(), dtype,
+            cache_dtype, page, n_seq, most, input_pos.dtype is torch.int64, n_head, n_kv, dim, scale))
         if status < 0:
             _C.check(status)
 
@@ -182,7 +183,8 @@ class CudaOps:
         ks, vs, cache_dtype = (0, 0, dtype) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr(), _C.E4M3)
         status = _C.lib.lri_paged_load(_C.LOAD_CALL.pack(
             k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, pages.data_ptr(), last_pos.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0), rows, dtype, cache_dtype, page, n_seq, most, last_pos.dtype is torch.int64, n_kv, dim))
+            torch._C._cuda_getCurrentRawStream(here), n_pages, pages.stride(0) if n_seq > 1 else most, rows, dtype, cache_dtype, page, n_seq, most,
+            last_pos.dtype is torch.int64, n_kv, dim))
         if status < 0:
             _C.check(status)
 
