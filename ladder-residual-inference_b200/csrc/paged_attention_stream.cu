@@ -808,6 +808,8 @@ int tile_heads_of(int group) {
   return (group + tiles - 1) / tiles;
 }
 
+size_t workspace_bytes(int ctas, int group, int dim) { return kCounterBytes + static_cast<size_t>(ctas) * 2 * tile_heads_of(group) * ((dim <= 64 ? 64 : 128) + 2) * 4; }
+
 constexpr int64_t kLine = 1ll << 30;  // places are 32-bit numbers
 
 constexpr int unit_of(int bytes, int hd) { return hd * bytes > 128 ? 16 : 32; }
@@ -876,8 +878,6 @@ bool paged_attn_stream_supports(int cache_dtype, int dim) { return dim <= 128 &&
 // Tables of so many positions that the longest sequence would not fit the line go to the plain kernel, whatever the lengths are: of more than about 2^32
 // positions times KV heads (units of 16 positions; of 32, twice as many).
 bool paged_attn_stream_fits(int cache_dtype, const PagedAttnParams& a) { return most_of_the_line(cache_dtype, a) <= kLine; }
-
-size_t workspace_bytes(int ctas, int group, int dim) { return kCounterBytes + static_cast<size_t>(ctas) * 2 * tile_heads_of(group) * ((dim <= 64 ? 64 : 128) + 2) * 4; }
 
 size_t paged_attn_stream_workspace_bytes(int n_head, int n_kv, int dim) { return workspace_bytes(max_ctas(), n_head / n_kv, dim); }
 
