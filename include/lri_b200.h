@@ -254,7 +254,8 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  *
  * lri_attn_prefill_pages: lri_attn_prefill of one sequence over such a copy of its pages (k_cache, v_cache [1, n_kv, smax, head_dim], read back up
  * to the largest position), with each query's own position input_pos[s]: it sees positions 0 .. input_pos[s], as far as they have pages, as the one new
- * token of lri_paged_attn_decode does; zeros with none visible (a negative position).  pages [max_pages]: the sequence's row of the table. */
+ * token of lri_paged_attn_decode does; zeros with none visible (a negative position).  pages [max_pages]: the sequence's row of the table;
+ * smax a multiple of 64.  Values that are not finite may reach queries in front of them, as in lri_attn_prefill. */
 typedef struct {
   const void *qkv, *rope_table, *input_pos;
   const int32_t *sequence, *pages;

@@ -711,6 +711,8 @@ extern "C" int lri_attn_prefill_pages(int dtype, const void* q, const void* k_ca
   LRI_REQUIRE(pages, LRI_ERR_ARG, "attn_prefill_pages: NULL pointer");
   LRI_REQUIRE(max_pages >= 1 && n_pages >= 1 && page_size >= 8 && page_size <= 4096 && page_size % 8 == 0 && t.capacity() <= (1ll << 30), LRI_ERR_ARG,
               "attn_prefill_pages: %d of %lld pages of %d positions", max_pages, (long long)n_pages, page_size);
+  // a tile of 64 keys that reached into the next head's rows would multiply what they hold, which may be a NaN, by zero
+  LRI_REQUIRE(smax % 64 == 0, LRI_ERR_ARG, "attn_prefill_pages: smax=%lld (multiples of 64)", (long long)smax);
   t.by_page = FastDiv::of(page_size);
   return prefill("attn_prefill_pages", dtype, q, k_cache, v_cache, input_pos, pos_is_i64, out, 1, S, n_head, n_kv, head_dim, smax, &t,
                  static_cast<cudaStream_t>(stream));

@@ -24,8 +24,12 @@
 // P = 0); the cache module zero-initialises them, as the reference's does (gpt_fast/utils.py:47-48).
 //
 // PAGES: the cache is a dense copy of a sequence's pages.  Every query has a position of its own, negative for none, and keys without a page are
-// masked, so that a prompt sees what single tokens at its positions would.  A softmax warp looks the pages of a tile's keys up (two a lane) before it
-// waits for the tile's scores.
+// masked, so that a prompt sees what single tokens at its positions would.  Mostly every page is there: while the first tiles come, the softmax warps look
+// through the table once, and only where one is missing do they look up the pages of each tile's keys, two a lane (32 query and 8 KV heads of 128, us,
+// dense, over pages, with one missing: 2000 tokens 62, 61, 64; 512 behind 1500 35, 35, 35; 512 behind 30000 607, 625, 622; with every tile looked up 2000
+// tokens took 66 and 70).
+#include <climits>
+
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -41,6 +45,16 @@ constexpr int kFaThreads = 192;  // TMA warp, MMA warp, 4 softmax warps
 constexpr float kFaRescaleLog2 = 8.0f;
 
 __device__ int g_attn_tc_status = 0;
+
+// whether it holds in any of the softmax warps' 128 threads
+__device__ __forceinline__ bool any_of_128(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(static_cast<uint32_t>(x))
+               : "memory");
+  return r != 0;
+}
 
 struct FaParams {
   void* out;  // [B, S, n_head * HD]
@@ -111,12 +125,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  int own_pos = -1;  // PAGES: of this thread's query
+  int own_pos = -1, first_pos = 0;  // PAGES: of this thread's query, and the least of its warp's
   if (PAGES && warp >= 2) {
     const int s = q0 + (warp & 3) * 32 + lane;
     if (s < p.S) own_pos = p.table.clamped(load_pos(p.input_pos, p.pos_is_i64, s), p.smax);
     const int last = __reduce_max_sync(0xffffffffu, own_pos);
     if (lane == 0) last_of[warp & 3] = last;
+    first_pos = __reduce_min_sync(0xffffffffu, s < p.S ? own_pos : INT_MAX);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -217,11 +232,14 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int64_t qpos = PAGES ? own_pos : pos0 + q0 + i;
     float m_ref = -INFINITY, l = 0.f;
-    bool alive = true;
+    bool alive = true, holes = false;  // PAGES: whether a page is missing up to the last position
+    if (PAGES) {
+      for (int i = threadIdx.x - 64; i < p.table.max_pages && static_cast<int64_t>(i) * p.table.page < kv_end; i += 128)
+        holes = holes || !p.table.names(p.table.ids[i]);
+      holes = any_of_128(holes);
+    }
     for (int j = 0; j < n_tiles; ++j) {
       const uint32_t sb = static_cast<uint32_t>(j & 1);
-      uint64_t paged = ~0ull;  // the keys of this tile that have a page
-      if (PAGES) paged = p.table.named64(j * kFaN, lane);
       const bool ready = mbar_wait(s_full0 + 8 * sb, (static_cast<uint32_t>(j) >> 1) & 1u, &abort_flag, 5, &g_attn_tc_status);
       if (!__all_sync(0xffffffffu, ready)) {
         alive = false;
@@ -243,10 +261,19 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const int64_t key0 = static_cast<int64_t>(j) * kFaN;
       // tiles that reach past the first row's position or past the end of the visible keys need the mask
       if constexpr (PAGES) {
-        if (__any_sync(0xffffffffu, key0 + kFaN - 1 > qpos) || paged != ~0ull) {
+        const int seen = own_pos - j * kFaN;
+        if (j * kFaN + kFaN - 1 > first_pos) {
 #pragma unroll
           for (int e = 0; e < kFaN; ++e)
-            if (key0 + e > qpos || !((paged >> e) & 1u)) sv[e] = -INFINITY;
+            if (e > seen) sv[e] = -INFINITY;
+        }
+        if (holes) {
+          const uint64_t paged = p.table.named64(j * kFaN, lane);
+          if (paged != ~0ull) {
+#pragma unroll
+            for (int e = 0; e < kFaN; ++e)
+              if (!((paged >> e) & 1u)) sv[e] = -INFINITY;
+          }
         }
       } else if (key0 + kFaN - 1 > pos0 + q0 || key0 + kFaN > kv_end) {
 #pragma unroll

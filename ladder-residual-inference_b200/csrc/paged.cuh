@@ -68,10 +68,11 @@ struct PageTable {
   int64_t n_pages;
   FastDiv by_page;
   __host__ __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(max_pages) * page; }
+  __device__ __forceinline__ bool names(int id) const { return id >= 0 && id < n_pages; }
   // page that holds position pos (0 <= pos < capacity()) of sequence b, -1: none
   __device__ __forceinline__ int find(int64_t b, int pos) const {
     const int id = ids[b * ld + by_page(pos)];
-    return id >= 0 && id < n_pages ? id : -1;
+    return names(id) ? id : -1;
   }
   __device__ __forceinline__ int row_of(int pos) const { return pos - by_page(pos) * page; }  // within its page
   // a position as attention takes it: -1 where it is negative, the last of the pages (or of `most` rows) where it lies behind them

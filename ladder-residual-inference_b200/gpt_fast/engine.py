@@ -46,7 +46,7 @@ class Engine:
         self.comm = comm if comm is not None else make_comm()
         self.ready = False
         self.paged = False  # whether the layers' caches are pages (setup_paged)
-        self._pages = self._last = None  # the table of the pass in hand, and a prompt's last position
+        self._pages = self._prompt = None  # of the pass in hand: the table; what a prompt's layers share (_body)
         self._norm_pushes = False  # set per step by _reduce_plan
 
     # ------------------------------------------------------------------------------------------
@@ -176,11 +176,12 @@ class Engine:
         if S == 1:
             cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
         else:
-            n_pages, _, page, _ = cache.k_pages.shape
-            k, v = cache.load(self._last, self._pages, out=self._copy_for(self._pages, page))
-            if hasattr(ops, "attention_pages"):
+            last, copy, masked = self._prompt
+            k, v = cache.load(last, self._pages, out=copy)
+            if masked:
+                n_pages, _, page, _ = cache.k_pages.shape
                 ops.attention_pages(q, k, v, pos, self._pages, page, n_pages, self.y, S, self.nh, self.nkv, self.hd)
-            else:  # an ops object without it takes prompts whose positions all have pages
+            else:
                 ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)
 
     def _mlp(self, w1, w2, rows, out, addend=None, normed=None, push=0):
@@ -250,7 +251,10 @@ class Engine:
             # pass's queries.
             self.q[:rows].zero_()
             if S > 1:
-                self._last = input_pos.amax(0, keepdim=True)  # what a prompt's copy of its pages reaches to; padding may be anywhere
+                # what the copy of its pages reaches to (padding may be anywhere), the copy, and whether keys without a page can be left out: an ops
+                # object that cannot takes prompts whose positions all have pages
+                page = self.model.layers[0].attention.kv_cache.k_pages.shape[2]
+                self._prompt = input_pos.amax(0, keepdim=True), self._copy_for(self._pages, page), hasattr(self.ops, "attention_pages")
         self.ops.embedding(self.model.tok_embeddings.weight, idx, self.resid)
         if not self._run_native(B, S, input_pos):
             getattr(self, "_run_" + self.family)(rows, B, S, input_pos)

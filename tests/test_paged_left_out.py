@@ -151,6 +151,46 @@ def test_portions_behind_max_length(family, device, monkeypatch):
         _same(got, _singles(model, tokens, range(150, 200), table, device))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("family", ["ladder", "dense"])
+def test_captured_portions(family):
+    """A portion captured once, behind a table that is wider than max_length, and replayed while tokens, positions and pages change in place; another sequence's
+    prompt runs in between, and a smaller captured portion of before the copy grew still replays."""
+    with torch.no_grad():
+        model = _model(family, "cuda")
+        model.setup_paged_caches(1, 40, PAGE, max_length=64, max_prompt=64)
+
+        def capture(tokens, positions, table):
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                model(tokens, positions, table)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                return graph, model(tokens, positions, table)
+
+        calls = []
+        for most, n in ((4, 20), (10, 40)):
+            call = [torch.zeros(1, n, dtype=torch.int64, device="cuda"), torch.full((n,), -1, dtype=torch.int32, device="cuda"),
+                    torch.full((1, most), -1, dtype=torch.int32, device="cuda")]
+            calls.append((n, call) + capture(*call))
+        other = torch.arange(20, 30, dtype=torch.int32, device="cuda")[None]
+        for i, at in enumerate((0, 10, 24)):
+            for n, call, graph, logits in calls:
+                call[0].copy_(_tokens(n, i))
+                call[1].copy_(_positions(at, at + n, "cuda"))
+                call[1][n - i:] = -1
+                call[2].copy_(torch.arange(call[2].shape[1], device="cuda").int() + i)
+                if i == 2:
+                    call[2][0, 0] = -1
+                model(_tokens(60, 7).cuda(), _positions(90, 150, "cuda"), other)
+                graph.replay()
+                got = logits.clone()
+                model(_tokens(60, 8).cuda(), _positions(90, 150, "cuda"), other)
+                assert torch.equal(got, model(*call))  # the same portion again writes the same rows
+
+
 @pytest.mark.parametrize("kw,most", [(dict(), 256), (dict(max_length=100), 100), (dict(max_length=1), 1), (dict(max_prompt=40), 40), (dict(max_length=64, max_prompt=64), 64)])
 def test_the_longest_prompt(kw, most, monkeypatch):
     """By default 512 tokens, or as many as a sequence has."""
@@ -177,7 +217,7 @@ ARG, ALIGN, UNSUPPORTED = -1, -2, -3
 @pytest.mark.parametrize("kw,status", [
     (dict(pages=0), ARG), (dict(most=0), ARG), (dict(n_pages=0), ARG), (dict(page=12), ARG), (dict(page=0), ARG), (dict(page=8192), ARG),
     (dict(most=1 << 28), ARG), (dict(q=0), ARG), (dict(pos=0), ARG), (dict(out=BUF + 8), ALIGN), (dict(S=-1), ARG), (dict(n_head=3), ARG), (dict(dim=80), UNSUPPORTED),
-    (dict(smax=0), ARG), (dict(dtype=3), UNSUPPORTED), (dict(S=0), 0)])
+    (dict(smax=0), ARG), (dict(smax=72), ARG), (dict(dtype=3), UNSUPPORTED), (dict(S=0), 0)])
 def test_c_prompt_over_pages_refuses(kw, status):
     from gpt_fast import _C
     a = dict(dtype=0, q=BUF, k=BUF, v=BUF, pos=BUF, i64=0, out=BUF, S=4, n_head=4, n_kv=2, dim=64, smax=64, pages=BUF, most=4, page=16, n_pages=6, stream=0)
