@@ -11,6 +11,9 @@ constexpr int kWarps = 4;
 
 // One CTA per (query head, sequence); LANES threads hold a position, eight elements each.  Every group of lanes keeps its own running maximum,
 // sum and values in 32 bits; the groups of a warp are joined by shuffles, the warps through shared memory.
+// Simple and far from the bytes it has to read: each query head reads the cache for itself, and a sequence stays with one CTA, whose chain of loads bounds it
+// (32 query and 8 KV heads, us, floor in brackets: 24 sequences of 17 to 8000 positions, heads of 192 2029 (28), of 256 1994 (37), e4m3 2290 (19), e4m3 of
+// 72 1198 (5.6); 100 of 300 to 6000, 256 2151 (234); one of 1025 150 (1.3), of 32768 9279 (41)).
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_plain_kernel(const PagedAttnParams p) {
   constexpr int kGroups = 32 / LANES;

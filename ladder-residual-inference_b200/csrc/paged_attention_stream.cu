@@ -35,12 +35,15 @@ __device__ int g_paged_attn_status = 0;
 constexpr int kMaxGroup = 16;   // query heads that share a pass over the cache
 constexpr int kMaxSeqs = 1024;  // of a launch
 constexpr int kStep = 4, kGap = 2;  // a pair of n units takes kStep n + kGap of the line
-// of the line: a CTA without as much is not worth its part in the join (one sequence of 1025 positions, us: 4, 8, 12, 24 units 11.8, 11.0, 11.1, 13.1)
+// of the line: a CTA without as much is not worth its part in the join (heads of 128, 32 on 8, us with 4, 8, 12, 16 and 24 units: one sequence of 300
+// positions 8.5, 8.7, 9.2, 9.8, 9.9, of 1025 10.1, 9.0, 9.4, 10.1, 10.8, in e4m3 9.6, 10.0, 10.4, 11.6, 13.0, of 4000 12.5, 12.6, 12.6, 12.1, 12.3; four of 1025
+// 11.1, 11.1, 11.1, 11.1, 11.2, in e4m3 10.8, 10.6, 10.8, 12.0, 13.4; sixteen of 100 10.1, 9.8, 9.6, 10.3, 11.5: 8 and 12 are alike within half a microsecond)
 constexpr int kMinRun = 12 * kStep;
 // CTAs are placed in the order of their numbers, and the last find their SMs taken by the preceding kernel to its end: behind a store of 16 rows the
 // last 16 of 148 have their first tiles 3 us after the others.  Of a full grid they take kLateBy of the line less, half their stretch at most (store and
-// attention in a graph, us, without and with: 8 sequences of 50 to 950 positions 14.1, 13.5; 16 of 300 14.9, 13.8; 16 of 1025 21.3, 20.6; 16 of 4000
-// 48.8, 48.7; by half of it 21.0 for the third, by half as much again 20.5 with 15.1 for the second).
+// attention in a graph, us, with and without: 8 sequences of 500 positions 13.1, 14.2; 16 of 300 13.9, 14.6; 16 of 1025 20.0, 20.8; 16 of 4000 48.4, 48.4;
+// 64 of 500 31.8, 31.9; 128 of 300 37.9, 37.8; 128 of 2000 166.3, 164.9; 24 of 17 to 8000 29.2, 29.5; e4m3, in the same order 13.0, 13.0; 13.4, 13.5; 17.9, 18.2;
+// 33.2, 33.6; 24.8, 24.7; 28.9, 28.8; 96.0, 95.7; 22.5, 22.9; calls of attention alone gain up to 0.6: what is behind a larger store loses nothing that shows).
 constexpr int kLateCtas = 16, kLateBy = 10 * kStep;
 // of a warp's ring: the keys of a unit, the values of a unit (40 fp16 sequences, us: 2, 3, 4 places 64.1, 67.2, 67.6: SMs far from memory fall behind)
 constexpr int kStages = 2;
@@ -61,7 +64,9 @@ struct StreamParams {
 // NT: blocks of eight query heads
 template <typename C, int HD, int NT>
 struct Shape {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;  // as many as the registers of an SM hold (100 e4m3 sequences, us: 8, 12, 16 83.1, 76.2, 77.2)
+  // as many as the registers of an SM hold (100 e4m3 sequences, us: 8, 12, 16 83.1, 76.2, 77.2; 64 heads on 4, two blocks, with 6, 8, 10: 24 sequences of 17 to
+  // 8000 30.5, 26.4, 27.2, in e4m3 28.3, 25.5, 29.2; 100 of 300 to 6000 85.9, 76.3, 77.5, in e4m3 74.6, 60.1, 68.3; one of 32768 43.1, 34.2, 36.9)
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRow = HD * static_cast<int>(sizeof(C));
   static constexpr int kChunkRow = kRow < 128 ? kRow : 128;  // bytes of a row that a box holds: the swizzle's span

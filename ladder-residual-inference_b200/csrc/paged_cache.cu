@@ -86,9 +86,10 @@ __device__ __forceinline__ void rotate8_any(int rot, int halves, int e, const TT
 
 // LANES threads hold a head, eight elements each; blockIdx.y says which heads, blockIdx.x which `per` tokens.  The CTA first finds out where its
 // tokens go and brings their rows of the table into shared memory, while the first rows of the projection are on their way; then R tokens at a
-// time, the next R asked for before.  Bound by HBM for prompts (8192 tokens of 32 + 2 x 8 heads of 128, bf16: 38 us, 5.3 TB/s; e4m3 with halves from an
-// fp32 table, where the arithmetic is half of it: 59 us), so bytes in flight and what is repeated for every vector count: with each token's place
-// looked up by every thread, 186 instructions for a vector and 67 us.  For single tokens it is a chain of loads and a store (3 us).
+// time, the next R asked for before.  Prompts in the activations' type are bound by HBM (8192 tokens of 32 + 2 x 8 heads of 128, bf16: 38.5 us, 5.3 TB/s), so
+// bytes in flight and what is repeated for every vector count: with each token's place looked up by every thread, 186 instructions for a vector and
+// 67 us.  To e4m3 they are not (51 us, with halves from an fp32 table 59, for 29 of HBM): issue slots are busy for 56 %, and what belongs to a token, its row
+// of the table and the partners of its elements, is fetched again for every head.  For single tokens it is a chain of loads and a store (3 us).
 template <typename T, typename TT, bool E4M3, bool VECTORS, int LANES, int R>
 __global__ void __launch_bounds__(kThreads, kPerSm) rope_paged_store_kernel(const StoreParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
