@@ -39,6 +39,8 @@ enum lri_dtype { LRI_BF16 = 0, LRI_FP16 = 1, LRI_FP32 = 2, LRI_E4M3 = 3 /* pages
  * token rows) stays on the kernel that gives a tile to one SM.  For passes that run kernels of theirs on a second stream
  * beside their projections (see csrc/gemm_pair.cu). */
 enum { LRI_ONE_SM = 0x100 };
+/* Added to `dtype` of lri_rope_paged_store: the query rows of tokens that are skipped become zeros, for results in fresh memory. */
+enum { LRI_ZERO_SKIPPED = 0x200 };
 
 enum lri_status {
   LRI_OK = 0,
@@ -238,7 +240,7 @@ int lri_attn_prefill(int dtype, const void* q, const void* k_cache, const void* 
  * != 0) pairs (e, e + rot_dim / 2); rope_table [table_rows, rot_dim / 2, 2] = (cos, sin) in `dtype` or (table_is_f32 != 0) fp32;
  * rot_dim 0: no rotation, no table.  fp32 from the rounded projection, rounded once.  e4m3: a row's scale is its largest magnitude / 448,
  * its codes the nearest to value * 448 / largest magnitude; a row with an infinity or NaN gets a NaN scale.  A token whose position is
- * negative or behind the table's or the pages' end, or whose sequence or page does not exist, is skipped: nothing is written for it.
+ * negative or behind the table's or the pages' end, or whose sequence or page does not exist, is skipped: nothing is written for it (LRI_ZERO_SKIPPED: a query row of zeros).
  * A (page, row) may be named once in a call.  The calls are described by structs of the host: a step makes many of them, and a binding's
  * cost grows with the number of arguments.
  *

@@ -38,6 +38,7 @@ ATTN_CALL = struct.Struct("@10Q4q9if")   # lri_paged_attn_call
 LOAD_CALL = struct.Struct("@9Q3q8i")     # lri_paged_load_call
 
 ONE_SM = 0x100  # LRI_ONE_SM
+ZERO_SKIPPED = 0x200  # LRI_ZERO_SKIPPED
 DENSE, LADDER, LADDER_TWO_STREAMS, PARALLEL, DESYNC, PARALLEL_TWO_STREAMS = range(6)
 
 # name -> (restype, argtypes); the order of arguments is that of include/lri_b200.h

@@ -128,8 +128,8 @@ class CudaOps:
     # The pitch of a single row says nothing: it may be any number.)
     @staticmethod
     def rope_paged_store(qkv, table, input_pos, sequence, pages, q_out, k_pages, v_pages, k_scale, v_scale, n_head, halves, tokens, pages_shape,
-                         cache_shape):
-        """table None: no rotation; its second extent is half of the elements that rotate."""
+                         cache_shape, flags=0):
+        """table None: no rotation; its second extent is half of the elements that rotate.  flags: 0 or _C.ZERO_SKIPPED."""
         here = qkv.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == input_pos.get_device() == pages.get_device() == q_out.get_device() == k_pages.get_device() ==
                 v_pages.get_device() and (sequence is None or sequence.get_device() == here) and (table is None or table.get_device() == here) and
@@ -146,7 +146,8 @@ class CudaOps:
         status = _C.lib.lri_rope_paged_store(_C.STORE_CALL.pack(
             qkv.data_ptr(), at, input_pos.data_ptr(), 0 if sequence is None else sequence.data_ptr(), pages.data_ptr(), q_out.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, torch._C._cuda_getCurrentRawStream(here),
-            qkv.stride(0) if tokens > 1 else (n_head + 2 * n_kv) * dim, rows, pages.stride(0) if n_seq > 1 else most, n_pages, tokens, dtype, cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
+            qkv.stride(0) if tokens > 1 else (n_head + 2 * n_kv) * dim, rows, pages.stride(0) if n_seq > 1 else most, n_pages, tokens, dtype | flags,
+            cache_dtype, f32, rot, halves, input_pos.dtype is torch.int64, n_seq, most, page, n_head, n_kv, dim))
         if status < 0:
             _C.check(status)
 

@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
+from ._C import ZERO_SKIPPED
 from .ops import CudaOps
 
 _E4M3 = torch.float8_e4m3fn
@@ -85,8 +86,8 @@ class PagedKVCache(nn.Module):
         positions, writes keys and values into the pages, returns the queries [tokens, n_head, head_dim].  Token i has position
         input_pos[i] in sequence sequence[i] (None: in sequence i).  table [positions, rot / 2, 2] (cos, sin) in the activations' type or
         fp32, None for no rotation: the first rot elements of a head turn, in adjacent pairs (utils.precompute_freqs_cis) or in halves.
-        A token without a position (negative, behind the table) or without a page is left out, its query row too.  One call
-        may name a (sequence, position) once."""
+        A token without a position (negative, behind the table) or without a page is left out: its query row is zeros, and in an `out` of the caller's
+        stays as it was.  One call may name a (sequence, position) once."""
         k, v, ks, vs, cache_shape = self._tensors()
         _, n_kv, _, dim = cache_shape
         dtype, shape, pages_shape = self.dtype, qkv.shape, pages.shape
@@ -103,11 +104,13 @@ class PagedKVCache(nn.Module):
             if not (len(shape) == 3 and shape[2] == 2 and 2 <= 2 * shape[1] <= dim and table.is_contiguous() and
                     (table.dtype is dtype or table.dtype is torch.float32)):
                 raise ValueError(f"table: [positions, rot / 2, 2] in {dtype} or float32, rot up to {dim}, not {_said(table)}")
+        args = n_head, bool(halves), tokens, pages_shape, cache_shape
         if out is None:
             out = qkv.new_empty((tokens, n_head, dim))
+            self.ops.rope_paged_store(qkv, table, input_pos, sequence, pages, out, k, v, ks, vs, *args, ZERO_SKIPPED)
         else:
             _check_like(out, dtype, (tokens, n_head, dim))
-        self.ops.rope_paged_store(qkv, table, input_pos, sequence, pages, out, k, v, ks, vs, n_head, bool(halves), tokens, pages_shape, cache_shape)
+            self.ops.rope_paged_store(qkv, table, input_pos, sequence, pages, out, k, v, ks, vs, *args)
         return out
 
     def attend_workspace(self, n_head: int) -> Tensor:

@@ -48,6 +48,30 @@ def test_a_single_row_has_no_pitch(eight):
         assert all(torch.equal(a, b) for a, b in zip(other, got[0]))
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dim,rot,tokens", [(64, 64, 3), (128, 0, 700), (80, 20, 64), (192, 64, 65)])
+def test_fresh_queries_hold_nothing_of_other_memory(eight, dim, rot, tokens):
+    """Without `out`, the rows of tokens that are left out are zeros, whatever lay in the memory before; an `out` of the caller's keeps them."""
+    from gpt_fast import PagedKVCache
+    n_head, n_kv, page, dtype = 3, 1, 16, torch.bfloat16
+    x = torch.randn(tokens, (n_head + 2 * n_kv) * dim, device="cuda").to(dtype)
+    rope = torch.randn(tokens, rot // 2, 2, device="cuda").to(dtype) if rot else None
+    per = -(-tokens // page)
+    table = torch.arange(per, dtype=torch.int32, device="cuda")[None].clone()
+    table[0, -1] = -1
+    pos, seq = torch.arange(tokens, dtype=torch.int32, device="cuda"), torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    pos[::5] = -1
+    live = (pos >= 0) & (table[0, pos.clamp(min=0).long() // page] >= 0)
+    cache = PagedKVCache(per, page, n_kv, dim, dtype, cache_dtype=E4M3 if eight else dtype, device="cuda")
+    kept = torch.full((tokens, n_head, dim), 7.0, dtype=dtype, device="cuda")
+    cache.store(x, rope, pos, table, n_head, sequence=seq, out=kept)
+    for _ in range(3):
+        torch.full((tokens, n_head, dim), float("nan"), dtype=dtype, device="cuda")  # freed at once: the next allocation finds it
+        q = cache.store(x, rope, pos, table, n_head, sequence=seq)
+        assert not q[~live].any() and torch.equal(q[live], kept[live])
+    assert (kept[~live] == 7).all()
+
+
 # ---- what the other tests would not notice -------------------------------------------------------------------------------------------
 def _cancelling(dtype, eight, dim, n, seqs, group):
     """Sequences of n positions whose values cancel: the result is far smaller than what it is made of, so that the rounding of probabilities shows.  The
