@@ -163,8 +163,6 @@ def prepare(case, seed):
             sys.path.insert(0, package)
         from gpt_fast import e4m3
         s["e4m3"] = e4m3
-        if "w" in s:  # what a program keeps for its projections
-            s["workspace"] = e4m3.linear_workspace(m, s["w"][0].shape[0], s["w"][0].device)
     return s
 
 
@@ -183,9 +181,9 @@ def run(s):
             return {"codes": codes, "scale": scale}
         if case["op"] == "linear":
             act = None if case["act"] == "none" else case["act"]
-            return e4m3.linear(s["x"], s["w"], bias=s["bias"], activation=act, addend=s["addend"], out=s["out"], workspace=s["workspace"])
+            return e4m3.linear(s["x"], s["w"], bias=s["bias"], activation=act, addend=s["addend"], out=s["out"])
         glu = case["alpha"], float(case["limit"]), case["offset"]
-        return e4m3.gateup_glu(s["x"], s["w"], glu=glu, out=s["out"], workspace=s["workspace"])
+        return e4m3.gateup_glu(s["x"], s["w"], glu=glu, out=s["out"])
     return {"norm": _plain_norm, "rows": _plain_rows, "linear": _plain_linear, "gateup": _plain_gateup}[case["op"]](s)
 
 
