@@ -34,7 +34,7 @@ extern "C" {
 typedef void* lri_stream_t; /* a cudaStream_t */
 
 /* LRI_FP32 is taken by the entry points that say so (every product and sum a true 32-bit operation). */
-enum lri_dtype { LRI_BF16 = 0, LRI_FP16 = 1, LRI_FP32 = 2, LRI_E4M3 = 3 /* pages of a key-value cache only */ };
+enum lri_dtype { LRI_BF16 = 0, LRI_FP16 = 1, LRI_FP32 = 2, LRI_E4M3 = 3 /* pages of a key-value cache only */ };  /* (the entry points of 8-bit projections have e4m3 in their names) */
 /* Added to `dtype` of lri_linear, lri_linear_f32, lri_gateup_glu or their _early forms: a prompt projection (more than 128
  * token rows) stays on the kernel that gives a tile to one SM.  For passes that run kernels of theirs on a second stream
  * beside their projections (see csrc/gemm_pair.cu). */
@@ -295,6 +295,64 @@ int lri_paged_load(const lri_paged_load_call* call);
 int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const void* v_cache, const void* input_pos, int pos_is_i64, void* out,
                            int S, int n_head, int n_kv, int head_dim, int64_t smax, const int32_t* pages, int max_pages, int page_size,
                            int64_t n_pages, lri_stream_t stream);
+
+/* ---- projections in 8 bits (e4m3) ------------------------------------------------------------------
+ * Activations as codes with a scale for each row, weights as codes with a scale for each output: value = code * scale.  Half the bytes of
+ * 16-bit weights for a decode step, twice the rate of the tensor cores for a prompt.  No counterpart in the reference, whose projections are
+ * nn.Linear in 16 bits (gpt_fast/utils.py:142-148, 187-198, 258).
+ * `dtype` bfloat16 or float16: the type of everything that is neither codes nor scales.  Codes: rows of k elements, a multiple of 8, that
+ * start at multiples of 16 bytes (pitch x_ld, w_ld, codes_ld; what lies between the rows is neither read nor written).  All arithmetic in
+ * fp32, rounded once where a result is stored.  Codes, 16-bit rows and results are 16-byte aligned, and results overlap nothing else (one exception: see addend).
+ *
+ * A row's codes are the nearest to value * (448 / top), its scale top / 448, top the largest magnitude of its values and at least 2^-100.
+ * A row with an infinity or NaN gets zeros and a NaN scale.
+ *
+ * lri_quantize_rows_e4m3: rows of x (pitch x_ld, a multiple of 8) to codes and scales; cols a multiple of 8 up to 65536.  Also what stores a weight.
+ *
+ * lri_add_rmsnorm_e4m3: lri_add_rmsnorm with the normed rows as codes: residual_out exactly as there, and
+ *     top = max |residual_out * weight|,  codes = nearest(residual_out * weight * (448 / top)),  scale = top * rsqrt(mean(residual_out^2) + eps) / 448,
+ * so that nothing is rounded between the norm and the codes, and the codes do not depend on the order of the sum of squares.  dim a multiple of 8 up to 16384.
+ *
+ * lri_linear_e4m3: y[m, j] = act(x_scale[m] * w_scale[j] * sum_k x[m, k] w[j, k] + bias[j]) + addend[m, j], j < n.  bias [n], addend [rows, n]
+ * may be NULL; addend may be y.  activation: LRI_ACT_*; GELU by the error function or by tanh.  LRI_ACT_GLU: w has 2 n rows [up | gate] and
+ * w_scale 2 n scales, without bias and addend, and y = g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit), u = clamp(up, -limit, limit):
+ * SwiGLU with alpha 1, limit infinity, offset 0. */
+enum lri_activation { LRI_ACT_NONE = 0, LRI_ACT_SILU = 1, LRI_ACT_GELU = 2, LRI_ACT_GELU_TANH = 3, LRI_ACT_GLU = 4 };
+typedef struct {
+  const void* x;
+  void* codes;
+  float* scale;
+  lri_stream_t stream;
+  int64_t rows, x_ld, codes_ld;
+  int dtype, cols;
+} lri_quantize_e4m3_call;
+int lri_quantize_rows_e4m3(const lri_quantize_e4m3_call* call);
+typedef struct {
+  const void *residual, *add1, *add2, *weight;
+  void *residual_out, *codes;
+  float* scale;
+  lri_stream_t stream;
+  int64_t rows, codes_ld;
+  int dtype, dim;
+  float residual_scale, eps;
+} lri_norm_e4m3_call;
+int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call);
+typedef struct {
+  const void *x, *w;
+  const float *x_scale, *w_scale;
+  const void *bias, *addend;
+  void* y;
+  lri_stream_t stream;
+  int64_t rows, x_ld, w_ld;
+  int dtype, n, k, activation;
+  float alpha, limit, offset;
+} lri_linear_e4m3_call;
+int lri_linear_e4m3(const lri_linear_e4m3_call* call);
+/* The second half of lri_qkv_rope_kvcache: rows [q heads | k heads | v heads] of a projection, qkv [B*S, (n_head + 2 n_kv) * head_dim],
+ * to rotated queries and to the caches; arguments as there. */
+int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_table, const void* input_pos, int pos_is_i64, void* q_out, void* k_cache,
+                     void* v_cache, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax, int64_t table_rows, int table_gathered,
+                     lri_stream_t stream);
 
 /* ---- F8: all-reduce over peer memory (one process per GPU) -----------------------------------
  * A communicator owns, on every rank, one inbox buffer that all peers can write.  One-shot

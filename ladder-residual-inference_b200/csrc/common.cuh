@@ -42,6 +42,11 @@ void count_launch(int n = 1);
     ::lri::count_launch();                                                                     \
   } while (0)
 
+// Whether two ranges of memory share a byte.
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- tuning options ----------------------------------------------------------------------------

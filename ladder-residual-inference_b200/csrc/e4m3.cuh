@@ -1,0 +1,51 @@
+// What the kernels of 8-bit projections share: codes of rows, and what becomes of a projection's sums.
+#pragma once
+
+#include "common.cuh"
+
+namespace lri {
+
+constexpr float kE4m3Largest = 448.f;              // the largest number of e4m3
+constexpr float kE4m3Smallest = 7.888609052e-31f;  // 2^-100: a row of smaller values is stored against it, so that 448 / top stays finite
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// The magnitude as an ordered number; infinity and NaN, which a maximum of floats would drop, are the largest.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Codes of four values of a row: the nearest to v * factor, factor = 448 / top.  The product may pass 448 by its rounding; the conversion
+// keeps it at 448.
+__device__ __forceinline__ uint32_t e4m3_codes4(float a, float b, float c, float d, float factor) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * factor), "f"(a * factor));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * factor), "f"(c * factor));
+  return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+}
+
+// What a projection works on, and what becomes of its sums.
+struct E4m3Linear {
+  const uint8_t *x, *w;  // codes [rows, k], [n, k] (ACT_GLU: [2 n, k], up rows first)
+  const float *x_scale, *w_scale;
+  const void *bias, *addend;
+  void* y;
+  int64_t x_ld, w_ld;
+  int rows, n, k;
+  GluParams glu;
+};
+
+// Activations of a sum in fp32.  NaN stays NaN, which minima and maxima of floats would turn into a limit.
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if (ACT == LRI_ACT_SILU) return silu_f(z);
+  if (ACT == LRI_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if (ACT == LRI_ACT_GELU_TANH) return 0.5f * z * (1.f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+  return z;
+}
+__device__ __forceinline__ float gated_unit(float gate, float up, const GluParams& p) {
+  const float g = gate > p.limit ? p.limit : gate;
+  const float u = up > p.limit ? p.limit : (up < -p.limit ? -p.limit : up);
+  return g * sigmoid_f(p.alpha * g) * (u + p.offset);
+}
+
+int e4m3_simple_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
+
+}  // namespace lri

@@ -1,0 +1,223 @@
+// Rows to 8 bits (e4m3) with a scale for each: rows of activations or weights as they are, or the residual's pending adds and its
+// root-mean-square norm on the way.
+//
+// With x the residual after its adds and w the norm's weight, a row of the norm is x w r, r = 1 / sqrt(mean(x^2) + eps).  Its largest
+// magnitude is r max|x w|, so the codes, nearest(x w r * 448 / (r max|x w|)), are nearest(x w * 448 / max|x w|): the row is looked at
+// once, for the sum of x^2 and the maximum of |x w| together, and r goes into the scale alone.  x w is exact in fp32 (two factors of at
+// most 11 bits), so codes do not depend on the order of any sum.
+//
+// Bound by memory: 2 bytes an element in for each tensor, 2 for the residual and 1 for the codes out.  The row stays in registers, as it
+// was rounded, between the two passes over it.
+#include "e4m3.cuh"
+
+namespace lri {
+namespace {
+
+struct RowsParams {
+  const void *x, *add1, *add2, *weight;  // weight: NORM
+  void* residual_out;
+  uint8_t* codes;
+  float* scale;
+  int64_t x_ld, codes_ld;
+  int cols;
+  float factor, eps;  // NORM: the residual's scale
+};
+
+constexpr int kRowThreads = 256;  // of a CTA when there are many rows
+constexpr int kFewRows = 148;     // up to here a row gets up to 1024 threads: the kernel is a latency chain
+
+// NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
+template <typename T, bool NORM, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) {
+  constexpr int kWarps = THREADS / 32;
+  const int64_t row = blockIdx.x;
+  const int nvec = p.cols >> 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float part_sum[kWarps];
+  __shared__ uint32_t part_top[kWarps];
+
+  uint4 w[NV];
+  if (NORM) {  // a constant of the model: fetched while the preceding kernel drains
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = threadIdx.x + i * THREADS;
+      if (v < nvec) w[i] = __ldg(static_cast<const uint4*>(p.weight) + v);
+    }
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_ld);
+  const uint4* a1 = NORM && p.add1 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add1) + row * p.cols) : nullptr;
+  const uint4* a2 = NORM && p.add2 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add2) + row * p.cols) : nullptr;
+  uint4* out = NORM && p.residual_out ? reinterpret_cast<uint4*>(static_cast<T*>(p.residual_out) + row * p.cols) : nullptr;
+
+  uint4 x[NV];
+  float ss = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = threadIdx.x + i * THREADS;
+    if (v < nvec) x[i] = in[v];
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = threadIdx.x + i * THREADS;
+    if (v >= nvec) continue;
+    float f[8];
+    unpack8<T>(x[i], f);
+    if (NORM) {
+      // each sum is rounded as lri_add_rmsnorm rounds it: the residual is kept in its type
+      if (p.factor != 1.f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] * p.factor);
+      }
+      if (a1) {
+        float a[8];
+        unpack8<T>(a1[v], a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + a[e]);
+      }
+      if (a2) {
+        float a[8];
+        unpack8<T>(a2[v], a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + a[e]);
+      }
+      x[i] = pack8<T>(f);
+      if (out) out[v] = x[i];
+      float g[8];
+      unpack8<T>(w[i], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss += f[e] * f[e];
+        f[e] *= g[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(f[e]));
+  }
+  if (NORM) {
+    ss = warp_sum(ss);
+    if (lane == 0) part_sum[warp] = ss;
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) part_top[warp] = top;
+  __syncthreads();
+  // every warp joins the parts by itself: no second barrier
+  top = __reduce_max_sync(0xffffffffu, lane < kWarps ? part_top[lane] : 0u);
+  if (NORM) ss = warp_sum(lane < kWarps ? part_sum[lane] : 0.f);
+
+  const bool bad = top >= kInfBits;
+  const float most = fmaxf(__uint_as_float(top), kE4m3Smallest);
+  if (threadIdx.x == 0) {
+    const float s = NORM ? most * rsqrtf(ss / static_cast<float>(p.cols) + p.eps) / kE4m3Largest : most / kE4m3Largest;
+    p.scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
+  }
+  const float factor = kE4m3Largest / most;
+  uint2* codes = reinterpret_cast<uint2*>(p.codes + row * p.codes_ld);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = threadIdx.x + i * THREADS;
+    if (v >= nvec) continue;
+    float f[8];
+    unpack8<T>(x[i], f);
+    if (NORM) {
+      float g[8];
+      unpack8<T>(w[i], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= g[e];
+    }
+    codes[v] = bad ? make_uint2(0, 0) : make_uint2(e4m3_codes4(f[0], f[1], f[2], f[3], factor), e4m3_codes4(f[4], f[5], f[6], f[7], factor));
+  }
+}
+
+template <typename T, bool NORM, int NV, int THREADS>
+int launch_nv(const RowsParams& p, int64_t rows, cudaStream_t st) {
+  LRI_CUDA(launch_pdl(rows_e4m3_kernel<T, NORM, NV, THREADS>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, p));
+  LRI_LAUNCH_CHECK(NORM ? "rows_e4m3_kernel<norm>" : "rows_e4m3_kernel");
+  return LRI_OK;
+}
+
+template <typename T, bool NORM>
+int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {
+  const int nvec = p.cols / 8;
+  if (nvec <= 256) return launch_nv<T, NORM, 1, kRowThreads>(p, rows, st);
+  if (rows <= kFewRows || nvec > 8 * kRowThreads) {
+    if (nvec <= 512) return launch_nv<T, NORM, 1, 512>(p, rows, st);
+    if (nvec <= 1024) return launch_nv<T, NORM, 1, 1024>(p, rows, st);
+    if (nvec <= 2048) return launch_nv<T, NORM, 2, 1024>(p, rows, st);
+    if constexpr (!NORM) {
+      if (nvec <= 4096) return launch_nv<T, NORM, 4, 1024>(p, rows, st);
+      return launch_nv<T, NORM, 8, 1024>(p, rows, st);
+    }
+  }
+  if (nvec <= 512) return launch_nv<T, NORM, 2, kRowThreads>(p, rows, st);
+  if (nvec <= 1024) return launch_nv<T, NORM, 4, kRowThreads>(p, rows, st);
+  return launch_nv<T, NORM, 8, kRowThreads>(p, rows, st);
+}
+
+constexpr int kMostNormCols = 16384, kMostCols = 65536;
+
+int check_rows(const char* who, int dtype, int64_t rows, int cols, int most, int64_t codes_ld, const void* codes, const float* scale) {
+  LRI_REQUIRE(dtype == LRI_BF16 || dtype == LRI_FP16, LRI_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  LRI_REQUIRE(rows >= 0 && rows < (1ll << 31), LRI_ERR_ARG, "%s: rows=%lld", who, (long long)rows);
+  LRI_REQUIRE(cols > 0 && cols % 8 == 0 && cols <= most, LRI_ERR_UNSUPPORTED, "%s: rows of %d elements: a multiple of 8 up to %d", who, cols, most);
+  LRI_REQUIRE(rows == 0 || (codes && scale), LRI_ERR_ARG, "%s: codes or scale is NULL", who);
+  LRI_REQUIRE(aligned16(codes) && codes_ld % 16 == 0 && codes_ld >= cols, LRI_ERR_ALIGN, "%s: rows of codes start at multiples of 16 bytes (pitch %lld for %d)", who,
+              (long long)codes_ld, cols);
+  LRI_REQUIRE((reinterpret_cast<uintptr_t>(scale) & 3u) == 0, LRI_ERR_ALIGN, "%s: scale is not 4-byte aligned", who);
+  return LRI_OK;
+}
+
+}  // namespace
+}  // namespace lri
+
+extern "C" int lri_quantize_rows_e4m3(const lri_quantize_e4m3_call* call) {
+  using namespace lri;
+  LRI_REQUIRE(call != nullptr, LRI_ERR_ARG, "quantize_rows_e4m3: NULL call");
+  const lri_quantize_e4m3_call& c = *call;
+  int rc = check_rows("quantize_rows_e4m3", c.dtype, c.rows, c.cols, kMostCols, c.codes_ld, c.codes, c.scale);
+  if (rc != LRI_OK) return rc;
+  LRI_REQUIRE(c.rows == 0 || c.x, LRI_ERR_ARG, "quantize_rows_e4m3: x is NULL");
+  LRI_REQUIRE(aligned16(c.x) && c.x_ld % 8 == 0 && c.x_ld >= c.cols, LRI_ERR_ALIGN, "quantize_rows_e4m3: rows of x start at multiples of 16 bytes (pitch %lld for %d)",
+              (long long)c.x_ld, c.cols);
+  if (c.rows == 0) return LRI_OK;
+  const int64_t x_bytes = ((c.rows - 1) * c.x_ld + c.cols) * 2, codes_bytes = (c.rows - 1) * c.codes_ld + c.cols, scale_bytes = c.rows * 4;
+  LRI_REQUIRE(!overlap(c.codes, codes_bytes, c.x, x_bytes) && !overlap(c.scale, scale_bytes, c.x, x_bytes) &&
+                  !overlap(c.scale, scale_bytes, c.codes, codes_bytes), LRI_ERR_ARG, "quantize_rows_e4m3: results overlap each other or x");
+  RowsParams p{};
+  p.x = c.x, p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.x_ld, p.codes_ld = c.codes_ld, p.cols = c.cols;
+  cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, false>(p, c.rows, st) : launch<__half, false>(p, c.rows, st);
+}
+
+extern "C" int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call) {
+  using namespace lri;
+  LRI_REQUIRE(call != nullptr, LRI_ERR_ARG, "add_rmsnorm_e4m3: NULL call");
+  const lri_norm_e4m3_call& c = *call;
+  int rc = check_rows("add_rmsnorm_e4m3", c.dtype, c.rows, c.dim, kMostNormCols, c.codes_ld, c.codes, c.scale);
+  if (rc != LRI_OK) return rc;
+  LRI_REQUIRE(c.rows == 0 || (c.residual && c.weight), LRI_ERR_ARG, "add_rmsnorm_e4m3: residual or weight is NULL");
+  LRI_REQUIRE(aligned16(c.residual) && aligned16(c.add1) && aligned16(c.add2) && aligned16(c.weight) && aligned16(c.residual_out), LRI_ERR_ALIGN,
+              "add_rmsnorm_e4m3: pointers must be 16-byte aligned");
+  if (c.rows == 0) return LRI_OK;
+  const int64_t bytes = c.rows * c.dim * 2, codes_bytes = (c.rows - 1) * c.codes_ld + c.dim, scale_bytes = c.rows * 4;
+  const void* const dense[] = {c.residual, c.add1, c.add2, c.residual_out};
+  for (const void* t : dense) {
+    if (t == nullptr) continue;
+    LRI_REQUIRE(!overlap(c.codes, codes_bytes, t, bytes) && !overlap(c.scale, scale_bytes, t, bytes), LRI_ERR_ARG,
+                "add_rmsnorm_e4m3: results overlap each other or the inputs");
+    // (an input that is the residual's place is read and written by the same threads)
+    LRI_REQUIRE(t == c.residual_out || !c.residual_out || !overlap(c.residual_out, bytes, t, bytes), LRI_ERR_ARG,
+                "add_rmsnorm_e4m3: residual_out overlaps an input that it is not");
+  }
+  LRI_REQUIRE(!overlap(c.codes, codes_bytes, c.scale, scale_bytes) && !overlap(c.codes, codes_bytes, c.weight, c.dim * 2ll) &&
+                  !overlap(c.scale, scale_bytes, c.weight, c.dim * 2ll) && !(c.residual_out && overlap(c.residual_out, bytes, c.weight, c.dim * 2ll)),
+              LRI_ERR_ARG, "add_rmsnorm_e4m3: results overlap each other or the weight");
+  RowsParams p{};
+  p.x = c.residual, p.add1 = c.add1, p.add2 = c.add2, p.weight = c.weight, p.residual_out = c.residual_out;
+  p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.dim, p.codes_ld = c.codes_ld, p.cols = c.dim;
+  p.factor = c.residual_scale, p.eps = c.eps;
+  cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, true>(p, c.rows, st) : launch<__half, true>(p, c.rows, st);
+}

@@ -670,3 +670,19 @@ extern "C" int lri_qkv_rope_kvcache(int dtype, const void* x, const void* wqkv, 
   return lri::qkv_rope_kvcache(dtype, x, wqkv, rope_table, input_pos, pos_is_i64, q_out, k_cache, v_cache, B, S, K, n_head, n_kv, head_dim, smax,
                                table_rows, table_gathered, workspace, workspace_bytes, {}, stream);
 }
+
+extern "C" int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_table, const void* input_pos, int pos_is_i64, void* q_out, void* k_cache,
+                                void* v_cache, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax, int64_t table_rows, int table_gathered,
+                                lri_stream_t stream) {
+  LRI_REQUIRE(dtype == LRI_BF16 || dtype == LRI_FP16, LRI_ERR_UNSUPPORTED, "rope_kvcache: dtype %d", dtype);
+  LRI_REQUIRE(B >= 0 && S >= 0 && static_cast<int64_t>(B) * S < (1ll << 31), LRI_ERR_ARG, "rope_kvcache: B=%d S=%d", B, S);
+  const int rc = check_qkv(rope_table, input_pos, q_out, k_cache, v_cache, n_head, n_kv, head_dim, smax, table_rows);
+  if (rc != LRI_OK) return rc;
+  LRI_REQUIRE(qkv && aligned16(qkv), LRI_ERR_ALIGN, "rope_kvcache: qkv must be 16-byte aligned and not NULL");
+  if (B == 0 || S == 0) return LRI_OK;
+  LinearParams p{};
+  p.m = B * S, p.rope_table = rope_table, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64;
+  p.q_out = q_out, p.k_cache = k_cache, p.v_cache = v_cache;
+  p.S = S, p.n_head = n_head, p.n_kv = n_kv, p.head_dim = head_dim, p.smax = smax, p.table_rows = table_rows, p.table_gathered = table_gathered;
+  return qkv_scatter_launch(dtype, qkv, p, static_cast<cudaStream_t>(stream));
+}

@@ -36,6 +36,9 @@ class LlamaPass(ctypes.Structure):
 STORE_CALL = struct.Struct("@11Q5q12i")  # lri_paged_store_call
 ATTN_CALL = struct.Struct("@10Q4q9if")   # lri_paged_attn_call
 LOAD_CALL = struct.Struct("@9Q3q8i")     # lri_paged_load_call
+QUANTIZE_CALL = struct.Struct("@4Q3q2i")   # lri_quantize_e4m3_call
+NORM8_CALL = struct.Struct("@8Q2q2i2f")    # lri_norm_e4m3_call
+LINEAR8_CALL = struct.Struct("@8Q3q4i3f0Q")  # lri_linear_e4m3_call
 
 ONE_SM = 0x100  # LRI_ONE_SM
 ZERO_SKIPPED = 0x200  # LRI_ZERO_SKIPPED
@@ -81,6 +84,11 @@ _SIGNATURES = {
     "lri_paged_load": (c_int, [c_void_p]),
     "lri_attn_prefill_pages": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_void_p,
                                        c_int, c_int, c_int64, c_void_p]),
+    "lri_quantize_rows_e4m3": (c_int, [c_void_p]),
+    "lri_add_rmsnorm_e4m3": (c_int, [c_void_p]),
+    "lri_linear_e4m3": (c_int, [c_void_p]),
+    "lri_rope_kvcache": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64,
+                                 c_int64, c_int, c_void_p]),
     "lri_comm_create": (c_int, [c_int, c_int, c_int64, ctypes.POINTER(c_void_p), ctypes.c_char_p]),
     "lri_comm_connect": (c_int, [c_void_p, ctypes.c_char_p]),
     "lri_allreduce": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
@@ -178,6 +186,8 @@ for _name, (_res, _args) in _SIGNATURES.items():
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 BF16, FP16, FP32, E4M3 = 0, 1, 2, 3
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}  # LRI_ACT_*
+ACT_GLU = 4
 CODES = {torch.bfloat16: BF16, torch.float16: FP16}
 GATE_SIGMOID, GATE_SILU = 0, 1
 GEMM_AUTO, GEMM_TCGEN05, GEMM_SIMT = 0, 1, 2

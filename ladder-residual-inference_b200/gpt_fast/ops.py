@@ -197,6 +197,61 @@ class CudaOps:
                                                int(input_pos.dtype == torch.int64), out.data_ptr(), S, n_head, n_kv, head_dim, k_cache.shape[2],
                                                pages.data_ptr(), pages.shape[1], page, n_pages, _C.stream_handle()))
 
+    # ---- projections in 8 bits ----------------------------------------------------------------------
+    # (codes, scale) pairs as gpt_fast.e4m3 checks them.  As above, the pitch of a single row may be any number.
+    @staticmethod
+    def quantize_rows_e4m3(x, codes, scale, shape):
+        here = x.get_device()
+        if not 0 <= here == torch._C._cuda_getDevice() == codes.get_device() == scale.get_device():
+            _C.refuse_devices(x, codes, scale)
+        rows, cols = shape
+        status = _C.lib.lri_quantize_rows_e4m3(_C.QUANTIZE_CALL.pack(
+            x.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x.stride(0) if rows > 1 else cols,
+            codes.stride(0) if rows > 1 else -(-cols // 16) * 16, _C.CODES[x.dtype], cols))
+        if status < 0:
+            _C.check(status)
+
+    @staticmethod
+    def add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, codes, scale, rows, residual_scale=1.0):
+        here = residual.get_device()
+        if not (0 <= here == torch._C._cuda_getDevice() == weight.get_device() == codes.get_device() == scale.get_device() and
+                (add1 is None or add1.get_device() == here) and (add2 is None or add2.get_device() == here) and
+                (residual_out is None or residual_out.get_device() == here)):
+            _C.refuse_devices(residual, weight, codes, scale, add1, add2, residual_out)
+        dim = weight.shape[0]
+        status = _C.lib.lri_add_rmsnorm_e4m3(_C.NORM8_CALL.pack(
+            residual.data_ptr(), 0 if add1 is None else add1.data_ptr(), 0 if add2 is None else add2.data_ptr(), weight.data_ptr(),
+            0 if residual_out is None else residual_out.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows,
+            codes.stride(0) if rows > 1 else -(-dim // 16) * 16, _C.CODES[residual.dtype], dim, residual_scale, eps))
+        if status < 0:
+            _C.check(status)
+
+    @staticmethod
+    def linear_e4m3(x, w, out, rows, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0)):
+        """x, w: (codes, scale); activation: a number of LRI_ACT_*."""
+        (xc, xs), (wc, ws) = x, w
+        here = xc.get_device()
+        if not (0 <= here == torch._C._cuda_getDevice() == xs.get_device() == wc.get_device() == ws.get_device() == out.get_device() and
+                (bias is None or bias.get_device() == here) and (addend is None or addend.get_device() == here)):
+            _C.refuse_devices(xc, xs, wc, ws, out, bias, addend)
+        n, k = wc.shape
+        pitch = -(-k // 16) * 16
+        status = _C.lib.lri_linear_e4m3(_C.LINEAR8_CALL.pack(
+            xc.data_ptr(), wc.data_ptr(), xs.data_ptr(), ws.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if addend is None else addend.data_ptr(),
+            out.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, xc.stride(0) if rows > 1 else pitch, wc.stride(0) if n > 1 else pitch,
+            _C.CODES[out.dtype], n // 2 if activation == _C.ACT_GLU else n, k, activation, *glu))
+        if status < 0:
+            _C.check(status)
+
+    @staticmethod
+    def rope_kvcache(qkv, table, table_gathered, input_pos, q_out, k_cache, v_cache, B, S, n_head, n_kv, head_dim):
+        """The second half of qkv_rope_kvcache, from rows of the projection."""
+        _C.require_cuda(qkv, table, input_pos, q_out, k_cache, v_cache)
+        _C.check(_C.lib.lri_rope_kvcache(
+            _C.dtype_code(qkv.dtype), qkv.data_ptr(), table.data_ptr(), input_pos.data_ptr(), int(input_pos.dtype == torch.int64), q_out.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), B, S, n_head, n_kv, head_dim, k_cache.shape[2], table.shape[0], int(table_gathered),
+            _C.stream_handle()))
+
     # ---- all layers of a pass ------------------------------------------------------------------------
     @staticmethod
     def run_layers(schedule, layers, above, events, main, side, sizes, eps, workspaces, row_ws, **tensors):

@@ -1,0 +1,192 @@
+"""The operators of projections in 8 bits against their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from e4m3_util import E4M3, U, check, glu64, linear64, quantised, random_rows, step, values
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def e4m3():
+    from gpt_fast import e4m3
+    return e4m3
+
+
+def _raw(codes):
+    return codes.view(torch.uint8)
+
+
+def _poisoned(e4m3, rows, cols, pad=0):
+    """Rows for results: what lies between and behind them must stay as it is."""
+    room = torch.full((rows + 2, (-(-cols // 16) + pad) * 16), 0x55, dtype=torch.uint8, device="cuda")
+    scale = torch.full((rows + 2,), -3.0, device="cuda")
+    return room, scale, (room.view(E4M3)[:rows, :cols], scale[:rows])
+
+
+def _untouched(room, scale, rows, cols):
+    assert (room[rows:] == 0x55).all() and (room[:rows, cols:] == 0x55).all() and (scale[rows:] == -3).all()
+
+
+# ---- rows ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,apart,pad", [(1, 8, 0, 0), (3, 24, 8, 1), (2, 2048, 0, 0), (149, 2056, 0, 0), (5, 4096, 1024, 0), (400, 4096, 0, 2), (2, 4104, 0, 0),
+                                                 (200, 8200, 8, 0), (3, 8200, 0, 0), (150, 11000, 0, 0), (2, 16392, 0, 1), (3, 32768, 0, 0), (2, 65536, 0, 0), (160, 288, 40, 0)])
+def test_rows(e4m3, dtype, rows, cols, apart, pad):
+    g = torch.Generator().manual_seed(rows + cols)
+    wide = torch.randn(rows, cols + apart, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))
+    wide[:, cols:] = math.nan
+    x = wide.to(dtype).cuda()[:, :cols]
+    room, scale, out = _poisoned(e4m3, rows, cols, pad)
+    codes, got = e4m3.quantize_rows(x, out=out)
+    assert codes is out[0] and got is out[1]
+    want, want_scale = quantised(x)
+    assert torch.equal(_raw(codes), _raw(want)) and torch.equal(got, want_scale)
+    _untouched(room, scale, rows, cols)
+    # and by the definition in 64 bits: the nearest code, to two roundings of the factor and one of the product
+    y = x.double() / x.double().abs().amax(-1, keepdim=True) * 448
+    assert ((codes.double() - y).abs() <= step(y) / 2 + 3 * U * y.abs() + 1e-30).all()
+    fresh = e4m3.quantize_rows(x)
+    assert torch.equal(_raw(fresh[0]), _raw(want)) and torch.equal(fresh[1], want_scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_no_and_of_unusual_values(e4m3, dtype):
+    x = torch.randn(9, 4096).to(dtype)
+    x[1] = 0.0
+    x[2] = 0.0
+    x[2, 77] = -0.0
+    x[3] *= torch.finfo(dtype).tiny
+    x[4, 4095] = math.inf
+    x[5, 0] = -math.inf
+    x[6, 123] = math.nan
+    x[7, 5] = torch.finfo(dtype).max
+    x[8] = torch.finfo(dtype).min
+    x = x.cuda()
+    codes, scale = e4m3.quantize_rows(x)
+    want, want_scale = quantised(x)
+    assert torch.equal(_raw(codes), _raw(want))
+    assert torch.equal(scale.isnan(), want_scale.isnan()) and torch.equal(scale.nan_to_num(), want_scale.nan_to_num())
+    assert scale.isnan().tolist() == [False] * 4 + [True] * 3 + [False] * 2
+    assert (values((codes, scale))[1] == 0).all()
+
+
+# ---- norm ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,adds,factor,keep", [(1, 8, 0, 1.0, "none"), (1, 4096, 1, 1.0, "own"), (7, 288, 2, 0.5, "in place"), (148, 2048, 1, 1.0, "in place"),
+                                                       (149, 2304, 1, 0.125, "own"), (3, 4104, 2, 1.0, "own"), (200, 4096, 2, 1.0, "add1"), (33, 8192, 0, 1.0, "none"),
+                                                       (150, 8192, 1, 1.0, "own"), (151, 11000, 1, 1.0, "own"), (2, 16384, 2, 0.25, "own"), (155, 16384, 1, 1.0, "own")])
+def test_norm(e4m3, dtype, rows, dim, adds, factor, keep):
+    from gpt_fast.ops import CudaOps
+    g = torch.Generator().manual_seed(rows * dim)
+    residual = (torch.randn(rows, dim, generator=g) * torch.exp(torch.randn(dim, generator=g)) * 3).to(dtype).cuda()
+    added = [torch.randn(rows, dim, generator=g).to(dtype).cuda() for _ in range(adds)] + [None] * (2 - adds)
+    weight = torch.randn(dim, generator=g).to(dtype).cuda()
+    eps = 1e-5
+    # the residual, bit for bit as the operator of 16 bits leaves it
+    kept, normed = torch.empty_like(residual), torch.empty_like(residual)
+    CudaOps.add_rmsnorm(residual, *added, weight, eps, kept, normed, rows, factor)
+    x = kept.double()
+    room, scale, out = _poisoned(e4m3, rows, dim)
+    to = {"none": None, "own": torch.full_like(residual, 7.0), "in place": residual, "add1": added[0]}[keep]
+    codes, got = e4m3.add_rmsnorm(residual, weight, eps, *added, residual_scale=factor, residual_out=to, out=out)
+    if to is not None:
+        assert torch.equal(to, kept)
+    want, top = quantised(kept.float() * weight.float())  # (the product is exact)
+    assert torch.equal(_raw(codes), _raw(want))
+    _untouched(room, scale, rows, dim)
+    rms = (x.square().mean(-1) + eps).sqrt()
+    exact = (x * weight.double()).abs().amax(-1) / (448 * rms)
+    # the sum of squares: at most 64 terms a thread, 10 levels of joining, half of it in the root; rsqrtf to 2 ulp, five more roundings
+    assert ((got.double() - exact).abs() <= (37 + 4 + 5) * U * exact).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_unusual_rows(e4m3, dtype):
+    residual = torch.randn(6, 512).to(dtype)
+    add = torch.randn(6, 512).to(dtype)
+    residual[1], add[1] = 0.0, 0.0
+    residual[2, 3] = math.inf
+    add[3, 511] = math.nan
+    residual[4], add[4] = torch.finfo(dtype).tiny, 0.0
+    residual[5, 0], add[5, 0] = math.inf, -math.inf
+    residual, add, weight = residual.cuda(), add.cuda(), torch.randn(512).to(dtype).cuda()
+    codes, scale = e4m3.add_rmsnorm(residual, weight, 1e-6, add)
+    assert scale.isnan().tolist() == [False, False, True, True, False, True]
+    assert (_raw(codes)[2] == 0).all() and (values((codes, scale))[1] == 0).all()
+    want, _ = quantised((residual + add).float() * weight.float())
+    assert torch.equal(_raw(codes), _raw(want))
+    assert torch.isfinite(scale[[0, 1, 4]]).all()
+
+
+# ---- linear ----------------------------------------------------------------------------------------------------------------------
+SIZES = [(1, 8), (8, 8), (17, 24), (130, 136), (100, 1000), (2001, 264), (256, 4096), (1280, 2048), (4096, 1024), (640, 11000), (129, 16384)]
+
+
+@pytest.mark.parametrize("n,k", SIZES)
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 33, 64, 65, 127, 128, 129, 200, 257, 384, 1000])
+def test_linear(e4m3, rows, n, k):
+    dtype = TYPES[(rows + n) % 2]
+    x, w = random_rows(rows, k, rows + k, pad=rows % 3), random_rows(n, k, n, pad=n % 2, size=k ** -0.5)
+    room = torch.full((rows + 1, n), 5.0, dtype=dtype, device="cuda")
+    y = e4m3.linear(x, w, out=room[:rows])
+    check(y, *linear64(x, w, dtype=dtype))
+    assert (room[rows:] == 5).all()
+    assert torch.equal(y, e4m3.linear(x, w, dtype=dtype)), "the same call twice"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", [None, "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("bias,addend", [(True, "none"), (False, "own"), (True, "in place")])
+@pytest.mark.parametrize("rows,n,k", [(1, 520, 264), (5, 333, 1000), (40, 1056, 512), (100, 257, 128), (300, 520, 640), (513, 203, 72)])
+def test_what_follows_the_sums(e4m3, dtype, activation, bias, addend, rows, n, k):
+    x, w = random_rows(rows, k, 1), random_rows(n, k, 2, size=2 * k ** -0.5)
+    g = torch.Generator().manual_seed(3)
+    b = (2 * torch.randn(n, generator=g)).to(dtype).cuda() if bias else None
+    a = None if addend == "none" else torch.randn(rows, n, generator=g).to(dtype).cuda()
+    want = linear64(x, w, b, activation, a, dtype)
+    y = e4m3.linear(x, w, bias=b, activation=activation, addend=a, dtype=dtype, out=a if addend == "in place" else None)
+    check(y, *want)
+
+
+GLUS = [(1.0, math.inf, 0.0), (1.702, 7.0, 1.0), (1.0, 0.5, 0.0)]
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 16, 33, 64, 65, 128, 129, 300, 520])
+@pytest.mark.parametrize("inter,k,glu", [(1, 8, GLUS[0]), (60, 136, GLUS[1]), (129, 1000, GLUS[0]), (1024, 2048, GLUS[2]), (2001, 264, GLUS[1]), (500, 11000, GLUS[0])])
+def test_gateup(e4m3, rows, inter, k, glu):
+    dtype = TYPES[(rows + inter) % 2]
+    x, w = random_rows(rows, k, rows), random_rows(2 * inter, k, inter, size=2 * k ** -0.5)
+    room = torch.full((rows + 1, inter), 5.0, dtype=dtype, device="cuda")
+    h = e4m3.gateup_glu(x, w, glu, out=room[:rows])
+    check(h, *glu64(x, w, glu, dtype))
+    assert (room[rows:] == 5).all()
+
+
+@pytest.mark.parametrize("rows", [2, 20, 100, 300])
+@pytest.mark.parametrize("kind", ["linear", "gateup"])
+def test_rows_that_are_nan_stay_alone(e4m3, rows, kind):
+    """A NaN scale makes its row NaN, a NaN code of a weight its output; an infinite limit lets NaN through."""
+    x, w = random_rows(rows, 256, 1), random_rows(200, 256, 2, size=1 / 16)
+    x[1][1] = math.nan
+    _raw(w[0])[7, 9] = 0x7F
+    w[1][150] = math.nan
+    y = e4m3.linear(x, w) if kind == "linear" else e4m3.gateup_glu(x, w, (1.0, 7.0, 0.0))
+    bad = torch.zeros(rows, 200, dtype=torch.bool, device="cuda")
+    bad[1], bad[:, 7], bad[:, 150] = True, True, True
+    if kind == "gateup":
+        bad = bad[:, :100] | bad[:, 100:]
+    assert torch.equal(y.isnan(), bad)
+
+
+@pytest.mark.parametrize("rows", [1, 30, 100, 400])
+def test_zero_rows_and_zero_weights(e4m3, rows):
+    x, w = random_rows(rows, 512, 1), random_rows(96, 512, 2)
+    _raw(x[0])[0] = 0
+    x[1][0] = 0.0
+    assert (e4m3.linear(x, w)[0] == 0).all()
+    none = e4m3.linear((x[0][:0], x[1][:0]), w)
+    assert none.shape == (0, 96)
