@@ -46,6 +46,9 @@ __device__ __forceinline__ float gated_unit(float gate, float up, const GluParam
   return g * sigmoid_f(p.alpha * g) * (u + p.offset);
 }
 
-int e4m3_simple_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
+// activation: lri_activation.  One (e4m3_few.cu) for up to kE4m3FewRows rows, the other (e4m3_pair.cu) for any number.
+constexpr int kE4m3FewRows = 128;
+int e4m3_few_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
+int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
 
 }  // namespace lri

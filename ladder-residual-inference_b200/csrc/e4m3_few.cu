@@ -1,0 +1,276 @@
+// Projections in 8 bits of few rows (up to kE4m3FewRows tokens): a decode step of a batch, a short prompt.
+//
+// Bound by reading the weights once.  As in gemm_streamk.cu the weights are the 128-row operand of tcgen05.mma and the tokens its N side (16
+// to 128 wide).  What differs is how the work is spread and joined.  A tile of 128 outputs is one cluster's: its 1, 2, 4 or 8 CTAs take
+// equal runs of the depth, leave their fp32 sums in shared memory, and each of them joins its share of the tile's results out of the others'
+// (distributed shared memory) in the order of the ranks.  So a projection is one launch without a workspace, the sums do not
+// depend on when a CTA runs, and the epilogue's loads are spread over the cluster.
+//
+// Two CTAs fit an SM: with 96 to 108 KB of ring each, 200 KB of weights are under way per SM whichever the tile's share.
+//
+// Gated unit: a tile is 64 up rows and the 64 matching gate rows; up and gate of an output meet where the sums are joined.
+//
+// Warp roles: warp 0 fetches (TMA; the weights of the first stages before the preceding kernel is complete, since it does not write
+// them), warp 1 owns the tensor memory and issues the products, warps 2-5 take the sums out of tensor memory; all warps join.  Every wait on
+// an mbarrier is bounded (lri_gemm_status); every CTA reaches the cluster barriers in every case.
+#include "e4m3_tc.cuh"
+
+namespace lri {
+namespace {
+
+using namespace tc;
+
+__device__ int g_e4m3_few_status = 0;
+
+constexpr int kTileBytes = kBM * kStep;  // of 128 weight rows
+constexpr int kMostSplit = 8;
+constexpr int kRing = 108 * 1024;  // of a CTA, two of which share an SM
+
+template <int BN>
+struct Ring {
+  static constexpr int kStageBytes = kTileBytes + BN * kStep;
+  static constexpr int kStages = kRing / kStageBytes;
+  static constexpr int kBytes = kStages * kStageBytes + 1024;
+  static_assert(kStages * kStageBytes >= BN * kBM * 4, "the sums of a tile take the ring's place");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank) {
+  uint32_t there;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(there) : "memory");
+  return v;
+}
+
+template <typename T, int ACT, int BN>
+__global__ void __launch_bounds__(kGemmThreads)
+e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const E4m3Linear p, int split) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+  constexpr int kOut = kGlu ? kBM / 2 : kBM;  // results of a tile for each token
+  constexpr uint32_t kStages = Ring<BN>::kStages, kStageBytes = Ring<BN>::kStageBytes;
+  constexpr uint32_t kCols = BN < 32 ? 32 : BN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the same in every CTA of the cluster
+  __shared__ uint64_t bars[2 * kStages + 1];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = split == 1 ? 0 : static_cast<int>(cluster_rank());
+  const int tile = blockIdx.x / split;
+  const int steps = (p.k + kStep - 1) / kStep;
+  const int kt0 = steps * rank / split, kt1 = steps * (rank + 1) / split;  // (the host keeps split <= steps)
+
+  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[kStages]), done = smem_u32(&bars[2 * kStages]);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (uint32_t s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
+
+  // warp-uniform loops, one elected lane issues (see gemm_pair.cu)
+  if (warp == 0) {
+    auto fetch_weights = [&](uint32_t s, int kt) {
+      mbar_expect_tx(full0 + 8 * s, kStageBytes);
+      const uint32_t dst = base + s * kStageBytes;
+      tma_load_2d(dst, &tmap_w, full0 + 8 * s, kt * kStep, tile * kOut);
+      if (kGlu) tma_load_2d(dst + kTileBytes / 2, &tmap_w, full0 + 8 * s, kt * kStep, p.n + tile * kOut);
+    };
+    auto fetch_rows = [&](uint32_t s, int kt) { tma_load_2d(base + s * kStageBytes + kTileBytes, &tmap_x, full0 + 8 * s, kt * kStep, 0); };
+    const int ahead = min(static_cast<int>(kStages), kt1 - kt0);
+    for (int i = 0; i < ahead; ++i)
+      if (elect_one()) fetch_weights(i, kt0 + i);
+    __syncwarp();
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int i = 0; i < ahead; ++i)
+      if (elect_one()) fetch_rows(i, kt0 + i);
+    __syncwarp();
+    uint32_t s = ahead == static_cast<int>(kStages) ? 0 : ahead, parity = 0;
+    for (int kt = kt0 + ahead; kt < kt1; ++kt) {
+      if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 71, &g_e4m3_few_status))) break;
+      if (elect_one()) {
+        fetch_weights(s, kt);
+        fetch_rows(s, kt);
+      }
+      __syncwarp();
+      if (++s == kStages) s = 0, parity ^= 1u;
+    }
+  } else if (warp == 1) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t idesc = e4m3_idesc(kBM, BN);
+    uint32_t s = 0, parity = 0;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 72, &g_e4m3_few_status))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_one()) {
+        const uint64_t wdesc = smem_desc_sw128(base + s * kStageBytes);
+        const uint64_t xdesc = smem_desc_sw128(base + s * kStageBytes + kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < kStep / kUmmaBytes; ++kk)
+          umma_e4m3(tmem_base, wdesc + 2 * kk, xdesc + 2 * kk, idesc, (kt > kt0 || kk > 0) ? 1u : 0u);
+        umma_commit(empty0 + 8 * s);
+        if (kt == kt1 - 1) umma_commit(done);
+      }
+      __syncwarp();
+      if (++s == kStages) s = 0, parity ^= 1u;
+    }
+  } else {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int quarter = warp & 3;
+    const bool ok = mbar_wait(done, 0, &abort_flag, 73, &g_e4m3_few_status);
+    if (__all_sync(0xffffffffu, ok)) {
+      // every copy has landed and every product has read it: the ring's place is free for the sums, [token][output of the tile]
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t to = base + (quarter * 32 + lane) * 4;
+#pragma unroll
+      for (int cc = 0; cc < BN; cc += 16) {
+        uint32_t r[16];
+        tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + (cc + e) * kBM * 4), "r"(r[e]) : "memory");
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kCols) : "memory");
+  }
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+  // ---- join: this CTA's share of the (token, pair of outputs) of the tile -----------------------------------------------------------
+  if (!abort_flag) {
+    constexpr int kPairs = kOut / 2;
+    const int items = p.rows * kPairs, i0 = items * rank / split, i1 = items * (rank + 1) / split;
+    const bool pairs_aligned = (p.n & 1) == 0;
+    for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += kGemmThreads) {
+      const int tok = i / kPairs, c = 2 * (i - tok * kPairs);
+      const int64_t j = static_cast<int64_t>(tile) * kOut + c;
+      if (j >= p.n) continue;
+      const bool both = j + 1 < p.n;
+      const uint32_t from = base + (tok * kBM + c) * 4;
+      float2 v[kMostSplit], g[kGlu ? kMostSplit : 1];
+#pragma unroll
+      for (int z = 0; z < kMostSplit; ++z) {
+        v[z] = z < split ? ld_cluster2(from, z) : make_float2(0.f, 0.f);
+        if (kGlu) g[kGlu ? z : 0] = z < split ? ld_cluster2(from + kOut * 4, z) : make_float2(0.f, 0.f);
+      }
+      const float sx = p.x_scale[tok];
+      const float w0 = p.w_scale[j], w1 = both ? p.w_scale[j + 1] : 0.f;
+      float a0 = v[0].x, a1 = v[0].y;
+#pragma unroll
+      for (int z = 1; z < kMostSplit; ++z)
+        if (z < split) a0 += v[z].x, a1 += v[z].y;
+      a0 = a0 * sx * w0, a1 = a1 * sx * w1;
+      const int64_t at = static_cast<int64_t>(tok) * p.n + j;
+      if (kGlu) {
+        float g0 = g[0].x, g1 = g[0].y;
+#pragma unroll
+        for (int z = 1; z < kMostSplit; ++z)
+          if (z < split) g0 += g[kGlu ? z : 0].x, g1 += g[kGlu ? z : 0].y;
+        a0 = gated_unit(g0 * sx * p.w_scale[p.n + j], a0, p.glu);
+        a1 = both ? gated_unit(g1 * sx * p.w_scale[p.n + j + 1], a1, p.glu) : 0.f;
+      } else {
+        if (p.bias) {
+          a0 += Num<T>::to_f(static_cast<const T*>(p.bias)[j]);
+          if (both) a1 += Num<T>::to_f(static_cast<const T*>(p.bias)[j + 1]);
+        }
+        a0 = activate<ACT>(a0), a1 = activate<ACT>(a1);
+        if (p.addend) {
+          const T* add = static_cast<const T*>(p.addend) + at;
+          a0 += Num<T>::to_f(add[0]);
+          if (both) a1 += Num<T>::to_f(add[1]);
+        }
+      }
+      T* y = static_cast<T*>(p.y) + at;
+      if (pairs_aligned) {
+        *reinterpret_cast<uint32_t*>(y) = pack2<T>(a0, a1);
+      } else {
+        y[0] = Num<T>::from_f(a0);
+        if (both) y[1] = Num<T>::from_f(a1);
+      }
+    }
+  } else if (threadIdx.x == 0) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
+  }
+  // nobody leaves while the others read its sums
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// CTAs of a tile: as many as fill the places that two CTAs an SM give, with four steps (64 KB of weights) or more for each.
+int split_of(int tiles, int steps) {
+  int split = 1;
+  while (split < kMostSplit && tiles * split * 2 <= 2 * sm_count() && steps >= 4 * split * 2) split *= 2;
+  return split;
+}
+
+template <typename T, int ACT, int BN>
+int launch(const E4m3Linear& p, cudaStream_t st) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+  constexpr int kOut = kGlu ? kBM / 2 : kBM;
+  CUtensorMap tw, tx;
+  int rc = make_tmap_e4m3(&tw, p.w, kGlu ? 2ll * p.n : p.n, p.k, p.w_ld, kOut);
+  if (rc != LRI_OK) return rc;
+  rc = make_tmap_e4m3(&tx, p.x, p.rows, p.k, p.x_ld, BN);
+  if (rc != LRI_OK) return rc;
+  auto kern = e4m3_few_kernel<T, ACT, BN>;
+  static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
+  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<BN>::kBytes));
+  const int tiles = (p.n + kOut - 1) / kOut, split = split_of(tiles, (p.k + kStep - 1) / kStep);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = Ring<BN>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  LRI_CUDA(cudaLaunchKernelEx(&cfg, kern, tw, tx, p, split));
+  LRI_LAUNCH_CHECK("e4m3_few_kernel");
+  return LRI_OK;
+}
+
+}  // namespace
+
+int e4m3_few_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st) {
+  return by_activation(dtype, activation, [&](auto t, auto act) {
+    using T = typename decltype(t)::type;
+    constexpr int kAct = decltype(act)::value;
+    if (p.rows <= 16) return launch<T, kAct, 16>(p, st);
+    if (p.rows <= 32) return launch<T, kAct, 32>(p, st);
+    if (p.rows <= 64) return launch<T, kAct, 64>(p, st);
+    return launch<T, kAct, 128>(p, st);
+  });
+}
+
+int e4m3_few_status_read_and_clear(int* status_out) { return status_read_and_clear(g_e4m3_few_status, status_out); }
+
+}  // namespace lri

@@ -1,0 +1,375 @@
+// Prompt projections in 8 bits on pairs of SMs (cta_group::2):  y[m, n] = act(sx[m] sw[n] sum_k x[m, k] w[n, k] + bias[n]) + addend[m, n].
+//
+// A cluster of two CTAs works through output tiles of 256 tokens x bn outputs, as in gemm_pair.cu, where the split is explained: each CTA
+// fetches its own 128 tokens and its own half of the tile's weight rows, one instruction multiplies 256 x bn x 32 codes.  A K step is 128
+// codes, 128 bytes a row: the copies, the swizzle and the descriptors are those of 64 elements of 16 bits, and so are the tensor pipe's cycles
+// a step, for twice the products.
+//
+// The codes' products are exact in fp32 and are summed there; the scales come in with the sums.  A token's scale belongs to an accumulator row
+// (a thread of the epilogue), an output's to a column, which all threads read at the same time.
+//
+// Gated unit: a tile is bn / 2 up rows and the bn / 2 matching gate rows, fetched by one CTA of the pair each.
+//
+// Roles per CTA: warp 0 fetches (TMA, no multicast), warp 1 owns the tensor memory and, in the first CTA, issues the products, warps 2-5
+// store.  Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
+// uses, is said in gemm_pair.cu and holds here.
+#include "e4m3.cuh"
+#include "e4m3_tc.cuh"
+#include "gemm_tile.cuh"
+
+namespace lri {
+namespace {
+
+using namespace tc;
+
+__device__ int g_e4m3_pair_status = 0;
+
+constexpr int kMaxStages = 8;
+constexpr int kTileBytes = kBM * kStep;  // of 128 operand rows
+constexpr int kAccCols = 256;            // TMEM columns of one of the two accumulators
+constexpr int kMaxBn = 256;
+constexpr int kSmemLimit = 226 * 1024;
+constexpr int kOwnSmem = 181 * 1024;
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// `bar` may lie in either CTA of the pair
+__device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* tmap, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_dst), "l"(tmap), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// arrives on the barrier at this offset in both CTAs
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Stores `V` consecutive results of a row, the first of which is column j (j < n).
+template <typename T, int V>
+__device__ __forceinline__ void store_results(T* dst, const float (&f)[V], int64_t j, int n, bool vectors) {
+  if (vectors && j + V <= n) {
+#pragma unroll
+    for (int v = 0; v < V / 8; ++v) {
+      float g[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = f[v * 8 + e];
+      reinterpret_cast<uint4*>(dst)[v] = pack8<T>(g);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (j + e < n) dst[e] = Num<T>::from_f(f[e]);
+  }
+}
+// Loads `V` consecutive elements of T as floats; zeros behind column n.
+template <typename T, int V>
+__device__ __forceinline__ void load_columns(const T* src, float (&f)[V], int64_t j, int n, bool vectors) {
+  if (vectors && j + V <= n) {
+#pragma unroll
+    for (int v = 0; v < V / 8; ++v) {
+      float g[8];
+      load8<T>(src + v * 8, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[v * 8 + e] = g[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = j + e < n ? Num<T>::to_f(src[e]) : 0.f;
+  }
+}
+
+// One row of an output tile from the TMEM lane at `tacc`; row = the token.  The loads from TMEM are warp-collective: the lanes meet before
+// each of them, rows outside the problem store nothing.
+template <typename T, int ACT>
+__device__ __forceinline__ void store_row(const E4m3Linear& p, int64_t row, int tile_q, int bn, uint32_t tacc) {
+  const bool live = row < p.rows, vectors = (p.n & 7) == 0;
+  const float sx = live ? p.x_scale[row] : 0.f;
+  if (ACT == LRI_ACT_GLU) {
+#pragma unroll 1
+    for (int cc = 0; cc < bn / 2; cc += 16) {
+      uint32_t up[16], gate[16];
+      __syncwarp();
+      tmem_ld16_issue(tacc + cc, up);
+      tmem_ld16_issue(tacc + bn / 2 + cc, gate);
+      tmem_wait_ld();
+      const int64_t j = static_cast<int64_t>(tile_q) * (bn / 2) + cc;
+      if (live && j < p.n) {
+        float su[16], sg[16], out[16];
+        load_columns<float, 16>(p.w_scale + j, su, j, p.n, true);
+        load_columns<float, 16>(p.w_scale + p.n + j, sg, j, p.n, (p.n & 3) == 0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          out[e] = gated_unit(__uint_as_float(gate[e]) * sx * sg[e], __uint_as_float(up[e]) * sx * su[e], p.glu);
+        store_results<T, 16>(static_cast<T*>(p.y) + row * p.n + j, out, j, p.n, vectors);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int cc = 0; cc < bn; cc += 32) {
+      uint32_t r[32];
+      __syncwarp();
+      tmem_ld32_issue(tacc + cc, r);
+      const int64_t j = static_cast<int64_t>(tile_q) * bn + cc;
+      const bool here = live && j < p.n;
+      float add[32];
+      if (here && p.addend) load_columns<T, 32>(static_cast<const T*>(p.addend) + row * p.n + j, add, j, p.n, vectors);
+      tmem_wait_ld();
+      if (here) {
+        float out[32], s[32];
+        load_columns<float, 32>(p.w_scale + j, s, j, p.n, true);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) out[e] = __uint_as_float(r[e]) * sx * s[e];
+        if (p.bias) {
+          load_columns<T, 32>(static_cast<const T*>(p.bias) + j, s, j, p.n, true);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) out[e] += s[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) out[e] = activate<ACT>(out[e]);
+        if (p.addend) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) out[e] += add[e];
+        }
+        store_results<T, 32>(static_cast<T*>(p.y) + row * p.n + j, out, j, p.n, vectors);
+      }
+    }
+  }
+}
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const E4m3Linear p, GemmGrid grid, int bn,
+                 uint32_t stages) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzle atoms need 1024-byte alignment; the same in both CTAs
+  __shared__ uint64_t bars[2 * kMaxStages + 4];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // uniform for the compiler too
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = blockIdx.x & 1;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int num_kt = (p.k + kStep - 1) / kStep;
+  const int half = bn >> 1;
+  const uint32_t stage_bytes = static_cast<uint32_t>(kTileBytes + half * kStep);  // 128 token rows and bn / 2 weight rows
+
+  const uint32_t full0 = smem_u32(&bars[0]);
+  const uint32_t empty0 = smem_u32(&bars[kMaxStages]);
+  const uint32_t acc_full0 = smem_u32(&bars[2 * kMaxStages]);       // products -> stores, one per accumulator
+  const uint32_t acc_empty0 = smem_u32(&bars[2 * kMaxStages + 2]);  // stores -> products (first CTA)
+
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (uint32_t s = 0; s < stages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full0 + 8 * a, 1);
+      mbar_init(acc_empty0 + 8 * a, 8);  // four warps of each CTA
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the other CTA runs
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
+                 "r"(2 * kAccCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_barrier();  // the barriers of both CTAs exist before either is used from the other
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int items = grid.tiles_p * grid.tiles_q;
+
+  if (warp == 0) {
+    const uint32_t full_first = in_cta(full0, 0);
+    uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait on parity 1, so the first round does not block
+    bool ok = true;
+    for (int item = pair; item < items && ok; item += pairs) {
+      const WorkItem w = work_item(item, grid);
+      // the weight rows of this CTA: half of the tile's, or all its up rows (first CTA) and all its gate rows (second)
+      const int w_row = kGlu ? static_cast<int>(rank) * p.n + w.tile_q * half : w.tile_q * bn + static_cast<int>(rank) * half;
+      const int x_row = w.tile_p * 2 * kBM + static_cast<int>(rank) * kBM;
+      for (int kt = 0; kt < num_kt; ++kt) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 61, &g_e4m3_pair_status));
+        if (!ok) break;
+        if (elect_one()) {
+          // (the second CTA's bytes may arrive before this: the phase cannot end before the arrival counted here)
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * stage_bytes);
+          const uint32_t dst = base + s * stage_bytes;
+          tma_load_pair(dst, &tmap_x, full_first + 8 * s, kt * kStep, x_row);
+          tma_load_pair(dst + kTileBytes, &tmap_w, full_first + 8 * s, kt * kStep, w_row);
+        }
+        if (++s == stages) s = 0, parity ^= 1u;
+      }
+    }
+    // the commits that free the last stages arrive in both CTAs: neither leaves before it has seen its own
+    for (uint32_t left = 0; left < stages && ok; ++left) {
+      ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 65, &g_e4m3_pair_status));
+      if (++s == stages) s = 0, parity ^= 1u;
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t idesc = e4m3_idesc(2 * kBM, bn);
+      uint32_t s = 0, parity = 0;
+      bool ok = true;
+      int it = 0;
+      for (int item = pair; item < items && ok; item += pairs, ++it) {
+        const uint32_t a = it & 1;
+        const uint32_t use = static_cast<uint32_t>(it) >> 1;
+        // the stores of both CTAs must have drained this accumulator (its first use does not block)
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_empty0 + 8 * a, (use & 1u) ^ 1u, &abort_flag, 64, &g_e4m3_pair_status));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d_tmem = tmem_base + a * kAccCols;
+        for (int kt = 0; kt < num_kt; ++kt) {
+          ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, parity, &abort_flag, 62, &g_e4m3_pair_status));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_one()) {
+            const uint64_t xdesc = smem_desc_sw128(base + s * stage_bytes);
+            const uint64_t wdesc = smem_desc_sw128(base + s * stage_bytes + kTileBytes);
+#pragma unroll
+            for (int kk = 0; kk < kStep / kUmmaBytes; ++kk)
+              umma_pair_e4m3(d_tmem, xdesc + 2 * kk, wdesc + 2 * kk, idesc, (kt > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(empty0 + 8 * s);  // both CTAs' stage is free once these products have read it
+            if (kt == num_kt - 1) umma_commit_pair(acc_full0 + 8 * a);
+          }
+          __syncwarp();
+          if (++s == stages) s = 0, parity ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id mod 4
+    const int i = quarter * 32 + lane;
+    int it = 0;
+    for (int item = pair; item < items; item += pairs, ++it) {
+      const WorkItem w = work_item(item, grid);
+      const uint32_t a = it & 1;
+      const uint32_t use = static_cast<uint32_t>(it) >> 1;
+      // the tcgen05.ld of the epilogue are warp-collective: the warp leaves together or not at all
+      const bool ready = mbar_wait(acc_full0 + 8 * a, use & 1u, &abort_flag, 63, &g_e4m3_pair_status);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * kAccCols;
+      store_row<T, ACT>(p, static_cast<int64_t>(w.tile_p) * 2 * kBM + rank * kBM + i, w.tile_q, bn, tacc);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_in_cluster(in_cta(acc_empty0 + 8 * a, 0));
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (abort_flag && threadIdx.x == 0) {
+    // give copies that were already issued time to land before the pair's shared memory is released
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);
+  }
+  __syncthreads();
+  cluster_barrier();  // the products read both CTAs' shared memory, and the stores arrive on the first CTA's barriers
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kAccCols) : "memory");
+  }
+}
+
+// Width of the tile: a K step costs about bn + 64 columns' worth (see gemm_pair.cu), so the narrower tile wins where it fills the last round.
+int tile_width(int64_t rows, int64_t w_rows) {
+  const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+  int best = kMaxBn;
+  int64_t cost = 0;
+  for (int bn = kMaxBn; bn >= 64; bn -= 32) {
+    const int64_t tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
+    const int64_t c = (tiles + pairs - 1) / pairs * (bn + 64);
+    if (bn == kMaxBn || c < cost) best = bn, cost = c;
+  }
+  return best;
+}
+
+template <typename T, int ACT>
+int launch(const E4m3Linear& p, cudaStream_t st) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+  const int64_t w_rows = kGlu ? 2ll * p.n : p.n;
+  const int bn = tile_width(p.rows, w_rows);
+  CUtensorMap tx, tw;
+  int rc = make_tmap_e4m3(&tx, p.x, p.rows, p.k, p.x_ld, kBM);
+  if (rc != LRI_OK) return rc;
+  rc = make_tmap_e4m3(&tw, p.w, w_rows, p.k, p.w_ld, bn / 2);
+  if (rc != LRI_OK) return rc;
+  auto kern = e4m3_pair_kernel<T, ACT>;
+  static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
+  LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+  const int stage_bytes = kTileBytes + bn / 2 * kStep;
+  int stages = (kSmemLimit - 1024) / stage_bytes;
+  stages = stages > kMaxStages ? kMaxStages : stages;
+
+  const int64_t tiles_p = (static_cast<int64_t>(p.rows) + 2 * kBM - 1) / (2 * kBM);
+  const int64_t tiles_q = kGlu ? (p.n + bn / 2 - 1) / (bn / 2) : (p.n + bn - 1) / bn;
+  const int64_t items = tiles_p * tiles_q;
+  if (items >= (1ll << 31)) return fail(LRI_ERR_UNSUPPORTED, "linear_e4m3: %lld output tiles", (long long)items);
+  // panel of token tiles: about 32 MB of tokens, between 2 and 16 tiles
+  int64_t group = (32ll << 20) / (2ll * kBM * p.k);
+  group = group < 2 ? 2 : (group > 16 ? 16 : group);
+  group = group > tiles_p ? tiles_p : group;
+  GemmGrid grid{static_cast<int>(tiles_p), static_cast<int>(tiles_q), static_cast<int>(group), nullptr, 0};
+  int usable = (sm_count() - option(OPT_GEMM_RESERVE_SMS)) / 2;
+  usable = usable < 1 ? 1 : usable;
+  const int64_t clusters = items < usable ? items : usable;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
+  cfg.blockDim = dim3(kGemmThreads);
+  const int smem = stages * stage_bytes + 1024;
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem > kOwnSmem ? smem : kOwnSmem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  LRI_CUDA(cudaLaunchKernelEx(&cfg, kern, tx, tw, p, grid, bn, static_cast<uint32_t>(stages)));
+  LRI_LAUNCH_CHECK("e4m3_pair_kernel");
+  return LRI_OK;
+}
+
+}  // namespace
+
+int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st) {
+  return by_activation(dtype, activation, [&](auto t, auto act) { return launch<typename decltype(t)::type, decltype(act)::value>(p, st); });
+}
+
+int e4m3_pair_status_read_and_clear(int* status_out) { return status_read_and_clear(g_e4m3_pair_status, status_out); }
+
+}  // namespace lri

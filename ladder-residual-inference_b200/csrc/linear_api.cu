@@ -21,6 +21,8 @@ int window_attention_tc_status_read_and_clear(int* status_out);
 int attn_decode_stream_status_read_and_clear(int* status_out);
 int paged_attn_status_read_and_clear(int* status_out);
 int state_scan_status_read_and_clear(int* status_out);
+int e4m3_few_status_read_and_clear(int* status_out);
+int e4m3_pair_status_read_and_clear(int* status_out);
 bool gemm_tcgen05_fused_supports(int epi, const LinearParams& p, int64_t m);
 int gemm_tcgen05_fused_launch(int dtype, int epi, const LinearParams& p, int64_t m, cudaStream_t st);
 
@@ -376,6 +378,12 @@ extern "C" int lri_gemm_status(void) {
   rc = paged_attn_status_read_and_clear(&v7);
   if (rc != LRI_OK) return rc;
   if (v7 != 0) return fail(LRI_ERR_TIMEOUT, "paged decode attention: a bounded mbarrier wait gave up (site %d)", v7);
+  int v8 = 0, v9 = 0;
+  rc = e4m3_few_status_read_and_clear(&v8);
+  if (rc != LRI_OK) return rc;
+  rc = e4m3_pair_status_read_and_clear(&v9);
+  if (rc != LRI_OK) return rc;
+  if (v8 != 0 || v9 != 0) return fail(LRI_ERR_TIMEOUT, "projection in 8 bits: a bounded mbarrier wait gave up (site %d)", v8 != 0 ? v8 : v9);
   int v4 = 0;
   rc = state_scan_status_read_and_clear(&v4);
   if (rc != LRI_OK) return rc;
