@@ -160,58 +160,81 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kCols) : "memory");
   }
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-  // ---- join: this CTA's share of the (token, pair of outputs) of the tile -----------------------------------------------------------
+  // ---- join: this CTA's share of the tokens, a thread for a pair of outputs ---------------------------------------------------------
+  constexpr int kPairs = kOut / 2, kGroups = kGemmThreads / kPairs;
+  const int c = 2 * static_cast<int>(threadIdx.x % kPairs);
+  const int64_t j = static_cast<int64_t>(tile) * kOut + c;
+  const bool there = j < p.n, both = j + 1 < p.n, pairs_aligned = (p.n & 1) == 0;
+  float2 s = make_float2(0.f, 0.f), more = s;  // scales of the outputs; bias, or scales of the gate
+  if (there) {
+    s = make_float2(p.w_scale[j], both ? p.w_scale[j + 1] : 0.f);
+    if (kGlu) {
+      more = make_float2(p.w_scale[p.n + j], both ? p.w_scale[p.n + j + 1] : 0.f);
+    } else if (p.bias) {
+      const T* bias = static_cast<const T*>(p.bias) + j;
+      more = make_float2(Num<T>::to_f(bias[0]), both ? Num<T>::to_f(bias[1]) : 0.f);
+    }
+  }
+  const int t0 = p.rows * rank / split, t1 = p.rows * (rank + 1) / split;
+  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (!abort_flag) {
-    constexpr int kPairs = kOut / 2;
-    const int items = p.rows * kPairs, i0 = items * rank / split, i1 = items * (rank + 1) / split;
-    const bool pairs_aligned = (p.n & 1) == 0;
-    for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += kGemmThreads) {
-      const int tok = i / kPairs, c = 2 * (i - tok * kPairs);
-      const int64_t j = static_cast<int64_t>(tile) * kOut + c;
-      if (j >= p.n) continue;
-      const bool both = j + 1 < p.n;
-      const uint32_t from = base + (tok * kBM + c) * 4;
-      float2 v[kMostSplit], g[kGlu ? kMostSplit : 1];
+    // two tokens at a time: their loads out of the cluster's shared memory are under way together
+    for (int t = t0 + static_cast<int>(threadIdx.x / kPairs); there && t < t1; t += 2 * kGroups) {
+      float2 v[2], g[2], add[2];
+      float sx[2];
+      uint32_t from[2];
 #pragma unroll
-      for (int z = 0; z < kMostSplit; ++z) {
-        v[z] = z < split ? ld_cluster2(from, z) : make_float2(0.f, 0.f);
-        if (kGlu) g[kGlu ? z : 0] = z < split ? ld_cluster2(from + kOut * 4, z) : make_float2(0.f, 0.f);
-      }
-      const float sx = p.x_scale[tok];
-      const float w0 = p.w_scale[j], w1 = both ? p.w_scale[j + 1] : 0.f;
-      float a0 = v[0].x, a1 = v[0].y;
-#pragma unroll
-      for (int z = 1; z < kMostSplit; ++z)
-        if (z < split) a0 += v[z].x, a1 += v[z].y;
-      a0 = a0 * sx * w0, a1 = a1 * sx * w1;
-      const int64_t at = static_cast<int64_t>(tok) * p.n + j;
-      if (kGlu) {
-        float g0 = g[0].x, g1 = g[0].y;
-#pragma unroll
-        for (int z = 1; z < kMostSplit; ++z)
-          if (z < split) g0 += g[kGlu ? z : 0].x, g1 += g[kGlu ? z : 0].y;
-        a0 = gated_unit(g0 * sx * p.w_scale[p.n + j], a0, p.glu);
-        a1 = both ? gated_unit(g1 * sx * p.w_scale[p.n + j + 1], a1, p.glu) : 0.f;
-      } else {
-        if (p.bias) {
-          a0 += Num<T>::to_f(static_cast<const T*>(p.bias)[j]);
-          if (both) a1 += Num<T>::to_f(static_cast<const T*>(p.bias)[j + 1]);
+      for (int u = 0; u < 2; ++u) {
+        const int tok = t + u * kGroups < t1 ? t + u * kGroups : t;
+        from[u] = base + (tok * kBM + c) * 4;
+        sx[u] = p.x_scale[tok];
+        add[u] = make_float2(0.f, 0.f);
+        if (!kGlu && p.addend) {
+          const T* a = static_cast<const T*>(p.addend) + static_cast<int64_t>(tok) * p.n + j;
+          add[u] = make_float2(Num<T>::to_f(a[0]), both ? Num<T>::to_f(a[1]) : 0.f);
         }
-        a0 = activate<ACT>(a0), a1 = activate<ACT>(a1);
-        if (p.addend) {
-          const T* add = static_cast<const T*>(p.addend) + at;
-          a0 += Num<T>::to_f(add[0]);
-          if (both) a1 += Num<T>::to_f(add[1]);
-        }
+        v[u] = g[u] = make_float2(0.f, 0.f);
       }
-      T* y = static_cast<T*>(p.y) + at;
-      if (pairs_aligned) {
-        *reinterpret_cast<uint32_t*>(y) = pack2<T>(a0, a1);
-      } else {
-        y[0] = Num<T>::from_f(a0);
-        if (both) y[1] = Num<T>::from_f(a1);
+      float2 part[kMostSplit][2], gate[kGlu ? kMostSplit : 1][2];
+#pragma unroll
+      for (int z = 0; z < kMostSplit; ++z)
+        if (z < split) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            part[z][u] = ld_cluster2(from[u], z);
+            if (kGlu) gate[kGlu ? z : 0][u] = ld_cluster2(from[u] + kOut * 4, z);
+          }
+        }
+#pragma unroll
+      for (int z = 0; z < kMostSplit; ++z)
+        if (z < split) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            v[u].x += part[z][u].x, v[u].y += part[z][u].y;
+            if (kGlu) g[u].x += gate[kGlu ? z : 0][u].x, g[u].y += gate[kGlu ? z : 0][u].y;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tok = t + u * kGroups;
+        if (tok >= t1) continue;
+        float a0 = v[u].x * sx[u] * s.x, a1 = v[u].y * sx[u] * s.y;
+        if (kGlu) {
+          a0 = gated_unit(g[u].x * sx[u] * more.x, a0, p.glu);
+          a1 = gated_unit(g[u].y * sx[u] * more.y, a1, p.glu);
+        } else {
+          a0 = activate<ACT>(a0 + more.x) + add[u].x;
+          a1 = activate<ACT>(a1 + more.y) + add[u].y;
+        }
+        T* y = static_cast<T*>(p.y) + static_cast<int64_t>(tok) * p.n + j;
+        if (pairs_aligned) {
+          *reinterpret_cast<uint32_t*>(y) = pack2<T>(a0, a1);
+        } else {
+          y[0] = Num<T>::from_f(a0);
+          if (both) y[1] = Num<T>::from_f(a1);
+        }
       }
     }
   } else if (threadIdx.x == 0) {

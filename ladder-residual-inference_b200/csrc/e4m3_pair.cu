@@ -10,7 +10,7 @@
 //
 // Gated unit: a tile is bn / 2 up rows and the bn / 2 matching gate rows, fetched by one CTA of the pair each.
 //
-// Roles per CTA: warp 0 fetches (TMA, no multicast), warp 1 owns the tensor memory and, in the first CTA, issues the products, warps 2-5
+// Roles per CTA: warp 0 fetches (TMA, no multicast), warp 1 owns the tensor memory and, in the first CTA, issues the products, warps 2-9
 // store.  Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
 // uses, is said in gemm_pair.cu and holds here.
 #include "e4m3.cuh"
@@ -30,6 +30,8 @@ constexpr int kAccCols = 256;            // TMEM columns of one of the two accum
 constexpr int kMaxBn = 256;
 constexpr int kSmemLimit = 226 * 1024;
 constexpr int kOwnSmem = 181 * 1024;
+constexpr int kStoreWarps = 8;  // two for each quarter of the tensor memory's lanes, which take its columns in turn
+constexpr int kThreads = 64 + 32 * kStoreWarps;
 
 __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -64,100 +66,126 @@ __device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Stores `V` consecutive results of a row, the first of which is column j (j < n).
-template <typename T, int V>
-__device__ __forceinline__ void store_results(T* dst, const float (&f)[V], int64_t j, int n, bool vectors) {
-  if (vectors && j + V <= n) {
-#pragma unroll
-    for (int v = 0; v < V / 8; ++v) {
-      float g[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = f[v * 8 + e];
-      reinterpret_cast<uint4*>(dst)[v] = pack8<T>(g);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (j + e < n) dst[e] = Num<T>::from_f(f[e]);
-  }
-}
-// Loads `V` consecutive elements of T as floats; zeros behind column n.
-template <typename T, int V>
-__device__ __forceinline__ void load_columns(const T* src, float (&f)[V], int64_t j, int n, bool vectors) {
-  if (vectors && j + V <= n) {
-#pragma unroll
-    for (int v = 0; v < V / 8; ++v) {
-      float g[8];
-      load8<T>(src + v * 8, g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[v * 8 + e] = g[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = j + e < n ? Num<T>::to_f(src[e]) : 0.f;
-  }
-}
+// ---- from the sums to the results -----------------------------------------------------------------------------------------------
+// A warp takes 32 rows x 32 columns of sums at a time.  Out of tensor memory a thread gets a row; the results want threads along the
+// columns, where memory is contiguous and an output's scale and bias are needed once for many rows.  So the block goes through shared
+// memory, scaled by its rows' scales on the way: kPitch words a row, a multiple of 4 whose vectors fall into different banks both ways.
+//   n a multiple of 8: a thread has 8 columns of every eighth row, moved as vectors of 16 bytes
+//   otherwise: a thread has one column of every row (rows of the result start anywhere)
+constexpr int kPitch = 36;
+constexpr int kBlockBytes = 32 * kPitch * 4;
 
-// One row of an output tile from the TMEM lane at `tacc`; row = the token.  The loads from TMEM are warp-collective: the lanes meet before
-// each of them, rows outside the problem store nothing.
-template <typename T, int ACT>
-__device__ __forceinline__ void store_row(const E4m3Linear& p, int64_t row, int tile_q, int bn, uint32_t tacc) {
-  const bool live = row < p.rows, vectors = (p.n & 7) == 0;
-  const float sx = live ? p.x_scale[row] : 0.f;
-  if (ACT == LRI_ACT_GLU) {
-#pragma unroll 1
-    for (int cc = 0; cc < bn / 2; cc += 16) {
-      uint32_t up[16], gate[16];
-      __syncwarp();
-      tmem_ld16_issue(tacc + cc, up);
-      tmem_ld16_issue(tacc + bn / 2 + cc, gate);
-      tmem_wait_ld();
-      const int64_t j = static_cast<int64_t>(tile_q) * (bn / 2) + cc;
-      if (live && j < p.n) {
-        float su[16], sg[16], out[16];
-        load_columns<float, 16>(p.w_scale + j, su, j, p.n, true);
-        load_columns<float, 16>(p.w_scale + p.n + j, sg, j, p.n, (p.n & 3) == 0);
+__device__ __forceinline__ void put_row(uint32_t block, int lane, const uint32_t (&r)[32], float sx) {
+  const uint32_t to = block + lane * kPitch * 4;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          out[e] = gated_unit(__uint_as_float(gate[e]) * sx * sg[e], __uint_as_float(up[e]) * sx * su[e], p.glu);
-        store_results<T, 16>(static_cast<T*>(p.y) + row * p.n + j, out, j, p.n, vectors);
-      }
-    }
-  } else {
-#pragma unroll 1
-    for (int cc = 0; cc < bn; cc += 32) {
-      uint32_t r[32];
-      __syncwarp();
-      tmem_ld32_issue(tacc + cc, r);
-      const int64_t j = static_cast<int64_t>(tile_q) * bn + cc;
-      const bool here = live && j < p.n;
-      float add[32];
-      if (here && p.addend) load_columns<T, 32>(static_cast<const T*>(p.addend) + row * p.n + j, add, j, p.n, vectors);
-      tmem_wait_ld();
-      if (here) {
-        float out[32], s[32];
-        load_columns<float, 32>(p.w_scale + j, s, j, p.n, true);
+  for (int v = 0; v < 8; ++v)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16 * v), "f"(__uint_as_float(r[4 * v]) * sx), "f"(__uint_as_float(r[4 * v + 1]) * sx),
+                 "f"(__uint_as_float(r[4 * v + 2]) * sx), "f"(__uint_as_float(r[4 * v + 3]) * sx)
+                 : "memory");
+}
+// this thread's 32 values of the block, VEC: [it][e] = row it * 8 + lane / 4, column lane % 4 * 8 + e; else [i / 8][i % 8] = row i, column lane
+template <bool VEC>
+__device__ __forceinline__ void get_values(uint32_t block, int lane, float (&f)[4][8]) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) out[e] = __uint_as_float(r[e]) * sx * s[e];
-        if (p.bias) {
-          load_columns<T, 32>(static_cast<const T*>(p.bias) + j, s, j, p.n, true);
+  for (int it = 0; it < 4; ++it) {
+    if (VEC) {
+      const uint32_t from = block + ((it * 8 + (lane >> 2)) * kPitch + (lane & 3) * 8) * 4;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) out[e] += s[e];
-        }
+      for (int h = 0; h < 2; ++h)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(f[it][4 * h]), "=f"(f[it][4 * h + 1]), "=f"(f[it][4 * h + 2]), "=f"(f[it][4 * h + 3])
+                     : "r"(from + 16 * h)
+                     : "memory");
+    } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) out[e] = activate<ACT>(out[e]);
-        if (p.addend) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) out[e] += add[e];
-        }
-        store_results<T, 32>(static_cast<T*>(p.y) + row * p.n + j, out, j, p.n, vectors);
-      }
+      for (int e = 0; e < 8; ++e)
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[it][e]) : "r"(block + ((it * 8 + e) * kPitch + lane) * 4) : "memory");
     }
   }
 }
 
+// One block: rows row0 .. row0 + 31, columns j0 .. j0 + 31 (j0 < n), sums at `tacc` (GLU: of the gate at `tgate`).
+template <typename T, int ACT, bool VEC>
+__device__ __forceinline__ void store_block(const E4m3Linear& p, int64_t row0, int64_t j0, float sx, uint32_t block, uint32_t tacc, uint32_t tgate) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+  constexpr int kCols = VEC ? 8 : 1;
+  const int lane = threadIdx.x & 31;
+  const int64_t j = j0 + (VEC ? (lane & 3) * 8 : lane);
+  const bool there = j < p.n;
+  auto row_of = [&](int it, int e) { return row0 + (VEC ? it * 8 + (lane >> 2) : it * 8 + e); };
+
+  // what does not depend on the sums is asked for before they are waited for
+  uint32_t r[32];
+  __syncwarp();
+  tmem_ld32_issue(tacc, r);
+  float s[kCols] = {}, more[kCols] = {};  // scales of the columns; their biases, or the scales of the gate
+  uint4 add[4] = {};
+  if (there) {
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) s[e] = p.w_scale[j + e];
+    if (kGlu) {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) more[e] = p.w_scale[p.n + j + e];
+    } else if (p.bias) {
+      const T* bias = static_cast<const T*>(p.bias) + j;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) more[e] = Num<T>::to_f(bias[e]);
+    }
+    if (!kGlu && VEC && p.addend) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        if (row_of(it, 0) < p.rows) add[it] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.addend) + row_of(it, 0) * p.n + j);
+    }
+  }
+  float f[4][8];
+  tmem_wait_ld();
+  put_row(block, lane, r, sx);
+  __syncwarp();
+  get_values<VEC>(block, lane, f);
+  __syncwarp();
+  if (kGlu) {
+    tmem_ld32_issue(tgate, r);
+    tmem_wait_ld();
+    put_row(block, lane, r, sx);
+    __syncwarp();
+    float g[4][8];
+    get_values<VEC>(block, lane, g);
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[it][e] = gated_unit(g[it][e] * more[VEC ? e : 0], f[it][e] * s[VEC ? e : 0], p.glu);
+  } else {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      float a[8] = {};
+      if (VEC) {
+        unpack8<T>(add[it], a);
+      } else if (there && p.addend) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (row_of(it, e) < p.rows) a[e] = Num<T>::to_f(static_cast<const T*>(p.addend)[row_of(it, e) * p.n + j]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[it][e] = activate<ACT>(f[it][e] * s[VEC ? e : 0] + more[VEC ? e : 0]) + a[e];
+    }
+  }
+  if (there) {
+    T* y = static_cast<T*>(p.y) + j;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      if (VEC) {
+        if (row_of(it, 0) < p.rows) *reinterpret_cast<uint4*>(y + row_of(it, 0) * p.n) = pack8<T>(f[it]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (row_of(it, e) < p.rows) y[row_of(it, e) * p.n] = Num<T>::from_f(f[it][e]);
+      }
+    }
+  }
+}
+
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const E4m3Linear p, GemmGrid grid, int bn,
                  uint32_t stages) {
   constexpr bool kGlu = ACT == LRI_ACT_GLU;
@@ -189,7 +217,7 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full0 + 8 * a, 1);
-      mbar_init(acc_empty0 + 8 * a, 8);  // four warps of each CTA
+      mbar_init(acc_empty0 + 8 * a, 2 * kStoreWarps);  // of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -272,18 +300,30 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
   } else {
     const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id mod 4
-    const int i = quarter * 32 + lane;
+    const uint32_t block = base + stages * stage_bytes + (warp - 2) * kBlockBytes;
+    const bool vectors = (p.n & 7) == 0;
+    const int cols = kGlu ? half : bn;  // results of a tile for each row
     int it = 0;
     for (int item = pair; item < items; item += pairs, ++it) {
       const WorkItem w = work_item(item, grid);
       const uint32_t a = it & 1;
       const uint32_t use = static_cast<uint32_t>(it) >> 1;
+      const int64_t row0 = static_cast<int64_t>(w.tile_p) * 2 * kBM + rank * kBM + quarter * 32;
+      const float sx = row0 + lane < p.rows ? p.x_scale[row0 + lane] : 0.f;
       // the tcgen05.ld of the epilogue are warp-collective: the warp leaves together or not at all
       const bool ready = mbar_wait(acc_full0 + 8 * a, use & 1u, &abort_flag, 63, &g_e4m3_pair_status);
       if (!__all_sync(0xffffffffu, ready)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * kAccCols;
-      store_row<T, ACT>(p, static_cast<int64_t>(w.tile_p) * 2 * kBM + rank * kBM + i, w.tile_q, bn, tacc);
+#pragma unroll 1
+      for (int cc = (warp - 2) / 4 * 32; cc < cols; cc += kStoreWarps / 4 * 32) {
+        const int64_t j0 = static_cast<int64_t>(w.tile_q) * cols + cc;
+        if (j0 >= p.n || row0 >= p.rows) break;
+        if (vectors)
+          store_block<T, ACT, true>(p, row0, j0, sx, block, tacc + cc, tacc + half + cc);
+        else
+          store_block<T, ACT, false>(p, row0, j0, sx, block, tacc + cc, tacc + half + cc);
+      }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive_in_cluster(in_cta(acc_empty0 + 8 * a, 0));
@@ -305,11 +345,12 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 }
 
 // Width of the tile: a K step costs about bn + 64 columns' worth (see gemm_pair.cu), so the narrower tile wins where it fills the last round.
-int tile_width(int64_t rows, int64_t w_rows) {
+// (GLU: half a tile's columns in blocks of 32.)
+int tile_width(int64_t rows, int64_t w_rows, int by) {
   const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
   int best = kMaxBn;
   int64_t cost = 0;
-  for (int bn = kMaxBn; bn >= 64; bn -= 32) {
+  for (int bn = kMaxBn; bn >= 64; bn -= by) {
     const int64_t tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
     const int64_t c = (tiles + pairs - 1) / pairs * (bn + 64);
     if (bn == kMaxBn || c < cost) best = bn, cost = c;
@@ -321,7 +362,7 @@ template <typename T, int ACT>
 int launch(const E4m3Linear& p, cudaStream_t st) {
   constexpr bool kGlu = ACT == LRI_ACT_GLU;
   const int64_t w_rows = kGlu ? 2ll * p.n : p.n;
-  const int bn = tile_width(p.rows, w_rows);
+  const int bn = tile_width(p.rows, w_rows, kGlu ? 64 : 32);
   CUtensorMap tx, tw;
   int rc = make_tmap_e4m3(&tx, p.x, p.rows, p.k, p.x_ld, kBM);
   if (rc != LRI_OK) return rc;
@@ -331,7 +372,7 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
   static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
   LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
   const int stage_bytes = kTileBytes + bn / 2 * kStep;
-  int stages = (kSmemLimit - 1024) / stage_bytes;
+  int stages = (kSmemLimit - 1024 - kStoreWarps * kBlockBytes) / stage_bytes;
   stages = stages > kMaxStages ? kMaxStages : stages;
 
   const int64_t tiles_p = (static_cast<int64_t>(p.rows) + 2 * kBM - 1) / (2 * kBM);
@@ -348,8 +389,8 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
   const int64_t clusters = items < usable ? items : usable;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
-  cfg.blockDim = dim3(kGemmThreads);
-  const int smem = stages * stage_bytes + 1024;
+  cfg.blockDim = dim3(kThreads);
+  const int smem = stages * stage_bytes + 1024 + kStoreWarps * kBlockBytes;
   cfg.dynamicSmemBytes = static_cast<size_t>(smem > kOwnSmem ? smem : kOwnSmem);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];

@@ -23,8 +23,7 @@ struct RowsParams {
   float factor, eps;  // NORM: the residual's scale
 };
 
-constexpr int kRowThreads = 256;  // of a CTA when there are many rows
-constexpr int kFewRows = 148;     // up to here a row gets up to 1024 threads: the kernel is a latency chain
+constexpr int kFewRows = 148;  // up to here a row gets up to 1024 threads: the kernel is a latency chain
 
 // NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
 template <typename T, bool NORM, int NV, int THREADS>
@@ -51,13 +50,18 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   const uint4* a2 = NORM && p.add2 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add2) + row * p.cols) : nullptr;
   uint4* out = NORM && p.residual_out ? reinterpret_cast<uint4*>(static_cast<T*>(p.residual_out) + row * p.cols) : nullptr;
 
-  uint4 x[NV];
+  // everything is asked for before anything is looked at: the sums' place may be an input's, and no load passes a store to it
+  uint4 x[NV], a[NV], b[NV];
   float ss = 0.f;
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = threadIdx.x + i * THREADS;
-    if (v < nvec) x[i] = in[v];
+    if (v < nvec) {
+      x[i] = in[v];
+      if (a1) a[i] = a1[v];
+      if (a2) b[i] = a2[v];
+    }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -72,16 +76,16 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
         for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] * p.factor);
       }
       if (a1) {
-        float a[8];
-        unpack8<T>(a1[v], a);
+        float g[8];
+        unpack8<T>(a[i], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + a[e]);
+        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + g[e]);
       }
       if (a2) {
-        float a[8];
-        unpack8<T>(a2[v], a);
+        float g[8];
+        unpack8<T>(b[i], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + a[e]);
+        for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + g[e]);
       }
       x[i] = pack8<T>(f);
       if (out) out[v] = x[i];
@@ -141,19 +145,16 @@ int launch_nv(const RowsParams& p, int64_t rows, cudaStream_t st) {
 template <typename T, bool NORM>
 int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {
   const int nvec = p.cols / 8;
-  if (nvec <= 256) return launch_nv<T, NORM, 1, kRowThreads>(p, rows, st);
-  if (rows <= kFewRows || nvec > 8 * kRowThreads) {
-    if (nvec <= 512) return launch_nv<T, NORM, 1, 512>(p, rows, st);
-    if (nvec <= 1024) return launch_nv<T, NORM, 1, 1024>(p, rows, st);
-    if (nvec <= 2048) return launch_nv<T, NORM, 2, 1024>(p, rows, st);
-    if constexpr (!NORM) {
-      if (nvec <= 4096) return launch_nv<T, NORM, 4, 1024>(p, rows, st);
-      return launch_nv<T, NORM, 8, 1024>(p, rows, st);
-    }
+  const bool few = rows <= kFewRows;
+  if (nvec <= 256) return launch_nv<T, NORM, 1, 256>(p, rows, st);
+  if (nvec <= 512) return few ? launch_nv<T, NORM, 1, 512>(p, rows, st) : launch_nv<T, NORM, 2, 256>(p, rows, st);
+  if (nvec <= 1024) return few ? launch_nv<T, NORM, 1, 1024>(p, rows, st) : launch_nv<T, NORM, 2, 512>(p, rows, st);
+  if (nvec <= 2048) return launch_nv<T, NORM, 2, 1024>(p, rows, st);
+  if constexpr (!NORM) {
+    if (nvec <= 4096) return launch_nv<T, NORM, 4, 1024>(p, rows, st);
+    return launch_nv<T, NORM, 8, 1024>(p, rows, st);
   }
-  if (nvec <= 512) return launch_nv<T, NORM, 2, kRowThreads>(p, rows, st);
-  if (nvec <= 1024) return launch_nv<T, NORM, 4, kRowThreads>(p, rows, st);
-  return launch_nv<T, NORM, 8, kRowThreads>(p, rows, st);
+  return fail(LRI_ERR_UNSUPPORTED, "add_rmsnorm_e4m3: rows of %d elements", p.cols);
 }
 
 constexpr int kMostNormCols = 16384, kMostCols = 65536;
