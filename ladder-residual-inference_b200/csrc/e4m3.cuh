@@ -40,11 +40,23 @@ __device__ __forceinline__ float sigmoid_fast(float t) {
   return r;
 }
 
+// z * Phi(z), Phi the normal distribution: Phi(-x) = erfc(x / sqrt 2) / 2 for x >= 0 by Abramowitz and Stegun's 7.1.26, (a1 t + .. + a5 t^5) exp(-x^2 / 2)
+// / 2 with t = 1 / (1 + p x / sqrt 2), to 0.75e-7 (1.3 * 2^-24), and Phi(x) = 1 - Phi(-x).  (erff, which chooses between two ranges: 88 us
+// for 4096 x 4096 x 4096 with GELU.)
+__device__ __forceinline__ float gelu(float z) {
+  const float x = fabsf(z);
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(1.f + 0.3275911f * 0.70710678f * x));
+  const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * poly * exp2_approx(x * x * (-0.5f * 1.44269504f));
+  return z * (z > 0.f ? 1.f - tail : tail);
+}
+
 // Activations of a sum in fp32.  NaN stays NaN, which minima and maxima of floats would turn into a limit.
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if (ACT == LRI_ACT_SILU) return z * sigmoid_fast(z);
-  if (ACT == LRI_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if (ACT == LRI_ACT_GELU) return gelu(z);
   if (ACT == LRI_ACT_GELU_TANH) return z * sigmoid_fast(1.59576912f * (z + 0.044715f * z * z * z));  // (1 + tanh u) / 2 = sigmoid(2 u)
   return z;
 }
