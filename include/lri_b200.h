@@ -316,7 +316,11 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * lri_linear_e4m3: y[m, j] = act(x_scale[m] * w_scale[j] * sum_k x[m, k] w[j, k] + bias[j]) + addend[m, j], j < n.  bias [n], addend [rows, n]
  * may be NULL; addend may be y.  activation: LRI_ACT_*; GELU by the error function or by tanh.  LRI_ACT_GLU: w has 2 n rows [up | gate] and
  * w_scale 2 n scales, without bias and addend, and y = g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit), u = clamp(up, -limit, limit):
- * SwiGLU with alpha 1, limit infinity, offset 0. */
+ * SwiGLU with alpha 1, limit infinity, offset 0.
+ *
+ * lri_linear_e4m3 starts on its weights (w and w_scale, bias) while the kernel before it on the stream still runs, as the projections in 16 bits do.  So
+ * lri_quantize_rows_e4m3 and lri_add_rmsnorm_e4m3, whose results may be weights, let the next kernel start only when they are complete, unless `early`
+ * is not 0: for a caller whose next calls read the results as x, or not at all. */
 enum lri_activation { LRI_ACT_NONE = 0, LRI_ACT_SILU = 1, LRI_ACT_GELU = 2, LRI_ACT_GELU_TANH = 3, LRI_ACT_GLU = 4 };
 typedef struct {
   const void* x;
@@ -324,7 +328,7 @@ typedef struct {
   float* scale;
   lri_stream_t stream;
   int64_t rows, x_ld, codes_ld;
-  int dtype, cols;
+  int dtype, cols, early;
 } lri_quantize_e4m3_call;
 int lri_quantize_rows_e4m3(const lri_quantize_e4m3_call* call);
 typedef struct {
@@ -333,7 +337,7 @@ typedef struct {
   float* scale;
   lri_stream_t stream;
   int64_t rows, codes_ld;
-  int dtype, dim;
+  int dtype, dim, early;
   float residual_scale, eps;
 } lri_norm_e4m3_call;
 int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call);

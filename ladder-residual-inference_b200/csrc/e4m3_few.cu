@@ -2,9 +2,12 @@
 //
 // Bound by reading the weights once.  As in gemm_streamk.cu the weights are the 128-row operand of tcgen05.mma and the tokens its N side (16
 // to 128 wide).  What differs is how the work is spread and joined.  A tile of 128 outputs is one cluster's: its 1, 2, 4 or 8 CTAs take
-// equal runs of the depth, leave their fp32 sums in shared memory, and each of them joins its share of the tile's results out of the others'
-// (distributed shared memory) in the order of the ranks.  So a projection is one launch without a workspace, the sums do not
-// depend on when a CTA runs, and the epilogue's loads are spread over the cluster.
+// equal runs of the depth, and each joins the sums of its share of the tokens, four by four, in the order of the ranks.  So a projection is one
+// launch without a workspace, the sums do not depend on when a CTA runs, and the work behind the products is spread over the cluster.
+//
+// A sum travels once: a CTA that is through with its products says so to the others, and where all are (their rings are free) it stores
+// each sum into the shared memory of the CTA that joins it, which counts the bytes (st.async).  (Sums left in place, a cluster barrier, loads out of
+// the others' shared memory and a barrier at the end took 2.2 to 2.7 us behind the last product: the barrier alone 0.5.)
 //
 // Two CTAs fit an SM: with 96 to 108 KB of ring each, 200 KB of weights are under way per SM whichever the tile's share.
 //
@@ -31,7 +34,7 @@ struct Ring {
   static constexpr int kStageBytes = kTileBytes + BN * kStep;
   static constexpr int kStages = kRing / kStageBytes;
   static constexpr int kBytes = kStages * kStageBytes + 1024;
-  static_assert(kStages * kStageBytes >= BN * kBM * 4, "the sums of a tile take the ring's place");
+  static_assert(kStages * kStageBytes >= (BN < 4 * kMostSplit ? 4 * kMostSplit : BN) * kBM * 4, "the sums of a tile take the ring's place");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -39,12 +42,42 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank) {
-  uint32_t there;
-  float2 v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(there) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// four sums to a place in the cluster's shared memory, whose barrier counts the bytes
+__device__ __forceinline__ void send4(uint32_t to, uint32_t bar, const uint32_t* v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void ld_shared4(uint32_t from, float (&v)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from) : "memory");
+}
+// Relaxed: what the others may do after it is overwrite a ring whose last reads this thread has seen complete; there is nothing of its own to
+// publish.  (A release waits for the memory system, which is busy with weights: 0.7 to 1.1 us.)
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait for what other CTAs of the cluster have done
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code, int* status) {
+  for (uint32_t i = 0; i < kPollBudget; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 1023u) == 1023u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  atomicCAS(status, 0, code);
+  return false;
 }
 
 template <typename T, int ACT, int BN>
@@ -56,7 +89,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   constexpr uint32_t kCols = BN < 32 ? 32 : BN;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the same in every CTA of the cluster
-  __shared__ uint64_t bars[2 * kStages + 1];
+  __shared__ uint64_t bars[2 * kStages + 3];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -68,6 +101,9 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const int kt0 = steps * rank / split, kt1 = steps * (rank + 1) / split;  // (the host keeps split <= steps)
 
   const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[kStages]), done = smem_u32(&bars[2 * kStages]);
+  const uint32_t all_done = smem_u32(&bars[2 * kStages + 1]), landed = smem_u32(&bars[2 * kStages + 2]);
+  // this CTA joins the groups rank, rank + split, .. of four tokens
+  const int groups = (p.rows + 3) / 4, mine = (groups - rank + split - 1) / split;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < kStages; ++s) {
@@ -75,8 +111,11 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       mbar_init(empty0 + 8 * s, 1);
     }
     mbar_init(done, 1);
+    mbar_init(all_done, split);
+    mbar_init(landed, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mbar_expect_tx(landed, static_cast<uint32_t>(mine * split * kBM * 16));
   }
   __shared__ float row_scale[BN];
   if (warp == 1) {
@@ -87,10 +126,11 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's barriers exist (published by the fence above)
 
   // What joining the sums needs of memory is asked for at the start, and a part of the addend brought to the L2: behind the last product each of
   // these was a trip to memory of its own (64 rows of 8192 gated outputs from 2048: 11.7 us, NOW here).
-  constexpr int kPairs = kOut / 2, kGroups = kGemmThreads / kPairs;
+  constexpr int kPairs = kOut / 2, kAtOnce = kGemmThreads / kPairs;
   const int c = 2 * static_cast<int>(threadIdx.x % kPairs);
   const int64_t j = static_cast<int64_t>(tile) * kOut + c;
   const bool there = j < p.n, both = j + 1 < p.n, pairs_aligned = (p.n & 1) == 0;
@@ -104,7 +144,6 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       more = make_float2(Num<T>::to_f(bias[0]), both ? Num<T>::to_f(bias[1]) : 0.f);
     }
   }
-  const int t0 = p.rows * rank / split, t1 = p.rows * (rank + 1) / split;
 
   // warp-uniform loops, one elected lane issues (see gemm_pair.cu)
   if (warp == 0) {
@@ -162,99 +201,121 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (!kGlu && p.addend) {
       const char* add = reinterpret_cast<const char*>(static_cast<const T*>(p.addend) + static_cast<int64_t>(tile) * kOut);
       const int bytes = static_cast<int>(min(static_cast<int64_t>(kOut), p.n - static_cast<int64_t>(tile) * kOut)) * 2;
-      for (int q = i; q < 2 * (t1 - t0); q += 128) {
-        const int at = (q & 1) * 128;
-        if (at < bytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(add + static_cast<int64_t>(t0 + (q >> 1)) * p.n * 2 + at));
+      for (int q = i; q < 8 * mine; q += 128) {
+        const int at = (q & 1) * 128, tok = 4 * ((q >> 3) * split + rank) + (q >> 1 & 3);
+        if (at < bytes && tok < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(add + static_cast<int64_t>(tok) * p.n * 2 + at));
       }
     }
     const bool ok = mbar_wait(done, 0, &abort_flag, 73, &g_e4m3_few_status);
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers exist (long since)
     if (__all_sync(0xffffffffu, ok)) {
-      // every copy has landed and every product has read it: the ring's place is free for the sums, [token][output of the tile]
+      // every copy has landed and every product has read it: the ring's place is free, which the others are told
+      if (i < split) arrive_in_cluster(in_cta(all_done, i));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t to = base + (quarter * 32 + lane) * 4;
+      const bool free = mbar_wait_cluster(all_done, 0, &abort_flag, 74, &g_e4m3_few_status);
+      if (__all_sync(0xffffffffu, free)) {
+        // [group of the joining CTA][rank][output of the tile] of four tokens
+        const uint32_t to = base + (rank * kBM + quarter * 32 + lane) * 16;
 #pragma unroll
-      for (int cc = 0; cc < BN; cc += 16) {
-        uint32_t r[16];
-        tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
-        tmem_wait_ld();
+        for (int cc = 0; cc < BN; cc += 16) {
+          if (cc >= p.rows) break;
+          uint32_t r[16];
+          tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
+          tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + (cc + e) * kBM * 4), "r"(r[e]) : "memory");
+          for (int e = 0; e < 16; e += 4) {
+            const int group = (cc + e) / 4, owner = group & (split - 1);
+            if (group < groups) send4(in_cta(to + (group - owner) * kBM * 16, owner), in_cta(landed, owner), r + e);
+          }
+        }
       }
     }
   }
+  if (warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kCols) : "memory");
   }
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-  // ---- join: this CTA's share of the tokens, a thread for a pair of outputs ---------------------------------------------------------
-  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (!abort_flag) {
-    // two tokens at a time: their loads out of the cluster's shared memory are under way together
-    for (int t = t0 + static_cast<int>(threadIdx.x / kPairs); there && t < t1; t += 2 * kGroups) {
-      float2 v[2], g[2], add[2];
-      float sx[2];
-      uint32_t from[2];
+  // ---- join: a thread for a pair of outputs and four tokens -------------------------------------------------------------------------
+  bool waited = false, ok = !abort_flag;
+  for (int g = static_cast<int>(threadIdx.x / kPairs); there && ok && g < mine; g += kAtOnce) {
+    const int tok0 = 4 * (g * split + rank);
+    T* y = static_cast<T*>(p.y) + static_cast<int64_t>(tok0) * p.n + j;
+    // (without branches around what has to be waited for: one after the other these loads took 1.5 us)
+    uint32_t add[4] = {};
+    if (!kGlu && p.addend) {
+      const uint16_t* from = static_cast<const uint16_t*>(p.addend) + static_cast<int64_t>(tok0) * p.n + j;
+      if (pairs_aligned) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int tok = t + u * kGroups < t1 ? t + u * kGroups : t;
-        from[u] = base + (tok * kBM + c) * 4;
-        sx[u] = row_scale[tok];
-        add[u] = make_float2(0.f, 0.f);
-        if (!kGlu && p.addend) {
-          const T* a = static_cast<const T*>(p.addend) + static_cast<int64_t>(tok) * p.n + j;
-          add[u] = make_float2(Num<T>::to_f(a[0]), both ? Num<T>::to_f(a[1]) : 0.f);
+        for (int u = 0; u < 4; ++u)
+          if (tok0 + u < p.rows) add[u] = *reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(u) * p.n);
+      } else {
+        uint16_t lo[4] = {}, hi[4] = {};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (tok0 + u < p.rows) lo[u] = from[static_cast<int64_t>(u) * p.n];
+          if (tok0 + u < p.rows && both) hi[u] = from[static_cast<int64_t>(u) * p.n + 1];
         }
-        v[u] = g[u] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) add[u] = lo[u] | static_cast<uint32_t>(hi[u]) << 16;
       }
-      float2 part[kMostSplit][2], gate[kGlu ? kMostSplit : 1][2];
+    }
+    if (!waited) ok = mbar_wait_cluster(landed, 0, &abort_flag, 75, &g_e4m3_few_status), waited = true;
+    const uint32_t from = base + (g * split * kBM + c) * 16;
+    float v[2][4] = {}, w[kGlu ? 2 : 1][4] = {};
+    for (int z = 0; z < split; ++z) {
 #pragma unroll
-      for (int z = 0; z < kMostSplit; ++z)
-        if (z < split) {
+      for (int h = 0; h < 2; ++h) {
+        float a[4];
+        ld_shared4(from + (z * kBM + h) * 16, a);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            part[z][u] = ld_cluster2(from[u], z);
-            if (kGlu) gate[kGlu ? z : 0][u] = ld_cluster2(from[u] + kOut * 4, z);
-          }
-        }
-#pragma unroll
-      for (int z = 0; z < kMostSplit; ++z)
-        if (z < split) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            v[u].x += part[z][u].x, v[u].y += part[z][u].y;
-            if (kGlu) g[u].x += gate[kGlu ? z : 0][u].x, g[u].y += gate[kGlu ? z : 0][u].y;
-          }
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int tok = t + u * kGroups;
-        if (tok >= t1) continue;
-        float a0 = v[u].x * sx[u] * s.x, a1 = v[u].y * sx[u] * s.y;
+        for (int u = 0; u < 4; ++u) v[h][u] += a[u];
         if (kGlu) {
-          a0 = gated_unit(g[u].x * sx[u] * more.x, a0, p.glu);
-          a1 = gated_unit(g[u].y * sx[u] * more.y, a1, p.glu);
-        } else {
-          a0 = activate<ACT>(a0 + more.x) + add[u].x;
-          a1 = activate<ACT>(a1 + more.y) + add[u].y;
-        }
-        T* y = static_cast<T*>(p.y) + static_cast<int64_t>(tok) * p.n + j;
-        if (pairs_aligned) {
-          *reinterpret_cast<uint32_t*>(y) = pack2<T>(a0, a1);
-        } else {
-          y[0] = Num<T>::from_f(a0);
-          if (both) y[1] = Num<T>::from_f(a1);
+          ld_shared4(from + (z * kBM + kOut + h) * 16, a);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[kGlu ? h : 0][u] += a[u];
         }
       }
     }
-  } else if (threadIdx.x == 0) {
-    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
+    float out[4][2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float sx = row_scale[tok0 + u];  // (behind the last row: anything, and not stored)
+      float a0 = v[0][u] * sx * s.x, a1 = v[1][u] * sx * s.y;
+      if (kGlu) {
+        a0 = gated_unit(w[0][u] * sx * more.x, a0, p.glu);
+        a1 = gated_unit(w[kGlu ? 1 : 0][u] * sx * more.y, a1, p.glu);
+      } else {
+        float b0, b1;
+        Num<T>::unpack2(add[u], b0, b1);
+        a0 = activate<ACT>(a0 + more.x) + b0;
+        a1 = activate<ACT>(a1 + more.y) + b1;
+      }
+      out[u][0] = a0, out[u][1] = a1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (tok0 + u >= p.rows) continue;
+      if (pairs_aligned) {
+        *reinterpret_cast<uint32_t*>(y + static_cast<int64_t>(u) * p.n) = pack2<T>(out[u][0], out[u][1]);
+      } else {
+        y[static_cast<int64_t>(u) * p.n] = Num<T>::from_f(out[u][0]);
+        if (both) y[static_cast<int64_t>(u) * p.n + 1] = Num<T>::from_f(out[u][1]);
+      }
+    }
   }
-  // nobody leaves while the others read its sums
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // A CTA that has got all its sums is nobody's target any more: those who send have arrived at its barrier before.  One that gave up stays until the
+  // others have left or given up too, and gives copies in flight time to land.
+  __syncthreads();
+  if (abort_flag) {
+    if (threadIdx.x == 0)
+      for (int i = 0; i < 2000; ++i) __nanosleep(100);
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
 }
 
 // CTAs of a tile: as many as fill the places that two CTAs an SM give, with four steps (64 KB of weights) or more for each.

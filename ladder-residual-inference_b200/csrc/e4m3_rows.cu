@@ -21,6 +21,7 @@ struct RowsParams {
   int64_t x_ld, codes_ld;
   int cols;
   float factor, eps;  // NORM: the residual's scale
+  bool early;         // the next kernel may start: it waits for this one before it reads the results
 };
 
 constexpr int kFewRows = 148;  // up to here a row gets up to 1024 threads: the kernel is a latency chain
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
       if (v < nvec) w[i] = __ldg(static_cast<const uint4*>(p.weight) + v);
     }
   }
-  pdl_launch_dependents();
+  if (p.early) pdl_launch_dependents();
   pdl_wait();
   const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_ld);
   const uint4* a1 = NORM && p.add1 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add1) + row * p.cols) : nullptr;
@@ -187,7 +188,7 @@ extern "C" int lri_quantize_rows_e4m3(const lri_quantize_e4m3_call* call) {
   LRI_REQUIRE(!overlap(c.codes, codes_bytes, c.x, x_bytes) && !overlap(c.scale, scale_bytes, c.x, x_bytes) &&
                   !overlap(c.scale, scale_bytes, c.codes, codes_bytes), LRI_ERR_ARG, "quantize_rows_e4m3: results overlap each other or x");
   RowsParams p{};
-  p.x = c.x, p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.x_ld, p.codes_ld = c.codes_ld, p.cols = c.cols;
+  p.x = c.x, p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.x_ld, p.codes_ld = c.codes_ld, p.cols = c.cols, p.early = c.early != 0;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, false>(p, c.rows, st) : launch<__half, false>(p, c.rows, st);
 }
@@ -218,7 +219,7 @@ extern "C" int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call) {
   RowsParams p{};
   p.x = c.residual, p.add1 = c.add1, p.add2 = c.add2, p.weight = c.weight, p.residual_out = c.residual_out;
   p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.dim, p.codes_ld = c.codes_ld, p.cols = c.dim;
-  p.factor = c.residual_scale, p.eps = c.eps;
+  p.factor = c.residual_scale, p.eps = c.eps, p.early = c.early != 0;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, true>(p, c.rows, st) : launch<__half, true>(p, c.rows, st);
 }

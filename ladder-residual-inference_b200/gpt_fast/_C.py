@@ -36,8 +36,8 @@ class LlamaPass(ctypes.Structure):
 STORE_CALL = struct.Struct("@11Q5q12i")  # lri_paged_store_call
 ATTN_CALL = struct.Struct("@10Q4q9if")   # lri_paged_attn_call
 LOAD_CALL = struct.Struct("@9Q3q8i")     # lri_paged_load_call
-QUANTIZE_CALL = struct.Struct("@4Q3q2i")   # lri_quantize_e4m3_call
-NORM8_CALL = struct.Struct("@8Q2q2i2f")    # lri_norm_e4m3_call
+QUANTIZE_CALL = struct.Struct("@4Q3q3i0Q")   # lri_quantize_e4m3_call
+NORM8_CALL = struct.Struct("@8Q2q3i2f0Q")    # lri_norm_e4m3_call
 LINEAR8_CALL = struct.Struct("@8Q3q4i3f0Q")  # lri_linear_e4m3_call
 
 ONE_SM = 0x100  # LRI_ONE_SM

@@ -49,9 +49,9 @@ def _check_dense(what, t, dtype, shape):
         raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)}, not {_said(t)}")
 
 
-def quantize_rows(x: Tensor, out: Optional[Rows] = None) -> Rows:
+def quantize_rows(x: Tensor, out: Optional[Rows] = None, early: bool = False) -> Rows:
     """Rows of x [rows, cols] (bfloat16 or float16; rows may lie apart, as parts of a wider buffer) as codes and scales; cols a multiple of 8
-    up to 65536."""
+    up to 65536.  early: the projection that follows may start on its weights before these rows are complete; not for rows that are themselves its weights."""
     shape = x.shape
     if not (x.dtype in _WIDE and len(shape) == 2 and shape[1] % 8 == 0 and 0 < shape[1] <= 65536 and x.stride(1) == 1 and
             (shape[0] <= 1 or x.stride(0) % 8 == 0 and x.stride(0) >= shape[1])):
@@ -60,14 +60,14 @@ def quantize_rows(x: Tensor, out: Optional[Rows] = None) -> Rows:
         out = empty_rows(*shape, x.device)
     else:
         _check_rows("out", out, shape)
-    CudaOps.quantize_rows_e4m3(x, *out, shape)
+    CudaOps.quantize_rows_e4m3(x, *out, shape, early)
     return out
 
 
 def add_rmsnorm(residual: Tensor, weight: Tensor, eps: float, add1: Optional[Tensor] = None, add2: Optional[Tensor] = None, residual_scale: float = 1.0,
-                residual_out: Optional[Tensor] = None, out: Optional[Rows] = None) -> Rows:
+                residual_out: Optional[Tensor] = None, out: Optional[Rows] = None, early: bool = False) -> Rows:
     """round(round(residual * residual_scale) + add1) + add2 to residual_out (None: not kept; may be residual), each sum rounded to the residual's
-    type, and RMSNorm of that times weight as codes and scales.  residual, add1, add2 [rows, dim]; dim a multiple of 8 up to 16384."""
+    type, and RMSNorm of that times weight as codes and scales.  residual, add1, add2 [rows, dim]; dim a multiple of 8 up to 16384.  early: as in quantize_rows."""
     shape, dtype = residual.shape, residual.dtype
     if not (dtype in _WIDE and len(shape) == 2 and shape[1] % 8 == 0 and 0 < shape[1] <= 16384 and residual.is_contiguous()):
         raise ValueError(f"residual: contiguous bfloat16 or float16 rows of a multiple of 8 elements up to 16384, not {_said(residual)}")
@@ -82,7 +82,7 @@ def add_rmsnorm(residual: Tensor, weight: Tensor, eps: float, add1: Optional[Ten
         out = empty_rows(*shape, residual.device)
     else:
         _check_rows("out", out, shape)
-    CudaOps.add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, *out, shape[0], residual_scale)
+    CudaOps.add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, *out, shape[0], residual_scale, early)
     return out
 
 

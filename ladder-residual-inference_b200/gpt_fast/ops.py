@@ -200,19 +200,20 @@ class CudaOps:
     # ---- projections in 8 bits ----------------------------------------------------------------------
     # (codes, scale) pairs as gpt_fast.e4m3 checks them.  As above, the pitch of a single row may be any number.
     @staticmethod
-    def quantize_rows_e4m3(x, codes, scale, shape):
+    def quantize_rows_e4m3(x, codes, scale, shape, early=False):
+        """early: what follows on the stream reads the rows as the x of a projection, or not at all (include/lri_b200.h)."""
         here = x.get_device()
         if not 0 <= here == torch._C._cuda_getDevice() == codes.get_device() == scale.get_device():
             _C.refuse_devices(x, codes, scale)
         rows, cols = shape
         status = _C.lib.lri_quantize_rows_e4m3(_C.QUANTIZE_CALL.pack(
             x.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x.stride(0) if rows > 1 else cols,
-            codes.stride(0) if rows > 1 else -(-cols // 16) * 16, _C.CODES[x.dtype], cols))
+            codes.stride(0) if rows > 1 else -(-cols // 16) * 16, _C.CODES[x.dtype], cols, early))
         if status < 0:
             _C.check(status)
 
     @staticmethod
-    def add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, codes, scale, rows, residual_scale=1.0):
+    def add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, codes, scale, rows, residual_scale=1.0, early=False):
         here = residual.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == weight.get_device() == codes.get_device() == scale.get_device() and
                 (add1 is None or add1.get_device() == here) and (add2 is None or add2.get_device() == here) and
@@ -222,7 +223,7 @@ class CudaOps:
         status = _C.lib.lri_add_rmsnorm_e4m3(_C.NORM8_CALL.pack(
             residual.data_ptr(), 0 if add1 is None else add1.data_ptr(), 0 if add2 is None else add2.data_ptr(), weight.data_ptr(),
             0 if residual_out is None else residual_out.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows,
-            codes.stride(0) if rows > 1 else -(-dim // 16) * 16, _C.CODES[residual.dtype], dim, residual_scale, eps))
+            codes.stride(0) if rows > 1 else -(-dim // 16) * 16, _C.CODES[residual.dtype], dim, early, residual_scale, eps))
         if status < 0:
             _C.check(status)
 

@@ -97,11 +97,11 @@ def _refused(entry, packed, text):
 
 
 def _quantize(x=_AT, codes=2 * _AT, scale=3 * _AT, rows=4, x_ld=64, codes_ld=64, dtype=0, cols=64):
-    return _C.QUANTIZE_CALL.pack(x, codes, scale, 0, rows, x_ld, codes_ld, dtype, cols)
+    return _C.QUANTIZE_CALL.pack(x, codes, scale, 0, rows, x_ld, codes_ld, dtype, cols, 0)
 
 
 def _norm(residual=_AT, add1=0, add2=0, weight=2 * _AT, kept=0, codes=3 * _AT, scale=4 * _AT, rows=4, codes_ld=64, dtype=0, dim=64):
-    return _C.NORM8_CALL.pack(residual, add1, add2, weight, kept, codes, scale, 0, rows, codes_ld, dtype, dim, 1.0, 1e-5)
+    return _C.NORM8_CALL.pack(residual, add1, add2, weight, kept, codes, scale, 0, rows, codes_ld, dtype, dim, 0, 1.0, 1e-5)
 
 
 def _linear(x=_AT, w=2 * _AT, xs=3 * _AT, ws=4 * _AT, bias=0, addend=0, y=5 * _AT, rows=4, x_ld=64, w_ld=64, dtype=0, n=16, k=64, act=0, limit=7.0):
@@ -142,5 +142,5 @@ def test_no_call_and_no_rows(entry):
 
 
 def test_structs_have_the_sizes_of_the_header():
-    assert _C.QUANTIZE_CALL.size == 64 and _C.NORM8_CALL.size == 96 and _C.LINEAR8_CALL.size == 120
+    assert _C.QUANTIZE_CALL.size == 72 and _C.NORM8_CALL.size == 104 and _C.LINEAR8_CALL.size == 120
     assert ctypes.sizeof(ctypes.c_void_p) == 8

@@ -190,3 +190,22 @@ def test_zero_rows_and_zero_weights(e4m3, rows):
     assert (e4m3.linear(x, w)[0] == 0).all()
     none = e4m3.linear((x[0][:0], x[1][:0]), w)
     assert none.shape == (0, 96)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_weights_of_the_call_before(e4m3, rows):
+    """A projection starts on its weights before the kernel in front of it is complete; the rows that the operators store may be weights all the same."""
+    x = random_rows(rows, 4096, 1)
+    w = torch.randn(512, 4096, dtype=torch.bfloat16, device="cuda")
+    add = torch.randn_like(w)
+    ones = torch.ones(4096, dtype=torch.bfloat16, device="cuda")
+    codes, scale = e4m3.empty_rows(512, 4096, "cuda")
+    for turn in range(20):
+        _raw(codes).fill_(0x7F)
+        scale.fill_(math.nan)
+        if turn % 2:
+            e4m3.quantize_rows(w, out=(codes, scale))
+        else:
+            e4m3.add_rmsnorm(w, ones, 1e-5, add1=add, out=(codes, scale))
+        y = e4m3.linear(x, (codes, scale))
+        check(y, *linear64(x, (codes, scale)))
