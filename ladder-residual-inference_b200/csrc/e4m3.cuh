@@ -66,9 +66,11 @@ __device__ __forceinline__ float gated_unit(float gate, float up, const GluParam
   return g * sigmoid_fast(p.alpha * g) * (u + p.offset);
 }
 
-// activation: lri_activation.  One (e4m3_few.cu) for up to kE4m3FewRows rows, the other (e4m3_pair.cu) for any number.
-constexpr int kE4m3FewRows = 128;
+// The two kernels (e4m3_few.cu, e4m3_pair.cu); both take any number of rows.  _fetched: the bytes that the busiest SM would fetch (few: with more than
+// 32 rows; pair: with the width of tile that it says).
+int64_t e4m3_few_fetched(int activation, const E4m3Linear& p);
 int e4m3_few_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
-int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st);
+int64_t e4m3_pair_fetched(int activation, const E4m3Linear& p, int* width);
+int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, int width, cudaStream_t st);
 
 }  // namespace lri

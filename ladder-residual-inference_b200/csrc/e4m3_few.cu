@@ -1,13 +1,14 @@
 // Projections in 8 bits of few rows (up to kE4m3FewRows tokens): a decode step of a batch, a short prompt.
 //
 // Bound by reading the weights once.  As in gemm_streamk.cu the weights are the 128-row operand of tcgen05.mma and the tokens its N side (16
-// to 128 wide).  What differs is how the work is spread and joined.  A tile of 128 outputs is one cluster's: its 1, 2, 4 or 8 CTAs take
+// to 64 wide, in as many tiles as there are).  What differs is how the work is spread and joined.  A tile of 128 outputs is one cluster's: its 1, 2, 4 or 8 CTAs take
 // equal runs of the depth, and each joins the sums of its share of the tokens, four by four, in the order of the ranks.  So a projection is one
 // launch without a workspace, the sums do not depend on when a CTA runs, and the work behind the products is spread over the cluster.
 //
-// A sum travels once: a CTA that is through with its products says so to the others, and where all are (their rings are free) it stores
-// each sum into the shared memory of the CTA that joins it, which counts the bytes (st.async).  (Sums left in place, a cluster barrier, loads out of
-// the others' shared memory and a barrier at the end took 2.2 to 2.7 us behind the last product: the barrier alone 0.5.)
+// A sum travels once: a CTA that is through with its products says so to the others and lays its sums out in its ring, and where all are
+// through (their rings are free too) it copies each block of them, 128 outputs x 4 tokens, into the shared memory of the CTA that joins it, whose barrier
+// counts the bytes.  (Sums left in place, a cluster barrier, loads out of the others' shared memory and a barrier at the end took 2.2 to
+// 2.7 us behind the last product, the barrier alone 0.5; stores that count their own bytes, 16 at a time, take 1 ns each: 2 us for 64 rows.)
 //
 // Two CTAs fit an SM: with 96 to 108 KB of ring each, 200 KB of weights are under way per SM whichever the tile's share.
 //
@@ -15,7 +16,7 @@
 //
 // Warp roles: warp 0 fetches (TMA; the weights of the first stages before the preceding kernel is complete, since it does not write
 // them), warp 1 owns the tensor memory and issues the products, warps 2-5 take the sums out of tensor memory; all warps join.  Every wait on
-// an mbarrier is bounded (lri_gemm_status); every CTA reaches the cluster barriers in every case.
+// an mbarrier is bounded (lri_gemm_status); every CTA reaches the two cluster barriers in every case.
 #include "e4m3_tc.cuh"
 
 namespace lri {
@@ -27,14 +28,18 @@ __device__ int g_e4m3_few_status = 0;
 
 constexpr int kTileBytes = kBM * kStep;  // of 128 weight rows
 constexpr int kMostSplit = 8;
+
 constexpr int kRing = 108 * 1024;  // of a CTA, two of which share an SM
+constexpr int kBlockBytes = kBM * 16;  // sums of 128 outputs x 4 tokens
 
 template <int BN>
 struct Ring {
   static constexpr int kStageBytes = kTileBytes + BN * kStep;
   static constexpr int kStages = kRing / kStageBytes;
   static constexpr int kBytes = kStages * kStageBytes + 1024;
-  static_assert(kStages * kStageBytes >= (BN < 4 * kMostSplit ? 4 * kMostSplit : BN) * kBM * 4, "the sums of a tile take the ring's place");
+  // what takes the ring's place: a CTA's own sums, and in front of the joining the others' of its groups (fewer than BN / 4 + kMostSplit)
+  static constexpr int kOwn = BN / 4 * kBlockBytes;
+  static_assert(kStages * kStageBytes >= kOwn + (BN / 4 + kMostSplit) * kBlockBytes, "sums in the ring's place");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -47,10 +52,9 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// four sums to a place in the cluster's shared memory, whose barrier counts the bytes
-__device__ __forceinline__ void send4(uint32_t to, uint32_t bar, const uint32_t* v) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(bar)
+// from this CTA's shared memory to another's of the cluster, whose barrier counts the bytes
+__device__ __forceinline__ void send(uint32_t to, uint32_t bar, uint32_t from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "r"(from), "r"(bytes), "r"(bar)
                : "memory");
 }
 __device__ __forceinline__ void ld_shared4(uint32_t from, float (&v)[4]) {
@@ -96,14 +100,14 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int rank = split == 1 ? 0 : static_cast<int>(cluster_rank());
-  const int tile = blockIdx.x / split;
+  const int tile = blockIdx.x / split, row0 = blockIdx.y * BN, rows = min(BN, p.rows - row0);
   const int steps = (p.k + kStep - 1) / kStep;
   const int kt0 = steps * rank / split, kt1 = steps * (rank + 1) / split;  // (the host keeps split <= steps)
 
   const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[kStages]), done = smem_u32(&bars[2 * kStages]);
   const uint32_t all_done = smem_u32(&bars[2 * kStages + 1]), landed = smem_u32(&bars[2 * kStages + 2]);
   // this CTA joins the groups rank, rank + split, .. of four tokens
-  const int groups = (p.rows + 3) / 4, mine = (groups - rank + split - 1) / split;
+  const int groups = (rows + 3) / 4, mine = (groups - rank + split - 1) / split;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < kStages; ++s) {
@@ -115,7 +119,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     mbar_init(landed, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mbar_expect_tx(landed, static_cast<uint32_t>(mine * split * kBM * 16));
+    mbar_expect_tx(landed, static_cast<uint32_t>(mine * (split - 1) * kBlockBytes));
   }
   __shared__ float row_scale[BN];
   if (warp == 1) {
@@ -153,7 +157,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       tma_load_2d(dst, &tmap_w, full0 + 8 * s, kt * kStep, tile * kOut);
       if (kGlu) tma_load_2d(dst + kTileBytes / 2, &tmap_w, full0 + 8 * s, kt * kStep, p.n + tile * kOut);
     };
-    auto fetch_rows = [&](uint32_t s, int kt) { tma_load_2d(base + s * kStageBytes + kTileBytes, &tmap_x, full0 + 8 * s, kt * kStep, 0); };
+    auto fetch_rows = [&](uint32_t s, int kt) { tma_load_2d(base + s * kStageBytes + kTileBytes, &tmap_x, full0 + 8 * s, kt * kStep, row0); };
     const int ahead = min(static_cast<int>(kStages), kt1 - kt0);
     for (int i = 0; i < ahead; ++i)
       if (elect_one()) fetch_weights(i, kt0 + i);
@@ -197,37 +201,41 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     pdl_wait();
     pdl_launch_dependents();
     const int quarter = warp & 3, i = static_cast<int>(threadIdx.x) - 64;
-    if (i < p.rows && i < BN) row_scale[i] = p.x_scale[i];
+    if (i < rows) row_scale[i] = p.x_scale[row0 + i];
     if (!kGlu && p.addend) {
-      const char* add = reinterpret_cast<const char*>(static_cast<const T*>(p.addend) + static_cast<int64_t>(tile) * kOut);
+      const char* add = reinterpret_cast<const char*>(static_cast<const T*>(p.addend) + static_cast<int64_t>(row0) * p.n + static_cast<int64_t>(tile) * kOut);
       const int bytes = static_cast<int>(min(static_cast<int64_t>(kOut), p.n - static_cast<int64_t>(tile) * kOut)) * 2;
       for (int q = i; q < 8 * mine; q += 128) {
         const int at = (q & 1) * 128, tok = 4 * ((q >> 3) * split + rank) + (q >> 1 & 3);
-        if (at < bytes && tok < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(add + static_cast<int64_t>(tok) * p.n * 2 + at));
+        if (at < bytes && tok < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(add + static_cast<int64_t>(tok) * p.n * 2 + at));
       }
     }
     const bool ok = mbar_wait(done, 0, &abort_flag, 73, &g_e4m3_few_status);
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers exist (long since)
     if (__all_sync(0xffffffffu, ok)) {
       // every copy has landed and every product has read it: the ring's place is free, which the others are told
-      if (i < split) arrive_in_cluster(in_cta(all_done, i));
+      if (split > 1 && i < split) arrive_in_cluster(in_cta(all_done, i));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const bool free = mbar_wait_cluster(all_done, 0, &abort_flag, 74, &g_e4m3_few_status);
-      if (__all_sync(0xffffffffu, free)) {
-        // [group of the joining CTA][rank][output of the tile] of four tokens
-        const uint32_t to = base + (rank * kBM + quarter * 32 + lane) * 16;
+      const uint32_t to = base + (quarter * 32 + lane) * 16;  // [group][output of the tile] of four tokens
 #pragma unroll
-        for (int cc = 0; cc < BN; cc += 16) {
-          if (cc >= p.rows) break;
-          uint32_t r[16];
-          tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
-          tmem_wait_ld();
+      for (int cc = 0; cc < BN; cc += 16) {
+        if (cc >= rows) break;
+        uint32_t r[16];
+        tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
+        tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const int group = (cc + e) / 4, owner = group & (split - 1);
-            if (group < groups) send4(in_cta(to + (group - owner) * kBM * 16, owner), in_cta(landed, owner), r + e);
-          }
-        }
+        for (int e = 0; e < 16; e += 4)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (cc + e) / 4 * kBlockBytes), "r"(r[e]), "r"(r[e + 1]), "r"(r[e + 2]), "r"(r[e + 3]) : "memory");
+      }
+    }
+    if (split > 1) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      // block `i` to its CTA, behind the ring's part for own sums: [group of the joining CTA][other ranks in order]
+      const int owner = i & (split - 1);
+      if (ok && i < groups && owner != rank && mbar_wait_cluster(all_done, 0, &abort_flag, 74, &g_e4m3_few_status)) {
+        const int slot = (i - owner) / split * (split - 1) + (rank < owner ? rank : rank - 1);
+        send(in_cta(base + Ring<BN>::kOwn + slot * kBlockBytes, owner), in_cta(landed, owner), base + i * kBlockBytes, kBlockBytes);
       }
     }
   }
@@ -240,41 +248,50 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   }
 
   // ---- join: a thread for a pair of outputs and four tokens -------------------------------------------------------------------------
-  bool waited = false, ok = !abort_flag;
-  for (int g = static_cast<int>(threadIdx.x / kPairs); there && ok && g < mine; g += kAtOnce) {
+  int g = static_cast<int>(threadIdx.x / kPairs);
+  uint32_t add[4] = {};
+  // (without branches around what has to be waited for: one after the other these loads took 1.5 us)
+  auto load_addend = [&]() {
+    if (kGlu || !p.addend || !there || g >= mine) return;
     const int tok0 = 4 * (g * split + rank);
-    T* y = static_cast<T*>(p.y) + static_cast<int64_t>(tok0) * p.n + j;
-    // (without branches around what has to be waited for: one after the other these loads took 1.5 us)
-    uint32_t add[4] = {};
-    if (!kGlu && p.addend) {
-      const uint16_t* from = static_cast<const uint16_t*>(p.addend) + static_cast<int64_t>(tok0) * p.n + j;
-      if (pairs_aligned) {
+    const uint16_t* from = static_cast<const uint16_t*>(p.addend) + static_cast<int64_t>(row0 + tok0) * p.n + j;
+    if (pairs_aligned) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (tok0 + u < p.rows) add[u] = *reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(u) * p.n);
-      } else {
-        uint16_t lo[4] = {}, hi[4] = {};
+      for (int u = 0; u < 4; ++u)
+        if (tok0 + u < rows) add[u] = *reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(u) * p.n);
+    } else {
+      uint16_t lo[4] = {}, hi[4] = {};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (tok0 + u < p.rows) lo[u] = from[static_cast<int64_t>(u) * p.n];
-          if (tok0 + u < p.rows && both) hi[u] = from[static_cast<int64_t>(u) * p.n + 1];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add[u] = lo[u] | static_cast<uint32_t>(hi[u]) << 16;
+      for (int u = 0; u < 4; ++u) {
+        if (tok0 + u < rows) lo[u] = from[static_cast<int64_t>(u) * p.n];
+        if (tok0 + u < rows && both) hi[u] = from[static_cast<int64_t>(u) * p.n + 1];
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add[u] = lo[u] | static_cast<uint32_t>(hi[u]) << 16;
     }
-    if (!waited) ok = mbar_wait_cluster(landed, 0, &abort_flag, 75, &g_e4m3_few_status), waited = true;
-    const uint32_t from = base + (g * split * kBM + c) * 16;
+  };
+  load_addend();
+  bool ok = !abort_flag;
+  if (split > 1) {
+    ok = mbar_wait_cluster(landed, 0, &abort_flag, 75, &g_e4m3_few_status) && ok;
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // nothing is copied into this CTA any more
+  }
+  for (; there && ok && g < mine; g += kAtOnce, load_addend()) {
+    const int tok0 = 4 * (g * split + rank);
+    T* y = static_cast<T*>(p.y) + static_cast<int64_t>(row0 + tok0) * p.n + j;
     float v[2][4] = {}, w[kGlu ? 2 : 1][4] = {};
     for (int z = 0; z < split; ++z) {
+      const uint32_t from = base + c * 16 + (z == rank ? (g * split + rank) * kBlockBytes
+                                                       : Ring<BN>::kOwn + (g * (split - 1) + (z < rank ? z : z - 1)) * kBlockBytes);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float a[4];
-        ld_shared4(from + (z * kBM + h) * 16, a);
+        ld_shared4(from + h * 16, a);
 #pragma unroll
         for (int u = 0; u < 4; ++u) v[h][u] += a[u];
         if (kGlu) {
-          ld_shared4(from + (z * kBM + kOut + h) * 16, a);
+          ld_shared4(from + (kOut + h) * 16, a);
 #pragma unroll
           for (int u = 0; u < 4; ++u) w[kGlu ? h : 0][u] += a[u];
         }
@@ -298,7 +315,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (tok0 + u >= p.rows) continue;
+      if (tok0 + u >= rows) continue;
       if (pairs_aligned) {
         *reinterpret_cast<uint32_t*>(y + static_cast<int64_t>(u) * p.n) = pack2<T>(out[u][0], out[u][1]);
       } else {
@@ -307,19 +324,16 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       }
     }
   }
-  // A CTA that has got all its sums is nobody's target any more: those who send have arrived at its barrier before.  One that gave up stays until the
-  // others have left or given up too, and gives copies in flight time to land.
-  __syncthreads();
-  if (abort_flag) {
-    if (threadIdx.x == 0)
-      for (int i = 0; i < 2000; ++i) __nanosleep(100);
-    __syncthreads();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (abort_flag && threadIdx.x == 0) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
   }
+  // what is copied out of this CTA has been copied once all the others have theirs
+  __syncwarp();
+  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// CTAs of a tile: as many as fill the places that two CTAs an SM give, with four steps (64 KB of weights) or more for each.
-int split_of(int tiles, int steps) {
+// CTAs of a tile: as many as there are places for, with four steps (64 KB of weights) or more for each.
+int split_of(int64_t tiles, int steps) {
   int split = 1;
   while (split < kMostSplit && tiles * split * 2 <= 2 * sm_count() && steps >= 4 * split * 2) split *= 2;
   return split;
@@ -337,9 +351,10 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
   auto kern = e4m3_few_kernel<T, ACT, BN>;
   static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
   LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<BN>::kBytes));
-  const int tiles = (p.n + kOut - 1) / kOut, split = split_of(tiles, (p.k + kStep - 1) / kStep);
+  const int tiles = (p.n + kOut - 1) / kOut, row_tiles = (p.rows + BN - 1) / BN;
+  const int split = split_of(static_cast<int64_t>(tiles) * row_tiles, (p.k + kStep - 1) / kStep);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split);
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split, static_cast<unsigned>(row_tiles));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = Ring<BN>::kBytes;
   cfg.stream = st;
@@ -357,14 +372,20 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
 
 }  // namespace
 
+int64_t e4m3_few_fetched(int activation, const E4m3Linear& p) {
+  const int tile = activation == LRI_ACT_GLU ? kBM / 2 : kBM, steps = (p.k + kStep - 1) / kStep;
+  const int64_t tiles = (static_cast<int64_t>(p.n) + tile - 1) / tile * ((p.rows + 63) / 64);
+  const int split = split_of(tiles, steps);
+  return (tiles * split + sm_count() - 1) / sm_count() * ((steps + split - 1) / split) * Ring<64>::kStageBytes;
+}
+
 int e4m3_few_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st) {
   return by_activation(dtype, activation, [&](auto t, auto act) {
     using T = typename decltype(t)::type;
     constexpr int kAct = decltype(act)::value;
     if (p.rows <= 16) return launch<T, kAct, 16>(p, st);
     if (p.rows <= 32) return launch<T, kAct, 32>(p, st);
-    if (p.rows <= 64) return launch<T, kAct, 64>(p, st);
-    return launch<T, kAct, 128>(p, st);
+    return launch<T, kAct, 64>(p, st);
   });
 }
 

@@ -28,5 +28,13 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   p.bias = c.bias, p.addend = c.addend, p.y = c.y, p.x_ld = c.x_ld, p.w_ld = c.w_ld;
   p.rows = static_cast<int>(c.rows), p.n = c.n, p.k = c.k, p.glu = GluParams{c.alpha, c.limit, c.offset};
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
-  return c.rows <= kE4m3FewRows ? e4m3_few_launch(c.dtype, c.activation, p, st) : e4m3_pair_launch(c.dtype, c.activation, p, st);
+  // Which kernel.  What both wait for from some tens of rows on is what an SM can take in, about 57 bytes a cycle (108 KB a us): the one with less to
+  // fetch is the faster, where kAhead is what the shorter start and end of the one for few rows are worth.  us, few / pair: 128 rows, 4096 x 14336 17.0 / 22.7, 2001 x 2568
+  // 6.7 / 10.6, gated 14336 x 4096 38.4 / 32.0; 256 rows, 1280 x 8192 10.7 / 13.8, 4096 x 4096 11.0 / 10.4; 512 rows, 6144 x 4096 27.6 / 15.8.  With up to 64 rows
+  // the pairs' tiles are mostly padding (65 rows: 4096 x 4096 8.1 / 9.9, gated 8192 x 2048 11.6 / 15.7).
+  constexpr int64_t kAhead = 64 << 10;
+  int width = 0;
+  if (c.rows <= 64 || e4m3_few_fetched(c.activation, p) <= e4m3_pair_fetched(c.activation, p, &width) + kAhead)
+    return e4m3_few_launch(c.dtype, c.activation, p, st);
+  return e4m3_pair_launch(c.dtype, c.activation, p, width, st);
 }

@@ -344,25 +344,24 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
 }
 
-// Width of the tile: a K step costs about bn + 64 columns' worth (see gemm_pair.cu), so the narrower tile wins where it fills the last round.
-// (GLU: half a tile's columns in blocks of 32.)
-int tile_width(int64_t rows, int64_t w_rows, int by) {
-  const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
-  int best = kMaxBn;
-  int64_t cost = 0;
+// Width of the tile: the one with which the busiest SM fetches least.  (A K step of 128 x bn takes 337, 382, 436, 505, 563 cycles at 128 .. 256 by 32, see gemm_pair.cu,
+// as its bytes do at 57 a cycle; so the narrower tile wins where it fills the last round.  GLU: half a tile's columns in blocks of 32.)
+int64_t fetched(const E4m3Linear& p, bool glu, int* width) {
+  const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, by = glu ? 64 : 32;
+  const int64_t w_rows = glu ? 2ll * p.n : p.n, steps = (p.k + kStep - 1) / kStep;
+  int64_t least = 0;
   for (int bn = kMaxBn; bn >= 64; bn -= by) {
-    const int64_t tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
-    const int64_t c = (tiles + pairs - 1) / pairs * (bn + 64);
-    if (bn == kMaxBn || c < cost) best = bn, cost = c;
+    const int64_t tiles = ((p.rows + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
+    const int64_t bytes = (tiles + pairs - 1) / pairs * steps * (kTileBytes + bn / 2 * kStep);
+    if (bn == kMaxBn || bytes < least) *width = bn, least = bytes;
   }
-  return best;
+  return least;
 }
 
 template <typename T, int ACT>
-int launch(const E4m3Linear& p, cudaStream_t st) {
+int launch(const E4m3Linear& p, int bn, cudaStream_t st) {
   constexpr bool kGlu = ACT == LRI_ACT_GLU;
   const int64_t w_rows = kGlu ? 2ll * p.n : p.n;
-  const int bn = tile_width(p.rows, w_rows, kGlu ? 64 : 32);
   CUtensorMap tx, tw;
   int rc = make_tmap_e4m3(&tx, p.x, p.rows, p.k, p.x_ld, kBM);
   if (rc != LRI_OK) return rc;
@@ -407,8 +406,10 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
 
 }  // namespace
 
-int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t st) {
-  return by_activation(dtype, activation, [&](auto t, auto act) { return launch<typename decltype(t)::type, decltype(act)::value>(p, st); });
+int64_t e4m3_pair_fetched(int activation, const E4m3Linear& p, int* width) { return fetched(p, activation == LRI_ACT_GLU, width); }
+
+int e4m3_pair_launch(int dtype, int activation, const E4m3Linear& p, int width, cudaStream_t st) {
+  return by_activation(dtype, activation, [&](auto t, auto act) { return launch<typename decltype(t)::type, decltype(act)::value>(p, width, st); });
 }
 
 int e4m3_pair_status_read_and_clear(int* status_out) { return status_read_and_clear(g_e4m3_pair_status, status_out); }

@@ -24,11 +24,12 @@ struct RowsParams {
   bool early;         // the next kernel may start: it waits for this one before it reads the results
 };
 
-constexpr int kFewRows = 148;  // up to here a row gets up to 1024 threads: the kernel is a latency chain
+constexpr int kFewRows = 148;  // one CTA an SM: up to here a row gets up to 1024 threads, and the kernel is a latency chain
 
-// NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
-template <typename T, bool NORM, int NV, int THREADS>
+// ADDS: pending addends of a norm, -1: rows as they are.  NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
+template <typename T, int ADDS, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) {
+  constexpr bool NORM = ADDS >= 0;
   constexpr int kWarps = THREADS / 32;
   const int64_t row = blockIdx.x;
   const int nvec = p.cols >> 3;
@@ -47,8 +48,8 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   if (p.early) pdl_launch_dependents();
   pdl_wait();
   const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_ld);
-  const uint4* a1 = NORM && p.add1 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add1) + row * p.cols) : nullptr;
-  const uint4* a2 = NORM && p.add2 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add2) + row * p.cols) : nullptr;
+  const uint4* a1 = ADDS > 0 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add1) + row * p.cols) : nullptr;
+  const uint4* a2 = ADDS > 1 ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.add2) + row * p.cols) : nullptr;
   uint4* out = NORM && p.residual_out ? reinterpret_cast<uint4*>(static_cast<T*>(p.residual_out) + row * p.cols) : nullptr;
 
   // everything is asked for before anything is looked at: the sums' place may be an input's, and no load passes a store to it
@@ -60,8 +61,8 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
     const int v = threadIdx.x + i * THREADS;
     if (v < nvec) {
       x[i] = in[v];
-      if (a1) a[i] = a1[v];
-      if (a2) b[i] = a2[v];
+      if (ADDS > 0) a[i] = a1[v];
+      if (ADDS > 1) b[i] = a2[v];
     }
   }
 #pragma unroll
@@ -76,13 +77,13 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] * p.factor);
       }
-      if (a1) {
+      if (ADDS > 0) {
         float g[8];
         unpack8<T>(a[i], g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = rnd<T>(f[e] + g[e]);
       }
-      if (a2) {
+      if (ADDS > 1) {
         float g[8];
         unpack8<T>(b[i], g);
 #pragma unroll
@@ -136,26 +137,34 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   }
 }
 
-template <typename T, bool NORM, int NV, int THREADS>
+template <typename T, int ADDS, int NV, int THREADS>
 int launch_nv(const RowsParams& p, int64_t rows, cudaStream_t st) {
-  LRI_CUDA(launch_pdl(rows_e4m3_kernel<T, NORM, NV, THREADS>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, p));
-  LRI_LAUNCH_CHECK(NORM ? "rows_e4m3_kernel<norm>" : "rows_e4m3_kernel");
+  LRI_CUDA(launch_pdl(rows_e4m3_kernel<T, ADDS, NV, THREADS>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, p));
+  LRI_LAUNCH_CHECK(ADDS >= 0 ? "rows_e4m3_kernel<norm>" : "rows_e4m3_kernel");
   return LRI_OK;
 }
 
-template <typename T, bool NORM>
+template <typename T, int ADDS>
 int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {
   const int nvec = p.cols / 8;
   const bool few = rows <= kFewRows;
-  if (nvec <= 256) return launch_nv<T, NORM, 1, 256>(p, rows, st);
-  if (nvec <= 512) return few ? launch_nv<T, NORM, 1, 512>(p, rows, st) : launch_nv<T, NORM, 2, 256>(p, rows, st);
-  if (nvec <= 1024) return few ? launch_nv<T, NORM, 1, 1024>(p, rows, st) : launch_nv<T, NORM, 2, 512>(p, rows, st);
-  if (nvec <= 2048) return launch_nv<T, NORM, 2, 1024>(p, rows, st);
-  if constexpr (!NORM) {
-    if (nvec <= 4096) return launch_nv<T, NORM, 4, 1024>(p, rows, st);
-    return launch_nv<T, NORM, 8, 1024>(p, rows, st);
+  if (nvec <= 256) return launch_nv<T, ADDS, 1, 256>(p, rows, st);
+  if (few) {
+    if (nvec <= 512) return launch_nv<T, ADDS, 1, 512>(p, rows, st);
+    if (nvec <= 1024) return launch_nv<T, ADDS, 1, 1024>(p, rows, st);
+    if (nvec <= 2048) return launch_nv<T, ADDS, 2, 1024>(p, rows, st);
   }
-  return fail(LRI_ERR_UNSUPPORTED, "add_rmsnorm_e4m3: rows of %d elements", p.cols);
+  if (nvec <= 512) return launch_nv<T, ADDS, 2, 256>(p, rows, st);
+  if constexpr (ADDS >= 0) {
+    if (nvec <= 1024) return launch_nv<T, ADDS, 2, 512>(p, rows, st);
+    if (nvec <= 2048) return launch_nv<T, ADDS, 4, 512>(p, rows, st);
+  } else {
+    if (nvec <= 1024) return launch_nv<T, ADDS, 4, 256>(p, rows, st);
+    if (nvec <= 2048) return launch_nv<T, ADDS, 8, 256>(p, rows, st);
+    if (nvec <= 4096) return few ? launch_nv<T, ADDS, 4, 1024>(p, rows, st) : launch_nv<T, ADDS, 8, 512>(p, rows, st);
+    if (nvec <= 8192) return launch_nv<T, ADDS, 8, 1024>(p, rows, st);
+  }
+  return fail(LRI_ERR_UNSUPPORTED, "rows of %d elements to e4m3", p.cols);
 }
 
 constexpr int kMostNormCols = 16384, kMostCols = 65536;
@@ -190,7 +199,7 @@ extern "C" int lri_quantize_rows_e4m3(const lri_quantize_e4m3_call* call) {
   RowsParams p{};
   p.x = c.x, p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.x_ld, p.codes_ld = c.codes_ld, p.cols = c.cols, p.early = c.early != 0;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
-  return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, false>(p, c.rows, st) : launch<__half, false>(p, c.rows, st);
+  return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, -1>(p, c.rows, st) : launch<__half, -1>(p, c.rows, st);
 }
 
 extern "C" int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call) {
@@ -221,5 +230,11 @@ extern "C" int lri_add_rmsnorm_e4m3(const lri_norm_e4m3_call* call) {
   p.codes = static_cast<uint8_t*>(c.codes), p.scale = c.scale, p.x_ld = c.dim, p.codes_ld = c.codes_ld, p.cols = c.dim;
   p.factor = c.residual_scale, p.eps = c.eps, p.early = c.early != 0;
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
-  return c.dtype == LRI_BF16 ? launch<__nv_bfloat16, true>(p, c.rows, st) : launch<__half, true>(p, c.rows, st);
+  if (!p.add1) p.add1 = p.add2, p.add2 = nullptr;  // (one addend is added alike whichever it is)
+  auto with = [&](auto t) {
+    using T = decltype(t);
+    if (p.add2) return launch<T, 2>(p, c.rows, st);
+    return p.add1 ? launch<T, 1>(p, c.rows, st) : launch<T, 0>(p, c.rows, st);
+  };
+  return c.dtype == LRI_BF16 ? with(__nv_bfloat16()) : with(__half());
 }

@@ -18,7 +18,7 @@ from .ops import CudaOps
 E4M3 = torch.float8_e4m3fn
 SWIGLU = (1.0, math.inf, 0.0)
 Rows = Tuple[Tensor, Tensor]
-_WIDE = (torch.bfloat16, torch.float16)
+_WIDE, _F32 = (torch.bfloat16, torch.float16), torch.float32
 
 
 def _said(t):
@@ -31,104 +31,105 @@ def empty_rows(rows: int, cols: int, device=None) -> Rows:
     return (codes if codes.shape[1] == cols else codes[:, :cols]), torch.empty(rows, device=device)
 
 
-def _check_rows(what, rows, shape=None):
-    """The shape of a pair (codes, scale)."""
+def _looked_at(what, rows, cols=None, count=None):
+    """Rows, columns and pitch of a pair (codes, scale), which are to be `count` x `cols` if that is given."""
     codes, scale = rows
-    got = codes.shape
-    if not (codes.dtype is E4M3 and len(got) == 2 and (shape is None or got == shape) and got[1] % 8 == 0 and got[1] > 0 and
-            (got[0] <= 1 or codes.stride(0) % 16 == 0 and codes.stride(0) >= got[1]) and codes.stride(1) == 1):
-        raise ValueError(f"{what}: float8_e4m3fn codes {'[rows, a multiple of 8]' if shape is None else tuple(shape)} whose rows start at multiples of 16 bytes "
-                         f"(e4m3.empty_rows), not {_said(codes)}")
-    if not (scale.dtype is torch.float32 and scale.shape == got[:1] and scale.is_contiguous()):
-        raise ValueError(f"{what}: {got[0]} contiguous fp32 scales, not {_said(scale)}")
-    return got
+    shape, strides = codes.shape, codes.stride()
+    if len(shape) == 2:
+        n, k = shape
+        pitch = strides[0] if n != 1 else -(-k // 16) * 16  # (the pitch of a single row may be any number)
+        if (codes.dtype is E4M3 and strides[1] == 1 and pitch % 16 == 0 and pitch >= k > 0 and k % 8 == 0 and (cols is None or k == cols and n == count) and
+                scale.dtype is _F32 and scale.numel() == n and scale.dim() == 1 and scale.is_contiguous()):
+            return n, k, pitch
+    want = "[rows, a multiple of 8]" if cols is None else f"[{count}, {cols}]"
+    raise ValueError(f"{what}: float8_e4m3fn codes {want} whose rows start at multiples of 16 bytes (e4m3.empty_rows) and a contiguous fp32 scale for "
+                     f"each, not {_said(codes)} and {_said(scale)}")
 
 
-def _check_dense(what, t, dtype, shape):
+def _dense(what, t, dtype, shape):
     if not (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
         raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)}, not {_said(t)}")
+
+
+def _result(out, dtype, rows, n, device):
+    if out is None:
+        if dtype not in _WIDE:
+            raise TypeError(f"results are bfloat16 or float16, not {dtype}")
+        return torch.empty(rows, n, dtype=dtype, device=device)
+    if out.dtype not in _WIDE:
+        raise TypeError(f"results are bfloat16 or float16, not {out.dtype}")
+    if not (out.shape == (rows, n) and out.is_contiguous()):
+        raise ValueError(f"out: contiguous [{rows}, {n}], not {_said(out)}")
+    return out
 
 
 def quantize_rows(x: Tensor, out: Optional[Rows] = None, early: bool = False) -> Rows:
     """Rows of x [rows, cols] (bfloat16 or float16; rows may lie apart, as parts of a wider buffer) as codes and scales; cols a multiple of 8
     up to 65536.  early: the projection that follows may start on its weights before these rows are complete; not for rows that are themselves its weights."""
-    shape = x.shape
-    if not (x.dtype in _WIDE and len(shape) == 2 and shape[1] % 8 == 0 and 0 < shape[1] <= 65536 and x.stride(1) == 1 and
-            (shape[0] <= 1 or x.stride(0) % 8 == 0 and x.stride(0) >= shape[1])):
+    shape, strides = x.shape, x.stride()
+    rows, cols = shape if len(shape) == 2 else (-1, 0)
+    x_ld = cols if rows == 1 else strides[0] if strides else 0
+    if not (rows >= 0 and x.dtype in _WIDE and cols % 8 == 0 and 0 < cols <= 65536 and strides[1] == 1 and x_ld % 8 == 0 and x_ld >= cols):
         raise ValueError(f"x: bfloat16 or float16 rows of a multiple of 8 elements up to 65536 that start at multiples of 16 bytes, not {_said(x)}")
     if out is None:
-        out = empty_rows(*shape, x.device)
-    else:
-        _check_rows("out", out, shape)
-    CudaOps.quantize_rows_e4m3(x, *out, shape, early)
+        out = empty_rows(rows, cols, x.device)
+    _, _, codes_ld = _looked_at("out", out, cols, rows)
+    CudaOps.quantize_rows_e4m3(x, out[0], out[1], rows, cols, x_ld, codes_ld, early)
     return out
 
 
 def add_rmsnorm(residual: Tensor, weight: Tensor, eps: float, add1: Optional[Tensor] = None, add2: Optional[Tensor] = None, residual_scale: float = 1.0,
                 residual_out: Optional[Tensor] = None, out: Optional[Rows] = None, early: bool = False) -> Rows:
     """round(round(residual * residual_scale) + add1) + add2 to residual_out (None: not kept; may be residual), each sum rounded to the residual's
-    type, and RMSNorm of that times weight as codes and scales.  residual, add1, add2 [rows, dim]; dim a multiple of 8 up to 16384.  early: as in quantize_rows."""
+    type, and RMSNorm of that times weight as codes and scales.  residual, add1, add2 [rows, dim]; dim a multiple of 8 up to 16384.  early: as in
+    quantize_rows."""
     shape, dtype = residual.shape, residual.dtype
-    if not (dtype in _WIDE and len(shape) == 2 and shape[1] % 8 == 0 and 0 < shape[1] <= 16384 and residual.is_contiguous()):
+    rows, dim = shape if len(shape) == 2 else (-1, 0)
+    if not (rows >= 0 and dtype in _WIDE and dim % 8 == 0 and 0 < dim <= 16384 and residual.is_contiguous()):
         raise ValueError(f"residual: contiguous bfloat16 or float16 rows of a multiple of 8 elements up to 16384, not {_said(residual)}")
-    _check_dense("weight", weight, dtype, shape[1:])
+    _dense("weight", weight, dtype, (dim,))
     if add1 is not None:
-        _check_dense("add1", add1, dtype, shape)
+        _dense("add1", add1, dtype, shape)
     if add2 is not None:
-        _check_dense("add2", add2, dtype, shape)
+        _dense("add2", add2, dtype, shape)
     if residual_out is not None:
-        _check_dense("residual_out", residual_out, dtype, shape)
+        _dense("residual_out", residual_out, dtype, shape)
     if out is None:
-        out = empty_rows(*shape, residual.device)
-    else:
-        _check_rows("out", out, shape)
-    CudaOps.add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, *out, shape[0], residual_scale, early)
+        out = empty_rows(rows, dim, residual.device)
+    _, _, codes_ld = _looked_at("out", out, dim, rows)
+    CudaOps.add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, out[0], out[1], rows, dim, codes_ld, residual_scale, early)
     return out
 
 
 def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional[str] = None, addend: Optional[Tensor] = None,
            dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None) -> Tensor:
     """activation(x w^T + bias) + addend, [rows, outputs], summed in fp32 and rounded once.  activation: None, "silu", "gelu" (by the error
-    function) or "gelu_tanh"; bias [outputs] and addend [rows, outputs] in the result's type; the addend may be `out`.  dtype: of the result where `out` is None."""
-    rows, k = _check_rows("x", x)
-    n, depth = _check_rows("w", w)
+    function) or "gelu_tanh"; bias [outputs] and addend [rows, outputs] in the result's type; the addend may be `out`.  dtype: of the result where `out`
+    is None."""
+    rows, k, x_ld = _looked_at("x", x)
+    n, depth, w_ld = _looked_at("w", w)
     if k != depth:
         raise ValueError(f"rows of {k} codes times weights of {depth}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation={activation!r}: one of {list(ACTIVATIONS)}")
-    if out is None:
-        if dtype not in _WIDE:
-            raise TypeError(f"results are bfloat16 or float16, not {dtype}")
-        out = torch.empty(rows, n, dtype=dtype, device=x[0].device)
-    else:
-        dtype = out.dtype
-        if dtype not in _WIDE:
-            raise TypeError(f"results are bfloat16 or float16, not {dtype}")
-        _check_dense("out", out, dtype, (rows, n))
+    out = _result(out, dtype, rows, n, x[0].device)
     if bias is not None:
-        _check_dense("bias", bias, dtype, (n,))
+        _dense("bias", bias, out.dtype, (n,))
     if addend is not None:
-        _check_dense("addend", addend, dtype, (rows, n))
-    CudaOps.linear_e4m3(x, w, out, rows, bias, addend, ACTIVATIONS[activation])
+        _dense("addend", addend, out.dtype, (rows, n))
+    CudaOps.linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias, addend, ACTIVATIONS[activation])
     return out
 
 
 def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None) -> Tensor:
     """The gated unit of x w1^T, w1 [2 inter, k] = [up | gate]: g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit),
     u = clamp(up, -limit, limit), glu = (alpha, limit, offset); SwiGLU by default.  In fp32, rounded once to [rows, inter]."""
-    rows, k = _check_rows("x", x)
-    n, depth = _check_rows("w1", w1)
+    rows, k, x_ld = _looked_at("x", x)
+    n, depth, w_ld = _looked_at("w1", w1)
     if k != depth or n % 2 or not n:
         raise ValueError(f"rows of {k} codes times [up | gate] weights [{n}, {depth}]")
     if not glu[1] >= 0:
         raise ValueError(f"glu={glu}: the limit is not below 0")
-    if out is None:
-        if dtype not in _WIDE:
-            raise TypeError(f"results are bfloat16 or float16, not {dtype}")
-        out = torch.empty(rows, n // 2, dtype=dtype, device=x[0].device)
-    else:
-        if out.dtype not in _WIDE:
-            raise TypeError(f"results are bfloat16 or float16, not {out.dtype}")
-        _check_dense("out", out, out.dtype, (rows, n // 2))
-    CudaOps.linear_e4m3(x, w1, out, rows, activation=ACT_GLU, glu=glu)
+    out = _result(out, dtype, rows, n // 2, x[0].device)
+    CudaOps.linear_e4m3(x, w1, out, rows, n // 2, k, x_ld, w_ld, activation=ACT_GLU, glu=glu)
     return out

@@ -198,49 +198,43 @@ class CudaOps:
                                                pages.data_ptr(), pages.shape[1], page, n_pages, _C.stream_handle()))
 
     # ---- projections in 8 bits ----------------------------------------------------------------------
-    # (codes, scale) pairs as gpt_fast.e4m3 checks them.  As above, the pitch of a single row may be any number.
+    # (As above: a look at a tensor's shape or strides costs the host 100 to 200 ns, and the callers have looked.)
     @staticmethod
-    def quantize_rows_e4m3(x, codes, scale, shape, early=False):
+    def quantize_rows_e4m3(x, codes, scale, rows, cols, x_ld, codes_ld, early=False):
         """early: what follows on the stream reads the rows as the x of a projection, or not at all (include/lri_b200.h)."""
         here = x.get_device()
         if not 0 <= here == torch._C._cuda_getDevice() == codes.get_device() == scale.get_device():
             _C.refuse_devices(x, codes, scale)
-        rows, cols = shape
         status = _C.lib.lri_quantize_rows_e4m3(_C.QUANTIZE_CALL.pack(
-            x.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x.stride(0) if rows > 1 else cols,
-            codes.stride(0) if rows > 1 else -(-cols // 16) * 16, _C.CODES[x.dtype], cols, early))
+            x.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x_ld, codes_ld, _C.CODES[x.dtype], cols, early))
         if status < 0:
             _C.check(status)
 
     @staticmethod
-    def add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, codes, scale, rows, residual_scale=1.0, early=False):
+    def add_rmsnorm_e4m3(residual, add1, add2, weight, eps, residual_out, codes, scale, rows, dim, codes_ld, residual_scale=1.0, early=False):
         here = residual.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == weight.get_device() == codes.get_device() == scale.get_device() and
                 (add1 is None or add1.get_device() == here) and (add2 is None or add2.get_device() == here) and
                 (residual_out is None or residual_out.get_device() == here)):
             _C.refuse_devices(residual, weight, codes, scale, add1, add2, residual_out)
-        dim = weight.shape[0]
         status = _C.lib.lri_add_rmsnorm_e4m3(_C.NORM8_CALL.pack(
             residual.data_ptr(), 0 if add1 is None else add1.data_ptr(), 0 if add2 is None else add2.data_ptr(), weight.data_ptr(),
             0 if residual_out is None else residual_out.data_ptr(), codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows,
-            codes.stride(0) if rows > 1 else -(-dim // 16) * 16, _C.CODES[residual.dtype], dim, early, residual_scale, eps))
+            codes_ld, _C.CODES[residual.dtype], dim, early, residual_scale, eps))
         if status < 0:
             _C.check(status)
 
     @staticmethod
-    def linear_e4m3(x, w, out, rows, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0)):
-        """x, w: (codes, scale); activation: a number of LRI_ACT_*."""
+    def linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0)):
+        """x, w: (codes, scale); n outputs; activation: a number of LRI_ACT_*."""
         (xc, xs), (wc, ws) = x, w
         here = xc.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == xs.get_device() == wc.get_device() == ws.get_device() == out.get_device() and
                 (bias is None or bias.get_device() == here) and (addend is None or addend.get_device() == here)):
             _C.refuse_devices(xc, xs, wc, ws, out, bias, addend)
-        n, k = wc.shape
-        pitch = -(-k // 16) * 16
         status = _C.lib.lri_linear_e4m3(_C.LINEAR8_CALL.pack(
             xc.data_ptr(), wc.data_ptr(), xs.data_ptr(), ws.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if addend is None else addend.data_ptr(),
-            out.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, xc.stride(0) if rows > 1 else pitch, wc.stride(0) if n > 1 else pitch,
-            _C.CODES[out.dtype], n // 2 if activation == _C.ACT_GLU else n, k, activation, *glu))
+            out.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x_ld, w_ld, _C.CODES[out.dtype], n, k, activation, *glu))
         if status < 0:
             _C.check(status)
 
