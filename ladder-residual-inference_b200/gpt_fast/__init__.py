@@ -3,6 +3,7 @@
 Importing the package initialises the process group when none exists (one process per GPU,
 torchrun environment), as the reference does at import time.
 """
+from . import e4m3
 from .gpt_dense_TP import GPTDense
 from .gpt_desync_TP import GPTDesync
 from .gpt_ladder_TP import GPTLadder
@@ -12,4 +13,4 @@ from .gpt_patevik_TP import GPTPatevik
 from .paged import PagedKVCache
 from .tp import maybe_init_dist
 
-__all__ = ["GPTDense", "GPTDesync", "GPTLadder", "GPTMigosun", "GPTParallel", "GPTPatevik", "PagedKVCache", "maybe_init_dist"]
+__all__ = ["GPTDense", "GPTDesync", "GPTLadder", "GPTMigosun", "GPTParallel", "GPTPatevik", "PagedKVCache", "e4m3", "maybe_init_dist"]

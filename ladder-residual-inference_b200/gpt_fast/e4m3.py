@@ -133,3 +133,48 @@ def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtyp
     out = _result(out, dtype, rows, n // 2, x[0].device)
     CudaOps.linear_e4m3(x, w1, out, rows, n // 2, k, x_ld, w_ld, activation=ACT_GLU, glu=glu)
     return out
+
+
+class E4M3Weight:
+    """Rows of a weight in 8 bits: (codes, scale) = weight.  Slices are rows of the same memory."""
+    __slots__ = ("codes", "scale")
+
+    def __init__(self, codes: Tensor, scale: Tensor):
+        self.codes, self.scale = codes, scale
+
+    def __iter__(self):
+        yield self.codes
+        yield self.scale
+
+    def __getitem__(self, rows: slice) -> "E4M3Weight":
+        return E4M3Weight(self.codes[rows], self.scale[rows])
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+class E4M3Linear(nn.Module):
+    """Stands where a model's nn.Linear was: owns the codes and scales of its weight [outputs, k].  `codes` [outputs, k up to a multiple of 16]."""
+
+    def __init__(self, weight: Tensor):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("codes", torch.zeros(self.out_features, -(-self.in_features // 16) * 16, dtype=E4M3, device=weight.device))
+        self.register_buffer("scale", torch.empty(self.out_features, device=weight.device))
+        quantize_rows(weight.detach(), out=(self.codes[:, :self.in_features], self.scale))
+
+    @property
+    def weight(self) -> E4M3Weight:
+        b = self._buffers
+        codes, scale = b["codes"], b["scale"]
+        if codes.dtype is not E4M3 or scale.dtype is not _F32:
+            raise TypeError("a module that was cast after its weights went to 8 bits holds codes without their meaning")
+        return E4M3Weight(codes if codes.shape[1] == self.in_features else codes[:, :self.in_features], scale)
+
+    def forward(self, x: Tensor) -> Tensor:
+        rows = x.reshape(-1, self.in_features)
+        return linear(quantize_rows(rows, early=True), self.weight, dtype=x.dtype).view(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}"

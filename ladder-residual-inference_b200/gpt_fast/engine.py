@@ -26,8 +26,9 @@ import os
 
 import torch
 
-from ._C import DENSE, DESYNC, LADDER, LADDER_TWO_STREAMS, PARALLEL, PARALLEL_TWO_STREAMS, dtype_code, option
+from ._C import ACT_GLU, DENSE, DESYNC, LADDER, LADDER_TWO_STREAMS, PARALLEL, PARALLEL_TWO_STREAMS, dtype_code, option
 from .comm import NoComm, make_comm
+from .e4m3 import SWIGLU, E4M3Linear, empty_rows
 from .ops import CudaOps, decode_splits
 
 _MAX_SPLITS = 64
@@ -45,6 +46,7 @@ class Engine:
         self.ops = ops if ops is not None else CudaOps
         self.comm = comm if comm is not None else make_comm()
         self.ready = False
+        self.eight = False  # whether the layers' projections are in 8 bits
         self.paged = False  # whether the layers' caches are pages (setup_paged)
         self._pages = self._prompt = None  # of the pass in hand: the table; what a prompt's layers share (_body)
         self._norm_pushes = False  # set per step by _reduce_plan
@@ -59,6 +61,7 @@ class Engine:
         self.max_batch, self.max_seq = max_batch, max_seq
         rows = max_batch * max_seq if rows is None else rows
         self.max_rows = rows
+        self.eight = isinstance(self.model.layers[0].attention.wo, E4M3Linear)
 
         def buf(cols, n=rows):
             return torch.empty(n, cols, dtype=dtype, device=device)
@@ -71,7 +74,7 @@ class Engine:
         def workspace(size_fn, *shape):
             # large enough for a prefill of all rows and for a decode step of up to 64 rows (whose
             # split-K partial sums can take more room than a longer prefill's raw projection)
-            n = max(size_fn(rows, *shape), size_fn(min(rows, 64), *shape))
+            n = 0 if self.eight else max(size_fn(rows, *shape), size_fn(min(rows, 64), *shape))
             return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
         self.ws_qkv = workspace(self.ops.qkv_workspace_bytes, self.nh, self.nkv, self.hd)
@@ -81,6 +84,9 @@ class Engine:
         self.ws_w2 = workspace(self.ops.linear_workspace_bytes, self.d)
         nbytes = self.ops.attn_decode_scratch_bytes(max_batch, self.nh, self.nkv, self.hd, _MAX_SPLITS)
         self.scratch = torch.zeros(max(nbytes, 16), dtype=torch.uint8, device=device)
+        if self.eight:
+            self.qkv = buf((self.nh + 2 * self.nkv) * self.hd)
+            self.normed8, self.y8, self.h8 = (empty_rows(rows, n, device) for n in (self.d, self.nh * self.hd, self.inter))
         # one sequence: the second residual of passes whose projections take the norms
         self.row_ws = buf(self.d, 1)
         self._setup_head(max_batch, device, dtype)
@@ -90,6 +96,7 @@ class Engine:
         if self.overlap_sublayers:
             if self.family == "ladder":
                 self.normed_m = buf(self.d)
+                self.normed8_m = empty_rows(rows, self.d, device) if self.eight else None
             # (same priority as the main stream: giving the MLP chain, four fifths of a layer's bytes, the higher
             # priority was measured slower on B200, 2.80 against 2.58 ms per 8B step)
             self.side_stream = torch.cuda.Stream()
@@ -104,8 +111,9 @@ class Engine:
         sequences of up to max_length positions."""
         self.setup(max_sequences, max_prompt, device, dtype, rows=max(max_sequences, max_prompt))
         n = (self.nh + 2 * self.nkv) * self.hd
-        self.qkv = torch.empty(self.max_rows, n, dtype=dtype, device=device)
-        nbytes = max(self.ops.linear_workspace_bytes(self.max_rows, n), self.ops.linear_workspace_bytes(min(self.max_rows, 64), n))
+        if not self.eight:
+            self.qkv = torch.empty(self.max_rows, n, dtype=dtype, device=device)
+        nbytes = 0 if self.eight else max(self.ops.linear_workspace_bytes(self.max_rows, n), self.ops.linear_workspace_bytes(min(self.max_rows, 64), n))
         self.ws_qkv_rows = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         caches = [layer.attention.kv_cache for layer in self.model.layers]
         self.ws_paged = caches[0].attend_workspace(self.nh)
@@ -160,18 +168,38 @@ class Engine:
             self._paged_attention(att.kv_cache, w_qkv, rows, S, pos)
         else:
             kc, vc = att.kv_cache.k_cache, att.kv_cache.v_cache
-            ops.qkv_rope_kvcache(self.normed, w_qkv, self.model.freqs_cis, False, pos, self.q, kc, vc, B, S, self.nh,
-                                 self.nkv, self.hd, self.ws_qkv)
+            if self.eight:
+                self._linear_e4m3(self.normed8, w_qkv, self.qkv, rows)
+                ops.rope_kvcache(self.qkv, self.model.freqs_cis, False, pos, self.q, kc, vc, B, S, self.nh, self.nkv, self.hd)
+            else:
+                ops.qkv_rope_kvcache(self.normed, w_qkv, self.model.freqs_cis, False, pos, self.q, kc, vc, B, S, self.nh,
+                                     self.nkv, self.hd, self.ws_qkv)
             ops.attention(self.q, kc, vc, pos, self.y, B, S, self.nh, self.nkv, self.hd, self.scratch, self._splits)
-        if push:
+        if self.eight:
+            self._linear_e4m3(self._rows_e4m3(self.y, self.y8, rows), att.wo.weight, out, rows)
+        elif push:
             self.comm.linear_push(self.y, att.wo.weight, out, rows, push)
         else:
             ops.linear(self.y, att.wo.weight, out, rows, workspace=self.ws_wo)
 
+    def _rows_e4m3(self, x, to, rows):
+        """The first rows of a buffer in 8 bits.  (early: what follows reads them as the x of a projection.)"""
+        cols = x.shape[1]
+        self.ops.quantize_rows_e4m3(x, *to, rows, cols, cols, to[0].stride(0), early=True)
+        return to
+
+    def _linear_e4m3(self, x, w, out, rows, addend=None, glu=False):
+        n, k = w.shape
+        self.ops.linear_e4m3(x, w, out, rows, n // 2 if glu else n, k, x[0].stride(0), w.codes.stride(0), addend=addend, activation=ACT_GLU if glu else 0,
+                             glu=SWIGLU)
+
     def _paged_attention(self, cache, w_qkv, rows, S, pos):
         """self.normed -> self.y: one new token of each sequence over its pages, or a prompt of one sequence over a dense copy of them."""
         ops, qkv, q = self.ops, self.qkv[:rows], self.q[:rows].view(rows, self.nh, self.hd)
-        ops.linear(self.normed, w_qkv, qkv, rows, workspace=self.ws_qkv_rows)
+        if self.eight:
+            self._linear_e4m3(self.normed8, w_qkv, qkv, rows)
+        else:
+            ops.linear(self.normed, w_qkv, qkv, rows, workspace=self.ws_qkv_rows)
         cache.store(qkv, self.model.freqs_cis, pos, self._pages, self.nh, sequence=None if S == 1 else self.one_sequence[:rows], out=q)
         if S == 1:
             cache.attend(q, pos, self._pages, out=self.y[:rows].view(rows, self.nh, self.hd), workspace=self.ws_paged)
@@ -185,6 +213,10 @@ class Engine:
                 ops.attention(q, k, v, pos, self.y, 1, S, self.nh, self.nkv, self.hd, None, 1)
 
     def _mlp(self, w1, w2, rows, out, addend=None, normed=None, push=0):
+        if self.eight:
+            self._linear_e4m3(self.normed8 if normed is None else self.normed8_m, w1, self.h, rows, glu=True)
+            self._linear_e4m3(self._rows_e4m3(self.h, self.h8, rows), w2, out, rows, addend=addend)
+            return
         self.ops.gateup_swiglu(self.normed if normed is None else normed, w1, self.h, rows, self.ws_ug)
         if push:
             self.comm.linear_push(self.h, w2, out, rows, push, addend=addend)
@@ -197,7 +229,11 @@ class Engine:
         message pushed on that channel (the reduction half of the all-reduce)."""
         res_out = self.resid if (write_residual and (add1 is not None or add2 is not None or scale != 1.0)) else None
         out = self.normed if normed is None else normed
-        if (ch1 and add1 is not None) or (ch2 and add2 is not None):
+        if self.eight and write_residual:  # (the final norm, which does not write the residual, feeds the output projection)
+            codes, scale_out = self.normed8 if normed is None else self.normed8_m
+            self.ops.add_rmsnorm_e4m3(self.resid, add1, add2, weight, self.cfg.norm_eps, res_out, codes, scale_out, rows, self.d, codes.stride(0), scale,
+                                      early=True)
+        elif (ch1 and add1 is not None) or (ch2 and add2 is not None):
             self.comm.add_rmsnorm_gather(self.resid, ch1 if add1 is not None else 0, add1,
                                          ch2 if add2 is not None else 0, add2, weight, self.cfg.norm_eps, res_out, out,
                                          rows, scale, self_push=self._norm_pushes)
@@ -209,7 +245,7 @@ class Engine:
         (0: they read an all-reduced buffer), the channels on which the projections push from their
         epilogue (0: they do not; with the fused form the norm pushes itself), and whether the
         reduction happens inside the norm at all."""
-        mode = self.comm.reduce_mode(rows * self.d, rows, hidden=hidden)
+        mode = "kernel" if self.eight else self.comm.reduce_mode(rows * self.d, rows, hidden=hidden)
         self._norm_pushes = mode == "fused"
         if mode == "kernel":
             return 0, 0, 0, 0, False
@@ -284,7 +320,7 @@ class Engine:
     def _run_native(self, B, S, pos):
         """The schedule's kernels in one native call, on one GPU; False where it has to run from here: with communication, another ops object,
         blocks of both kinds, layers of unequal sizes."""
-        if type(self.comm) is not NoComm or self.ops is not CudaOps or self.model.norm.weight is None:
+        if self.eight or type(self.comm) is not NoComm or self.ops is not CudaOps or self.model.norm.weight is None:
             return False
         m, family = self.model, self.family
         mixed = getattr(self.cfg, "ladder_layers", None)
@@ -470,9 +506,15 @@ class Engine:
         mixed = getattr(self.cfg, "ladder_layers", None)
         if mixed is not None and len(set(mixed)) != self.cfg.n_layer:
             return self._run_hybrid(rows, B, S, pos, set(mixed))
+        # (in 8 bits up to 64 rows: more may run on pairs of SMs)
+        if self.eight and rows > 64:
+            return self._run_ladder_one_stream(rows, B, S, pos)
         # (beyond 64 rows only where the kernel on pairs of SMs is not forced upon every projection, as in lri_llama_run)
         if S == 1 and self.overlap_sublayers and (rows <= 64 or rows <= _TWO_STREAM_ROWS and option("gemm_pair") <= 1):
             return self._run_ladder_two_streams(rows, B, S, pos)
+        self._run_ladder_one_stream(rows, B, S, pos)
+
+    def _run_ladder_one_stream(self, rows, B, S, pos):
         comm, m = self.comm, self.model
         ca, cm, pa, pm, split = self._reduce_plan(rows, hidden=True)
         h_a = h_m = None

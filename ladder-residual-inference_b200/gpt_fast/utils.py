@@ -122,18 +122,32 @@ class FeedForward(nn.Module):
         self.w2 = nn.Linear(config.intermediate_size // tp_world_size, config.dim, bias=False)
 
     def forward(self, x: Tensor) -> Tensor:
-        ops = _ops()
         shape = x.shape
         x2 = x.reshape(-1, shape[-1]).contiguous()
-        rows = x2.shape[0]
-        inter = self.w1.weight.shape[0] // 2
-        h = torch.empty(rows, inter, dtype=x.dtype, device=x.device)
-        ws_bytes = ops.gateup_workspace_bytes(rows, inter)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-        ops.gateup_swiglu(x2, self.w1.weight, h, rows, ws)
-        y = torch.empty(rows, self.w2.weight.shape[0], dtype=x.dtype, device=x.device)
-        ops.linear(h, self.w2.weight, y, rows)
-        return y.view(*shape[:-1], -1)
+        return _linear(self.w2, _gated(self.w1.weight, x2)).view(*shape[:-1], -1)
+
+
+def _linear(lin, x2):
+    """x2 [rows, k] through a projection in 16 or 8 bits."""
+    if not isinstance(lin, nn.Linear):
+        return lin(x2)
+    y = torch.empty(x2.shape[0], lin.weight.shape[0], dtype=x2.dtype, device=x2.device)
+    _ops().linear(x2, lin.weight, y, x2.shape[0])
+    return y
+
+
+def _gated(weight, x2):
+    """The gated unit of x2 [rows, k] times weight rows [up | gate], in 16 or 8 bits."""
+    rows, inter = x2.shape[0], weight.shape[0] // 2
+    if not isinstance(weight, Tensor):
+        from . import e4m3
+        return e4m3.gateup_glu(e4m3.quantize_rows(x2, early=True), weight, dtype=x2.dtype)
+    ops = _ops()
+    h = torch.empty(rows, inter, dtype=x2.dtype, device=x2.device)
+    ws_bytes = ops.gateup_workspace_bytes(rows, inter)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2.device) if ws_bytes else None
+    ops.gateup_swiglu(x2, weight, h, rows, ws)
+    return h
 
 
 def _attention_core(mod, q, input_pos, bsz, seqlen):
@@ -155,6 +169,12 @@ def _qkv(mod, x2, weight_rows, freqs_cis, input_pos, bsz, seqlen):
     ops = _ops()
     rows = bsz * seqlen
     q = torch.empty(rows, mod.n_head * mod.head_dim, dtype=x2.dtype, device=x2.device)
+    if not isinstance(weight_rows, Tensor):
+        from . import e4m3
+        qkv = e4m3.linear(e4m3.quantize_rows(x2, early=True), weight_rows, dtype=x2.dtype)
+        ops.rope_kvcache(qkv, freqs_cis.contiguous(), True, input_pos, q, mod.kv_cache.k_cache, mod.kv_cache.v_cache, bsz, seqlen, mod.n_head,
+                         mod.n_local_heads, mod.head_dim)
+        return q
     ws_bytes = ops.qkv_workspace_bytes(rows, mod.n_head, mod.n_local_heads, mod.head_dim)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2.device) if ws_bytes else None
     # freqs_cis arrives already indexed by position (freqs_cis[input_pos]), as the reference passes it
@@ -194,15 +214,12 @@ class Attention(nn.Module):
 
     def forward(self, x: Tensor, freqs_cis: Tensor, mask: Tensor, input_pos: Optional[Tensor] = None) -> Tensor:
         assert self.kv_cache is not None, "Caches must be initialized first"
-        ops = _ops()
         bsz, seqlen, _ = x.shape
         pos = _as_pos(input_pos)
         x2 = x.reshape(bsz * seqlen, -1).contiguous()
         q = _qkv(self, x2, self.wqkv.weight, freqs_cis, pos, bsz, seqlen)
         y = _attention_core(self, q, pos, bsz, seqlen)
-        out = torch.empty(bsz * seqlen, self.wo.weight.shape[0], dtype=x.dtype, device=x.device)
-        ops.linear(y, self.wo.weight, out, bsz * seqlen)
-        return out.view(bsz, seqlen, -1)
+        return _linear(self.wo, y).view(bsz, seqlen, -1)
 
 
 class FuseAttentionMLP(nn.Module):
@@ -249,12 +266,11 @@ class FuseAttentionMLP(nn.Module):
         w = self.wqkv1.weight
         q = _qkv(self, x2, w[: self.qkv_rows], freqs_cis, pos, bsz, seqlen)
         y = _attention_core(self, q, pos, bsz, seqlen)
-        attn = torch.empty(rows, self.wo.weight.shape[0], dtype=x.dtype, device=x.device)
-        ops.linear(y, self.wo.weight, attn, rows)
-        h = torch.empty(rows, self.intermediate_size, dtype=x.dtype, device=x.device)
-        ws_bytes = ops.gateup_workspace_bytes(rows, self.intermediate_size)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-        ops.gateup_swiglu(x2, w[self.qkv_rows:], h, rows, ws)
+        attn = _linear(self.wo, y)
+        h = _gated(w[self.qkv_rows:], x2)
+        if not isinstance(self.w2, nn.Linear):
+            from . import e4m3
+            return e4m3.linear(e4m3.quantize_rows(h, early=True), self.w2.weight, addend=attn, out=attn).view(bsz, seqlen, -1)
         out = torch.empty_like(attn)
         ops.linear(h, self.w2.weight, out, rows, addend=attn)
         return out.view(bsz, seqlen, -1)
