@@ -302,7 +302,8 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * nn.Linear in 16 bits (gpt_fast/utils.py:142-148, 187-198, 258).
  * `dtype` bfloat16 or float16: the type of everything that is neither codes nor scales.  Codes: rows of k elements, a multiple of 8, that
  * start at multiples of 16 bytes (pitch x_ld, w_ld, codes_ld; what lies between the rows is neither read nor written).  All arithmetic in
- * fp32, rounded once where a result is stored.  Codes, 16-bit rows and results are 16-byte aligned, and results overlap nothing else (one exception: see addend).
+ * fp32, rounded once where a result is stored.  Codes, rows in 16 bits (but a bias) and results but scales are 16-byte aligned, and results overlap
+ * nothing else, but where it says that one may be an input.
  *
  * A row's codes are the nearest to value * (448 / top), its scale top / 448, top the largest magnitude of its values and at least 2^-100.
  * A row with an infinity or NaN gets zeros and a NaN scale.
@@ -318,9 +319,10 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * w_scale 2 n scales, without bias and addend, and y = g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit), u = clamp(up, -limit, limit):
  * SwiGLU with alpha 1, limit infinity, offset 0.
  *
- * lri_linear_e4m3 starts on its weights (w and w_scale, bias) while the kernel before it on the stream still runs, as the projections in 16 bits do.  So
+ * lri_linear_e4m3 starts on its weights (w and w_scale) while the kernel before it on the stream still runs, as the projections in 16 bits do.  So
  * lri_quantize_rows_e4m3 and lri_add_rmsnorm_e4m3, whose results may be weights, let the next kernel start only when they are complete, unless `early`
- * is not 0: for a caller whose next calls read the results as x, or not at all. */
+ * is not 0: for a caller whose next calls read the results as x, or not at all.  Codes that something else has just stored (the pages of a cache) become
+ * weights behind an operation that is complete before the next begins, such as a copy. */
 enum lri_activation { LRI_ACT_NONE = 0, LRI_ACT_SILU = 1, LRI_ACT_GELU = 2, LRI_ACT_GELU_TANH = 3, LRI_ACT_GLU = 4 };
 typedef struct {
   const void* x;

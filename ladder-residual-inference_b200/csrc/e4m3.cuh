@@ -61,8 +61,10 @@ __device__ __forceinline__ float activate(float z) {
   return z;
 }
 __device__ __forceinline__ float gated_unit(float gate, float up, const GluParams& p) {
-  const float g = gate > p.limit ? p.limit : gate;
-  const float u = up > p.limit ? p.limit : (up < -p.limit ? -p.limit : up);
+  float g, u;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(g) : "f"(gate), "f"(p.limit));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(u) : "f"(up), "f"(p.limit));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(u) : "f"(u), "f"(-p.limit));
   return g * sigmoid_fast(p.alpha * g) * (u + p.offset);
 }
 

@@ -121,7 +121,8 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_expect_tx(landed, static_cast<uint32_t>(mine * (split - 1) * kBlockBytes));
   }
-  __shared__ float row_scale[BN];
+  __shared__ float4 row_scale[BN / 4];
+  __shared__ float2 bias[kGlu ? 1 : kOut / 2];
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -138,15 +139,10 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const int c = 2 * static_cast<int>(threadIdx.x % kPairs);
   const int64_t j = static_cast<int64_t>(tile) * kOut + c;
   const bool there = j < p.n, both = j + 1 < p.n, pairs_aligned = (p.n & 1) == 0;
-  float2 s = make_float2(0.f, 0.f), more = s;  // scales of the outputs; bias, or scales of the gate
+  float2 s = make_float2(0.f, 0.f), more = s;  // scales of the outputs, of their gates
   if (there) {
     s = make_float2(p.w_scale[j], both ? p.w_scale[j + 1] : 0.f);
-    if (kGlu) {
-      more = make_float2(p.w_scale[p.n + j], both ? p.w_scale[p.n + j + 1] : 0.f);
-    } else if (p.bias) {
-      const T* bias = static_cast<const T*>(p.bias) + j;
-      more = make_float2(Num<T>::to_f(bias[0]), both ? Num<T>::to_f(bias[1]) : 0.f);
-    }
+    if (kGlu) more = make_float2(p.w_scale[p.n + j], both ? p.w_scale[p.n + j + 1] : 0.f);
   }
 
   // warp-uniform loops, one elected lane issues (see gemm_pair.cu)
@@ -201,7 +197,11 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     pdl_wait();
     pdl_launch_dependents();
     const int quarter = warp & 3, i = static_cast<int>(threadIdx.x) - 64;
-    if (i < rows) row_scale[i] = p.x_scale[row0 + i];
+    if (i < rows) reinterpret_cast<float*>(row_scale)[i] = p.x_scale[row0 + i];
+    if (!kGlu && i < kOut) {
+      const int64_t o = static_cast<int64_t>(tile) * kOut + i;
+      reinterpret_cast<float*>(bias)[i] = p.bias && o < p.n ? Num<T>::to_f(static_cast<const T*>(p.bias)[o]) : 0.f;
+    }
     if (!kGlu && p.addend) {
       const char* add = reinterpret_cast<const char*>(static_cast<const T*>(p.addend) + static_cast<int64_t>(row0) * p.n + static_cast<int64_t>(tile) * kOut);
       const int bytes = static_cast<int>(min(static_cast<int64_t>(kOut), p.n - static_cast<int64_t>(tile) * kOut)) * 2;
@@ -277,6 +277,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     __syncwarp();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // nothing is copied into this CTA any more
   }
+  if (!kGlu) more = bias[c / 2];
   for (; there && ok && g < mine; g += kAtOnce, load_addend()) {
     const int tok0 = 4 * (g * split + rank);
     T* y = static_cast<T*>(p.y) + static_cast<int64_t>(row0 + tok0) * p.n + j;
@@ -297,10 +298,12 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         }
       }
     }
+    const float4 four = row_scale[tok0 >> 2];  // (behind the last row: anything, and not stored)
+    const float sxs[4] = {four.x, four.y, four.z, four.w};
     float out[4][2];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float sx = row_scale[tok0 + u];  // (behind the last row: anything, and not stored)
+      const float sx = sxs[u];
       float a0 = v[0][u] * sx * s.x, a1 = v[1][u] * sx * s.y;
       if (kGlu) {
         a0 = gated_unit(w[0][u] * sx * more.x, a0, p.glu);
@@ -334,8 +337,9 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 
 // CTAs of a tile: as many as there are places for, with four steps (64 KB of weights) or more for each.
 int split_of(int64_t tiles, int steps) {
+  const int places = 2 * sm_count();
   int split = 1;
-  while (split < kMostSplit && tiles * split * 2 <= 2 * sm_count() && steps >= 4 * split * 2) split *= 2;
+  while (split < kMostSplit && tiles * split * 2 <= places && steps >= 4 * split * 2) split *= 2;
   return split;
 }
 

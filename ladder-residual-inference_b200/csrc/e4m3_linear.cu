@@ -15,8 +15,10 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   LRI_REQUIRE(c.rows == 0 || (c.x && c.w && c.x_scale && c.w_scale && c.y), LRI_ERR_ARG, "linear_e4m3: NULL pointer");
   LRI_REQUIRE(aligned16(c.x) && aligned16(c.w) && c.x_ld % 16 == 0 && c.w_ld % 16 == 0 && c.x_ld >= c.k && c.w_ld >= c.k, LRI_ERR_ALIGN,
               "linear_e4m3: rows of codes start at multiples of 16 bytes (pitches %lld and %lld for %d)", (long long)c.x_ld, (long long)c.w_ld, c.k);
-  LRI_REQUIRE(aligned16(c.y) && aligned16(c.bias) && aligned16(c.addend) && aligned16(c.x_scale) && aligned16(c.w_scale), LRI_ERR_ALIGN,
-              "linear_e4m3: y, bias, addend and the scales must be 16-byte aligned");
+  // (rows of a weight may be a part of a larger one's: their scales and biases start where those of the part do)
+  const auto at = [](const void* p, unsigned by) { return (reinterpret_cast<uintptr_t>(p) & (by - 1)) == 0; };
+  LRI_REQUIRE(aligned16(c.y) && aligned16(c.addend) && at(c.bias, 2) && at(c.x_scale, 4) && at(c.w_scale, 4), LRI_ERR_ALIGN,
+              "linear_e4m3: y and addend must be 16-byte aligned, bias and scales as their elements");
   if (c.rows == 0) return LRI_OK;
   const int64_t w_rows = glu ? 2ll * c.n : c.n, y_bytes = c.rows * c.n * 2;
   LRI_REQUIRE(!overlap(c.y, y_bytes, c.x, (c.rows - 1) * c.x_ld + c.k) && !overlap(c.y, y_bytes, c.w, (w_rows - 1) * c.w_ld + c.k) &&
@@ -32,9 +34,10 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   // fetch is the faster, where kAhead is what the shorter start and end of the one for few rows are worth.  us, few / pair: 128 rows, 4096 x 14336 17.0 / 22.7, 2001 x 2568
   // 6.7 / 10.6, gated 14336 x 4096 38.4 / 32.0; 256 rows, 1280 x 8192 10.7 / 13.8, 4096 x 4096 11.0 / 10.4; 512 rows, 6144 x 4096 27.6 / 15.8.  With up to 64 rows
   // the pairs' tiles are mostly padding (65 rows: 4096 x 4096 8.1 / 9.9, gated 8192 x 2048 11.6 / 15.7).
-  constexpr int64_t kAhead = 64 << 10;
+  constexpr int64_t kAhead = 64 << 10, kMostTiles = 65535;  // (of 64 rows: the second extent of a grid)
+  if (c.rows <= 64) return e4m3_few_launch(c.dtype, c.activation, p, st);
   int width = 0;
-  if (c.rows <= 64 || e4m3_few_fetched(c.activation, p) <= e4m3_pair_fetched(c.activation, p, &width) + kAhead)
-    return e4m3_few_launch(c.dtype, c.activation, p, st);
+  const int64_t pair = e4m3_pair_fetched(c.activation, p, &width);
+  if (c.rows <= 64 * kMostTiles && e4m3_few_fetched(c.activation, p) <= pair + kAhead) return e4m3_few_launch(c.dtype, c.activation, p, st);
   return e4m3_pair_launch(c.dtype, c.activation, p, width, st);
 }

@@ -105,7 +105,8 @@ def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional
            dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None) -> Tensor:
     """activation(x w^T + bias) + addend, [rows, outputs], summed in fp32 and rounded once.  activation: None, "silu", "gelu" (by the error
     function) or "gelu_tanh"; bias [outputs] and addend [rows, outputs] in the result's type; the addend may be `out`.  dtype: of the result where `out`
-    is None."""
+    is None.  The kernel reads w before the call in front of it on the stream is complete: weights, or what quantize_rows and add_rmsnorm have stored
+    (without `early`), not codes that another operator has just written."""
     rows, k, x_ld = _looked_at("x", x)
     n, depth, w_ld = _looked_at("w", w)
     if k != depth:

@@ -209,3 +209,109 @@ def test_weights_of_the_call_before(e4m3, rows):
             e4m3.add_rmsnorm(w, ones, 1e-5, add1=add, out=(codes, scale))
         y = e4m3.linear(x, (codes, scale))
         check(y, *linear64(x, (codes, scale)))
+
+
+# ---- calls around calls ------------------------------------------------------------------------------------------------------------
+SHAPES = [(1, 640, 1024, False), (40, 1100, 512, True), (100, 300, 2048, False), (300, 1100, 512, True), (700, 512, 264, False)]
+
+
+def _call(e4m3, rows, n, k, glu, seed=0):
+    x, w = random_rows(rows, k, seed), random_rows(n, k, seed + 1, size=2 * k ** -0.5)
+    return (lambda: e4m3.gateup_glu(x, w, GLUS[1])) if glu else (lambda: e4m3.linear(x, w, activation="silu"))
+
+
+def test_two_streams_at_once(e4m3):
+    """Calls share nothing on the device."""
+    calls = [_call(e4m3, *s, seed=i) for i, s in enumerate(SHAPES)]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(20):
+        for i, c in enumerate(calls):
+            with torch.cuda.stream(streams[(i + turn) % 3]):
+                got.append((i, c()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+
+
+@pytest.mark.parametrize("rows", [3, 90, 400])
+def test_captured(e4m3, rows):
+    """A run of the operators in a graph, replayed with other inputs in place."""
+    d, inter = 512, 1000
+    g = torch.Generator().manual_seed(5)
+    r, a, wt = torch.zeros(rows, d, dtype=torch.float16, device="cuda"), torch.zeros(rows, d, dtype=torch.float16, device="cuda"), torch.ones(d, dtype=torch.float16, device="cuda")
+    w1, w2 = random_rows(2 * inter, d, 1, size=d ** -0.5), random_rows(d, inter, 2, size=inter ** -0.5)
+
+    def run():
+        kept = torch.empty_like(r)
+        x = e4m3.add_rmsnorm(r, wt, 1e-5, a, residual_out=kept, early=True)
+        h = e4m3.gateup_glu(x, w1, dtype=torch.float16)
+        return e4m3.linear(e4m3.quantize_rows(h, early=True), w2, addend=kept, out=kept)
+
+    run()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = run()
+    for _ in range(4):
+        r.copy_(torch.randn(rows, d, generator=g))
+        a.copy_(torch.randn(rows, d, generator=g))
+        graph.replay()
+        assert torch.equal(y, run())
+
+
+def test_without_dependent_launches(e4m3):
+    from gpt_fast import _C
+    calls = [_call(e4m3, *s, seed=i) for i, s in enumerate(SHAPES)]
+    x = torch.randn(50, 2048, dtype=torch.float16, device="cuda")
+    want, rows = [c() for c in calls], e4m3.quantize_rows(x)
+    _C.check(_C.lib.lri_set_option(b"pdl", 0))
+    try:
+        assert all(torch.equal(c(), w) for c, w in zip(calls, want))
+        assert torch.equal(_raw(e4m3.quantize_rows(x)[0]), _raw(rows[0]))
+    finally:
+        _C.check(_C.lib.lri_set_option(b"pdl", 1))
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("lo,hi", [(0, 7), (3, 200), (197, 333)])
+def test_parts_of_weights_and_rows(e4m3, rows, lo, hi):
+    """Rows lo .. hi of a weight and of activations: scales and biases that start anywhere."""
+    x, w = random_rows(rows + 9, 264, 1), random_rows(333, 264, 2, pad=1)
+    bias = torch.randn(333, dtype=torch.bfloat16, device="cuda")
+    part = w[0][lo:hi], w[1][lo:hi]
+    few = x[0][5:5 + rows], x[1][5:5 + rows]
+    check(e4m3.linear(few, part, bias=bias[lo:hi]), *linear64(few, part, bias[lo:hi]))
+    if (hi - lo) % 2 == 0:
+        check(e4m3.gateup_glu(few, part), *glu64(few, part, GLUS[0]))
+
+
+def test_many_rows(e4m3):
+    """More rows than a grid's second extent has tiles."""
+    x, w = random_rows(64 * 65535 + 70, 16, 1), random_rows(8, 16, 2)
+    y = e4m3.linear(x, w)
+    at = torch.cat([torch.arange(300), torch.arange(x[0].shape[0] - 300, x[0].shape[0])]).cuda()
+    check(y[at], *linear64((x[0][at], x[1][at]), w))
+    assert torch.equal(y[:128], e4m3.linear((x[0][:128], x[1][:128]), w))
+
+
+def test_another_device_is_refused(e4m3):
+    x, w = random_rows(3, 64, 1), random_rows(8, 64, 2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        e4m3.linear(x, (w[0], w[1].cpu()))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        e4m3.quantize_rows(torch.zeros(3, 64, dtype=torch.bfloat16, device="cuda"), out=e4m3.empty_rows(3, 64, "cpu"))
+
+
+def test_addends_and_biases_of_the_call_before(e4m3):
+    """Only weights are read ahead: what a call has just computed may be the next one's bias or addend."""
+    x, w = random_rows(1, 2048, 1), random_rows(2048, 2048, 2, size=2048 ** -0.5)
+    first = e4m3.linear(x, w)
+    torch.cuda.synchronize()
+    want = e4m3.linear(x, w, bias=first[0], addend=first)
+    for _ in range(20):
+        y = torch.full_like(first, math.nan)
+        e4m3.linear(x, w, out=y)
+        assert torch.equal(e4m3.linear(x, w, bias=y[0], addend=y), want)
