@@ -226,6 +226,8 @@ __global__ void __launch_bounds__(256) swiglu_rows_kernel(const T* __restrict__ 
 template <typename T>
 __global__ void __launch_bounds__(256) qkv_scatter_kernel(const T* __restrict__ qkv, const LinearParams p) {
   // one thread per adjacent pair of the projection output
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t width = static_cast<int64_t>(p.n_head + 2 * p.n_kv) * p.head_dim;
   const int64_t pairs_per_row = width >> 1;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -300,9 +302,9 @@ int swiglu_rows_launch(int dtype, const void* ug, void* h, int64_t m, int n, cud
 int qkv_scatter_launch(int dtype, const void* qkv, const LinearParams& p, cudaStream_t st) {
   const int64_t items = static_cast<int64_t>(p.m) * ((static_cast<int64_t>(p.n_head + 2 * p.n_kv) * p.head_dim) >> 1);
   if (dtype == LRI_BF16)
-    qkv_scatter_kernel<__nv_bfloat16><<<blocks_for(items, 256), 256, 0, st>>>(static_cast<const __nv_bfloat16*>(qkv), p);
+    LRI_CUDA(launch_pdl(qkv_scatter_kernel<__nv_bfloat16>, dim3(blocks_for(items, 256)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(qkv), p));
   else
-    qkv_scatter_kernel<__half><<<blocks_for(items, 256), 256, 0, st>>>(static_cast<const __half*>(qkv), p);
+    LRI_CUDA(launch_pdl(qkv_scatter_kernel<__half>, dim3(blocks_for(items, 256)), dim3(256), 0, st, static_cast<const __half*>(qkv), p));
   LRI_LAUNCH_CHECK("qkv_scatter_kernel");
   return LRI_OK;
 }
