@@ -233,7 +233,8 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       asm volatile("barrier.sync 1, 128;" ::: "memory");
       // block `i` to its CTA, behind the ring's part for own sums: [group of the joining CTA][other ranks in order]
       const int owner = i & (split - 1);
-      if (ok && i < groups && owner != rank && mbar_wait_cluster(all_done, 0, &abort_flag, 74, &g_e4m3_few_status)) {
+      const bool free = ok && mbar_wait_cluster(all_done, 0, &abort_flag, 74, &g_e4m3_few_status);  // (all threads: none leaves before the others have arrived)
+      if (free && i < groups && owner != rank) {
         const int slot = (i - owner) / split * (split - 1) + (rank < owner ? rank : rank - 1);
         send(in_cta(base + Ring<BN>::kOwn + slot * kBlockBytes, owner), in_cta(landed, owner), base + i * kBlockBytes, kBlockBytes);
       }

@@ -232,32 +232,52 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  cluster_barrier();  // the barriers of both CTAs exist before either is used from the other
+  // the barriers of both CTAs exist before either is used from the other (published by the fence above: a release here waits for a busy memory system)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
-  pdl_wait();
-  pdl_launch_dependents();
+  if (warp != 0) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   const int items = grid.tiles_p * grid.tiles_q;
 
   if (warp == 0) {
     const uint32_t full_first = in_cta(full0, 0);
-    uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait on parity 1, so the first round does not block
+    // the weight rows of this CTA: half of the tile's, or all its up rows (first CTA) and all its gate rows (second)
+    auto fetch_weights = [&](uint32_t s, int kt, const WorkItem& w) {
+      // (the second CTA's bytes may arrive before this: the phase cannot end before the arrival counted here)
+      if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * stage_bytes);
+      const int w_row = kGlu ? static_cast<int>(rank) * p.n + w.tile_q * half : w.tile_q * bn + static_cast<int>(rank) * half;
+      tma_load_pair(base + s * stage_bytes + kTileBytes, &tmap_w, full_first + 8 * s, kt * kStep, w_row);
+    };
+    auto fetch_rows = [&](uint32_t s, int kt, const WorkItem& w) {
+      tma_load_pair(base + s * stage_bytes, &tmap_x, full_first + 8 * s, kt * kStep, w.tile_p * 2 * kBM + static_cast<int>(rank) * kBM);
+    };
+    // the weights of the first stages do not depend on the preceding kernel
+    const int ahead = min(static_cast<int>(stages), num_kt);  // (every pair has an item)
+    const WorkItem first = work_item(pair, grid);
+    for (int i = 0; i < ahead; ++i)
+      if (elect_one()) fetch_weights(i, i, first);
+    __syncwarp();
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int i = 0; i < ahead; ++i)
+      if (elect_one()) fetch_rows(i, i, first);
+    __syncwarp();
+    uint32_t s = ahead, parity = 1;  // a fresh barrier passes a wait on parity 1, so the first round does not block
+    if (s == stages) s = 0, parity = 0;
     bool ok = true;
     for (int item = pair; item < items && ok; item += pairs) {
       const WorkItem w = work_item(item, grid);
-      // the weight rows of this CTA: half of the tile's, or all its up rows (first CTA) and all its gate rows (second)
-      const int w_row = kGlu ? static_cast<int>(rank) * p.n + w.tile_q * half : w.tile_q * bn + static_cast<int>(rank) * half;
-      const int x_row = w.tile_p * 2 * kBM + static_cast<int>(rank) * kBM;
-      for (int kt = 0; kt < num_kt; ++kt) {
+      for (int kt = item == pair ? ahead : 0; kt < num_kt; ++kt) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 61, &g_e4m3_pair_status));
         if (!ok) break;
         if (elect_one()) {
-          // (the second CTA's bytes may arrive before this: the phase cannot end before the arrival counted here)
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * stage_bytes);
-          const uint32_t dst = base + s * stage_bytes;
-          tma_load_pair(dst, &tmap_x, full_first + 8 * s, kt * kStep, x_row);
-          tma_load_pair(dst + kTileBytes, &tmap_w, full_first + 8 * s, kt * kStep, w_row);
+          fetch_weights(s, kt, w);
+          fetch_rows(s, kt, w);
         }
+        __syncwarp();
         if (++s == stages) s = 0, parity ^= 1u;
       }
     }
