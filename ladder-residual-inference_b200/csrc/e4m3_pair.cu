@@ -104,39 +104,53 @@ __device__ __forceinline__ void get_values(uint32_t block, int lane, float (&f)[
   }
 }
 
-// One block: rows row0 .. row0 + 31, columns j0 .. j0 + 31 (j0 < n), sums at `tacc` (GLU: of the gate at `tgate`).
+// What a block needs of memory, asked for one block ahead (the first one's while its sums are still being made): behind the sums an addend's trip to memory took
+// 3200 cycles a block, four to eight times a tile, which short sums do not hide (2048 x 8192 x 1024 with addend NOWA).
+template <bool VEC>
+struct Beside {
+  float s[VEC ? 8 : 1], more[VEC ? 8 : 1];  // scales of the columns; their biases, or the scales of the gate
+  uint4 add[VEC ? 4 : 1];
+};
+
+// Rows row0 .. row0 + 31, columns j0 .. j0 + 31.  VEC: this thread's columns are the 8 from j0 + lane % 4 * 8 on, of every eighth row; else column j0 + lane of
+// every row.
 template <typename T, int ACT, bool VEC>
-__device__ __forceinline__ void store_block(const E4m3Linear& p, int64_t row0, int64_t j0, float sx, uint32_t block, uint32_t tacc, uint32_t tgate) {
-  constexpr bool kGlu = ACT == LRI_ACT_GLU;
+__device__ __forceinline__ void load_beside(const E4m3Linear& p, int64_t row0, int64_t j0, Beside<VEC>& b) {
+  const int lane = threadIdx.x & 31;
+  const int64_t j = j0 + (VEC ? (lane & 3) * 8 : lane);
   constexpr int kCols = VEC ? 8 : 1;
+  if (j >= p.n) return;
+#pragma unroll
+  for (int e = 0; e < kCols; ++e) b.s[e] = p.w_scale[j + e];
+  if (ACT == LRI_ACT_GLU) {
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) b.more[e] = p.w_scale[p.n + j + e];
+  } else {
+    const T* bias = static_cast<const T*>(p.bias) + j;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) b.more[e] = p.bias ? Num<T>::to_f(bias[e]) : 0.f;
+  }
+  if (ACT != LRI_ACT_GLU && VEC && p.addend) {
+#pragma unroll
+    for (int it = 0; it < (VEC ? 4 : 1); ++it) {
+      const int64_t row = row0 + it * 8 + (lane >> 2);
+      if (row < p.rows) b.add[it] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.addend) + row * p.n + j);
+    }
+  }
+}
+
+// One block (j0 < n), sums at `tacc` (GLU: of the gate at `tgate`).
+template <typename T, int ACT, bool VEC>
+__device__ __forceinline__ void store_block(const E4m3Linear& p, int64_t row0, int64_t j0, float sx, uint32_t block, uint32_t tacc, uint32_t tgate,
+                                            const Beside<VEC>& b) {
+  constexpr bool kGlu = ACT == LRI_ACT_GLU;
   const int lane = threadIdx.x & 31;
   const int64_t j = j0 + (VEC ? (lane & 3) * 8 : lane);
   const bool there = j < p.n;
   auto row_of = [&](int it, int e) { return row0 + (VEC ? it * 8 + (lane >> 2) : it * 8 + e); };
-
-  // what does not depend on the sums is asked for before they are waited for
   uint32_t r[32];
   __syncwarp();
   tmem_ld32_issue(tacc, r);
-  float s[kCols] = {}, more[kCols] = {};  // scales of the columns; their biases, or the scales of the gate
-  uint4 add[4] = {};
-  if (there) {
-#pragma unroll
-    for (int e = 0; e < kCols; ++e) s[e] = p.w_scale[j + e];
-    if (kGlu) {
-#pragma unroll
-      for (int e = 0; e < kCols; ++e) more[e] = p.w_scale[p.n + j + e];
-    } else if (p.bias) {
-      const T* bias = static_cast<const T*>(p.bias) + j;
-#pragma unroll
-      for (int e = 0; e < kCols; ++e) more[e] = Num<T>::to_f(bias[e]);
-    }
-    if (!kGlu && VEC && p.addend) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-        if (row_of(it, 0) < p.rows) add[it] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.addend) + row_of(it, 0) * p.n + j);
-    }
-  }
   float f[4][8];
   tmem_wait_ld();
   put_row(block, lane, r, sx);
@@ -153,20 +167,20 @@ __device__ __forceinline__ void store_block(const E4m3Linear& p, int64_t row0, i
 #pragma unroll
     for (int it = 0; it < 4; ++it)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[it][e] = gated_unit(g[it][e] * more[VEC ? e : 0], f[it][e] * s[VEC ? e : 0], p.glu);
+      for (int e = 0; e < 8; ++e) f[it][e] = gated_unit(g[it][e] * b.more[VEC ? e : 0], f[it][e] * b.s[VEC ? e : 0], p.glu);
   } else {
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
       float a[8] = {};
       if (VEC) {
-        unpack8<T>(add[it], a);
+        if (p.addend) unpack8<T>(b.add[VEC ? it : 0], a);
       } else if (there && p.addend) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (row_of(it, e) < p.rows) a[e] = Num<T>::to_f(static_cast<const T*>(p.addend)[row_of(it, e) * p.n + j]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[it][e] = activate<ACT>(f[it][e] * s[VEC ? e : 0] + more[VEC ? e : 0]) + a[e];
+      for (int e = 0; e < 8; ++e) f[it][e] = activate<ACT>(f[it][e] * b.s[VEC ? e : 0] + b.more[VEC ? e : 0]) + a[e];
     }
   }
   if (there) {
@@ -182,6 +196,25 @@ __device__ __forceinline__ void store_block(const E4m3Linear& p, int64_t row0, i
       }
     }
   }
+}
+
+// This warp's blocks of a tile of `cols` columns, every second one from the first + `turn` on; `ready` waits for the sums.
+template <typename T, int ACT, bool VEC, typename F>
+__device__ __forceinline__ bool store_tile(const E4m3Linear& p, int64_t row0, int64_t tile0, int cols, int turn, float sx, uint32_t block, uint32_t tacc, uint32_t tgate,
+                                           const F& ready) {
+  constexpr int kStride = kStoreWarps / 4 * 32;
+  const int end = row0 < p.rows ? static_cast<int>(min(static_cast<int64_t>(cols), p.n - tile0)) : 0;
+  Beside<VEC> now{}, next{};
+  int cc = turn * 32;
+  if (cc < end) load_beside<T, ACT, VEC>(p, row0, tile0 + cc, now);
+  if (!ready()) return false;
+#pragma unroll 1
+  for (; cc < end; cc += kStride) {
+    if (cc + kStride < end) load_beside<T, ACT, VEC>(p, row0, tile0 + cc + kStride, next);
+    store_block<T, ACT, VEC>(p, row0, tile0 + cc, sx, block, tacc + cc, tgate + cc, now);
+    now = next;
+  }
+  return true;
 }
 
 template <typename T, int ACT>
@@ -331,19 +364,16 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       const int64_t row0 = static_cast<int64_t>(w.tile_p) * 2 * kBM + rank * kBM + quarter * 32;
       const float sx = row0 + lane < p.rows ? p.x_scale[row0 + lane] : 0.f;
       // the tcgen05.ld of the epilogue are warp-collective: the warp leaves together or not at all
-      const bool ready = mbar_wait(acc_full0 + 8 * a, use & 1u, &abort_flag, 63, &g_e4m3_pair_status);
-      if (!__all_sync(0xffffffffu, ready)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      auto ready = [&]() {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * a, use & 1u, &abort_flag, 63, &g_e4m3_pair_status));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return there;
+      };
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * kAccCols;
-#pragma unroll 1
-      for (int cc = (warp - 2) / 4 * 32; cc < cols; cc += kStoreWarps / 4 * 32) {
-        const int64_t j0 = static_cast<int64_t>(w.tile_q) * cols + cc;
-        if (j0 >= p.n || row0 >= p.rows) break;
-        if (vectors)
-          store_block<T, ACT, true>(p, row0, j0, sx, block, tacc + cc, tacc + half + cc);
-        else
-          store_block<T, ACT, false>(p, row0, j0, sx, block, tacc + cc, tacc + half + cc);
-      }
+      const int64_t tile0 = static_cast<int64_t>(w.tile_q) * cols;
+      const bool stored = vectors ? store_tile<T, ACT, true>(p, row0, tile0, cols, (warp - 2) / 4, sx, block, tacc, tacc + half, ready)
+                                  : store_tile<T, ACT, false>(p, row0, tile0, cols, (warp - 2) / 4, sx, block, tacc, tacc + half, ready);
+      if (!stored) break;
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive_in_cluster(in_cta(acc_empty0 + 8 * a, 0));

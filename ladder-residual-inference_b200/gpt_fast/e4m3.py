@@ -39,7 +39,7 @@ def _looked_at(what, rows, cols=None, count=None):
         n, k = shape
         pitch = strides[0] if n != 1 else -(-k // 16) * 16  # (the pitch of a single row may be any number)
         if (codes.dtype is E4M3 and strides[1] == 1 and pitch % 16 == 0 and pitch >= k > 0 and k % 8 == 0 and (cols is None or k == cols and n == count) and
-                scale.dtype is _F32 and scale.numel() == n and scale.dim() == 1 and scale.is_contiguous()):
+                scale.dtype is _F32 and scale.numel() == n and scale.is_contiguous()):
             return n, k, pitch
     want = "[rows, a multiple of 8]" if cols is None else f"[{count}, {cols}]"
     raise ValueError(f"{what}: float8_e4m3fn codes {want} whose rows start at multiples of 16 bytes (e4m3.empty_rows) and a contiguous fp32 scale for "
@@ -87,13 +87,11 @@ def add_rmsnorm(residual: Tensor, weight: Tensor, eps: float, add1: Optional[Ten
     rows, dim = shape if len(shape) == 2 else (-1, 0)
     if not (rows >= 0 and dtype in _WIDE and dim % 8 == 0 and 0 < dim <= 16384 and residual.is_contiguous()):
         raise ValueError(f"residual: contiguous bfloat16 or float16 rows of a multiple of 8 elements up to 16384, not {_said(residual)}")
-    _dense("weight", weight, dtype, (dim,))
-    if add1 is not None:
-        _dense("add1", add1, dtype, shape)
-    if add2 is not None:
-        _dense("add2", add2, dtype, shape)
-    if residual_out is not None:
-        _dense("residual_out", residual_out, dtype, shape)
+    if not (weight.dtype is dtype and weight.numel() == dim and weight.is_contiguous()):
+        _dense("weight", weight, dtype, (dim,))
+    for name, t in (("add1", add1), ("add2", add2), ("residual_out", residual_out)):
+        if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+            _dense(name, t, dtype, shape)
     if out is None:
         out = empty_rows(rows, dim, residual.device)
     _, _, codes_ld = _looked_at("out", out, dim, rows)
@@ -113,7 +111,8 @@ def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional
         raise ValueError(f"rows of {k} codes times weights of {depth}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation={activation!r}: one of {list(ACTIVATIONS)}")
-    out = _result(out, dtype, rows, n, x[0].device)
+    if out is None or not (out.dtype in _WIDE and out.shape == (rows, n) and out.is_contiguous()):
+        out = _result(out, dtype, rows, n, x[0].device)
     if bias is not None:
         _dense("bias", bias, out.dtype, (n,))
     if addend is not None:
