@@ -10,7 +10,13 @@
 // counts the bytes.  (Sums left in place, a cluster barrier, loads out of the others' shared memory and a barrier at the end took 2.2 to
 // 2.7 us behind the last product, the barrier alone 0.5; stores that count their own bytes, 16 at a time, take 1 ns each: 2 us for 64 rows.)
 //
-// Two CTAs fit an SM: with 96 to 108 KB of ring each, 200 KB of weights are under way per SM whichever the tile's share.
+// Two CTAs fit an SM: with 96 to 108 KB of ring each, 200 KB are under way per SM whichever the tile's share.  us with rings of 36, 54, 72, 108 KB (an earlier
+// form): 1 x 6144 x 4096 8.6, 8.2, 7.8, 7.1; 24 x 4096 x 14336 20.0, 16.7, 15.3, 14.1; 4 gated rows of 14336 from 4096 24.2, 22.4, 21.5, 20.3; with one CTA of 200 KB 7.9, 14.0,
+// 24.8.
+//
+// us and TB/s, one B200, weights out of memory, calls behind one another in a graph: 1 x 6144 x 4096 6.0 (4.2), 24 x 4096 x 14336 with addend 12.5 (4.8), 4 gated rows of 14336
+// from 4096 19.6 (6.0), of 28672 from 8192 70 (6.7), 64 gated rows of 8192 from 2048 9.9 (3.5).  What a call takes beside its bytes is about 3 us: 1 to
+// 1.7 until the last CTA runs and its first bytes come, 1 from the last product to the sums in the joining CTA, 0.5 to 1 for joining.
 //
 // Gated unit: a tile is 64 up rows and the 64 matching gate rows; up and gate of an output meet where the sums are joined.
 //
@@ -134,7 +140,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's barriers exist (published by the fence above)
 
   // What joining the sums needs of memory is asked for at the start, and a part of the addend brought to the L2: behind the last product each of
-  // these was a trip to memory of its own (64 rows of 8192 gated outputs from 2048: 11.7 us, NOW here).
+  // these was a trip to memory of its own (64 rows of 8192 gated outputs from 2048: 11.7 us, 11.1 here).
   constexpr int kPairs = kOut / 2, kAtOnce = kGemmThreads / kPairs;
   const int c = 2 * static_cast<int>(threadIdx.x % kPairs);
   const int64_t j = static_cast<int64_t>(tile) * kOut + c;
@@ -336,7 +342,9 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// CTAs of a tile: as many as there are places for, with four steps (64 KB of weights) or more for each.
+// CTAs of a tile: as many as there are places for, with four steps (64 KB of weights) or more for each.  us with at most 2 / 4 / 8: 1 x 1280 x 8192 8.8 / 6.2 / 4.7,
+// 16 x 4096 x 14336 16.0 / 14.0 / 12.1.  With one place an SM 1 x 6144 x 4096 8.5 (6.4), 16 gated rows of 8192 from 2048 9.8 (8.0).  At least 2 / 4 / 8 steps: 1 x 2048 x 1024
+// 2.95 / 3.28 / 3.77, 1 x 2048 x 2048 3.48 / 3.39 / 4.13, 64 x 2048 x 2048 5.61 / 4.84 / 6.25.
 int split_of(int64_t tiles, int steps) {
   const int places = 2 * sm_count();
   int split = 1;
@@ -388,6 +396,7 @@ int e4m3_few_launch(int dtype, int activation, const E4m3Linear& p, cudaStream_t
   return by_activation(dtype, activation, [&](auto t, auto act) {
     using T = typename decltype(t)::type;
     constexpr int kAct = decltype(act)::value;
+    // (a narrower tile leaves the ring more stages; us, 16 rows in tiles of 16 / 32 / 64: 6144 x 4096 6.4 / 6.6 / 7.7, gated 14336 from 4096 20.2 / 20.4 / 23.3)
     if (p.rows <= 16) return launch<T, kAct, 16>(p, st);
     if (p.rows <= 32) return launch<T, kAct, 32>(p, st);
     return launch<T, kAct, 64>(p, st);

@@ -11,7 +11,16 @@
 // Gated unit: a tile is bn / 2 up rows and the bn / 2 matching gate rows, fetched by one CTA of the pair each.
 //
 // Roles per CTA: warp 0 fetches (TMA, no multicast), warp 1 owns the tensor memory and, in the first CTA, issues the products, warps 2-9
-// store.  Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
+// store.  A block of 32 x 32 takes them some 1100 cycles, 1800 with what surrounds it, 3000 with GELU or the gated unit (the special-function unit), so a tile of
+// 256 x 256 takes 7000 to 12000: hidden behind the products of 128 x 256 from a depth of 1500 (GELU, gated 2000) on, and the pace of a projection below
+// (2048 x 8192 x 1024 23.8 us, 2.9 times its products).  Four storing warps instead of eight: us, 1000 x 4096 x 14336 47.0 / 45.9, 4096 x 4096 x 4096 with GELU 58.0 / 55.0,
+// 2048 x 8192 x 1024 with addend 37.9 / 31.0.
+//
+// us and TFLOP/s, one B200, weights and tokens out of memory: 2048 x 6144 x 4096 40.1 (2570), 4096 x 8192 x 8192 with addend 185 (2970), 4096 gated rows of 14336 from 4096
+// 332 (2900), 8192 x 8192 x 8192 379 (2900; the 1000 W cap sets the clock); the tensor pipe is busy for 83 to 88 % of a launch.  With 129 to 512 rows an SM takes in
+// too much for too few products: 256 x 4096 x 14336 22.3 us, 2.3 times the weights' time.
+//
+// Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
 // uses, is said in gemm_pair.cu and holds here.
 #include "e4m3.cuh"
 #include "e4m3_tc.cuh"
@@ -104,8 +113,8 @@ __device__ __forceinline__ void get_values(uint32_t block, int lane, float (&f)[
   }
 }
 
-// What a block needs of memory, asked for one block ahead (the first one's while its sums are still being made): behind the sums an addend's trip to memory took
-// 3200 cycles a block, four to eight times a tile, which short sums do not hide (2048 x 8192 x 1024 with addend NOWA).
+// What a block needs of memory, asked for one block ahead, the first one's while its sums are still being made (us, behind the sums / here: 256 x 4096 x 4096 10.1 / 9.7,
+// 2048 gated rows of 8192 from 2048 52.9 / 52.1).
 template <bool VEC>
 struct Beside {
   float s[VEC ? 8 : 1], more[VEC ? 8 : 1];  // scales of the columns; their biases, or the scales of the gate
@@ -395,7 +404,9 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 }
 
 // Width of the tile: the one with which the busiest SM fetches least.  (A K step of 128 x bn takes 337, 382, 436, 505, 563 cycles at 128 .. 256 by 32, see gemm_pair.cu,
-// as its bytes do at 57 a cycle; so the narrower tile wins where it fills the last round.  GLU: half a tile's columns in blocks of 32.)
+// as its bytes do at 57 a cycle; so the narrower tile wins where it fills the last round.  us, chosen / 256 / 128 / 64: 512 x 6144 x 4096 15.5 / 18.2 / 17.4 / 20.5,
+// 1000 x 2048 x 8192 17.4 / 25.7 / 17.4 / 24.4, 2048 x 6144 x 4096 40.4 / 40.5 / 44.5 / 61.4, 256 x 4096 x 4096 10.1 / 11.1 / 11.0 / 10.1.  GLU: half a tile's
+// columns in blocks of 32.)
 int64_t fetched(const E4m3Linear& p, bool glu, int* width) {
   const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, by = glu ? 64 : 32;
   const int64_t w_rows = glu ? 2ll * p.n : p.n, steps = (p.k + kStep - 1) / kStep;

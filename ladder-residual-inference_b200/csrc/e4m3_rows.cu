@@ -7,7 +7,8 @@
 // most 11 bits), so codes do not depend on the order of any sum.
 //
 // Bound by memory: 2 bytes an element in for each tensor, 2 for the residual and 1 for the codes out.  The row stays in registers, as it
-// was rounded, between the two passes over it.
+// was rounded, between the two passes over it.  One B200, us and TB/s: norm of 8192 x 4096 with an addend 36.0 (6.5, the rate of a copy), of 1 and 40 rows 1.7; rows as they
+// are, 4096 x 14336 26.9 (6.6), 2047 x 11000 12.5 (5.4).  Kernels for 0, 1 and 2 addends: with the choice in the kernel their registers were there for all (8192 x 4096 43.4 us).
 #include "e4m3.cuh"
 
 namespace lri {
@@ -24,7 +25,9 @@ struct RowsParams {
   bool early;         // the next kernel may start: it waits for this one before it reads the results
 };
 
-constexpr int kFewRows = 148;  // one CTA an SM: up to here a row gets up to 1024 threads, and the kernel is a latency chain
+// One CTA an SM: up to here a row gets up to 1024 threads, and the kernel is a latency chain.  (us with 148 / 592: 500 rows of 8192 with an addend 7.3 / 8.3, 300 of 16384 9.1 /
+// 10.9, 500 of 28672 as they are 9.6 / 12.1; the other way, 16 rows of 4096 take 1.9 with 256 threads and 1.7 with 512.)
+constexpr int kFewRows = 148;
 
 // ADDS: pending addends of a norm, -1: rows as they are.  NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
 template <typename T, int ADDS, int NV, int THREADS>
@@ -154,6 +157,9 @@ int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {
     if (nvec <= 1024) return launch_nv<T, ADDS, 1, 1024>(p, rows, st);
     if (nvec <= 2048) return launch_nv<T, ADDS, 2, 1024>(p, rows, st);
   }
+  // Many rows: CTAs small enough that others run while one waits at its barrier.  us, threads x vectors: a norm of 16384 with an addend (2048 rows) 1024 x 2 48.3, 512 x 4
+  // 37.1, 256 x 8 37.9; of 11000 (3000) 57.3, 38.8, 41.5; of 8192 (4096) 512 x 2 36.6, 256 x 4 36.7.  As they are, 14336 (4096) 512 x 4 27.5, 256 x 8 26.9; 28672 (2048) 1024 x 4 36.9,
+  // 512 x 8 27.5.
   if (nvec <= 512) return launch_nv<T, ADDS, 2, 256>(p, rows, st);
   if constexpr (ADDS >= 0) {
     if (nvec <= 1024) return launch_nv<T, ADDS, 2, 512>(p, rows, st);
