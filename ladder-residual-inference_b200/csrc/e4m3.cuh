@@ -42,7 +42,7 @@ __device__ __forceinline__ float sigmoid_fast(float t) {
 
 // z * Phi(z), Phi the normal distribution: Phi(-x) = erfc(x / sqrt 2) / 2 for x >= 0 by Abramowitz and Stegun's 7.1.26, (a1 t + .. + a5 t^5) exp(-x^2 / 2)
 // / 2 with t = 1 / (1 + p x / sqrt 2), to 0.75e-7 (1.3 * 2^-24), and Phi(x) = 1 - Phi(-x).  (erff, which chooses between two ranges: 88 us
-// for 4096 x 4096 x 4096 with GELU.)
+// for 4096 x 4096 x 4096 with GELU, 63 with this.)
 __device__ __forceinline__ float gelu(float z) {
   const float x = fabsf(z);
   float t;

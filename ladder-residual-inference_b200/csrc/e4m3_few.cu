@@ -1,4 +1,4 @@
-// Projections in 8 bits of few rows (up to kE4m3FewRows tokens): a decode step of a batch, a short prompt.
+// Projections in 8 bits of few rows: a decode step of a batch, a short prompt.
 //
 // Bound by reading the weights once.  As in gemm_streamk.cu the weights are the 128-row operand of tcgen05.mma and the tokens its N side (16
 // to 64 wide, in as many tiles as there are).  What differs is how the work is spread and joined.  A tile of 128 outputs is one cluster's: its 1, 2, 4 or 8 CTAs take
@@ -34,8 +34,7 @@ __device__ int g_e4m3_few_status = 0;
 
 constexpr int kTileBytes = kBM * kStep;  // of 128 weight rows
 constexpr int kMostSplit = 8;
-
-constexpr int kRing = 108 * 1024;  // of a CTA, two of which share an SM
+constexpr int kRing = 108 * 1024;      // of a CTA, two of which share an SM
 constexpr int kBlockBytes = kBM * 16;  // sums of 128 outputs x 4 tokens
 
 template <int BN>

@@ -144,3 +144,12 @@ def test_no_call_and_no_rows(entry):
 def test_structs_have_the_sizes_of_the_header():
     assert _C.QUANTIZE_CALL.size == 72 and _C.NORM8_CALL.size == 104 and _C.LINEAR8_CALL.size == 120
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+@pytest.mark.parametrize("change,text", [(dict(dtype=2), "dtype"), (dict(B=-1), "B=-1"), (dict(head_dim=12), "multiple of 8"), (dict(smax=0), "smax"), (dict(qkv=0), "qkv"),
+                                         (dict(qkv=_AT + 8), "qkv"), (dict(table=0), "NULL"), (dict(k=3 * _AT + 4), "aligned")])
+def test_rotation_refuses(change, text):
+    a = dict(dtype=0, qkv=_AT, table=2 * _AT, pos=3 * _AT + 64, q=4 * _AT, k=5 * _AT, v=6 * _AT, B=1, S=2, n_head=4, n_kv=2, head_dim=64, smax=32, rows=32)
+    a.update(change)
+    status = _C.lib.lri_rope_kvcache(a["dtype"], a["qkv"], a["table"], a["pos"], 0, a["q"], a["k"], a["v"], a["B"], a["S"], a["n_head"], a["n_kv"], a["head_dim"], a["smax"], a["rows"], 0, None)
+    assert status < 0 and text in _C.lib.lri_last_error().decode(), _C.lib.lri_last_error()
