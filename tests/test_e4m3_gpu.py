@@ -166,6 +166,33 @@ def test_gateup(e4m3, rows, inter, k, glu):
     assert (room[rows:] == 5).all()
 
 
+@pytest.mark.parametrize("rows,n,k", [(257, 640, 11000), (256, 4096, 14336), (300, 1333, 8200), (1000, 1001, 12296), (512, 4096, 9000), (131, 2048, 16384), (1024, 200, 5000)])
+@pytest.mark.parametrize("how", ["plain", "all"])
+def test_few_tiles_of_long_sums(e4m3, rows, n, k, how):
+    """Few tiles, many steps each: the ends of the rounds of both kernels."""
+    dtype = TYPES[n % 2]
+    x, w = random_rows(rows, k, 1), random_rows(n, k, 2, size=2 * k ** -0.5)
+    g = torch.Generator().manual_seed(3)
+    more = {} if how == "plain" else dict(bias=torch.randn(n, generator=g).to(dtype).cuda(), activation="gelu", addend=torch.randn(rows, n, generator=g).to(dtype).cuda())
+    room = torch.full((rows + 1, n), 5.0, dtype=dtype, device="cuda")
+    y = e4m3.linear(x, w, out=room[:rows], **more)
+    check(y, *linear64(x, w, dtype=dtype, **more))
+    assert (room[rows:] == 5).all()
+    for _ in range(5):
+        assert torch.equal(y, e4m3.linear(x, w, dtype=dtype, **more))
+
+
+@pytest.mark.parametrize("rows,inter,k", [(1000, 1024, 8192), (257, 1500, 6000), (512, 2047, 9000), (1024, 130, 4104)])
+@pytest.mark.parametrize("glu", GLUS)
+def test_gateup_of_few_tiles_and_long_sums(e4m3, rows, inter, k, glu):
+    dtype = TYPES[inter % 2]
+    x, w = random_rows(rows, k, 1), random_rows(2 * inter, k, 2, size=2 * k ** -0.5)
+    h = e4m3.gateup_glu(x, w, glu, dtype=dtype)
+    check(h, *glu64(x, w, glu, dtype))
+    for _ in range(5):
+        assert torch.equal(h, e4m3.gateup_glu(x, w, glu, dtype=dtype))
+
+
 @pytest.mark.parametrize("rows", [2, 20, 100, 300])
 @pytest.mark.parametrize("kind", ["linear", "gateup"])
 def test_rows_that_are_nan_stay_alone(e4m3, rows, kind):
