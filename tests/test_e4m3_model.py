@@ -94,7 +94,7 @@ def test_what_is_refused(no_library):
 @pytest.mark.parametrize("world", [1, 2])
 def test_ranks(world):
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={world}", "--master-addr", "127.0.0.1",
-           "--master-port", str(29770 + world), os.path.join(ROOT, "tests", "e4m3_cpu_worker.py")]
+           "--master-port", str(29830 + world), os.path.join(ROOT, "tests", "e4m3_cpu_worker.py")]
     r = subprocess.run(cmd, capture_output=True, text=True, timeout=600, env=dict(os.environ, OMP_NUM_THREADS="2", CUDA_VISIBLE_DEVICES=""))
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
     assert "E4M3-CPU-OK" in r.stdout
