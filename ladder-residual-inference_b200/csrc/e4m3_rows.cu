@@ -29,22 +29,22 @@ struct RowsParams {
 // 10.9, 500 of 28672 as they are 9.6 / 12.1; the other way, 16 rows of 4096 take 1.9 with 256 threads and 1.7 with 512.)
 constexpr int kFewRows = 148;
 
-// ADDS: pending addends of a norm, -1: rows as they are.  NV: vectors of 8 elements that a thread keeps; a row has at most THREADS * NV of them
-template <typename T, int ADDS, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) {
+// ADDS: pending addends of a norm, -1: rows as they are.  NV: vectors of 8 elements that a thread keeps, of a row that has at most
+// blockDim * NV of them.  A CTA has as many threads as the row needs, up to MOST, or (ALL) MOST in any case.
+template <typename T, int ADDS, int NV, int MOST, bool ALL>
+__global__ void __launch_bounds__(MOST) rows_e4m3_kernel(const RowsParams p) {
   constexpr bool NORM = ADDS >= 0;
-  constexpr int kWarps = THREADS / 32;
   const int64_t row = blockIdx.x;
   const int nvec = p.cols >> 3;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ float part_sum[kWarps];
-  __shared__ uint32_t part_top[kWarps];
+  const int threads = ALL ? MOST : blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float part_sum[MOST / 32];
+  __shared__ uint32_t part_top[MOST / 32];
 
   uint4 w[NV];
   if (NORM) {  // a constant of the model: fetched while the preceding kernel drains
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * THREADS;
+      const int v = threadIdx.x + i * threads;
       if (v < nvec) w[i] = __ldg(static_cast<const uint4*>(p.weight) + v);
     }
   }
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * THREADS;
+    const int v = threadIdx.x + i * threads;
     if (v < nvec) {
       x[i] = in[v];
       if (ADDS > 0) a[i] = a1[v];
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * THREADS;
+    const int v = threadIdx.x + i * threads;
     if (v >= nvec) continue;
     float f[8];
     unpack8<T>(x[i], f);
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   if (lane == 0) part_top[warp] = top;
   __syncthreads();
   // every warp joins the parts by itself: no second barrier
-  top = __reduce_max_sync(0xffffffffu, lane < kWarps ? part_top[lane] : 0u);
-  if (NORM) ss = warp_sum(lane < kWarps ? part_sum[lane] : 0.f);
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? part_top[lane] : 0u);
+  if (NORM) ss = warp_sum(lane < warps ? part_sum[lane] : 0.f);
 
   const bool bad = top >= kInfBits;
   const float most = fmaxf(__uint_as_float(top), kE4m3Smallest);
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   uint2* codes = reinterpret_cast<uint2*>(p.codes + row * p.codes_ld);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * THREADS;
+    const int v = threadIdx.x + i * threads;
     if (v >= nvec) continue;
     float f[8];
     unpack8<T>(x[i], f);
@@ -140,35 +140,35 @@ __global__ void __launch_bounds__(THREADS) rows_e4m3_kernel(const RowsParams p) 
   }
 }
 
-template <typename T, int ADDS, int NV, int THREADS>
+template <typename T, int ADDS, int NV, int MOST, bool ALL = false>
 int launch_nv(const RowsParams& p, int64_t rows, cudaStream_t st) {
-  LRI_CUDA(launch_pdl(rows_e4m3_kernel<T, ADDS, NV, THREADS>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, p));
+  const int threads = ALL ? MOST : ((p.cols / 8 + NV - 1) / NV + 31) / 32 * 32;
+  LRI_CUDA(launch_pdl(rows_e4m3_kernel<T, ADDS, NV, MOST, ALL>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, st, p));
   LRI_LAUNCH_CHECK(ADDS >= 0 ? "rows_e4m3_kernel<norm>" : "rows_e4m3_kernel");
   return LRI_OK;
 }
 
+// Many rows: CTAs small enough that others run while one waits at its barrier, and no larger than the row (us, all threads / as many as it needs: norms with an addend
+// of 16000 x 768 25.9 / 16.6, 4096 x 5120 27.7 / 24.9; rows as they are 20000 x 768 20.5 / 12.5, 8192 x 5504 22.7 / 21.4; but as they are 2048 x 28672 27.2 / 40.9, where the
+// stride of a thread has to be a number the compiler knows).  us by vectors a thread, norms: 16000 x 768 1 16.6, 2 17.8, 4 15.2; 8192 x 2048 21.6, 19.3, 19.9; 8192 x 4096 1 41.2, 2 36.2,
+// 4 36.5; 4096 x 8192 1 44.2, 2 37.0, 4 36.6, and 500 of them 8.2, 7.4, 7.8; 2048 x 16384 2 48.8, 4 37.1, 8 38.4.  As they are: 16000 x 2048 1 21.4, 2 16.1, 4 16.1; 8192 x 4096 1 23.6,
+// 2 17.0, 4 16.2; 4096 x 8192 2 17.8, 4 16.2, 8 16.6; 4096 x 14336 2 32.9, 4 27.8, 8 27.2; 2048 x 28672 4 36.9, 8 27.2.
 template <typename T, int ADDS>
 int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {
   const int nvec = p.cols / 8;
   const bool few = rows <= kFewRows;
-  if (nvec <= 256) return launch_nv<T, ADDS, 1, 256>(p, rows, st);
-  if (few) {
-    if (nvec <= 512) return launch_nv<T, ADDS, 1, 512>(p, rows, st);
-    if (nvec <= 1024) return launch_nv<T, ADDS, 1, 1024>(p, rows, st);
-    if (nvec <= 2048) return launch_nv<T, ADDS, 2, 1024>(p, rows, st);
-  }
-  // Many rows: CTAs small enough that others run while one waits at its barrier.  us, threads x vectors: a norm of 16384 with an addend (2048 rows) 1024 x 2 48.3, 512 x 4
-  // 37.1, 256 x 8 37.9; of 11000 (3000) 57.3, 38.8, 41.5; of 8192 (4096) 512 x 2 36.6, 256 x 4 36.7.  As they are, 14336 (4096) 512 x 4 27.5, 256 x 8 26.9; 28672 (2048) 1024 x 4 36.9,
-  // 512 x 8 27.5.
-  if (nvec <= 512) return launch_nv<T, ADDS, 2, 256>(p, rows, st);
+  if (few && nvec <= 1024) return launch_nv<T, ADDS, 1, 1024>(p, rows, st);
+  if (few && nvec <= 2048) return launch_nv<T, ADDS, 2, 1024>(p, rows, st);
+  if (nvec <= 256) return launch_nv<T, ADDS, 4, 64>(p, rows, st);
   if constexpr (ADDS >= 0) {
+    if (nvec <= 512) return launch_nv<T, ADDS, 2, 256>(p, rows, st);
     if (nvec <= 1024) return launch_nv<T, ADDS, 2, 512>(p, rows, st);
     if (nvec <= 2048) return launch_nv<T, ADDS, 4, 512>(p, rows, st);
   } else {
     if (nvec <= 1024) return launch_nv<T, ADDS, 4, 256>(p, rows, st);
     if (nvec <= 2048) return launch_nv<T, ADDS, 8, 256>(p, rows, st);
-    if (nvec <= 4096) return few ? launch_nv<T, ADDS, 4, 1024>(p, rows, st) : launch_nv<T, ADDS, 8, 512>(p, rows, st);
-    if (nvec <= 8192) return launch_nv<T, ADDS, 8, 1024>(p, rows, st);
+    if (nvec <= 4096) return few ? launch_nv<T, ADDS, 4, 1024>(p, rows, st) : launch_nv<T, ADDS, 8, 512, true>(p, rows, st);
+    if (nvec <= 8192) return launch_nv<T, ADDS, 8, 1024, true>(p, rows, st);
   }
   return fail(LRI_ERR_UNSUPPORTED, "rows of %d elements to e4m3", p.cols);
 }

@@ -34,7 +34,7 @@ def _untouched(room, scale, rows, cols):
 # ---- rows ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols,apart,pad", [(1, 8, 0, 0), (3, 24, 8, 1), (2, 2048, 0, 0), (149, 2056, 0, 0), (5, 4096, 1024, 0), (400, 4096, 0, 2), (2, 4104, 0, 0),
-                                                 (200, 8200, 8, 0), (3, 8200, 0, 0), (150, 11000, 0, 0), (2, 16392, 0, 1), (3, 32768, 0, 0), (2, 65536, 0, 0), (160, 288, 40, 0)])
+                                                 (200, 8200, 8, 0), (3, 8200, 0, 0), (150, 11000, 0, 0), (2, 16392, 0, 1), (3, 32768, 0, 0), (2, 65536, 0, 0), (160, 288, 40, 0), (150, 8, 0, 0), (151, 2040, 0, 1), (150, 30000, 0, 0), (149, 40000, 8, 0)])
 def test_rows(e4m3, dtype, rows, cols, apart, pad):
     g = torch.Generator().manual_seed(rows + cols)
     wide = torch.randn(rows, cols + apart, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))
@@ -78,7 +78,8 @@ def test_rows_of_no_and_of_unusual_values(e4m3, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,dim,adds,factor,keep", [(1, 8, 0, 1.0, "none"), (1, 4096, 1, 1.0, "own"), (7, 288, 2, 0.5, "in place"), (148, 2048, 1, 1.0, "in place"),
                                                        (149, 2304, 1, 0.125, "own"), (3, 4104, 2, 1.0, "own"), (200, 4096, 2, 1.0, "add1"), (33, 8192, 0, 1.0, "none"),
-                                                       (150, 8192, 1, 1.0, "own"), (151, 11000, 1, 1.0, "own"), (2, 16384, 2, 0.25, "own"), (155, 16384, 1, 1.0, "own")])
+                                                       (150, 8192, 1, 1.0, "own"), (151, 11000, 1, 1.0, "own"), (2, 16384, 2, 0.25, "own"), (155, 16384, 1, 1.0, "own"), (150, 8, 1, 1.0, "in place"),
+                                                       (200, 768, 2, 1.0, "own"), (149, 2040, 0, 1.0, "none"), (160, 5120, 2, 1.0, "in place")])
 def test_norm(e4m3, dtype, rows, dim, adds, factor, keep):
     from gpt_fast.ops import CudaOps
     g = torch.Generator().manual_seed(rows * dim)
