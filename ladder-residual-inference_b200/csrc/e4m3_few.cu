@@ -23,6 +23,7 @@
 // Warp roles: warp 0 fetches (TMA; the weights of the first stages before the preceding kernel is complete, since it does not write
 // them), warp 1 owns the tensor memory and issues the products, warps 2-5 take the sums out of tensor memory; all warps join.  Every wait on
 // an mbarrier is bounded (lri_gemm_status); every CTA reaches the two cluster barriers in every case.
+#include "cluster.cuh"
 #include "e4m3_tc.cuh"
 
 namespace lri {
@@ -50,11 +51,6 @@ struct Ring {
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
 // from this CTA's shared memory to another's of the cluster, whose barrier counts the bytes
@@ -136,7 +132,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's barriers exist (published by the fence above)
+  cluster_arrive_relaxed();  // this CTA's barriers exist (published by the fence above)
 
   // What joining the sums needs of memory is asked for at the start, and a part of the addend brought to the L2: behind the last product each of
   // these was a trip to memory of its own (64 rows of 8192 gated outputs from 2048: 11.7 us, 11.1 here).
@@ -215,9 +211,9 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         if (at < bytes && tok < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(add + static_cast<int64_t>(tok) * p.n * 2 + at));
       }
     }
-    const bool ok = mbar_wait(done, 0, &abort_flag, 73, &g_e4m3_few_status);
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others' barriers exist (long since)
-    if (__all_sync(0xffffffffu, ok)) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, &abort_flag, 73, &g_e4m3_few_status));
+    cluster_wait();  // the others' barriers exist (long since)
+    if (ok) {
       // every copy has landed and every product has read it: the ring's place is free, which the others are told
       if (split > 1 && i < split) arrive_in_cluster(in_cta(all_done, i));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -226,6 +222,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       for (int cc = 0; cc < BN; cc += 16) {
         if (cc >= rows) break;
         uint32_t r[16];
+        __syncwarp();
         tmem_ld16_issue(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cc, r);
         tmem_wait_ld();
 #pragma unroll
@@ -245,7 +242,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       }
     }
   }
-  if (warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp < 2) cluster_wait();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
@@ -280,8 +277,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   bool ok = !abort_flag;
   if (split > 1) {
     ok = mbar_wait_cluster(landed, 0, &abort_flag, 75, &g_e4m3_few_status) && ok;
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // nothing is copied into this CTA any more
+    cluster_arrive_relaxed();  // nothing is copied into this CTA any more
   }
   if (!kGlu) more = bias[c / 2];
   for (; there && ok && g < mine; g += kAtOnce, load_addend()) {
@@ -337,8 +333,7 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     for (int i = 0; i < 2000; ++i) __nanosleep(100);  // let copies in flight land before shared memory is released
   }
   // what is copied out of this CTA has been copied once all the others have theirs
-  __syncwarp();
-  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (split > 1) cluster_wait();
 }
 
 // CTAs of a tile: as many as there are places for, with four steps (64 KB of weights) or more for each.  us with at most 2 / 4 / 8: 1 x 1280 x 8192 8.8 / 6.2 / 4.7,

@@ -22,6 +22,7 @@
 //
 // Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
 // uses, is said in gemm_pair.cu and holds here.
+#include "cluster.cuh"
 #include "e4m3.cuh"
 #include "e4m3_tc.cuh"
 #include "gemm_tile.cuh"
@@ -42,14 +43,6 @@ constexpr int kOwnSmem = 181 * 1024;
 constexpr int kStoreWarps = 8;  // two for each quarter of the tensor memory's lanes, which take its columns in turn
 constexpr int kThreads = 64 + 32 * kStoreWarps;
 
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // `bar` may lie in either CTA of the pair
 __device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* tmap, uint32_t bar, int x, int y) {
   asm volatile(
@@ -250,7 +243,7 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   const uint32_t acc_full0 = smem_u32(&bars[2 * kMaxStages]);       // products -> stores, one per accumulator
   const uint32_t acc_empty0 = smem_u32(&bars[2 * kMaxStages + 2]);  // stores -> products (first CTA)
 
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  cluster_arrive_relaxed();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < stages; ++s) {
@@ -264,8 +257,7 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the other CTA runs
+  cluster_wait();  // the other CTA runs
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
                  "r"(2 * kAccCols)
@@ -275,7 +267,8 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   // the barriers of both CTAs exist before either is used from the other (published by the fence above: a release here waits for a busy memory system)
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive_relaxed();
+  cluster_wait();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
   if (warp != 0) {
