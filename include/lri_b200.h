@@ -35,9 +35,9 @@ typedef void* lri_stream_t; /* a cudaStream_t */
 
 /* LRI_FP32 is taken by the entry points that say so (every product and sum a true 32-bit operation). */
 enum lri_dtype { LRI_BF16 = 0, LRI_FP16 = 1, LRI_FP32 = 2, LRI_E4M3 = 3 /* pages of a key-value cache only */ };  /* (the entry points of 8-bit projections have e4m3 in their names) */
-/* Added to `dtype` of lri_linear, lri_linear_f32, lri_gateup_glu or their _early forms: a prompt projection (more than 128
- * token rows) stays on the kernel that gives a tile to one SM.  For passes that run kernels of theirs on a second stream
- * beside their projections (see csrc/gemm_pair.cu). */
+/* Added to `dtype` of lri_linear, lri_linear_f32, lri_gateup_glu or their _early forms, or of an lri_linear_e4m3_call: a prompt projection
+ * (more than 128 token rows; in 8 bits more than 64) stays off the kernel on pairs of SMs.  For passes that run kernels of theirs on a second stream
+ * beside their projections (see csrc/gemm_pair.cu); option gemm_pair = 0 does it for a process. */
 enum { LRI_ONE_SM = 0x100 };
 /* Added to `dtype` of lri_rope_paged_store: the query rows of tokens that are skipped become zeros, for results in fresh memory. */
 enum { LRI_ZERO_SKIPPED = 0x200 };
@@ -354,6 +354,9 @@ typedef struct {
   float alpha, limit, offset;
 } lri_linear_e4m3_call;
 int lri_linear_e4m3(const lri_linear_e4m3_call* call);
+/* Which kernel a call of these sizes takes (w has n outputs, or 2 n rows with LRI_ACT_GLU; LRI_ONE_SM may be added to dtype): 0 the one for few rows, > 0 the
+ * width of the tiles of the one on pairs of SMs. */
+int lri_linear_e4m3_plan(int dtype, int64_t rows, int n, int k, int activation);
 /* The second half of lri_qkv_rope_kvcache: rows [q heads | k heads | v heads] of a projection, qkv [B*S, (n_head + 2 n_kv) * head_dim],
  * to rotated queries and to the caches; arguments as there. */
 int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_table, const void* input_pos, int pos_is_i64, void* q_out, void* k_cache,

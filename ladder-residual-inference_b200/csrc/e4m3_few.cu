@@ -101,7 +101,9 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int rank = split == 1 ? 0 : static_cast<int>(cluster_rank());
-  const int tile = blockIdx.x / split, row0 = blockIdx.y * BN, rows = min(BN, p.rows - row0);
+  const int64_t row0_ = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * BN;  // (a grid's second extent alone may be too short)
+  if (row0_ >= p.rows) return;
+  const int tile = blockIdx.x / split, row0 = static_cast<int>(row0_), rows = min(BN, p.rows - row0);
   const int steps = (p.k + kStep - 1) / kStep;
   const int kt0 = steps * rank / split, kt1 = steps * (rank + 1) / split;  // (the host keeps split <= steps)
 
@@ -358,10 +360,12 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
   auto kern = e4m3_few_kernel<T, ACT, BN>;
   static std::atomic<unsigned long long> attr_set{0};  // per template instantiation, one bit per device
   LRI_ONCE_PER_DEVICE(attr_set, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<BN>::kBytes));
-  const int tiles = (p.n + kOut - 1) / kOut, row_tiles = (p.rows + BN - 1) / BN;
-  const int split = split_of(static_cast<int64_t>(tiles) * row_tiles, (p.k + kStep - 1) / kStep);
+  const int tiles = (p.n + kOut - 1) / kOut;
+  const int64_t row_tiles = (static_cast<int64_t>(p.rows) + BN - 1) / BN, kMostY = 65535;
+  const int split = split_of(tiles * row_tiles, (p.k + kStep - 1) / kStep);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split, static_cast<unsigned>(row_tiles));
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split, static_cast<unsigned>(row_tiles < kMostY ? row_tiles : kMostY),
+                     static_cast<unsigned>((row_tiles + kMostY - 1) / kMostY));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = Ring<BN>::kBytes;
   cfg.stream = st;
@@ -381,7 +385,7 @@ int launch(const E4m3Linear& p, cudaStream_t st) {
 
 int64_t e4m3_few_fetched(int activation, const E4m3Linear& p) {
   const int tile = activation == LRI_ACT_GLU ? kBM / 2 : kBM, steps = (p.k + kStep - 1) / kStep;
-  const int64_t tiles = (static_cast<int64_t>(p.n) + tile - 1) / tile * ((p.rows + 63) / 64);
+  const int64_t tiles = (static_cast<int64_t>(p.n) + tile - 1) / tile * ((static_cast<int64_t>(p.rows) + 63) / 64);
   const int split = split_of(tiles, steps);
   return (tiles * split + sm_count() - 1) / sm_count() * ((steps + split - 1) / split) * Ring<64>::kStageBytes;
 }

@@ -1,15 +1,64 @@
 // Entry point of the projections in 8 bits: argument checks and the choice of the kernel.
 #include "e4m3.cuh"
 
+namespace lri {
+namespace {
+
+// As the projections in 16 bits (gemm_pair.cu says why): a program that runs tensor-memory kernels on another stream can keep a projection off the kernel on
+// pairs of SMs (LRI_ONE_SM, option gemm_pair = 0), and sums of one or two steps of 128 codes, which a pair has no time to fetch ahead of, never go there.
+constexpr int kMinDepth = 2 * 128;
+
+// 0: the kernel for few rows, else the width of the tiles of the one on pairs.  What both wait for from some tens of rows on is what an SM can take in, about 57
+// bytes a cycle (108 KB a us): the one with less to fetch is the faster, where kAhead is what the shorter start and end of the one for few rows are worth.  us, few /
+// pair: 128 rows, 4096 x 14336 17.0 / 22.7, 2001 x 2568 6.7 / 10.6, gated 14336 x 4096 38.4 / 32.0; 256 rows, 1280 x 8192 10.7 / 13.8, 4096 x 4096 11.0 / 10.4; 512 rows, 6144 x
+// 4096 27.6 / 15.8.  With up to 64 rows the pairs' tiles are mostly padding (65 rows: 4096 x 4096 8.1 / 9.9, gated 8192 x 2048 11.6 / 15.7).
+int width_on_pairs(int activation, const E4m3Linear& p, bool one_sm) {
+  constexpr int64_t kAhead = 64 << 10;
+  const int forced = option(OPT_GEMM_PAIR);
+  if (p.rows <= 64 || one_sm || forced == 0 || p.k <= kMinDepth) return 0;
+  const int by = activation == LRI_ACT_GLU ? 64 : 32;
+  if (forced > 1) return forced / by * by;
+  int width = 0;
+  const int64_t pair = e4m3_pair_fetched(activation, p, &width);
+  return e4m3_few_fetched(activation, p) <= pair + kAhead ? 0 : width;
+}
+
+// takes LRI_ONE_SM out of a call's dtype
+bool take_one_sm(int& dtype) {
+  const bool one_sm = dtype >= 0 && (dtype & LRI_ONE_SM) != 0;
+  if (one_sm) dtype &= ~LRI_ONE_SM;
+  return one_sm;
+}
+
+int check_sizes(int dtype, int64_t rows, int n, int k, int activation) {
+  LRI_REQUIRE(dtype == LRI_BF16 || dtype == LRI_FP16, LRI_ERR_UNSUPPORTED, "linear_e4m3: dtype %d", dtype);
+  LRI_REQUIRE(activation >= LRI_ACT_NONE && activation <= LRI_ACT_GLU, LRI_ERR_UNSUPPORTED, "linear_e4m3: activation %d", activation);
+  LRI_REQUIRE(rows >= 0 && rows < (1ll << 31) && n > 0 && n < (1 << 30), LRI_ERR_ARG, "linear_e4m3: rows=%lld n=%d", (long long)rows, n);
+  LRI_REQUIRE(k > 0 && k % 8 == 0, LRI_ERR_UNSUPPORTED, "linear_e4m3: k=%d must be a positive multiple of 8", k);
+  return LRI_OK;
+}
+
+}  // namespace
+}  // namespace lri
+
+extern "C" int lri_linear_e4m3_plan(int dtype, int64_t rows, int n, int k, int activation) {
+  using namespace lri;
+  const bool one_sm = take_one_sm(dtype);
+  const int rc = check_sizes(dtype, rows, n, k, activation);
+  if (rc != LRI_OK) return rc;
+  E4m3Linear p{};
+  p.rows = static_cast<int>(rows), p.n = n, p.k = k;
+  return width_on_pairs(activation, p, one_sm);
+}
+
 extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   using namespace lri;
   LRI_REQUIRE(call != nullptr, LRI_ERR_ARG, "linear_e4m3: NULL call");
-  const lri_linear_e4m3_call& c = *call;
-  LRI_REQUIRE(c.dtype == LRI_BF16 || c.dtype == LRI_FP16, LRI_ERR_UNSUPPORTED, "linear_e4m3: dtype %d", c.dtype);
-  LRI_REQUIRE(c.activation >= LRI_ACT_NONE && c.activation <= LRI_ACT_GLU, LRI_ERR_UNSUPPORTED, "linear_e4m3: activation %d", c.activation);
+  lri_linear_e4m3_call c = *call;
+  const bool one_sm = take_one_sm(c.dtype);
+  const int rc = check_sizes(c.dtype, c.rows, c.n, c.k, c.activation);
+  if (rc != LRI_OK) return rc;
   const bool glu = c.activation == LRI_ACT_GLU;
-  LRI_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) && c.n > 0 && c.n < (1 << 30), LRI_ERR_ARG, "linear_e4m3: rows=%lld n=%d", (long long)c.rows, c.n);
-  LRI_REQUIRE(c.k > 0 && c.k % 8 == 0, LRI_ERR_UNSUPPORTED, "linear_e4m3: k=%d must be a positive multiple of 8", c.k);
   LRI_REQUIRE(!glu || (!c.bias && !c.addend), LRI_ERR_UNSUPPORTED, "linear_e4m3: the gated unit takes no bias and no addend");
   LRI_REQUIRE(!glu || c.limit >= 0.f, LRI_ERR_ARG, "linear_e4m3: limit=%g", (double)c.limit);
   LRI_REQUIRE(c.rows == 0 || (c.x && c.w && c.x_scale && c.w_scale && c.y), LRI_ERR_ARG, "linear_e4m3: NULL pointer");
@@ -30,14 +79,6 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   p.bias = c.bias, p.addend = c.addend, p.y = c.y, p.x_ld = c.x_ld, p.w_ld = c.w_ld;
   p.rows = static_cast<int>(c.rows), p.n = c.n, p.k = c.k, p.glu = GluParams{c.alpha, c.limit, c.offset};
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
-  // Which kernel.  What both wait for from some tens of rows on is what an SM can take in, about 57 bytes a cycle (108 KB a us): the one with less to
-  // fetch is the faster, where kAhead is what the shorter start and end of the one for few rows are worth.  us, few / pair: 128 rows, 4096 x 14336 17.0 / 22.7, 2001 x 2568
-  // 6.7 / 10.6, gated 14336 x 4096 38.4 / 32.0; 256 rows, 1280 x 8192 10.7 / 13.8, 4096 x 4096 11.0 / 10.4; 512 rows, 6144 x 4096 27.6 / 15.8.  With up to 64 rows
-  // the pairs' tiles are mostly padding (65 rows: 4096 x 4096 8.1 / 9.9, gated 8192 x 2048 11.6 / 15.7).
-  constexpr int64_t kAhead = 64 << 10, kMostTiles = 65535;  // (of 64 rows: the second extent of a grid)
-  if (c.rows <= 64) return e4m3_few_launch(c.dtype, c.activation, p, st);
-  int width = 0;
-  const int64_t pair = e4m3_pair_fetched(c.activation, p, &width);
-  if (c.rows <= 64 * kMostTiles && e4m3_few_fetched(c.activation, p) <= pair + kAhead) return e4m3_few_launch(c.dtype, c.activation, p, st);
-  return e4m3_pair_launch(c.dtype, c.activation, p, width, st);
+  const int width = width_on_pairs(c.activation, p, one_sm);
+  return width ? e4m3_pair_launch(c.dtype, c.activation, p, width, st) : e4m3_few_launch(c.dtype, c.activation, p, st);
 }

@@ -405,7 +405,7 @@ int64_t fetched(const E4m3Linear& p, bool glu, int* width) {
   const int64_t w_rows = glu ? 2ll * p.n : p.n, steps = (p.k + kStep - 1) / kStep;
   int64_t least = 0;
   for (int bn = kMaxBn; bn >= 64; bn -= by) {
-    const int64_t tiles = ((p.rows + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
+    const int64_t tiles = ((static_cast<int64_t>(p.rows) + 2 * kBM - 1) / (2 * kBM)) * ((w_rows + bn - 1) / bn);
     const int64_t bytes = (tiles + pairs - 1) / pairs * steps * (kTileBytes + bn / 2 * kStep);
     if (bn == kMaxBn || bytes < least) *width = bn, least = bytes;
   }

@@ -87,6 +87,7 @@ _SIGNATURES = {
     "lri_quantize_rows_e4m3": (c_int, [c_void_p]),
     "lri_add_rmsnorm_e4m3": (c_int, [c_void_p]),
     "lri_linear_e4m3": (c_int, [c_void_p]),
+    "lri_linear_e4m3_plan": (c_int, [c_int, c_int64, c_int, c_int, c_int]),
     "lri_rope_kvcache": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64,
                                  c_int64, c_int, c_void_p]),
     "lri_comm_create": (c_int, [c_int, c_int, c_int64, ctypes.POINTER(c_void_p), ctypes.c_char_p]),

@@ -12,7 +12,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from ._C import ACT_GLU, ACTIVATIONS
+from ._C import ACT_GLU, ACTIVATIONS, ONE_SM
 from .ops import CudaOps
 
 E4M3 = torch.float8_e4m3fn
@@ -100,11 +100,12 @@ def add_rmsnorm(residual: Tensor, weight: Tensor, eps: float, add1: Optional[Ten
 
 
 def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional[str] = None, addend: Optional[Tensor] = None,
-           dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None) -> Tensor:
+           dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None, one_sm: bool = False) -> Tensor:
     """activation(x w^T + bias) + addend, [rows, outputs], summed in fp32 and rounded once.  activation: None, "silu", "gelu" (by the error
     function) or "gelu_tanh"; bias [outputs] and addend [rows, outputs] in the result's type; the addend may be `out`.  dtype: of the result where `out`
     is None.  The kernel reads w before the call in front of it on the stream is complete: weights, or what quantize_rows and add_rmsnorm have stored
-    (without `early`), not codes that another operator has just written."""
+    (without `early`), not codes that another operator has just written.  one_sm: not on pairs of SMs, for a call beside which another stream runs projections or prompt
+    attention (a process can keep off them altogether by option gemm_pair = 0)."""
     rows, k, x_ld = _looked_at("x", x)
     n, depth, w_ld = _looked_at("w", w)
     if k != depth:
@@ -117,13 +118,16 @@ def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional
         _dense("bias", bias, out.dtype, (n,))
     if addend is not None:
         _dense("addend", addend, out.dtype, (rows, n))
-    CudaOps.linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias, addend, ACTIVATIONS[activation])
+    CudaOps.linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias, addend, ACTIVATIONS[activation],
+                        flags=ONE_SM if one_sm else 0)
     return out
 
 
-def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None) -> Tensor:
+def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None,
+               one_sm: bool = False) -> Tensor:
     """The gated unit of x w1^T, w1 [2 inter, k] = [up | gate]: g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit),
-    u = clamp(up, -limit, limit), glu = (alpha, limit, offset); SwiGLU by default.  In fp32, rounded once to [rows, inter]."""
+    u = clamp(up, -limit, limit), glu = (alpha, limit, offset); SwiGLU by default.  In fp32, rounded once to [rows, inter].
+    one_sm: as in linear."""
     rows, k, x_ld = _looked_at("x", x)
     n, depth, w_ld = _looked_at("w1", w1)
     if k != depth or n % 2 or not n:
@@ -131,7 +135,7 @@ def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtyp
     if not glu[1] >= 0:
         raise ValueError(f"glu={glu}: the limit is not below 0")
     out = _result(out, dtype, rows, n // 2, x[0].device)
-    CudaOps.linear_e4m3(x, w1, out, rows, n // 2, k, x_ld, w_ld, activation=ACT_GLU, glu=glu)
+    CudaOps.linear_e4m3(x, w1, out, rows, n // 2, k, x_ld, w_ld, activation=ACT_GLU, glu=glu, flags=ONE_SM if one_sm else 0)
     return out
 
 

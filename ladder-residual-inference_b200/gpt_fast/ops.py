@@ -225,8 +225,8 @@ class CudaOps:
             _C.check(status)
 
     @staticmethod
-    def linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0)):
-        """x, w: (codes, scale); n outputs; activation: a number of LRI_ACT_*."""
+    def linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0), flags=0):
+        """x, w: (codes, scale); n outputs; activation: a number of LRI_ACT_*; flags: 0 or _C.ONE_SM."""
         (xc, xs), (wc, ws) = x, w
         here = xc.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == xs.get_device() == wc.get_device() == ws.get_device() == out.get_device() and
@@ -234,7 +234,7 @@ class CudaOps:
             _C.refuse_devices(xc, xs, wc, ws, out, bias, addend)
         status = _C.lib.lri_linear_e4m3(_C.LINEAR8_CALL.pack(
             xc.data_ptr(), wc.data_ptr(), xs.data_ptr(), ws.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if addend is None else addend.data_ptr(),
-            out.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x_ld, w_ld, _C.CODES[out.dtype], n, k, activation, *glu))
+            out.data_ptr(), torch._C._cuda_getCurrentRawStream(here), rows, x_ld, w_ld, _C.CODES[out.dtype] | flags, n, k, activation, *glu))
         if status < 0:
             _C.check(status)
 
