@@ -41,6 +41,9 @@ enum lri_dtype { LRI_BF16 = 0, LRI_FP16 = 1, LRI_FP32 = 2, LRI_E4M3 = 3 /* pages
 enum { LRI_ONE_SM = 0x100 };
 /* Added to `dtype` of lri_rope_paged_store: the query rows of tokens that are skipped become zeros, for results in fresh memory. */
 enum { LRI_ZERO_SKIPPED = 0x200 };
+/* Added to `dtype` of an lri_linear_e4m3_call: w and w_scale may be read while the kernel in front on the stream still runs.  For weights that have been
+ * complete since before an operation in front of that which begins when all before it is complete (a copy, a kernel of another library), as a model's are. */
+enum { LRI_WEIGHTS_AHEAD = 0x400 };
 
 enum lri_status {
   LRI_OK = 0,
@@ -319,10 +322,8 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * w_scale 2 n scales, without bias and addend, and y = g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit), u = clamp(up, -limit, limit):
  * SwiGLU with alpha 1, limit infinity, offset 0.
  *
- * lri_linear_e4m3 starts on its weights (w and w_scale) while the kernel before it on the stream still runs, as the projections in 16 bits do.  So
- * lri_quantize_rows_e4m3 and lri_add_rmsnorm_e4m3, whose results may be weights, let the next kernel start only when they are complete, unless `early`
- * is not 0: for a caller whose next calls read the results as x, or not at all.  Codes that something else has just stored (the pages of a cache) become
- * weights behind an operation that is complete before the next begins, such as a copy. */
+ * Everything is read when the kernel in front on the stream is complete, but weights with LRI_WEIGHTS_AHEAD: any operator's results may be any input of the
+ * next, weights among them.  `early` not 0: the next kernel may start before this one is complete, and waits for it by itself, as all of this library do. */
 enum lri_activation { LRI_ACT_NONE = 0, LRI_ACT_SILU = 1, LRI_ACT_GELU = 2, LRI_ACT_GELU_TANH = 3, LRI_ACT_GLU = 4 };
 typedef struct {
   const void* x;

@@ -29,6 +29,7 @@ struct E4m3Linear {
   void* y;
   int64_t x_ld, w_ld;
   int rows, n, k;
+  bool ahead;  // LRI_WEIGHTS_AHEAD
   GluParams glu;
 };
 

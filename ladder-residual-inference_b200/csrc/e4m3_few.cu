@@ -20,8 +20,12 @@
 //
 // Gated unit: a tile is 64 up rows and the 64 matching gate rows; up and gate of an output meet where the sums are joined.
 //
-// Warp roles: warp 0 fetches (TMA; the weights of the first stages before the preceding kernel is complete, since it does not write
-// them), warp 1 owns the tensor memory and issues the products, warps 2-5 take the sums out of tensor memory; all warps join.  Every wait on
+// While the preceding kernel still runs, the weights of the first stages go into the ring where the caller says that they are no result of calls before
+// (LRI_WEIGHTS_AHEAD), else to the L2: what other kernels have written is visible behind griddepcontrol.wait alone.  us, into the ring / to the L2 / neither: 1 x 6144 x
+// 4096 6.4 / 7.4 / 7.5, 16 x 2048 x 2048 3.6 / 3.8 / 4.3, 24 x 4096 x 14336 with addend 12.4 / 12.4 / 13.5, 4 gated rows of 14336 from 4096 19.7 / 21.0 / 21.0, 64 x 4096 x 4096 7.7 /
+// 7.9 / 8.8.  (To the L2 for more stages than the ring has: 12.4 -> 13.1, 21.0 -> 22.1.)
+//
+// Warp roles: warp 0 fetches (TMA), warp 1 owns the tensor memory and issues the products, warps 2-5 take the sums out of tensor memory; all warps join.  Every wait on
 // an mbarrier is bounded (lri_gemm_status); every CTA reaches the two cluster barriers in every case.
 #include "cluster.cuh"
 #include "e4m3_tc.cuh"
@@ -136,6 +140,29 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
   cluster_arrive_relaxed();  // this CTA's barriers exist (published by the fence above)
 
+  // warp-uniform loops, one elected lane issues (see gemm_pair.cu)
+  auto fetch_weights = [&](uint32_t s, int kt) {
+    mbar_expect_tx(full0 + 8 * s, kStageBytes);
+    const uint32_t dst = base + s * kStageBytes;
+    tma_load_2d(dst, &tmap_w, full0 + 8 * s, kt * kStep, tile * kOut);
+    if (kGlu) tma_load_2d(dst + kTileBytes / 2, &tmap_w, full0 + 8 * s, kt * kStep, p.n + tile * kOut);
+  };
+  const int first = min(static_cast<int>(kStages), kt1 - kt0);  // steps that the empty ring has room for
+  if (warp == 0) {
+    for (int i = 0; i < first; ++i) {
+      if (elect_one()) {
+        if (p.ahead) {
+          fetch_weights(i, kt0 + i);
+        } else {
+          tma_prefetch_2d(&tmap_w, (kt0 + i) * kStep, tile * kOut);
+          if (kGlu) tma_prefetch_2d(&tmap_w, (kt0 + i) * kStep, p.n + tile * kOut);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (!p.ahead) pdl_wait();
+
   // What joining the sums needs of memory is asked for at the start, and a part of the addend brought to the L2: behind the last product each of
   // these was a trip to memory of its own (64 rows of 8192 gated outputs from 2048: 11.7 us, 11.1 here).
   constexpr int kPairs = kOut / 2, kAtOnce = kGemmThreads / kPairs;
@@ -147,27 +174,20 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     s = make_float2(p.w_scale[j], both ? p.w_scale[j + 1] : 0.f);
     if (kGlu) more = make_float2(p.w_scale[p.n + j], both ? p.w_scale[p.n + j + 1] : 0.f);
   }
+  pdl_wait();
+  pdl_launch_dependents();
 
-  // warp-uniform loops, one elected lane issues (see gemm_pair.cu)
   if (warp == 0) {
-    auto fetch_weights = [&](uint32_t s, int kt) {
-      mbar_expect_tx(full0 + 8 * s, kStageBytes);
-      const uint32_t dst = base + s * kStageBytes;
-      tma_load_2d(dst, &tmap_w, full0 + 8 * s, kt * kStep, tile * kOut);
-      if (kGlu) tma_load_2d(dst + kTileBytes / 2, &tmap_w, full0 + 8 * s, kt * kStep, p.n + tile * kOut);
-    };
     auto fetch_rows = [&](uint32_t s, int kt) { tma_load_2d(base + s * kStageBytes + kTileBytes, &tmap_x, full0 + 8 * s, kt * kStep, row0); };
-    const int ahead = min(static_cast<int>(kStages), kt1 - kt0);
-    for (int i = 0; i < ahead; ++i)
-      if (elect_one()) fetch_weights(i, kt0 + i);
-    __syncwarp();
-    pdl_wait();
-    pdl_launch_dependents();
-    for (int i = 0; i < ahead; ++i)
-      if (elect_one()) fetch_rows(i, kt0 + i);
-    __syncwarp();
-    uint32_t s = ahead == static_cast<int>(kStages) ? 0 : ahead, parity = 0;
-    for (int kt = kt0 + ahead; kt < kt1; ++kt) {
+    for (int i = 0; i < first; ++i) {
+      if (elect_one()) {
+        if (!p.ahead) fetch_weights(i, kt0 + i);
+        fetch_rows(i, kt0 + i);
+      }
+      __syncwarp();
+    }
+    uint32_t s = first == static_cast<int>(kStages) ? 0 : first, parity = 0;
+    for (int kt = kt0 + first; kt < kt1; ++kt) {
       if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 71, &g_e4m3_few_status))) break;
       if (elect_one()) {
         fetch_weights(s, kt);
@@ -177,8 +197,6 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       if (++s == kStages) s = 0, parity ^= 1u;
     }
   } else if (warp == 1) {
-    pdl_wait();
-    pdl_launch_dependents();
     const uint32_t idesc = e4m3_idesc(kBM, BN);
     uint32_t s = 0, parity = 0;
     for (int kt = kt0; kt < kt1; ++kt) {
@@ -197,8 +215,6 @@ e4m3_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       if (++s == kStages) s = 0, parity ^= 1u;
     }
   } else {
-    pdl_wait();
-    pdl_launch_dependents();
     const int quarter = warp & 3, i = static_cast<int>(threadIdx.x) - 64;
     if (i < rows) reinterpret_cast<float*>(row_scale)[i] = p.x_scale[row0 + i];
     if (!kGlu && i < kOut) {

@@ -23,11 +23,11 @@ int width_on_pairs(int activation, const E4m3Linear& p, bool one_sm) {
   return e4m3_few_fetched(activation, p) <= pair + kAhead ? 0 : width;
 }
 
-// takes LRI_ONE_SM out of a call's dtype
-bool take_one_sm(int& dtype) {
-  const bool one_sm = dtype >= 0 && (dtype & LRI_ONE_SM) != 0;
-  if (one_sm) dtype &= ~LRI_ONE_SM;
-  return one_sm;
+// takes a flag out of a call's dtype
+bool take(int flag, int& dtype) {
+  const bool there = dtype >= 0 && (dtype & flag) != 0;
+  if (there) dtype &= ~flag;
+  return there;
 }
 
 int check_sizes(int dtype, int64_t rows, int n, int k, int activation) {
@@ -43,7 +43,7 @@ int check_sizes(int dtype, int64_t rows, int n, int k, int activation) {
 
 extern "C" int lri_linear_e4m3_plan(int dtype, int64_t rows, int n, int k, int activation) {
   using namespace lri;
-  const bool one_sm = take_one_sm(dtype);
+  const bool one_sm = take(LRI_ONE_SM, dtype);
   const int rc = check_sizes(dtype, rows, n, k, activation);
   if (rc != LRI_OK) return rc;
   E4m3Linear p{};
@@ -55,7 +55,7 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   using namespace lri;
   LRI_REQUIRE(call != nullptr, LRI_ERR_ARG, "linear_e4m3: NULL call");
   lri_linear_e4m3_call c = *call;
-  const bool one_sm = take_one_sm(c.dtype);
+  const bool one_sm = take(LRI_ONE_SM, c.dtype), ahead = take(LRI_WEIGHTS_AHEAD, c.dtype);
   const int rc = check_sizes(c.dtype, c.rows, c.n, c.k, c.activation);
   if (rc != LRI_OK) return rc;
   const bool glu = c.activation == LRI_ACT_GLU;
@@ -77,7 +77,7 @@ extern "C" int lri_linear_e4m3(const lri_linear_e4m3_call* call) {
   E4m3Linear p{};
   p.x = static_cast<const uint8_t*>(c.x), p.w = static_cast<const uint8_t*>(c.w), p.x_scale = c.x_scale, p.w_scale = c.w_scale;
   p.bias = c.bias, p.addend = c.addend, p.y = c.y, p.x_ld = c.x_ld, p.w_ld = c.w_ld;
-  p.rows = static_cast<int>(c.rows), p.n = c.n, p.k = c.k, p.glu = GluParams{c.alpha, c.limit, c.offset};
+  p.rows = static_cast<int>(c.rows), p.n = c.n, p.k = c.k, p.ahead = ahead, p.glu = GluParams{c.alpha, c.limit, c.offset};
   cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   const int width = width_on_pairs(c.activation, p, one_sm);
   return width ? e4m3_pair_launch(c.dtype, c.activation, p, width, st) : e4m3_few_launch(c.dtype, c.activation, p, st);

@@ -271,35 +271,32 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   cluster_wait();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
-  if (warp != 0) {
-    pdl_wait();
-    pdl_launch_dependents();
-  }
   const int items = grid.tiles_p * grid.tiles_q;
+  const WorkItem first = work_item(pair, grid);  // (every pair has an item)
+  // the weight rows of this CTA: half of the tile's, or all its up rows (first CTA) and all its gate rows (second)
+  auto weight_row = [&](const WorkItem& w) { return kGlu ? static_cast<int>(rank) * p.n + w.tile_q * half : w.tile_q * bn + static_cast<int>(rank) * half; };
+  const int ahead = min(static_cast<int>(stages), num_kt);
+  if (warp == 0) {
+    for (int i = 0; i < ahead; ++i) {
+      if (elect_one()) tma_prefetch_2d(&tmap_w, i * kStep, weight_row(first));
+      __syncwarp();
+    }
+  }
+  pdl_wait();
+  pdl_launch_dependents();
 
   if (warp == 0) {
     const uint32_t full_first = in_cta(full0, 0);
-    // the weight rows of this CTA: half of the tile's, or all its up rows (first CTA) and all its gate rows (second)
-    auto fetch_weights = [&](uint32_t s, int kt, const WorkItem& w) {
+    auto fetch = [&](uint32_t s, int kt, const WorkItem& w) {
       // (the second CTA's bytes may arrive before this: the phase cannot end before the arrival counted here)
       if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * stage_bytes);
-      const int w_row = kGlu ? static_cast<int>(rank) * p.n + w.tile_q * half : w.tile_q * bn + static_cast<int>(rank) * half;
-      tma_load_pair(base + s * stage_bytes + kTileBytes, &tmap_w, full_first + 8 * s, kt * kStep, w_row);
-    };
-    auto fetch_rows = [&](uint32_t s, int kt, const WorkItem& w) {
+      tma_load_pair(base + s * stage_bytes + kTileBytes, &tmap_w, full_first + 8 * s, kt * kStep, weight_row(w));
       tma_load_pair(base + s * stage_bytes, &tmap_x, full_first + 8 * s, kt * kStep, w.tile_p * 2 * kBM + static_cast<int>(rank) * kBM);
     };
-    // the weights of the first stages do not depend on the preceding kernel
-    const int ahead = min(static_cast<int>(stages), num_kt);  // (every pair has an item)
-    const WorkItem first = work_item(pair, grid);
-    for (int i = 0; i < ahead; ++i)
-      if (elect_one()) fetch_weights(i, i, first);
-    __syncwarp();
-    pdl_wait();
-    pdl_launch_dependents();
-    for (int i = 0; i < ahead; ++i)
-      if (elect_one()) fetch_rows(i, i, first);
-    __syncwarp();
+    for (int i = 0; i < ahead; ++i) {
+      if (elect_one()) fetch(i, i, first);
+      __syncwarp();
+    }
     uint32_t s = ahead, parity = 1;  // a fresh barrier passes a wait on parity 1, so the first round does not block
     if (s == stages) s = 0, parity = 0;
     bool ok = true;
@@ -308,10 +305,7 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       for (int kt = item == pair ? ahead : 0; kt < num_kt; ++kt) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, parity, &abort_flag, 61, &g_e4m3_pair_status));
         if (!ok) break;
-        if (elect_one()) {
-          fetch_weights(s, kt, w);
-          fetch_rows(s, kt, w);
-        }
+        if (elect_one()) fetch(s, kt, w);
         __syncwarp();
         if (++s == stages) s = 0, parity ^= 1u;
       }

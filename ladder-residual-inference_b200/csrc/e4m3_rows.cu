@@ -40,13 +40,9 @@ __global__ void __launch_bounds__(MOST) rows_e4m3_kernel(const RowsParams p) {
   __shared__ float part_sum[MOST / 32];
   __shared__ uint32_t part_top[MOST / 32];
 
-  uint4 w[NV];
-  if (NORM) {  // a constant of the model: fetched while the preceding kernel drains
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * threads;
-      if (v < nvec) w[i] = __ldg(static_cast<const uint4*>(p.weight) + v);
-    }
+  const uint4* weight = static_cast<const uint4*>(p.weight);
+  if (NORM && blockIdx.x == 0) {  // on its way to the L2 while the preceding kernel drains, whose result it may be
+    for (int v = 8 * threadIdx.x; v < nvec; v += 8 * threads) asm volatile("prefetch.global.L2 [%0];" ::"l"(weight + v));
   }
   if (p.early) pdl_launch_dependents();
   pdl_wait();
@@ -56,7 +52,7 @@ __global__ void __launch_bounds__(MOST) rows_e4m3_kernel(const RowsParams p) {
   uint4* out = NORM && p.residual_out ? reinterpret_cast<uint4*>(static_cast<T*>(p.residual_out) + row * p.cols) : nullptr;
 
   // everything is asked for before anything is looked at: the sums' place may be an input's, and no load passes a store to it
-  uint4 x[NV], a[NV], b[NV];
+  uint4 x[NV], a[NV], b[NV], w[NV];
   float ss = 0.f;
   uint32_t top = 0;
 #pragma unroll
@@ -66,6 +62,7 @@ __global__ void __launch_bounds__(MOST) rows_e4m3_kernel(const RowsParams p) {
       x[i] = in[v];
       if (ADDS > 0) a[i] = a1[v];
       if (ADDS > 1) b[i] = a2[v];
+      if (NORM) w[i] = weight[v];
     }
   }
 #pragma unroll

@@ -26,6 +26,12 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// A box on its way to the L2.  For weights, while the kernel in front still runs: what this asks for is read behind the wait, so it may be that kernel's own
+// result (memory that other kernels write is only visible there, and a copy into shared memory ahead of it may hold what was there before).
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* tmap, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y) : "memory");
+}
+
 }  // namespace tc
 
 // 2-D tensor of codes [rows, k], rows `ld` bytes apart (a multiple of 16), box = 128 codes x box_rows rows, 128-byte swizzle; codes past k

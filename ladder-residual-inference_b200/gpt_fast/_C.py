@@ -42,6 +42,7 @@ LINEAR8_CALL = struct.Struct("@8Q3q4i3f0Q")  # lri_linear_e4m3_call
 
 ONE_SM = 0x100  # LRI_ONE_SM
 ZERO_SKIPPED = 0x200  # LRI_ZERO_SKIPPED
+WEIGHTS_AHEAD = 0x400  # LRI_WEIGHTS_AHEAD
 DENSE, LADDER, LADDER_TWO_STREAMS, PARALLEL, DESYNC, PARALLEL_TWO_STREAMS = range(6)
 
 # name -> (restype, argtypes); the order of arguments is that of include/lri_b200.h

@@ -65,7 +65,7 @@ def _result(out, dtype, rows, n, device):
 
 def quantize_rows(x: Tensor, out: Optional[Rows] = None, early: bool = False) -> Rows:
     """Rows of x [rows, cols] (bfloat16 or float16; rows may lie apart, as parts of a wider buffer) as codes and scales; cols a multiple of 8
-    up to 65536.  early: the projection that follows may start on its weights before these rows are complete; not for rows that are themselves its weights."""
+    up to 65536.  early: the next kernel may start before these rows are complete, for which it waits by itself."""
     shape, strides = x.shape, x.stride()
     rows, cols = shape if len(shape) == 2 else (-1, 0)
     x_ld = cols if rows == 1 else strides[0] if strides else 0
@@ -103,8 +103,7 @@ def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional
            dtype: torch.dtype = torch.bfloat16, out: Optional[Tensor] = None, one_sm: bool = False) -> Tensor:
     """activation(x w^T + bias) + addend, [rows, outputs], summed in fp32 and rounded once.  activation: None, "silu", "gelu" (by the error
     function) or "gelu_tanh"; bias [outputs] and addend [rows, outputs] in the result's type; the addend may be `out`.  dtype: of the result where `out`
-    is None.  The kernel reads w before the call in front of it on the stream is complete: weights, or what quantize_rows and add_rmsnorm have stored
-    (without `early`), not codes that another operator has just written.  one_sm: not on pairs of SMs, for a call beside which another stream runs projections or prompt
+    is None.  A w with `ahead` set may be read before the call in front of this one is complete (E4M3Weight).  one_sm: not on pairs of SMs, for a call beside which another stream runs projections or prompt
     attention (a process can keep off them altogether by option gemm_pair = 0)."""
     rows, k, x_ld = _looked_at("x", x)
     n, depth, w_ld = _looked_at("w", w)
@@ -140,18 +139,20 @@ def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtyp
 
 
 class E4M3Weight:
-    """Rows of a weight in 8 bits: (codes, scale) = weight.  Slices are rows of the same memory."""
-    __slots__ = ("codes", "scale")
+    """Rows of a weight in 8 bits: (codes, scale) = weight.  Slices are rows of the same memory.  ahead: a projection may start on them while the kernel in front of it
+    on the stream still runs; for weights that have been complete since before an operation in front of that which begins when all before it is complete
+    (a copy, any kernel of torch), or since the host last waited."""
+    __slots__ = ("codes", "scale", "ahead")
 
-    def __init__(self, codes: Tensor, scale: Tensor):
-        self.codes, self.scale = codes, scale
+    def __init__(self, codes: Tensor, scale: Tensor, ahead: bool = False):
+        self.codes, self.scale, self.ahead = codes, scale, ahead
 
     def __iter__(self):
         yield self.codes
         yield self.scale
 
     def __getitem__(self, rows: slice) -> "E4M3Weight":
-        return E4M3Weight(self.codes[rows], self.scale[rows])
+        return E4M3Weight(self.codes[rows], self.scale[rows], self.ahead)
 
     @property
     def shape(self):

@@ -183,13 +183,14 @@ class Engine:
             ops.linear(self.y, att.wo.weight, out, rows, workspace=self.ws_wo)
 
     def _rows_e4m3(self, x, to, rows):
-        """The first rows of a buffer in 8 bits.  (early: what follows reads them as the x of a projection.)"""
+        """The first rows of a buffer in 8 bits."""
         cols = x.shape[1]
         self.ops.quantize_rows_e4m3(x, *to, rows, cols, cols, to[0].stride(0), early=True)
         return to
 
     def _linear_e4m3(self, x, w, out, rows, addend=None, glu=False):
         n, k = w.shape
+        w.ahead = True  # (the embedding in front of the layers begins when all before it, whatever last changed a weight too, is complete)
         self.ops.linear_e4m3(x, w, out, rows, n // 2 if glu else n, k, x[0].stride(0), w.codes.stride(0), addend=addend, activation=ACT_GLU if glu else 0,
                              glu=SWIGLU)
 

@@ -201,7 +201,7 @@ class CudaOps:
     # (As above: a look at a tensor's shape or strides costs the host 100 to 200 ns, and the callers have looked.)
     @staticmethod
     def quantize_rows_e4m3(x, codes, scale, rows, cols, x_ld, codes_ld, early=False):
-        """early: what follows on the stream reads the rows as the x of a projection, or not at all (include/lri_b200.h)."""
+        """early: the next kernel may start before this one is complete (include/lri_b200.h)."""
         here = x.get_device()
         if not 0 <= here == torch._C._cuda_getDevice() == codes.get_device() == scale.get_device():
             _C.refuse_devices(x, codes, scale)
@@ -228,6 +228,8 @@ class CudaOps:
     def linear_e4m3(x, w, out, rows, n, k, x_ld, w_ld, bias=None, addend=None, activation=0, glu=(0.0, 0.0, 0.0), flags=0):
         """x, w: (codes, scale); n outputs; activation: a number of LRI_ACT_*; flags: 0 or _C.ONE_SM."""
         (xc, xs), (wc, ws) = x, w
+        if getattr(w, "ahead", False):
+            flags |= _C.WEIGHTS_AHEAD
         here = xc.get_device()
         if not (0 <= here == torch._C._cuda_getDevice() == xs.get_device() == wc.get_device() == ws.get_device() == out.get_device() and
                 (bias is None or bias.get_device() == here) and (addend is None or addend.get_device() == here)):
