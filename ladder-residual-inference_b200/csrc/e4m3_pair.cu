@@ -390,12 +390,18 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
 }
 
+// Pairs that a launch has: those that option gemm_reserve_sms leaves.
+int usable_pairs() {
+  const int pairs = (sm_count() - option(OPT_GEMM_RESERVE_SMS)) / 2;
+  return pairs < 1 ? 1 : pairs;
+}
+
 // Width of the tile: the one with which the busiest SM fetches least.  (A K step of 128 x bn takes 337, 382, 436, 505, 563 cycles at 128 .. 256 by 32, see gemm_pair.cu,
 // as its bytes do at 57 a cycle; so the narrower tile wins where it fills the last round.  us, chosen / 256 / 128 / 64: 512 x 6144 x 4096 15.5 / 18.2 / 17.4 / 20.5,
 // 1000 x 2048 x 8192 17.4 / 25.7 / 17.4 / 24.4, 2048 x 6144 x 4096 40.4 / 40.5 / 44.5 / 61.4, 256 x 4096 x 4096 10.1 / 11.1 / 11.0 / 10.1.  GLU: half a tile's
 // columns in blocks of 32.)
 int64_t fetched(const E4m3Linear& p, bool glu, int* width) {
-  const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, by = glu ? 64 : 32;
+  const int pairs = usable_pairs(), by = glu ? 64 : 32;
   const int64_t w_rows = glu ? 2ll * p.n : p.n, steps = (p.k + kStep - 1) / kStep;
   int64_t least = 0;
   for (int bn = kMaxBn; bn >= 64; bn -= by) {
@@ -431,9 +437,7 @@ int launch(const E4m3Linear& p, int bn, cudaStream_t st) {
   group = group < 2 ? 2 : (group > 16 ? 16 : group);
   group = group > tiles_p ? tiles_p : group;
   GemmGrid grid{static_cast<int>(tiles_p), static_cast<int>(tiles_q), static_cast<int>(group), nullptr, 0};
-  int usable = (sm_count() - option(OPT_GEMM_RESERVE_SMS)) / 2;
-  usable = usable < 1 ? 1 : usable;
-  const int64_t clusters = items < usable ? items : usable;
+  const int64_t clusters = items < usable_pairs() ? items : usable_pairs();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
   cfg.blockDim = dim3(kThreads);

@@ -4,19 +4,23 @@ import contextlib
 import pytest
 import torch
 
-from e4m3_util import check, linear64, random_rows
+from e4m3_util import check, glu64, linear64, random_rows
 from gpt_fast import _C, e4m3
 
 BF16, GLU = 0, _C.ACT_GLU
 
 
 @contextlib.contextmanager
-def gemm_pair(value):
-    _C.check(_C.lib.lri_set_option(b"gemm_pair", value))
+def option(name, value, default):
+    _C.check(_C.lib.lri_set_option(name, value))
     try:
         yield
     finally:
-        _C.check(_C.lib.lri_set_option(b"gemm_pair", 1))
+        _C.check(_C.lib.lri_set_option(name, default))
+
+
+def gemm_pair(value):
+    return option(b"gemm_pair", value, 1)
 
 
 def plan(rows, n, k, activation=0, flags=0):
@@ -46,6 +50,13 @@ def test_off_pairs_by_flag_and_by_option():
 def test_forced_on_pairs():
     with gemm_pair(96):
         assert plan(65, 100, 512) == 96 and plan(65, 100, 512, GLU) == 64 and plan(64, 100, 512) == 0 and plan(300, 100, 512, flags=_C.ONE_SM) == 0
+
+
+def test_tiles_are_chosen_for_the_pairs_that_are_left():
+    """64 tiles of 256 x 128 take 42 pairs two rounds, 40 of 256 x 224 one."""
+    assert plan(1000, 2048, 8192) == 128
+    with option(b"gemm_reserve_sms", 64, 0):
+        assert plan(1000, 2048, 8192) == 224
 
 
 @pytest.mark.parametrize("rows", [64 * 65535, 64 * 65535 + 1, 2 ** 31 - 300, 2 ** 31 - 1])
@@ -93,3 +104,16 @@ def test_many_rows_off_pairs():
     check(want, *linear64(few, w))
     whole = rows // 4096 * 4096
     assert (y[:whole].view(-1, 4096, 8) == want).all() and torch.equal(y[whole:], want[:rows - whole])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,glu", [(1000, 2048, 1024, False), (600, 1500, 520, True), (300, 4096, 1024, False)])
+def test_fewer_pairs(rows, n, k, glu):
+    """The same results whatever is left of the chip: more rounds of tiles of other widths."""
+    x, w = random_rows(rows, k, 1), random_rows(2 * n if glu else n, k, 2, size=k ** -0.5)
+    call = (lambda: e4m3.gateup_glu(x, w)) if glu else (lambda: e4m3.linear(x, w))
+    want = call()
+    check(want, *(glu64(x, w, e4m3.SWIGLU) if glu else linear64(x, w)))
+    for reserved in (1, 20, 63, 64):
+        with option(b"gemm_reserve_sms", reserved, 0):
+            assert torch.equal(call(), want)
