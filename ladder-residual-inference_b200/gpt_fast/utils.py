@@ -127,21 +127,29 @@ class FeedForward(nn.Module):
         return _linear(self.w2, _gated(self.w1.weight, x2)).view(*shape[:-1], -1)
 
 
-def _linear(lin, x2):
-    """x2 [rows, k] through a projection in 16 or 8 bits."""
-    if not isinstance(lin, nn.Linear):
-        return lin(x2)
-    y = torch.empty(x2.shape[0], lin.weight.shape[0], dtype=x2.dtype, device=x2.device)
-    _ops().linear(x2, lin.weight, y, x2.shape[0])
+def _e4m3(weight):
+    """The operators of 8 bits where a weight is in 8 bits, else None.  (Whatever else stands where a projection was is its `weight`, as for the engine.)"""
+    from . import e4m3
+    return e4m3 if isinstance(weight, e4m3.E4M3Weight) else None
+
+
+def _linear(lin, x2, addend=None):
+    """x2 [rows, k] times the weight of a projection in 16 or 8 bits, + addend."""
+    weight = lin.weight
+    eight = _e4m3(weight)
+    if eight:
+        return eight.linear(eight.quantize_rows(x2, early=True), weight, addend=addend, dtype=x2.dtype)
+    y = torch.empty(x2.shape[0], weight.shape[0], dtype=x2.dtype, device=x2.device)
+    _ops().linear(x2, weight, y, x2.shape[0], addend=addend)
     return y
 
 
 def _gated(weight, x2):
     """The gated unit of x2 [rows, k] times weight rows [up | gate], in 16 or 8 bits."""
     rows, inter = x2.shape[0], weight.shape[0] // 2
-    if not isinstance(weight, Tensor):
-        from . import e4m3
-        return e4m3.gateup_glu(e4m3.quantize_rows(x2, early=True), weight, dtype=x2.dtype)
+    eight = _e4m3(weight)
+    if eight:
+        return eight.gateup_glu(eight.quantize_rows(x2, early=True), weight, dtype=x2.dtype)
     ops = _ops()
     h = torch.empty(rows, inter, dtype=x2.dtype, device=x2.device)
     ws_bytes = ops.gateup_workspace_bytes(rows, inter)
@@ -169,9 +177,9 @@ def _qkv(mod, x2, weight_rows, freqs_cis, input_pos, bsz, seqlen):
     ops = _ops()
     rows = bsz * seqlen
     q = torch.empty(rows, mod.n_head * mod.head_dim, dtype=x2.dtype, device=x2.device)
-    if not isinstance(weight_rows, Tensor):
-        from . import e4m3
-        qkv = e4m3.linear(e4m3.quantize_rows(x2, early=True), weight_rows, dtype=x2.dtype)
+    eight = _e4m3(weight_rows)
+    if eight:
+        qkv = eight.linear(eight.quantize_rows(x2, early=True), weight_rows, dtype=x2.dtype)
         ops.rope_kvcache(qkv, freqs_cis.contiguous(), True, input_pos, q, mod.kv_cache.k_cache, mod.kv_cache.v_cache, bsz, seqlen, mod.n_head,
                          mod.n_local_heads, mod.head_dim)
         return q
@@ -258,7 +266,6 @@ class FuseAttentionMLP(nn.Module):
 
     def forward(self, x: Tensor, freqs_cis: Tensor, mask: Tensor, input_pos: Optional[Tensor] = None) -> Tensor:
         assert self.kv_cache is not None, "Caches must be initialized first"
-        ops = _ops()
         bsz, seqlen, _ = x.shape
         rows = bsz * seqlen
         pos = _as_pos(input_pos)
@@ -268,12 +275,7 @@ class FuseAttentionMLP(nn.Module):
         y = _attention_core(self, q, pos, bsz, seqlen)
         attn = _linear(self.wo, y)
         h = _gated(w[self.qkv_rows:], x2)
-        if not isinstance(self.w2, nn.Linear):
-            from . import e4m3
-            return e4m3.linear(e4m3.quantize_rows(h, early=True), self.w2.weight, addend=attn, out=attn).view(bsz, seqlen, -1)
-        out = torch.empty_like(attn)
-        ops.linear(h, self.w2.weight, out, rows, addend=attn)
-        return out.view(bsz, seqlen, -1)
+        return _linear(self.w2, h, addend=attn).view(bsz, seqlen, -1)
 
 
 def all_reduce_func(x: torch.Tensor, clone: bool, async_op=False):
