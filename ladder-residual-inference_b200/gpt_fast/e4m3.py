@@ -112,7 +112,7 @@ def linear(x: Rows, w: Rows, bias: Optional[Tensor] = None, activation: Optional
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation={activation!r}: one of {list(ACTIVATIONS)}")
     if out is None or not (out.dtype in _WIDE and out.shape == (rows, n) and out.is_contiguous()):
-        out = _result(out, dtype, rows, n, x[0].device)
+        out = _result(out, dtype, rows, n, next(iter(x)).device)
     if bias is not None:
         _dense("bias", bias, out.dtype, (n,))
     if addend is not None:
@@ -133,7 +133,7 @@ def gateup_glu(x: Rows, w1: Rows, glu: Tuple[float, float, float] = SWIGLU, dtyp
         raise ValueError(f"rows of {k} codes times [up | gate] weights [{n}, {depth}]")
     if not glu[1] >= 0:
         raise ValueError(f"glu={glu}: the limit is not below 0")
-    out = _result(out, dtype, rows, n // 2, x[0].device)
+    out = _result(out, dtype, rows, n // 2, next(iter(x)).device)
     CudaOps.linear_e4m3(x, w1, out, rows, n // 2, k, x_ld, w_ld, activation=ACT_GLU, glu=glu, flags=ONE_SM if one_sm else 0)
     return out
 
