@@ -63,14 +63,20 @@ def _result(out, dtype, rows, n, device):
     return out
 
 
-def quantize_rows(x: Tensor, out: Optional[Rows] = None, early: bool = False) -> Rows:
-    """Rows of x [rows, cols] (bfloat16 or float16; rows may lie apart, as parts of a wider buffer) as codes and scales; cols a multiple of 8
-    up to 65536.  early: the next kernel may start before these rows are complete, for which it waits by itself."""
+def _wide_rows(x):
+    """Rows, columns and pitch of x, which are what quantize_rows takes."""
     shape, strides = x.shape, x.stride()
     rows, cols = shape if len(shape) == 2 else (-1, 0)
     x_ld = cols if rows == 1 else strides[0] if strides else 0
     if not (rows >= 0 and x.dtype in _WIDE and cols % 8 == 0 and 0 < cols <= 65536 and strides[1] == 1 and x_ld % 8 == 0 and x_ld >= cols):
         raise ValueError(f"x: bfloat16 or float16 rows of a multiple of 8 elements up to 65536 that start at multiples of 16 bytes, not {_said(x)}")
+    return rows, cols, x_ld
+
+
+def quantize_rows(x: Tensor, out: Optional[Rows] = None, early: bool = False) -> Rows:
+    """Rows of x [rows, cols] (bfloat16 or float16; rows may lie apart, as parts of a wider buffer) as codes and scales; cols a multiple of 8
+    up to 65536.  early: the next kernel may start before these rows are complete, for which it waits by itself."""
+    rows, cols, x_ld = _wide_rows(x)
     if out is None:
         out = empty_rows(rows, cols, x.device)
     _, _, codes_ld = _looked_at("out", out, cols, rows)
@@ -161,6 +167,15 @@ class E4M3Weight:
 
 class E4M3Linear(nn.Module):
     """Stands where a model's nn.Linear was: owns the codes and scales of its weight [outputs, k].  `codes` [outputs, k up to a multiple of 16]."""
+
+    @staticmethod
+    def check(lin: nn.Linear):
+        """Raises where a projection cannot go to 8 bits."""
+        if lin.bias is not None:
+            raise ValueError("a projection with a bias")
+        _wide_rows(lin.weight)
+        if lin.weight.data_ptr() % 16:
+            raise ValueError("a weight that does not start at a multiple of 16 bytes")
 
     def __init__(self, weight: Tensor):
         super().__init__()

@@ -97,13 +97,19 @@ class TPModelBase(nn.Module):
             raise TypeError(f"the layers of {type(self).__name__} keep their projections in 16 bits")
         if self._engine is not None:
             raise RuntimeError("projections go to 8 bits before caches are set up")
-        for block in self.layers:
-            for part in (block.attention, getattr(block, "feed_forward", None)):
-                if part is None:
-                    continue
-                for name, module in list(part.named_children()):
-                    if isinstance(module, nn.Linear):
-                        setattr(part, name, E4M3Linear(module.weight))
+        found = [(part, name, module) for block in self.layers for part in (block.attention, getattr(block, "feed_forward", None)) if part is not None
+                 for name, module in part.named_children() if isinstance(module, nn.Linear)]
+        for _, name, module in found:  # (all of them before the first is replaced)
+            try:
+                E4M3Linear.check(module)
+            except ValueError as e:
+                raise ValueError(f"{name}: {e}") from None
+        if len({module.weight.device for _, _, module in found}) > 1:
+            raise ValueError("the layers' projections are on several devices")
+        while found:
+            part, name, module = found.pop(0)
+            setattr(part, name, E4M3Linear(module.weight))
+            del module  # (a weight of 16 bits goes as soon as it has been read: a model may fill more than half of the memory)
         return self
 
     def _setup_layer_caches(self, max_batch_size, max_seq_length, dtype, device):

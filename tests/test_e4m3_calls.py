@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from e4m3_ops import E4M3Ops
 from e4m3_util import random_rows
 from gpt_fast import e4m3
 
@@ -20,3 +21,43 @@ def test_rows_of_a_weight_as_activations_on_the_gpu():
     x = w[:5]
     assert torch.equal(e4m3.linear(x, w), e4m3.linear(tuple(x), tuple(w)))
     assert torch.equal(e4m3.gateup_glu(x, w), e4m3.gateup_glu(tuple(x), tuple(w)))
+
+
+def _tiny(monkeypatch, **shape):
+    from gpt_fast import gpt_dense_TP
+    from test_paged_model import SHAPE
+    monkeypatch.setitem(gpt_dense_TP.transformer_configs, "eight-test", {**SHAPE, **shape})
+    monkeypatch.setattr(e4m3, "CudaOps", E4M3Ops)
+    return gpt_dense_TP.GPTDense.from_name("eight-test").to(torch.bfloat16)
+
+
+def _linears(model):
+    return [type(m) for m in model.layers.modules() if isinstance(m, (torch.nn.Linear, e4m3.E4M3Linear))]
+
+
+@pytest.mark.parametrize("fault", ["width", "bias", "type", "device", "address"])
+def test_a_model_is_quantised_as_a_whole_or_not_at_all(fault, monkeypatch):
+    """The last layer's last projection cannot go to 8 bits: the others stay as they are."""
+    model = _tiny(monkeypatch, **({"intermediate_size": 516} if fault == "width" else {}))
+    last = model.layers[-1].feed_forward.w2
+    if fault == "bias":
+        last.bias = torch.nn.Parameter(torch.zeros(256, dtype=torch.bfloat16))
+    elif fault == "type":
+        last.float()
+    elif fault == "device":
+        last.to("meta")
+    elif fault == "address":
+        n = last.weight.numel()
+        last.weight.data = torch.zeros(n + 4, dtype=torch.bfloat16)[4:].view(last.weight.shape)
+    before = _linears(model)
+    with pytest.raises(ValueError):
+        model.quantize_projections()
+    assert _linears(model) == before and e4m3.E4M3Linear not in before
+
+
+def test_quantised_twice(monkeypatch):
+    model = _tiny(monkeypatch)
+    assert model.quantize_projections() is model
+    kept = [m.codes.data_ptr() for m in model.modules() if isinstance(m, e4m3.E4M3Linear)]
+    model.quantize_projections()
+    assert kept and kept == [m.codes.data_ptr() for m in model.modules() if isinstance(m, e4m3.E4M3Linear)]
