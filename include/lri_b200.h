@@ -359,7 +359,7 @@ int lri_linear_e4m3(const lri_linear_e4m3_call* call);
  * width of the tiles of the one on pairs of SMs. */
 int lri_linear_e4m3_plan(int dtype, int64_t rows, int n, int k, int activation);
 /* The second half of lri_qkv_rope_kvcache: rows [q heads | k heads | v heads] of a projection, qkv [B*S, (n_head + 2 n_kv) * head_dim],
- * to rotated queries and to the caches; arguments as there. */
+ * to rotated queries and to the caches, which do not overlap it; arguments as there. */
 int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_table, const void* input_pos, int pos_is_i64, void* q_out, void* k_cache,
                      void* v_cache, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax, int64_t table_rows, int table_gathered,
                      lri_stream_t stream);

@@ -690,6 +690,10 @@ extern "C" int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_tab
   if (rc != LRI_OK) return rc;
   LRI_REQUIRE(qkv && aligned16(qkv), LRI_ERR_ALIGN, "rope_kvcache: qkv must be 16-byte aligned and not NULL");
   if (B == 0 || S == 0) return LRI_OK;
+  // (each pair is read by the thread that stores it, but results have other pitches than qkv)
+  const int64_t head = 2ll * head_dim, tokens = static_cast<int64_t>(B) * S, qkv_bytes = tokens * (n_head + 2ll * n_kv) * head, cache = smax * B * n_kv * head;
+  LRI_REQUIRE(!overlap(qkv, qkv_bytes, q_out, tokens * n_head * head) && !overlap(qkv, qkv_bytes, k_cache, cache) && !overlap(qkv, qkv_bytes, v_cache, cache), LRI_ERR_ARG,
+              "rope_kvcache: results overlap qkv");
   LinearParams p{};
   p.m = B * S, p.rope_table = rope_table, p.input_pos = input_pos, p.pos_is_i64 = pos_is_i64;
   p.q_out = q_out, p.k_cache = k_cache, p.v_cache = v_cache;

@@ -4,7 +4,7 @@ import torch
 
 from e4m3_ops import E4M3Ops
 from e4m3_util import random_rows
-from gpt_fast import e4m3
+from gpt_fast import _C, e4m3
 
 
 def test_rows_of_a_weight_as_activations():
@@ -61,3 +61,11 @@ def test_quantised_twice(monkeypatch):
     kept = [m.codes.data_ptr() for m in model.modules() if isinstance(m, e4m3.E4M3Linear)]
     model.quantize_projections()
     assert kept and kept == [m.codes.data_ptr() for m in model.modules() if isinstance(m, e4m3.E4M3Linear)]
+
+
+@pytest.mark.parametrize("q,k,v", [(0, 1 << 21, 1 << 22), (256, 1 << 21, 1 << 22), (1 << 20, 512, 1 << 22), (1 << 20, 1 << 21, 1008)])
+def test_rotation_in_place_is_refused(q, k, v):
+    """Queries have another pitch than the rows that they come from: a thread would overwrite what another has yet to read."""
+    at = 1 << 24
+    status = _C.lib.lri_rope_kvcache(0, at, 1 << 20, 1 << 21, 0, at + q, at + k, at + v, 1, 2, 4, 2, 64, 32, 32, 0, None)
+    assert status < 0 and b"overlap" in _C.lib.lri_last_error()
