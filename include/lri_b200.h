@@ -320,7 +320,8 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * lri_linear_e4m3: y[m, j] = act(x_scale[m] * w_scale[j] * sum_k x[m, k] w[j, k] + bias[j]) + addend[m, j], j < n.  bias [n], addend [rows, n]
  * may be NULL; addend may be y.  activation: LRI_ACT_*; GELU by the error function or by tanh.  LRI_ACT_GLU: w has 2 n rows [up | gate] and
  * w_scale 2 n scales, without bias and addend, and y = g * sigmoid(alpha g) * (u + offset) with g = min(gate, limit), u = clamp(up, -limit, limit):
- * SwiGLU with alpha 1, limit infinity, offset 0.
+ * SwiGLU with alpha 1, limit infinity, offset 0.  Activations of z are good to (16 + 1.25 z^2) 2^-24 of their value (GELU; the others to 8 roundings and as many of the
+ * exponential's argument), and zero where their logistic or normal distribution function is below 2^-126.
  *
  * Everything is read when the kernel in front on the stream is complete, but weights with LRI_WEIGHTS_AHEAD: any operator's results may be any input of the
  * next, weights among them.  `early` not 0: the next kernel may start before this one is complete, and waits for it by itself, as all of this library do. */
