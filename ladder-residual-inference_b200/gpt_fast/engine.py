@@ -85,6 +85,7 @@ class Engine:
         nbytes = self.ops.attn_decode_scratch_bytes(max_batch, self.nh, self.nkv, self.hd, _MAX_SPLITS)
         self.scratch = torch.zeros(max(nbytes, 16), dtype=torch.uint8, device=device)
         if self.eight:
+            self.layer_bytes = sum(m.codes.numel() for m in self.model.layers[0].modules() if isinstance(m, E4M3Linear))
             self.qkv = buf((self.nh + 2 * self.nkv) * self.hd)
             self.normed8, self.y8, self.h8 = (empty_rows(rows, n, device) for n in (self.d, self.nh * self.hd, self.inter))
         # one sequence: the second residual of passes whose projections take the norms
@@ -312,6 +313,17 @@ class Engine:
             return False
         return not parallel or self.hd != 128 or self.nh != self.nkv or not 7 * self.sms <= 8 * B * self.nkv <= 10 * self.sms
 
+    def _two_streams_e4m3(self, rows):
+        """Whether a ladder step in 8 bits runs its two sides on two streams.  Not beyond 64 rows, where projections may run on pairs of SMs (8B, 80, 96, 128 sequences
+        4491, 4810, 5577 us so, and 4141, 4614, 5488 on two streams with all of them off pairs).  Nor called eagerly where the host takes longer than the device: its calls take 87 us a
+        layer for two streams and 65 for one, and the device on one stream about 33 and what the weights and 0.8 us for each sequence make (us a layer on one stream and
+        two: 1024 wide, 1 and 64 sequences 65 and 87, 65 and 86; 2048 wide 65 and 86, 75 and 86; 4096, with 14336 hidden units, 1, 16, 24, 64 sequences 68 and 87, 78 and 86, 90 and 87, 126
+        and 106; 5120 with 16384, 1 and 16 82 and 88, 94 and 88; 8192 with 28672, 1 and 64 165 and 145, 231 and 216).  Ranks, whose all-reduces hide behind the other side, take two."""
+        if rows > 64:
+            return False
+        host_bound = self.resid.is_cuda and type(self.comm) is NoComm and self.layer_bytes + 5e6 * rows < 330e6
+        return not host_bound or torch.cuda.is_current_stream_capturing()
+
     def _many_of_a_small_ladder(self, B):
         """Two streams for a small ladder model called eagerly after all: with nine sequences and more the projections have two kernels each, and the
         device is as long as the host (stories110M, us on one stream and two, on two machines: 9 391 and 372, 441 and 421, 16 397 and 373, 445 and
@@ -507,8 +519,7 @@ class Engine:
         mixed = getattr(self.cfg, "ladder_layers", None)
         if mixed is not None and len(set(mixed)) != self.cfg.n_layer:
             return self._run_hybrid(rows, B, S, pos, set(mixed))
-        # (in 8 bits up to 64 rows: more may run on pairs of SMs)
-        if self.eight and rows > 64:
+        if self.eight and S == 1 and not self._two_streams_e4m3(rows):
             return self._run_ladder_one_stream(rows, B, S, pos)
         # (beyond 64 rows only where the kernel on pairs of SMs is not forced upon every projection, as in lri_llama_run)
         if S == 1 and self.overlap_sublayers and (rows <= 64 or rows <= _TWO_STREAM_ROWS and option("gemm_pair") <= 1):

@@ -125,3 +125,38 @@ def test_the_weight_of_a_norm_may_be_a_result(rows, dim):
     torch.cuda.synchronize()
     for turn, (codes, scale) in enumerate(got):
         assert torch.equal(codes.view(torch.uint8), want[turn % 2][0].view(torch.uint8)) and torch.equal(scale, want[turn % 2][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,batch,two", [(256, 1, False), (256, 50, False), (256, 65, False), (4096, 1, False), (4096, 30, True)])
+def test_streams_of_ladder_steps(dim, batch, two, monkeypatch):
+    """Two streams in a graph up to 64 sequences; called eagerly only where the device takes longer than the host.  The same bits."""
+    from gpt_fast.engine import Engine
+    from test_paged_model import SHAPE
+    if dim == 4096:
+        monkeypatch.setitem(SHAPE, "dim", 4096)
+        monkeypatch.setitem(SHAPE, "n_head", 32)
+        monkeypatch.setitem(SHAPE, "n_local_heads", 8)
+        monkeypatch.setitem(SHAPE, "intermediate_size", 14336)
+        monkeypatch.setitem(SHAPE, "n_layer", 2)
+    taken = []
+    for name in ("_run_ladder_one_stream", "_run_ladder_two_streams"):
+        def run(self, *args, _run=getattr(Engine, name), _two=name.endswith("two_streams")):
+            taken.append(_two)
+            _run(self, *args)
+        monkeypatch.setattr(Engine, name, run)
+    with torch.no_grad():
+        model = _model("ladder", "cuda").quantize_projections()
+        model.setup_caches(batch, 32)
+        idx = torch.randint(0, 512, (batch, 1), generator=torch.Generator().manual_seed(1)).cuda()
+        pos = torch.tensor([0], dtype=torch.int32, device="cuda")
+        eager = model(idx, pos).clone()
+        assert taken == [two]
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            logits = model(idx, pos)
+        assert taken[1:] == [batch <= 64]
+        graph.replay()
+        assert torch.equal(logits, eager)
