@@ -308,7 +308,8 @@ int lri_attn_prefill_pages(int dtype, const void* q, const void* k_cache, const 
  * fp32, rounded once where a result is stored.  Codes, rows in 16 bits (but a bias) and results but scales are 16-byte aligned, and results overlap
  * nothing else, but where it says that one may be an input.
  *
- * A row's codes are the nearest to value * (448 / top), its scale top / 448, top the largest magnitude of its values and at least 2^-100.
+ * A row's codes are the nearest to value * (448 / top), quotient and product in fp32 (a value midway between two codes may go to either), its scale top / 448, top
+ * the largest magnitude of its values and at least 2^-100.
  * A row with an infinity or NaN gets zeros and a NaN scale.
  *
  * lri_quantize_rows_e4m3: rows of x (pitch x_ld, a multiple of 8) to codes and scales; cols a multiple of 8 up to 65536.  Also what stores a weight.

@@ -14,7 +14,7 @@
 // form): 1 x 6144 x 4096 8.6, 8.2, 7.8, 7.1; 24 x 4096 x 14336 20.0, 16.7, 15.3, 14.1; 4 gated rows of 14336 from 4096 24.2, 22.4, 21.5, 20.3; with one CTA of 200 KB 7.9, 14.0,
 // 24.8.
 //
-// us and TB/s, one B200, weights out of memory, calls behind one another in a graph: 1 x 6144 x 4096 6.0 (4.2), 24 x 4096 x 14336 with addend 12.5 (4.8), 4 gated rows of 14336
+// us and TB/s, one B200, weights out of memory and into the ring ahead, calls behind one another in a graph: 1 x 6144 x 4096 6.0 (4.2), 24 x 4096 x 14336 with addend 12.5 (4.8), 4 gated rows of 14336
 // from 4096 19.6 (6.0), of 28672 from 8192 70 (6.7), 64 gated rows of 8192 from 2048 9.9 (3.5).  What a call takes beside its bytes is about 3 us: 1 to
 // 1.7 until the last CTA runs and its first bytes come, 1 from the last product to the sums in the joining CTA, 0.5 to 1 for joining.
 //

@@ -5,7 +5,8 @@ namespace lri {
 namespace {
 
 // As the projections in 16 bits (gemm_pair.cu says why): a program that runs tensor-memory kernels on another stream can keep a projection off the kernel on
-// pairs of SMs (LRI_ONE_SM, option gemm_pair = 0), and sums of one or two steps of 128 codes, which a pair has no time to fetch ahead of, never go there.
+// pairs of SMs (LRI_ONE_SM, option gemm_pair = 0), and sums of one or two steps of 128 codes, which are among what that kernel was suspected for, never go there.
+// (us on the other kernel: 4096 x 8192 x 256 79, 2048 x 4096 x 256 with addend 28, 1000 x 2048 x 256 6.0.  The pairs were not run at these depths.)
 constexpr int kMinDepth = 2 * 128;
 
 // 0: the kernel for few rows, else the width of the tiles of the one on pairs.  What both wait for from some tens of rows on is what an SM can take in, about 57

@@ -16,9 +16,13 @@
 // (2048 x 8192 x 1024 23.8 us, 2.9 times its products).  Four storing warps instead of eight: us, 1000 x 4096 x 14336 47.0 / 45.9, 4096 x 4096 x 4096 with GELU 58.0 / 55.0,
 // 2048 x 8192 x 1024 with addend 37.9 / 31.0.
 //
-// us and TFLOP/s, one B200, weights and tokens out of memory: 2048 x 6144 x 4096 40.1 (2570), 4096 x 8192 x 8192 with addend 185 (2970), 4096 gated rows of 14336 from 4096
-// 332 (2900), 8192 x 8192 x 8192 379 (2900; the 1000 W cap sets the clock); the tensor pipe is busy for 83 to 88 % of a launch.  With 129 to 512 rows an SM takes in
+// us and TFLOP/s, one B200, weights and tokens out of memory, some tens of calls behind one another: 2048 x 6144 x 4096 40.8 (2525), 4096 x 8192 x 8192 with addend 186 (2950), 4096
+// gated rows of 14336 from 4096 334 (2880), 8192 x 8192 x 8192 383 (2870); the tensor pipe is busy for 83 to 88 % of a launch.  For seconds on end the 1000 W cap sets
+// the clock: 4096 x 8192 x 8192 224 us at 1230 MHz, the gated rows 371 at 1250; one call at a time on an idle chip 190 and 319 at 1965 MHz.  With 129 to 512 rows an SM takes in
 // too much for too few products: 256 x 4096 x 14336 22.3 us, 2.3 times the weights' time.
+//
+// While the preceding kernel still runs, the weights of the first stages go to the L2 (into the ring, for which they would have to be no result of calls before: no
+// faster).  us, so / without: 300 x 4096 x 1024 6.80 / 6.99, 1000 x 4096 x 4096 17.9 / 18.1, 256 x 4096 x 4096 9.8 / 9.8.
 //
 // Every wait on an mbarrier is bounded (lri_gemm_status); what is not, and why the launch asks for more shared memory than it
 // uses, is said in gemm_pair.cu and holds here.

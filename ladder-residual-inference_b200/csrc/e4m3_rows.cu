@@ -148,7 +148,8 @@ int launch_nv(const RowsParams& p, int64_t rows, cudaStream_t st) {
 // Many rows: CTAs small enough that others run while one waits at its barrier, and no larger than the row (us, all threads / as many as it needs: norms with an addend
 // of 16000 x 768 25.9 / 16.6, 4096 x 5120 27.7 / 24.9; rows as they are 20000 x 768 20.5 / 12.5, 8192 x 5504 22.7 / 21.4; but with eight vectors a thread, rows as they
 // are, 2048 x 28672 27.2 / 40.9, 2047 x 11000 in fp16 12.6 / 17.0: there the stride of a thread has to be a number that the compiler knows).  us by vectors a thread, norms: 16000 x 768 1 16.6, 2 17.8, 4 15.2; 8192 x 2048 21.6, 19.3, 19.9; 8192 x 4096 1 41.2, 2 36.2,
-// 4 36.5; 4096 x 8192 1 44.2, 2 37.0, 4 36.6, and 500 of them 8.2, 7.4, 7.8; 2048 x 16384 2 48.8, 4 37.1, 8 38.4.  As they are: 16000 x 2048 1 21.4, 2 16.1, 4 16.1; 8192 x 4096 1 23.6,
+// 4 36.5; 4096 x 8192 1 44.2, 2 37.0, 4 36.6, and 500 of them 8.2, 7.4, 7.8; 2048 x 16384 2 48.8, 4 37.1, 8 38.4.  The widest rows, eight vectors for 1024 threads
+// / sixteen for 512: 1000 x 40000 26.2 / 27.8, 2048 x 53248 58.5 / 61.3, 149 x 40000 7.6 / 7.9.  As they are: 16000 x 2048 1 21.4, 2 16.1, 4 16.1; 8192 x 4096 1 23.6,
 // 2 17.0, 4 16.2; 4096 x 8192 2 17.8, 4 16.2, 8 16.6; 4096 x 14336 2 32.9, 4 27.8, 8 27.2; 2048 x 28672 4 36.9, 8 27.2.
 template <typename T, int ADDS>
 int launch(const RowsParams& p, int64_t rows, cudaStream_t st) {

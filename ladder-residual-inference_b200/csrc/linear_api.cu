@@ -681,6 +681,8 @@ extern "C" int lri_qkv_rope_kvcache(int dtype, const void* x, const void* wqkv, 
                                table_rows, table_gathered, workspace, workspace_bytes, {}, stream);
 }
 
+// The rotation and the caches behind a projection in 8 bits: one launch a layer.  us with 32 query and 8 key heads of 128: 1 token 1.6, 16 sequences 2.0, 64 3.1, a prompt of 256 7.0, of
+// 1024 23 (3.8 for its bytes: a thread has one pair of elements, with a division for its place).
 extern "C" int lri_rope_kvcache(int dtype, const void* qkv, const void* rope_table, const void* input_pos, int pos_is_i64, void* q_out, void* k_cache,
                                 void* v_cache, int B, int S, int n_head, int n_kv, int head_dim, int64_t smax, int64_t table_rows, int table_gathered,
                                 lri_stream_t stream) {
