@@ -47,13 +47,6 @@ constexpr int kOwnSmem = 181 * 1024;
 constexpr int kStoreWarps = 8;  // two for each quarter of the tensor memory's lanes, which take its columns in turn
 constexpr int kThreads = 64 + 32 * kStoreWarps;
 
-// `bar` may lie in either CTA of the pair
-__device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* tmap, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_dst), "l"(tmap), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
 __device__ __forceinline__ void umma_pair_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -61,15 +54,6 @@ __device__ __forceinline__ void umma_pair_e4m3(uint32_t d_tmem, uint64_t a_desc,
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
-}
-// arrives on the barrier at this offset in both CTAs
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"(static_cast<uint16_t>(3))
-               : "memory");
-}
-__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- from the sums to the results -----------------------------------------------------------------------------------------------
@@ -376,7 +360,7 @@ e4m3_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       if (!stored) break;
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_in_cluster(in_cta(acc_empty0 + 8 * a, 0));
+      if (lane == 0) arrive_and_publish(in_cta(acc_empty0 + 8 * a, 0));
     }
   }
 

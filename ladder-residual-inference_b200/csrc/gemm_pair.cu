@@ -22,6 +22,7 @@
 // stream while products of one K step ran here stopped for good (the form that allocated before the other CTA was known to run).
 // Whether that was the cause is not known, and the engines do not bring the two together: designs with side-by-side mixers
 // ask for single SMs (LRI_ONE_SM).  Option gemm_pair = 0 does the same for a program that runs passes on several streams at a time.
+#include "cluster.cuh"
 #include "gemm_tile.cuh"
 
 namespace lri {
@@ -38,21 +39,6 @@ constexpr int kMaxBn = 256;
 constexpr int kSmemLimit = 226 * 1024;  // of the 227 KB of an SM; the barriers take the rest
 constexpr int kOwnSmem = 181 * 1024;    // the smallest other tensor-memory kernel (prompt attention, heads of 64) takes 49 KB
 
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// `bar` may lie in either CTA of the pair
-__device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* tmap, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_dst), "l"(tmap), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
 __device__ __forceinline__ void umma_pair_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -60,15 +46,6 @@ __device__ __forceinline__ void umma_pair_f16(uint32_t d_tmem, uint64_t a_desc, 
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
-}
-// arrives on the barrier at this offset in both CTAs
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"(static_cast<uint16_t>(3))
-               : "memory");
-}
-__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename T, int EPI>
@@ -95,7 +72,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   const uint32_t acc_full0 = smem_u32(&bars[2 * kMaxStages]);       // products -> stores, one per accumulator
   const uint32_t acc_empty0 = smem_u32(&bars[2 * kMaxStages + 2]);  // stores -> products (first CTA)
 
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  cluster_arrive_relaxed();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < stages; ++s) {
@@ -109,8 +86,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the other CTA runs
+  cluster_wait();  // the other CTA runs
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
                  "r"(2 * kAccCols)
@@ -206,7 +182,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       store_row<T, EPI>(lin, c, shape, static_cast<int64_t>(w.tile_p) * 2 * kBM + rank * kBM + i, w.tile_q, bn, tacc);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_in_cluster(in_cta(acc_empty0 + 8 * a, 0));
+      if (lane == 0) arrive_and_publish(in_cta(acc_empty0 + 8 * a, 0));
     }
   }
 

@@ -16,7 +16,7 @@ def _statements(name):
     return [line for line in lines if line]
 
 
-@pytest.mark.parametrize("name", KERNELS)
+@pytest.mark.parametrize("name", KERNELS + ["gemm_pair.cu"])
 def test_cluster_barriers_are_the_converging_ones(name):
     assert not [line for line in _statements(name) if "barrier.cluster" in line]
 
